@@ -83,6 +83,18 @@ _SIGNATURES = {
     "cdx_linear_fwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp]),
     "cdx_linear_residual_fwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp]),
     "cdx_linear_accum_fwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp]),
+    "cdx_paged_append_fwd": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _vp, ctypes.c_float, _vp,
+                                            _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "cdx_paged_write": (ctypes.c_int, [_vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp,
+                                       _vp]),
+    "cdx_paged_attention_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32, _i32, _i64, _i32]),
+    "cdx_paged_attention_fwd": (ctypes.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp,
+                                               ctypes.c_float, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "cdx_paged_evict_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i32, _i64, _i64]),
+    "cdx_paged_evict": (ctypes.c_int, [_i64, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp,
+                                       _vp, _i64, _i64, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "cdx_sample_tokens": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _i32, _vp,
+                                         ctypes.c_float, _vp, ctypes.c_float, _vp, _vp]),
     "cdx_hbm_probe": (ctypes.c_int, [_i32, _vp, _vp, _i64, _vp]),
 }
 
@@ -193,6 +205,12 @@ def stream_of(t: torch.Tensor) -> int:
     torch.cuda.current_stream(t.device).cuda_stream returns, without building a Stream
     object on every launch)."""
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def on_device(t: torch.Tensor):
+    """A context in which t's device is the current one (a launch on a default stream goes to the
+    current device); the shared no-op context if it is already."""
+    return _NO_REGION if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -21,6 +21,7 @@
 //                     (2 x 777 tokens, 4 heads of 80: 3.6 us; a prompt's own V^T is written by
 //                     the pass above instead).
 #include "cdx_gemm.h"
+#include "cdx_paged.h"
 #include "cdx_skinny.h"
 
 namespace cdx {
@@ -49,28 +50,6 @@ struct QkvCacheParams {
   uint32_t row_blocks;  // blocks of 16 (token, head) rows; those after them copy, or write V
 };
 
-// Sum over each row of 16 lanes, returned to all of them.
-__device__ __forceinline__ float row16_sum(float v) {
-  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, false));
-  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, false));
-  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, false));
-  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, false));
-  return v;
-}
-
-__device__ __forceinline__ void load4(const float* p, float* f) {
-  const float4 v = *reinterpret_cast<const float4*>(p);
-  f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-}
-__device__ __forceinline__ void load4(const uint16_t* p, float* f) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-  f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xffff0000u);
-  f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xffff0000u);
-}
-__device__ __forceinline__ void store4(uint16_t* p, const float* f) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
-}
-
 // A staged tile of 64 tokens x D values in LDS (rows of D + 8) to columns s0 .. s0 + 63 of
 // V^T rows (vt_ld apart) in vt_col order: 16-byte writes along the tokens.
 __device__ __forceinline__ void store_vt_tile(const uint16_t* tile, int D, uint16_t* dst, int64_t vt_ld) {
@@ -91,8 +70,8 @@ __device__ __forceinline__ void store_vt_tile(const uint16_t* tile, int D, uint1
 
 __device__ __forceinline__ uint4 load8_bf16(const float* p) {
   float f[8];
-  load4(p, f);
-  load4(p + 4, f + 4);
+  head_load4(p, f);
+  head_load4(p + 4, f + 4);
   return pack8(f);
 }
 __device__ __forceinline__ uint4 load8_bf16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
@@ -171,26 +150,26 @@ __global__ __launch_bounds__(256) void qkv_cache_kernel(const QkvCacheParams p) 
   const int64_t base = (b * p.nkv + h / (p.nq / p.nkv)) * p.past * p.D + c;  // the query's old cache slab
   float x1[4], x2[4], t[8], w1[4] = {1.f, 1.f, 1.f, 1.f}, w2[4] = {1.f, 1.f, 1.f, 1.f};
   float k1[4], k2[4], v1[4], v2[4];
-  load4(src, x1);
-  load4(src + half, x2);
-  load4(cs, t);
-  load4(cs + 4, t + 4);
+  head_load4(src, x1);
+  head_load4(src + half, x2);
+  head_load4(cs, t);
+  head_load4(cs + 4, t + 4);
   if (nw != nullptr) {
-    load4(nw + c, w1);
-    load4(nw + c + half, w2);
+    head_load4(nw + c, w1);
+    head_load4(nw + c + half, w2);
   }
   if (attend && kind == 0) {
-    load4(p.past_k + base, k1);
-    load4(p.past_k + base + half, k2);
-    load4(p.past_v + base, v1);
-    load4(p.past_v + base + half, v2);
+    head_load4(p.past_k + base, k1);
+    head_load4(p.past_k + base + half, k2);
+    head_load4(p.past_v + base, v1);
+    head_load4(p.past_v + base + half, v2);
   }
   __builtin_amdgcn_sched_barrier(0);
   if (kind != 2) {
     float ss = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(x1[j], x1[j], __builtin_fmaf(x2[j], x2[j], ss));
-    const float rs = rsqrtf(row16_sum(on ? ss : 0.f) / (float)p.D + p.eps);
+    const float rs = rsqrtf(head16_sum(on ? ss : 0.f) / (float)p.D + p.eps);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       x1[j] = norm ? w1[j] * (x1[j] * rs) : x1[j];
@@ -206,15 +185,15 @@ __global__ __launch_bounds__(256) void qkv_cache_kernel(const QkvCacheParams p) 
   if (kind != 0) {
     if (!on) return;
     uint16_t* dst = (kind == 1 ? p.k : p.v) + ((b * p.nkv + h) * rows_out + p.past + s) * p.D + c;
-    store4(dst, x1);
-    store4(dst + half, x2);
+    head_store4(dst, x1);
+    head_store4(dst + half, x2);
     return;
   }
   if (!attend) {
     if (!on) return;
     uint16_t* dst = p.q + ((b * p.nq + h) * p.S + s) * p.D + c;
-    store4(dst, x1);
-    store4(dst + half, x2);
+    head_store4(dst, x1);
+    head_store4(dst + half, x2);
     return;
   }
   // Attention of query s over keys 0 .. s of the old cache (the host has past >= S):
@@ -223,15 +202,15 @@ __global__ __launch_bounds__(256) void qkv_cache_kernel(const QkvCacheParams p) 
   for (int j = 0; j <= s; ++j) {
     if (j > 0) {
       const int64_t at = base + (int64_t)j * p.D;
-      load4(p.past_k + at, k1);
-      load4(p.past_k + at + half, k2);
-      load4(p.past_v + at, v1);
-      load4(p.past_v + at + half, v2);
+      head_load4(p.past_k + at, k1);
+      head_load4(p.past_k + at + half, k2);
+      head_load4(p.past_v + at, v1);
+      head_load4(p.past_v + at + half, v2);
     }
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) dot = __builtin_fmaf(x1[i], k1[i], __builtin_fmaf(x2[i], k2[i], dot));
-    const float z = row16_sum(on ? dot : 0.f) * p.scale_log2;
+    const float z = head16_sum(on ? dot : 0.f) * p.scale_log2;
     // A score of -inf weighs nothing, also as the first (where z - m_new has no value); +inf and
     // NaN make the row NaN, as do scores of -inf alone (l stays 0).
     const float m_new = fmaxf(mx, z);
@@ -250,8 +229,8 @@ __global__ __launch_bounds__(256) void qkv_cache_kernel(const QkvCacheParams p) 
 #pragma unroll
   for (int i = 0; i < 4; ++i) o1[i] *= inv, o2[i] *= inv;
   uint16_t* dst = p.attn + (m * p.nq + h) * p.D + c;
-  store4(dst, o1);
-  store4(dst + half, o2);
+  head_store4(dst, o1);
+  head_store4(dst + half, o2);
 }
 
 // V [slabs][rows][D] (tokens 0 .. S - 1 of each slab) to V^T [slabs][D][vt_ld]: a block

@@ -1,0 +1,414 @@
+// Attention of one new token per sequence over a paged KV cache, for gfx950.
+//
+//   o[b, h] = sum_t p_t v_t,  p = softmax_t(scale q[b, h] . k_t),  t < length[b],
+//
+// with the query heads of a group sharing one head of K and V.  Every key and value is read
+// once for one row of scores, so the cache's bytes bound the operator; what the kernel arranges
+// is that they arrive in whole 16-byte pieces, enough of them at a time, and that each is used
+// for all query heads of its group.
+//
+//   * A wave walks tiles of 32 slots.  S^T = K Q^T with v_mfma_f32_16x16x32_bf16: the rows are
+//     slots, the 16 columns query heads of one group (unused columns cost nothing: the matrix
+//     cores wait for memory).  A lane holds one head's scores of 8 slots, 4 g .. 4 g + 3 of
+//     each half of the tile (g = lane / 16).
+//   * O^T = V^T P^T then wants, in the same lane, 8 slots of P and of V: P is there already, and
+//     V's 8 rows are loaded in that slot order, a piece of DPL columns each, and transposed in
+//     registers (two bf16 of neighbouring rows per v_perm).  Nothing goes through LDS.
+//   * One pass: the running maximum and sum of the softmax, in log2 units and fp32, per wave.
+//     The four waves of a block take every fourth tile and are joined through LDS.
+//   * A sequence is split into `splits` runs of tiles over blocks; the partial sums (fp32, with
+//     their maximum and sum) are joined by a second kernel, which also adds up the weights that
+//     each slot received, from the scores that the first kernel left.
+#include <algorithm>
+
+#include "cdx_paged.h"
+
+namespace cdx {
+namespace {
+
+constexpr int kTile = 32;   // slots of a wave's step
+constexpr int kWaves = 4;
+constexpr int kHeads = 16;  // query heads of a block: the columns of a matrix instruction
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct PagedAttnParams {
+  const uint16_t* q;  // [B][nq][D]
+  const uint16_t* k_pages;
+  const uint16_t* v_pages;
+  PagedTable t;
+  const int32_t* lengths;
+  int32_t B, nq, nkv, D, group, head_tiles, splits;
+  float scale_log2;
+  uint16_t* out;      // [B][nq][D]
+  float* part_o;      // [splits][B][nq][D], unnormalised
+  float2* part_ml;    // [splits][B][nq]: maximum (log2 units) and sum
+  float* scores;      // [B][nq][cap] in log2 units, or nullptr
+  const float* w_in;  // [B][nkv][cap]
+  float* w_out;
+};
+
+// Both values that lanes l and l ^ 16 (l ^ 32) hold, reduced.
+__device__ __forceinline__ float max_over_groups(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// The low (high) halves of two words, side by side.
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+template <int DPL>
+struct Piece;
+template <>
+struct Piece<4> {
+  typedef uint2 type;
+};
+template <>
+struct Piece<8> {
+  typedef uint4 type;
+};
+
+// NC: pieces of 32 dims in a head; DPL: columns of V that a lane holds (16 DPL >= D).
+template <int NC, int DPL>
+__global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttnParams p) {
+  typedef typename Piece<DPL>::type vpiece_t;
+  constexpr int PITCH = 16 * DPL + 4;
+  __shared__ float lds_o[kWaves][kHeads][PITCH];
+  __shared__ float lds_m[kWaves][kHeads], lds_l[kWaves][kHeads];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  // Splits run fastest, so that the blocks of one sequence and head lie together.
+  const uint32_t split = blockIdx.x % p.splits;
+  uint32_t rest = blockIdx.x / p.splits;
+  const int ht = rest % p.head_tiles;
+  rest /= p.head_tiles;
+  const int h = rest % p.nkv, b = rest / p.nkv;
+  const int heads = min(kHeads, p.group - ht * kHeads);
+  const int head0 = h * p.group + ht * kHeads;
+
+  const int32_t cap = p.t.capacity();
+  const int32_t len = min(p.lengths[b], cap);
+  const int32_t tiles = len > 0 ? (len + kTile - 1) / kTile : 0;
+  const int32_t per = (tiles + p.splits - 1) / p.splits;
+  const int32_t t_end = min(tiles, (int32_t)(split + 1) * per);
+
+  // Q^T: column n is head n, 8 dims per lane and piece; dims past the head and heads past the
+  // group are zero.
+  bf16x8 qf[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    const int d = c * 32 + g * 8;
+    if (n < heads && d < p.D) x = *reinterpret_cast<const uint4*>(p.q + ((int64_t)b * p.nq + head0 + n) * p.D + d);
+    qf[c] = __builtin_bit_cast(bf16x8, x);
+  }
+
+  f32x4 acc[DPL];
+#pragma unroll
+  for (int j = 0; j < DPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const int32_t* table = p.t.table + (int64_t)b * p.t.ld;
+  const int lps = p.t.log2_page;
+  const bool v_on = n * DPL < p.D;
+
+  for (int32_t tile = (int32_t)split * per + wave; tile < t_end; tile += kWaves) {
+    const int32_t s0 = tile * kTile;
+    // The two halves of 16 slots each lie inside one page.
+    int32_t page[2];
+    bool there[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int32_t s = s0 + 16 * i;
+      there[i] = false;
+      page[i] = 0;
+      if (s < len) {
+        const int32_t pg = table[s >> lps];
+        there[i] = (uint32_t)pg < (uint32_t)p.t.num_pages;
+        page[i] = there[i] ? pg : 0;
+      }
+    }
+    bf16x8 kf[2][NC];
+    vpiece_t vr[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t row0 = (((int64_t)page[i] * p.nkv + h) << lps) + ((s0 + 16 * i) & ((1 << lps) - 1));
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int d = c * 32 + g * 8;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (d < p.D) x = *reinterpret_cast<const uint4*>(p.k_pages + (row0 + n) * p.D + d);
+        kf[i][c] = __builtin_bit_cast(bf16x8, x);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        vpiece_t x{};
+        if (v_on) x = *reinterpret_cast<const vpiece_t*>(p.v_pages + (row0 + 4 * g + r) * p.D + n * DPL);
+        // A value that no key of the sequence stands for weighs 0, which 0 * NaN is not.
+        if (!there[i] || s0 + 16 * i + 4 * g + r >= len) x = vpiece_t{};
+        vr[4 * i + r] = x;
+      }
+    }
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][c], qf[c], a, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // (A page that is not in the pool makes the row NaN.)
+        const float z = there[i] ? a[r] * p.scale_log2 : __builtin_nanf("");
+        s[4 * i + r] = s0 + 16 * i + 4 * g + r < len ? z : -INFINITY;
+      }
+      if (p.scores != nullptr && n < heads && s0 + 16 * i < len)  // (then the 16 slots lie inside the capacity)
+        *reinterpret_cast<f32x4*>(p.scores + ((int64_t)b * p.nq + head0 + n) * cap + s0 + 16 * i + 4 * g) =
+            f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+    const float m_new = fmaxf(m, max_over_groups(mx));
+    const float m_ref = m_new == -INFINITY ? 0.f : m_new;  // scores of -inf weigh nothing, also the first ones
+    const float alpha = __builtin_amdgcn_exp2f(m - m_ref);
+    m = m_new;
+    l *= alpha;
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) acc[j] *= alpha;
+    float pf[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      pf[i] = __builtin_amdgcn_exp2f(s[i] - m_ref);
+      l += pf[i];
+    }
+    const bf16x8 pb = __builtin_bit_cast(bf16x8, pack8(pf));
+    const uint32_t* vw = reinterpret_cast<const uint32_t*>(vr);  // [8 rows][DPL / 2]
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) {
+      uint4 a;
+      const int w = j / 2;
+      constexpr int RW = DPL / 2;
+      if (j & 1) {
+        a.x = high_halves(vw[0 * RW + w], vw[1 * RW + w]);
+        a.y = high_halves(vw[2 * RW + w], vw[3 * RW + w]);
+        a.z = high_halves(vw[4 * RW + w], vw[5 * RW + w]);
+        a.w = high_halves(vw[6 * RW + w], vw[7 * RW + w]);
+      } else {
+        a.x = low_halves(vw[0 * RW + w], vw[1 * RW + w]);
+        a.y = low_halves(vw[2 * RW + w], vw[3 * RW + w]);
+        a.z = low_halves(vw[4 * RW + w], vw[5 * RW + w]);
+        a.w = low_halves(vw[6 * RW + w], vw[7 * RW + w]);
+      }
+      acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pb, acc[j], 0, 0, 0);
+    }
+  }
+
+  // Join the waves: lane (n, g) holds head n, columns (4 g + r) DPL + j.
+  l = sum_over_groups(l);
+  if (g == 0) {
+    lds_m[wave][n] = m;
+    lds_l[wave][n] = l;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) lds_o[wave][n][(4 * g + r) * DPL + j] = acc[j][r];
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * (p.D / 4); i += 64 * kWaves) {
+    const int hd = i / (p.D / 4), d = (i - hd * (p.D / 4)) * 4;
+    float M = lds_m[0][hd];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, lds_m[w][hd]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lds_m[w][hd] - ref);
+      L = __builtin_fmaf(f, lds_l[w][hd], L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f, lds_o[w][hd][d + e], o[e]);
+    }
+    const int64_t row = (int64_t)b * p.nq + head0 + hd;
+    if (p.splits > 1 || p.scores != nullptr) {
+      const int64_t at = (int64_t)split * p.B * p.nq + row;
+      if (d == 0) p.part_ml[at] = make_float2(M, L);
+      if (p.splits > 1) *reinterpret_cast<float4*>(p.part_o + at * p.D + d) = make_float4(o[0], o[1], o[2], o[3]);
+    }
+    if (p.splits == 1) {
+      // No keys at all: zeros.  Keys whose scores are all -inf: 0 / 0, as softmax has it.
+      const float inv = len > 0 ? 1.f / L : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= inv;
+      head_store4(p.out + row * p.D + d, o);
+    }
+  }
+}
+
+constexpr int kJoinThreads = 256;
+constexpr int kJoinSlots = 1024;  // slots of the weights that a block adds up
+
+// Blocks [0, B * nkv * chunks): chunk 0 joins the splits of one (sequence, KV head); with
+// weights every chunk adds the softmax weights of its slots, over the heads of the group.
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttnParams p, int chunks) {
+  const int chunk = blockIdx.x % chunks;
+  const uint32_t slab = blockIdx.x / chunks;
+  const int b = slab / p.nkv, h = slab - b * p.nkv;
+  const int32_t cap = p.t.capacity(), len = min(p.lengths[b], cap);
+  const int64_t row0 = (int64_t)b * p.nq + h * p.group, step = (int64_t)p.B * p.nq;
+  auto statistics = [&](int64_t row, float& M, float& L) {
+    M = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[s * step + row].x);
+    const float ref = M == -INFINITY ? 0.f : M;
+    L = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float2 ml = p.part_ml[s * step + row];
+      L = __builtin_fmaf(__builtin_amdgcn_exp2f(ml.x - ref), ml.y, L);
+    }
+    M = ref;
+  };
+  if (chunk == 0 && p.splits > 1) {
+    for (int i = threadIdx.x; i < p.group * (p.D / 4); i += kJoinThreads) {
+      const int hd = i / (p.D / 4), d = (i - hd * (p.D / 4)) * 4;
+      float M, L, o[4] = {0.f, 0.f, 0.f, 0.f};
+      statistics(row0 + hd, M, L);
+      for (int s = 0; s < p.splits; ++s) {
+        const int64_t at = s * step + row0 + hd;
+        const float f = __builtin_amdgcn_exp2f(p.part_ml[at].x - M);
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * p.D + d);
+        o[0] = __builtin_fmaf(f, x.x, o[0]), o[1] = __builtin_fmaf(f, x.y, o[1]);
+        o[2] = __builtin_fmaf(f, x.z, o[2]), o[3] = __builtin_fmaf(f, x.w, o[3]);
+      }
+      const float inv = len > 0 ? 1.f / L : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= inv;
+      head_store4(p.out + (row0 + hd) * p.D + d, o);
+    }
+  }
+  if (p.scores == nullptr) return;
+  const int32_t s0 = chunk * kJoinSlots;
+  float w[kJoinSlots / kJoinThreads];
+#pragma unroll
+  for (int u = 0; u < kJoinSlots / kJoinThreads; ++u) {
+    const int32_t s = s0 + u * kJoinThreads + threadIdx.x;
+    w[u] = s < cap ? p.w_in[(int64_t)slab * cap + s] : 0.f;
+  }
+  for (int hd = 0; hd < p.group && s0 < len; ++hd) {
+    float M, L;
+    statistics(row0 + hd, M, L);
+    const float inv = 1.f / L;
+#pragma unroll
+    for (int u = 0; u < kJoinSlots / kJoinThreads; ++u) {
+      const int32_t s = s0 + u * kJoinThreads + threadIdx.x;
+      if (s < len) w[u] = __builtin_fmaf(__builtin_amdgcn_exp2f(p.scores[(row0 + hd) * cap + s] - M), inv, w[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kJoinSlots / kJoinThreads; ++u) {
+    const int32_t s = s0 + u * kJoinThreads + threadIdx.x;
+    if (s < cap) p.w_out[(int64_t)slab * cap + s] = w[u];
+  }
+}
+
+// Blocks that a sequence and head is split over: enough of them for four blocks on each CU, each
+// with at least two tiles per wave when the sequences fill their tables.
+int paged_splits(int64_t blocks, int64_t cap) {
+  const int64_t want = (4 * (int64_t)device_cu_count() + blocks - 1) / blocks;
+  const int64_t most = (cap + 2 * kWaves * kTile - 1) / (2 * kWaves * kTile);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 256}));
+}
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+struct PagedWork {
+  size_t o, ml, scores, total;
+};
+PagedWork paged_work(int64_t B, int64_t nq, int64_t hd, int64_t cap, int splits, bool weights) {
+  PagedWork w{};
+  w.o = splits > 1 ? round16((size_t)(splits * B * nq * hd) * sizeof(float)) : 0;
+  w.ml = splits > 1 || weights ? round16((size_t)(splits * B * nq) * sizeof(float2)) : 0;
+  w.scores = weights ? round16((size_t)(B * nq * cap) * sizeof(float)) : 0;
+  w.total = w.o + w.ml + w.scores;
+  return w;
+}
+
+}  // namespace
+}  // namespace cdx
+
+extern "C" size_t cdx_paged_attention_workspace_bytes(int64_t B, int32_t nq, int32_t nkv, int32_t hd,
+                                                      int64_t capacity, int32_t with_weights) {
+  using namespace cdx;
+  if (B <= 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || hd <= 0 || capacity <= 0) return 0;
+  const int64_t head_tiles = (nq / nkv + kHeads - 1) / kHeads;
+  return paged_work(B, nq, hd, capacity, paged_splits(B * nkv * head_tiles, capacity), with_weights != 0).total;
+}
+
+extern "C" int cdx_paged_attention_fwd(const uint16_t* q, int64_t B, int32_t nq, int32_t nkv, int32_t hd,
+                                       const uint16_t* k_pages, const uint16_t* v_pages, const int32_t* table,
+                                       int64_t table_ld, int64_t width, int64_t num_pages, int32_t page_size,
+                                       const int32_t* lengths, float scale, uint16_t* out, const float* weights_in,
+                                       float* weights_out, void* work, size_t work_bytes, void* stream) {
+  using namespace cdx;
+  const char* name = "cdx_paged_attention_fwd";
+  clear_error();
+  PagedAttnParams p{};
+  if (int rc = paged_table(name, table, table_ld, width, num_pages, page_size, B, nkv, hd, &p.t)) return rc;
+  if (nq <= 0 || nq % nkv != 0) return fail(CDX_EINVAL, "%s: bad shape nq=%d nkv=%d", name, nq, nkv);
+  if (!(scale > 0.f) || scale > 3e38f) return fail(CDX_EINVAL, "%s: scale must be > 0 and finite", name);
+  if ((weights_in == nullptr) != (weights_out == nullptr))
+    return fail(CDX_EINVAL, "%s: weights_in and weights_out must both be given or both be NULL", name);
+  if (width == 0 || num_pages == 0) return fail(CDX_EINVAL, "%s: empty block table or pool", name);
+  if (B == 0) return CDX_OK;
+  const int64_t cap = width * page_size, group = nq / nkv, head_tiles = (group + kHeads - 1) / kHeads;
+  const int64_t blocks = B * nkv * head_tiles;
+  const int64_t chunks = weights_in ? (cap + kJoinSlots - 1) / kJoinSlots : 1;
+  const int splits = paged_splits(blocks, cap);
+  if (B * nq > INT32_MAX / 1024 || blocks * splits > INT32_MAX || B * nkv * chunks > INT32_MAX)
+    return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
+  if (!q || !k_pages || !v_pages || !table || !lengths || !out) return fail(CDX_EINVAL, "%s: null pointer", name);
+  const PagedWork ws = paged_work(B, nq, hd, cap, splits, weights_in != nullptr);
+  if (work_bytes < ws.total || (ws.total > 0 && !work))
+    return fail(CDX_EWORKSPACE, "%s: workspace needs %zu bytes, got %zu", name, ws.total, work ? work_bytes : 0);
+  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(work))
+    return fail(CDX_EUNSUPPORTED, "%s: pointers must be 16-byte aligned", name);
+  p.q = q;
+  p.k_pages = k_pages;
+  p.v_pages = v_pages;
+  p.lengths = lengths;
+  p.B = (int32_t)B;
+  p.nq = nq;
+  p.nkv = nkv;
+  p.D = hd;
+  p.group = (int32_t)group;
+  p.head_tiles = (int32_t)head_tiles;
+  p.splits = splits;
+  p.scale_log2 = scale * kLog2e;
+  p.out = out;
+  char* at = static_cast<char*>(work);
+  p.part_o = reinterpret_cast<float*>(at);
+  p.part_ml = reinterpret_cast<float2*>(at + ws.o);
+  p.scores = weights_in ? reinterpret_cast<float*>(at + ws.o + ws.ml) : nullptr;
+  p.w_in = weights_in;
+  p.w_out = weights_out;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(blocks * splits)), block(64 * kWaves);
+  if (hd <= 32)
+    paged_attn_kernel<1, 4><<<grid, block, 0, s>>>(p);
+  else if (hd <= 64)
+    paged_attn_kernel<2, 4><<<grid, block, 0, s>>>(p);
+  else if (hd <= 96)
+    paged_attn_kernel<3, 8><<<grid, block, 0, s>>>(p);
+  else
+    paged_attn_kernel<4, 8><<<grid, block, 0, s>>>(p);
+  if (int rc = check_launch(name)) return rc;
+  if (splits == 1 && !weights_in) return CDX_OK;
+  paged_join_kernel<<<dim3((unsigned)(B * nkv * chunks)), dim3(kJoinThreads), 0, s>>>(p, (int)chunks);
+  return check_launch(name);
+}

@@ -528,6 +528,97 @@ int cdx_linear_residual_fwd(const uint16_t* x_dev, int64_t ldx, const uint16_t* 
 int cdx_linear_accum_fwd(const uint16_t* x_dev, int64_t ldx, const uint16_t* w_dev, int64_t ldw, int64_t M,
                          int32_t K, int32_t N, uint16_t* residual_dev, int64_t ldr, void* stream);
 
+/* ---- paged generation: the cache in pages, its attention, its bound; sampling ---- */
+
+/*
+ * A paged KV cache.  k_pages and v_pages hold [num_pages, nkv, page_size, hd] bf16; sequence b's
+ * slot t is row t % page_size of page table[b * table_ld + t / page_size], t < width * page_size
+ * (its capacity).  Every entry point checks on the device what it reads there: a slot past the
+ * capacity, or on a page outside [0, num_pages), is neither read nor written.
+ *   page_size  16, 32, 64, 128 or 256
+ *   hd         a multiple of 8 up to 128
+ *   lengths    [B] int32, the slots in use; <= 0: none.  Larger than the capacity counts as it.
+ *
+ * The append of one new token per sequence, from its packed projection:
+ *   qkv        B rows of (nq + 2 nkv) * hd values at stride ldqkv, bf16, or fp32 (qkv_fp32)
+ *   q, k       RMSNorm over each head (weights q_norm_w, k_norm_w [hd]; NULL = none), then RoPE
+ *              at position positions[b] of the fp32 table cos_sin [n_pos, hd / 2, 2]; a position
+ *              outside the table gives NaN
+ *   q_out      [B, nq, hd] bf16
+ *   k, v       to slot lengths[b] - 1: the lengths count the new token already
+ * fp32 arithmetic, one rounding.
+ *
+ * No counterpart in the reference, whose step appends by torch.cat (core/attention.py:138-161).
+ */
+int cdx_paged_append_fwd(const void* qkv_dev, int32_t qkv_fp32, int64_t ldqkv, int64_t B, int32_t nq, int32_t nkv,
+                         int32_t hd, const uint16_t* q_norm_w_dev, const uint16_t* k_norm_w_dev, float eps,
+                         const float* cos_sin_dev, int64_t n_pos, const int32_t* lengths_dev,
+                         const int32_t* positions_dev, const int32_t* table_dev, int64_t table_ld, int64_t width,
+                         int64_t num_pages, int32_t page_size, uint16_t* k_pages_dev, uint16_t* v_pages_dev,
+                         uint16_t* q_out_dev, void* stream);
+
+/*
+ * Prompts into the pages: k, v [B, nkv, S, hd] bf16 (normalised and rotated, as the fused
+ * projection writes them), rows t < min(lengths[b], S) to slot t.
+ */
+int cdx_paged_write(const uint16_t* k_dev, const uint16_t* v_dev, int64_t B, int32_t nkv, int64_t S, int32_t hd,
+                    const int32_t* lengths_dev, const int32_t* table_dev, int64_t table_ld, int64_t width,
+                    int64_t num_pages, int32_t page_size, uint16_t* k_pages_dev, uint16_t* v_pages_dev,
+                    void* stream);
+
+/*
+ * Attention of one new token per sequence over all its slots:
+ *   out[b, h] = sum_t p_t v[t, g],  p = softmax over t < lengths[b] of scale * q[b, h] . k[t, g]
+ * with g = h / (nq / nkv).  q, out [B, nq, hd] bf16.  A sequence without slots gives zeros; one
+ * with a page outside the pool among its slots gives NaN.
+ * weights_in and weights_out [B, nkv, width * page_size] fp32, or NULL:
+ *   weights_out[b, g, t] = weights_in[b, g, t] + sum over g's query heads of p_t   (t < lengths[b])
+ * and a copy at the other slots; they may be the same memory.
+ * work: cdx_paged_attention_workspace_bytes bytes (may be 0), used until the call's work is done.
+ */
+size_t cdx_paged_attention_workspace_bytes(int64_t B, int32_t nq, int32_t nkv, int32_t hd, int64_t capacity,
+                                           int32_t with_weights);
+int cdx_paged_attention_fwd(const uint16_t* q_dev, int64_t B, int32_t nq, int32_t nkv, int32_t hd,
+                            const uint16_t* k_pages_dev, const uint16_t* v_pages_dev, const int32_t* table_dev,
+                            int64_t table_ld, int64_t width, int64_t num_pages, int32_t page_size,
+                            const int32_t* lengths_dev, float scale, uint16_t* out_dev, const float* weights_in_dev,
+                            float* weights_out_dev, void* work_dev, size_t work_bytes, void* stream);
+
+/*
+ * The bound of a cache by accumulated attention weight, for `layers` layers that share the block
+ * table (pages [layers, num_pages, nkv, page_size, hd]; weights and slot_positions [layers, B,
+ * nkv, width * page_size]).  Each head of each sequence that is longer than `keep` keeps the slots
+ * whose position exceeds positions[b] - recent, then those of the largest weight (equal ones
+ * by lower slot; NaN as -inf), `keep` in all.  The kept slots >= keep move, in ascending order,
+ * into the evicted slots < keep, in ascending order; the others stay.  new_* receive the lengths
+ * and, in the new order, the weights and positions (0 and -1 past the new length); they need
+ * memory of their own.  Pages that move rows must belong to one sequence only.
+ */
+size_t cdx_paged_evict_workspace_bytes(int64_t layers, int64_t B, int32_t nkv, int64_t capacity, int64_t keep);
+int cdx_paged_evict(int64_t layers, int64_t B, int32_t nkv, int32_t hd, const int32_t* lengths_dev,
+                    const int32_t* positions_dev, const int32_t* table_dev, int64_t table_ld, int64_t width,
+                    int64_t num_pages, int32_t page_size, uint16_t* k_pages_dev, uint16_t* v_pages_dev,
+                    const float* weights_dev, const int32_t* slot_positions_dev, int64_t keep, int64_t recent,
+                    int32_t* new_lengths_dev, float* new_weights_dev, int32_t* new_slot_positions_dev,
+                    void* work_dev, size_t work_bytes, void* stream);
+
+/*
+ * tokens[b] from logits [B, V] at stride ld (bf16, or fp32 with logits_fp32) and uniforms[b] in
+ * [0, 1): w_i = exp((x_i - max) / T), cut by top-k (all that tie with the k-th stay), then top-p
+ * (descending, equal ones by index: a token stays while the sum before it is <= p * total), then
+ * min-p (w_i >= min_p); the first i whose running sum of kept weights exceeds u * total.  T == 0 (or
+ * NaN) takes the first maximum; top_k <= 0 or >= V, top_p >= 1 and min_p <= 0 cut nothing.  A NaN
+ * logit counts as -inf; a row of -inf alone gives -1.  Each setting is a [B] array or, where
+ * that is NULL, the scalar beside it.  Weights are summed as integers of 62 - ceil(log2 V) bits:
+ * the result does not depend on any order.  V <= 2^20.
+ *
+ * Replaces: the sampling of models/modeling.py:258-283, with the random numbers given.
+ */
+int cdx_sample_tokens(const void* logits_dev, int32_t logits_fp32, int64_t ld, int64_t B, int64_t V,
+                      const float* uniforms_dev, const float* temperature_dev, float temperature,
+                      const int32_t* top_k_dev, int32_t top_k, const float* top_p_dev, float top_p,
+                      const float* min_p_dev, float min_p, int64_t* tokens_dev, void* stream);
+
 /* ---- measurement ---------------------------------------------------------- */
 
 /*

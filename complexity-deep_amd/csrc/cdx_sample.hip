@@ -8,12 +8,21 @@
 //   token   the first i whose running sum of kept weights exceeds u times their total
 //
 // A token is right or wrong, so the sums must not depend on the order in which threads add:
-// weights are integers, round(w 2^s) with s = 62 - ceil(log2 V), which 64 bits sum exactly in any
-// order.  The exponential is taken in 64 bits: with 2^-44 of the largest weight as the step
-// and a hundred thousand tokens, a border lies within rounding of u with probability 1e-8.
+// weights are integers, round(w 2^s) with s = 62 - ceil(log2 V) (at most 51), which 64 bits sum
+// exactly in any order.  The exponential is taken in 64 bits, to about 2^-47: with a hundred
+// thousand tokens a border lies within the rounding of u with a probability around 1e-8.
 //
-// One block per row.  Thresholds come from radix descents over the logits' bits, a byte at a
-// time: of counts for top-k, of weights for top-p.
+// One block per row, no sort.  Each of its 16 waves walks a contiguous part of the row, a span
+// of 64 pieces of 16 bytes at a time, so that a wave's order is the order of the indices.
+//   * The first pass takes the maximum, and each thread's own.  The k-th largest of those 1024
+//     is a lower bound of the k-th largest logit; min-p gives a bound as well (where no top-p
+//     needs the sum over the tokens below it).
+//   * Few tokens pass a bound: a second pass lists them, in order, in LDS, and everything else
+//     (the exact k-th, top-p, the draw) happens among at most 256 a wave, four to a lane.
+//   * Without a bound, or with more than the lists hold, thresholds come from a histogram over
+//     2048 bins of x (of counts for top-k, of weights for top-p), whose border bin is then
+//     resolved by a radix descent over its few tokens; the draw sums the kept weights by span.
+//     Those passes are paced by the exponentials, about 20 instructions in 64 bits a token.
 #include "cdx_common.h"
 
 namespace cdx {
@@ -21,10 +30,13 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kSampleWaves = kThreads / 64;
-constexpr int kVec = 8;                       // tokens that a lane takes at a time
-constexpr int kSpan = 64 * kVec;              // tokens that a wave takes at a time
 constexpr int64_t kMaxVocab = 1 << 20;
-constexpr int kMaxSpans = (int)(kMaxVocab / kSpan);
+constexpr int kListWave = 256;                // tokens that a wave can list
+constexpr int kLane = kListWave / 64;
+constexpr int kList = kListWave * kSampleWaves;
+constexpr int kBins = 2048;
+
+typedef unsigned long long u64;
 
 struct SampleParams {
   const void* logits;  // [B] rows of V at stride ld
@@ -51,208 +63,544 @@ __device__ __forceinline__ float key_logit(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-__device__ __forceinline__ float load_logit(const float* p, int64_t i) { return p[i]; }
-__device__ __forceinline__ float load_logit(const uint16_t* p, int64_t i) { return bf16_bits_to_f32(p[i]); }
-
-typedef unsigned long long u64;
-
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
   return v;
 }
+template <typename T>
+__device__ __forceinline__ T wave_inclusive(T v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T up = __shfl_up(v, d, 64);
+    if (lane >= d) v += up;
+  }
+  return v;
+}
+
+// One row, in pieces of 16 bytes at 16-byte addresses: piece c holds tokens c * VEC - head ..
+// + VEC - 1, those outside 0 .. V - 1 as -inf.
+template <typename TIn>
+struct Row {
+  static constexpr int VEC = 16 / sizeof(TIn);
+  const TIn* x;  // of token -head (not read before token 0)
+  int V, head, pieces;
+
+  __device__ __forceinline__ Row(const TIn* row, int V_) : V(V_) {
+    head = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(TIn));
+    x = row - head;
+    pieces = (head + V + VEC - 1) / VEC;
+  }
+  static __device__ __forceinline__ float value(const float* p) { return *p; }
+  static __device__ __forceinline__ float value(const uint16_t* p) { return bf16_bits_to_f32(*p); }
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) { unpack8(v, f); }
+  __device__ __forceinline__ bool whole(int c) const { return (c > 0 || head == 0) && (c + 1) * VEC - head <= V; }
+  __device__ __forceinline__ void load(int c, float (&f)[VEC]) const {
+    if (whole(c)) {
+      unpack(*reinterpret_cast<const uint4*>(x + (int64_t)c * VEC), f);
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int i = c * VEC + e - head;
+      f[e] = i >= 0 && i < V ? value(x + c * VEC + e) : -INFINITY;
+    }
+  }
+  // f(span, first token, values) over the spans s0 <= span < s1, four loads ahead.
+  template <typename F>
+  __device__ __forceinline__ void spans(int s0, int s1, int lane, F f) const {
+    constexpr int AHEAD = 4;
+    for (int s = s0; s < s1; s += AHEAD) {
+      float v[AHEAD][VEC];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int c = (s + a) * 64 + lane;
+        if (s + a < s1 && c < pieces) {
+          load(c, v[a]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[a][e] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a)
+        if (s + a < s1) f(s + a, ((s + a) * 64 + lane) * VEC - head, v[a]);
+    }
+  }
+};
+
+// exp((x - top) / T) and its integer.
+struct Weights {
+  double top, per_t, unit;  // unit: 2^shift
+
+  // 2^t for t <= 0 as p 2^n, 2^-0.5 <= p <= 2^0.5: the series of 2^r = exp(r ln 2) to r^11, whose
+  // remainder is below 0.35^12 / 12! = 7e-15.
+  static __device__ __forceinline__ double mantissa(double t, int& n) {
+    const double k = __builtin_rint(t), r = t - k;
+    n = (int)k;
+    double p = 4.44553827187081e-10;               // ln2^11 / 11!
+    p = __builtin_fma(p, r, 7.054911620801121e-09);  // ln2^10 / 10!
+    p = __builtin_fma(p, r, 1.0178086009239699e-07);
+    p = __builtin_fma(p, r, 1.3215486790144309e-06);
+    p = __builtin_fma(p, r, 1.5252733804059841e-05);
+    p = __builtin_fma(p, r, 0.0001540353039338161);
+    p = __builtin_fma(p, r, 0.0013333558146428441);
+    p = __builtin_fma(p, r, 0.009618129107628477);
+    p = __builtin_fma(p, r, 0.055504108664821576);
+    p = __builtin_fma(p, r, 0.24022650695910072);
+    p = __builtin_fma(p, r, 0.6931471805599453);
+    return __builtin_fma(p, r, 1.0);
+  }
+  // (x - top) log2(e) / T, no lower than -256; a logit of -inf, and any other beside a top of
+  // +inf, is as low (also at a temperature without bounds).
+  __device__ __forceinline__ double exponent(float x) const {
+    const double t = ((double)x - top) * per_t;
+    return t >= -256.0 ? t : (x == top ? 0.0 : -256.0);
+  }
+  __device__ __forceinline__ double fraction(float x) const {
+    int n;
+    const double p = mantissa(exponent(x), n);
+    return __builtin_ldexp(p, n);
+  }
+  static __device__ __forceinline__ u64 round_units(double w) {
+    // w < 2^52: its integer is the low part of w + 2^52.
+    return __builtin_bit_cast(u64, w + 4503599627370496.0) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ u64 units(float x) const { return round_units(fraction(x) * unit); }
+};
+
+struct Shared {
+  u64 bins[kBins];
+  u64 sums[kMaxVocab / 256 + 1];  // by span: at most 2^20 / 256 + 1 of them
+  int ties[kMaxVocab / 256 + 1];
+  uint32_t list_key[kList];
+  int list_index[kList];
+  u64 red[kSampleWaves];
+  u64 pick[3];
+  int count[kSampleWaves];
+  int total;
+};
+
+// Sum over the block, returned to every thread.
+__device__ __forceinline__ u64 block_sum(u64 v, Shared& sh) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  u64 t = 0;
+#pragma unroll
+  for (int w = 0; w < kSampleWaves; ++w) t += sh.red[w];
+  return t;
+}
+
+// By wave 0: the last of n bins, from the highest down, that holds something and before which
+// the sum is within the limit: (bin, that sum) into pick.
+__device__ __forceinline__ void pick_bin(Shared& sh, int n, u64 above, u64 limit, bool descending) {
+  const int lane = threadIdx.x, per = n / 64;
+  u64 mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int d = lane * per + i;
+    mine += sh.bins[descending ? n - 1 - d : d];
+  }
+  u64 before = above + wave_inclusive(mine, lane) - mine;
+  int last = -1;
+  u64 at = 0;
+  for (int i = 0; i < per && before <= limit; ++i) {
+    const int d = lane * per + i;
+    const u64 v = sh.bins[descending ? n - 1 - d : d];
+    if (v != 0) {
+      last = d;
+      at = before;
+    }
+    before += v;
+  }
+  const u64 lanes = __ballot(last >= 0);
+  if (lanes != 0 && lane == 63 - __builtin_clzll(lanes)) {
+    sh.pick[0] = (u64)(descending ? n - 1 - last : last);
+    sh.pick[1] = at;
+  }
+}
+
+// The smallest key before which the items of larger keys weigh no more than the limit, and that
+// weight.  each(f) calls f(key, weight) for the thread's items.  A byte at a time.
+template <typename Each>
+__device__ uint32_t descend(Shared& sh, u64& above, u64 limit, Each each) {
+  uint32_t prefix = 0;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    __syncthreads();
+    if (threadIdx.x < 256) sh.bins[threadIdx.x] = 0;
+    __syncthreads();
+    each([&](uint32_t key, u64 w) {
+      if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&sh.bins[(key >> shift) & 255], w);
+    });
+    __syncthreads();
+    if (threadIdx.x < 64) pick_bin(sh, 256, above, limit, true);
+    __syncthreads();
+    prefix = prefix << 8 | (uint32_t)sh.pick[0];
+    above = sh.pick[1];
+  }
+  return prefix;
+}
 
 template <typename TIn>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
-  __shared__ u64 hist[256];
-  __shared__ u64 spans[kMaxSpans];
-  __shared__ u64 red[kSampleWaves];
-  __shared__ u64 pick[3];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x;
-  const TIn* x = static_cast<const TIn*>(p.logits) + row * p.ld;
-  const int V = p.V;
-  const float T = p.temperature ? p.temperature[row] : p.temperature1;
-  const float top_p = p.top_p ? p.top_p[row] : p.top_p1, min_p = p.min_p ? p.min_p[row] : p.min_p1;
-  const int top_k = p.top_k ? p.top_k[row] : p.top_k1;
+  __shared__ Shared sh;
+  constexpr int VEC = Row<TIn>::VEC;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t b = blockIdx.x;
+  const Row<TIn> row(static_cast<const TIn*>(p.logits) + b * p.ld, p.V);
+  const int n_spans = (row.pieces + 63) / 64;
+  const int per_wave = (n_spans + kSampleWaves - 1) / kSampleWaves;
+  const int s0 = min(n_spans, wave * per_wave), s1 = min(n_spans, s0 + per_wave);
+  const float T = p.temperature ? p.temperature[b] : p.temperature1;
+  const float min_p = p.min_p ? p.min_p[b] : p.min_p1, u = p.uniforms[b];
+  float top_p = p.top_p ? p.top_p[b] : p.top_p1;
+  int top_k = p.top_k ? p.top_k[b] : p.top_k1;
 
-  // The largest logit and the first index that has it.
-  u64 best = 0;
-  for (int i = tid; i < V; i += kThreads) {
-    const u64 c = (u64)logit_key(load_logit(x, i)) << 32 | (uint32_t)~i;
-    best = c > best ? c : best;
-  }
+  // The largest logit (fmaxf passes over NaN), of the thread and of the row.
+  float mine = -INFINITY;
+  row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const u64 o = __shfl_xor(best, d, 64);
-    best = o > best ? o : best;
-  }
-  if (lane == 0) red[wave] = best;
+    for (int e = 0; e < VEC; ++e) mine = fmaxf(mine, v[e]);
+  });
+  float top = mine;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  if (lane == 0) sh.red[wave] = __float_as_uint(top);
   __syncthreads();
-  for (int w = 0; w < kSampleWaves; ++w) best = red[w] > best ? red[w] : best;
-  const uint32_t top = (uint32_t)(best >> 32);
-  const float top_x = key_logit(top);
-  if (top_x == -INFINITY || !(T > 0.f)) {
-    if (tid == 0) p.tokens[row] = top_x == -INFINITY ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
+#pragma unroll
+  for (int w = 0; w < kSampleWaves; ++w) top = fmaxf(top, __uint_as_float((uint32_t)sh.red[w]));
+  if (top == -INFINITY) {
+    if (tid == 0) p.tokens[b] = -1;
     return;
   }
-
-  const double one = (double)(1ull << p.shift);
-  // Weights as a fraction of the largest, and as integers.
-  auto weight = [&](uint32_t key) -> double {
-    if (key == top) return 1.0;
-    const float v = key_logit(key);
-    if (top_x == INFINITY || v == -INFINITY) return 0.0;  // (also at a temperature without bounds)
-    return exp(((double)v - (double)top_x) / (double)T);
-  };
-  auto units = [&](double w) -> u64 { return (u64)(w * one + 0.5); };
-
-  // top-k: the key of the k-th largest logit.
-  uint32_t low = 0;
-  if (top_k > 0 && top_k < V) {
-    uint32_t prefix = 0;
-    u64 need = top_k;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < V; i += kThreads) {
-        const uint32_t key = logit_key(load_logit(x, i));
-        if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1ull);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        u64 above = 0;
-        int d = 255;
-        while (d > 0 && above + hist[d] < need) above += hist[d--];
-        pick[0] = d;
-        pick[1] = above;
-      }
-      __syncthreads();
-      prefix = prefix << 8 | (uint32_t)pick[0];
-      need -= pick[1];
-    }
-    low = prefix;
-  }
-
-  // top-p: the smallest kept key, and how many of the tokens that have it are kept.
-  uint32_t border = low;
-  u64 border_count = ~0ull;
-  if (top_p < 1.f) {
-    u64 limit = 0, above = 0;
-    uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < V; i += kThreads) {
-        const uint32_t key = logit_key(load_logit(x, i));
-        if (key >= low && (shift == 24 || key >> (shift + 8) == prefix))
-          atomicAdd(&hist[(key >> shift) & 255], units(weight(key)));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        if (shift == 24) {
-          u64 total = 0;
-          for (int d = 0; d < 256; ++d) total += hist[d];
-          limit = (u64)((double)(top_p > 0.f ? top_p : 0.f) * (double)total);
-        }
-        // The last digit, from above, with weight before which the sum is within the limit.
-        u64 sum = above;
-        int last = 0;
-        for (int d = 255; d >= 0 && sum <= limit; --d) {
-          if (hist[d] == 0) continue;
-          last = d;
-          above = sum;
-          sum += hist[d];
-        }
-        pick[0] = last;
-        pick[1] = above;
-        pick[2] = limit;
-      }
-      __syncthreads();
-      prefix = prefix << 8 | (uint32_t)pick[0];
-      above = pick[1];
-      limit = pick[2];
-    }
-    border = prefix;
-    border_count = (limit - above) / units(weight(border)) + 1;
-  }
-
-  // First index whose running sum of f exceeds a target, from the sums of spans of 512 tokens.
-  const int n_spans = (V + kSpan - 1) / kSpan;
-  auto span_sums = [&](auto f) {
-    __syncthreads();
-    for (int s = wave; s < n_spans; s += kSampleWaves) {
-      u64 sum = 0;
+  if (!(T > 0.f)) {
+    int first = p.V;
+    if (mine == top)
+      row.spans(s0, s1, lane, [&](int, int i0, const float(&v)[VEC]) {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const int i = s * kSpan + e * 64 + lane;
-        if (i < V) sum += f(i, logit_key(load_logit(x, i)));
-      }
-      sum = wave_sum(sum);
-      if (lane == 0) spans[s] = sum;
-    }
+        for (int e = 0; e < VEC; ++e)
+          if (v[e] == top) first = min(first, i0 + e);
+      });
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) first = min(first, __shfl_xor(first, d, 64));
     __syncthreads();
-  };
-  // (Every thread returns the index; target < the sum over the row.)
-  auto find = [&](auto f, u64 target) -> int {
-    if (wave == 0) {
-      int s = 0;
+    if (lane == 0) sh.red[wave] = (u64)first;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSampleWaves; ++w) first = min(first, (int)sh.red[w]);
+    if (tid == 0) p.tokens[b] = first;
+    return;
+  }
+  const Weights wt{(double)top, 1.4426950408889634 / (double)T, (double)(1ull << p.shift)};
+  if (top_k >= p.V) top_k = 0;
+  if (!(top_p < 1.f)) top_p = 1.f;
+  if (top_p < 0.f) top_p = 0.f;
+  const bool cut_p = top_p < 1.f;
+
+  // A logit below `bound` is not kept, whatever the others are.
+  float bound = -INFINITY;
+  if (top_k > 0 && top_k <= min(row.pieces, kThreads)) {
+    // (A thread without tokens has -inf, which bounds nothing.)
+    u64 above = 0;
+    bound = key_logit(descend(sh, above, (u64)top_k - 1, [&](auto f) { f(logit_key(mine), 1); }));
+  }
+  if (min_p > 0.f && !cut_p) {
+    // x >= top + T ln(min_p), less what the rounding of a weight (far below 1e-9 of it), and here of
+    // the bound to 32 bits, could make of it.
+    const double low = (double)top + (double)T * (log((double)(min_p < 1.f ? min_p : 1.f)) - 1e-9);
+    bound = fmaxf(bound, (float)(low - 1e-6 * (fabs((double)top) + fabs(low))));
+  }
+  const bool bounded = bound > -INFINITY || row.pieces * VEC <= kList;
+
+  // The tokens that pass, in order, by wave; more than the list holds: count only.
+  int listed = kListWave + 1;
+  if (bounded) {
+    listed = 0;
+    row.spans(s0, s1, lane, [&](int, int i0, const float(&v)[VEC]) {
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) n += v[e] >= bound && v[e] > -INFINITY ? 1 : 0;
+      if (__ballot(n > 0) == 0) return;
+      const int incl = wave_inclusive(n, lane);
+      int at = listed + incl - n;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (v[e] >= bound && v[e] > -INFINITY) {
+          if (at < kListWave) {
+            sh.list_key[wave * kListWave + at] = logit_key(v[e]);
+            sh.list_index[wave * kListWave + at] = i0 + e;
+          }
+          ++at;
+        }
+      listed += __builtin_amdgcn_readlane(incl, 63);
+    });
+  }
+  __syncthreads();
+  if (lane == 0) sh.count[wave] = listed;
+  __syncthreads();
+  bool fits = true;
+#pragma unroll
+  for (int w = 0; w < kSampleWaves; ++w) fits = fits && sh.count[w] <= kListWave;
+
+  if (fits) {
+    uint32_t key[kLane];
+    int index[kLane];
+    u64 w[kLane];
+    double wf[kLane];
+    bool on[kLane];
+#pragma unroll
+    for (int r = 0; r < kLane; ++r) {
+      const int i = r * 64 + lane;
+      on[r] = i < listed;
+      key[r] = on[r] ? sh.list_key[wave * kListWave + i] : 0u;
+      index[r] = on[r] ? sh.list_index[wave * kListWave + i] : 0;
+    }
+    if (top_k > 0) {
+      u64 above = 0;
+      const uint32_t low = descend(sh, above, (u64)top_k - 1, [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < kLane; ++r)
+          if (on[r]) f(key[r], 1);
+      });
+#pragma unroll
+      for (int r = 0; r < kLane; ++r) on[r] = on[r] && key[r] >= low;
+    }
+#pragma unroll
+    for (int r = 0; r < kLane; ++r) {
+      wf[r] = on[r] ? wt.fraction(key_logit(key[r])) : 0.0;
+      w[r] = on[r] ? Weights::round_units(wf[r] * wt.unit) : 0;
+    }
+    if (cut_p) {
+      u64 s = 0;
+#pragma unroll
+      for (int r = 0; r < kLane; ++r) s += w[r];
+      const u64 total = block_sum(s, sh);
+      const u64 limit = (u64)((double)top_p * (double)total);
+      u64 above = 0;
+      const uint32_t border = descend(sh, above, limit, [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < kLane; ++r)
+          if (w[r] != 0) f(key[r], w[r]);
+      });
+      const u64 keep = (limit - above) / wt.units(key_logit(border)) + 1;
+      // Ties at the border by index: those of the waves before, then of this wave's items before.
+      int ties = 0;
+#pragma unroll
+      for (int r = 0; r < kLane; ++r) ties += __popcll(__ballot(on[r] && key[r] == border));
+      __syncthreads();
+      if (lane == 0) sh.count[wave] = ties;
+      __syncthreads();
       u64 before = 0;
-      while (s < n_spans - 1 && before + spans[s] <= target) before += spans[s++];
-      int at = -1;
-      for (int e = 0; e < kVec && at < 0; ++e) {
-        const int i = s * kSpan + e * 64 + lane;
-        u64 run = i < V ? f(i, logit_key(load_logit(x, i))) : 0;
+      for (int v = 0; v < wave; ++v) before += sh.count[v];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const u64 up = __shfl_up(run, d, 64);
-          if (lane >= d) run += up;
-        }
-        const u64 hit = __ballot(before + run > target);
-        if (hit != 0) at = s * kSpan + e * 64 + __builtin_ctzll(hit);
-        before += __shfl(run, 63, 64);
+      for (int r = 0; r < kLane; ++r) {
+        const u64 tie = __ballot(on[r] && key[r] == border);
+        const u64 rank = before + __popcll(tie & ((1ull << lane) - 1));
+        on[r] = on[r] && (key[r] > border || (key[r] == border && rank < keep));
+        before += __popcll(tie);
       }
-      if (lane == 0) pick[0] = (u64)(at < 0 ? V - 1 : at);
     }
-    __syncthreads();
-    return (int)pick[0];
-  };
-
-  // Ties at the border are kept in the order of their indices.
-  int last_tie = V;
-  if (border_count != ~0ull) {
-    auto tie = [&](int, uint32_t key) -> u64 { return key == border ? 1 : 0; };
-    span_sums(tie);
-    u64 count = 0;
-    for (int s = lane; s < n_spans; s += 64) count += spans[s];
-    count = wave_sum(count);
-    if (count > border_count) last_tie = find(tie, border_count - 1);
-  }
-  auto allowed = [&](int i, uint32_t key) {
-    if (key < border || (key == border && i > last_tie)) return false;
-    return !(min_p > 0.f) || key == top || weight(key) >= (double)min_p;
-  };
-  auto kept = [&](int i, uint32_t key) -> u64 { return allowed(i, key) ? units(weight(key)) : 0; };
-  const float u = p.uniforms[row];
-  if (!(u > 0.f)) {
-    // The first kept token of any weight, also of one that rounds to no unit.
-    auto any = [&](int i, uint32_t key) -> u64 { return allowed(i, key) && weight(key) > 0.0 ? 1 : 0; };
-    span_sums(any);
-    const int token = find(any, 0);
-    if (tid == 0) p.tokens[row] = token;
+    u64 s = 0;
+#pragma unroll
+    for (int r = 0; r < kLane; ++r) {
+      const bool is_top = key_logit(key[r]) == top;
+      on[r] = on[r] && (!(min_p > 0.f) || is_top || wf[r] >= (double)min_p);
+      // u == 0: the first kept token of any weight, also of one that rounds to no unit.
+      if (!(u > 0.f)) w[r] = on[r] && (is_top || exp(((double)key_logit(key[r]) - wt.top) / (double)T) > 0.0) ? 1 : 0;
+      w[r] = on[r] ? w[r] : 0;
+      s += w[r];
+    }
+    const u64 total = block_sum(s, sh);
+    u64 target = u > 0.f ? (u64)((double)(u < 1.f ? u : 1.f) * (double)total) : 0;
+    if (target >= total) target = total - 1;
+    u64 before = 0;
+    for (int v = 0; v < wave; ++v) before += sh.red[v];
+    if (target < before || target >= before + sh.red[wave]) return;  // another wave's
+#pragma unroll
+    for (int r = 0; r < kLane; ++r) {
+      const u64 run = before + wave_inclusive(w[r], lane);
+      const u64 hit = __ballot(run > target);
+      if (hit != 0) {
+        if (lane == __builtin_ctzll(hit)) p.tokens[b] = index[r];
+        return;
+      }
+      before = __shfl(run, 63, 64);
+    }
     return;
   }
-  span_sums(kept);
-  u64 total = 0;
-  for (int s = lane; s < n_spans; s += 64) total += spans[s];
-  total = wave_sum(total);
-  u64 target = (u64)((double)(u < 1.f ? u : 1.f) * (double)total);
+
+  // Whole rows.  The border of a sum over the row (of counts or of weights), from the highest logit
+  // down: by bins of equal width, then among the tokens of the border bin.
+  auto border_of = [&](float per_x, u64 above, auto limit_of, auto weight) -> uint32_t {
+    // Bins count down from the top; those past the last one are the last one.
+    auto bin = [&](float x) -> int {
+      const float d = (top - x) * per_x;
+      return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+    };
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
+    __syncthreads();
+    row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const u64 w = v[e] > -INFINITY ? weight(v[e]) : 0;
+        if (w != 0) atomicAdd(&sh.bins[bin(v[e])], w);
+      }
+    });
+    __syncthreads();
+    u64 t = 0;
+    for (int i = tid; i < kBins; i += kThreads) t += sh.bins[i];
+    const u64 limit = limit_of(block_sum(t, sh));
+    if (tid < 64) pick_bin(sh, kBins, above, limit, false);
+    if (tid == 0) sh.total = 0;
+    __syncthreads();
+    const int chosen = (int)sh.pick[0];
+    above = sh.pick[1];
+    row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (v[e] > -INFINITY && bin(v[e]) == chosen) {
+          const int at = atomicAdd(&sh.total, 1);
+          if (at < kList) sh.list_key[at] = logit_key(v[e]);
+        }
+    });
+    __syncthreads();
+    const int n = sh.total;
+    const uint32_t key = descend(sh, above, limit, [&](auto f) {
+      if (n <= kList) {
+        for (int i = tid; i < n; i += kThreads) {
+          const u64 w = weight(key_logit(sh.list_key[i]));
+          if (w != 0) f(sh.list_key[i], w);
+        }
+      } else {
+        row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (v[e] > -INFINITY && bin(v[e]) == chosen) {
+              const u64 w = weight(v[e]);
+              if (w != 0) f(logit_key(v[e]), w);
+            }
+        });
+      }
+    });
+    if (tid == 0) {
+      sh.pick[1] = above;
+      sh.pick[2] = limit;
+    }
+    __syncthreads();
+    return key;
+  };
+
+  float low = -INFINITY;
+  if (top_k > 0) {
+    // Bins over four times the spread of the threads' maxima.
+    float least = mine > -INFINITY ? mine : top;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) least = fminf(least, __shfl_xor(least, d, 64));
+    __syncthreads();
+    if (lane == 0) sh.red[wave] = __float_as_uint(least);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSampleWaves; ++w) least = fminf(least, __uint_as_float((uint32_t)sh.red[w]));
+    const float spread = top - least;
+    const float per_x = spread > 0.f && spread < INFINITY ? (float)(kBins / 4) / spread : 0.f;
+    low = key_logit(border_of(per_x, 0, [&](u64 n) { return (u64)top_k - 1 < n ? (u64)top_k - 1 : n - 1; },
+                              [](float) -> u64 { return 1; }));
+  }
+  float border = low;
+  u64 keep = ~0ull, tie_w = 0;
+  if (cut_p) {
+    // A weight past 2^-64 is no unit: bins over that many times T ln 2.
+    const float range = 44.4f * T, per_x = range < 1e30f && range > 1e-30f ? (float)kBins / range : 0.f;
+    border = key_logit(border_of(per_x, 0, [&](u64 n) { return (u64)((double)top_p * (double)n); },
+                                 [&](float x) -> u64 { return x >= low ? wt.units(x) : 0; }));
+    tie_w = wt.units(border);
+    keep = (sh.pick[2] - sh.pick[1]) / tie_w + 1;
+  }
+  // Kept weights by span, the ties at the border counted apart.
+  const bool any = !(u > 0.f);
+  auto kept = [&](float x) -> u64 {
+    if (x == top) return any ? 1 : wt.units(x);
+    const double w = wt.fraction(x);
+    if (min_p > 0.f && !(w >= (double)min_p)) return 0;
+    if (any) return exp(((double)x - wt.top) / (double)T) > 0.0 ? 1 : 0;
+    return Weights::round_units(w * wt.unit);
+  };
+  const bool by_ties = keep != ~0ull;
+  tie_w = by_ties ? kept(border) : 0;
+  __syncthreads();
+  row.spans(s0, s1, lane, [&](int s, int, const float(&v)[VEC]) {
+    u64 sum = 0;
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (v[e] > border || (!by_ties && v[e] == border && v[e] > -INFINITY)) sum += kept(v[e]);
+      ties += by_ties && v[e] == border ? 1 : 0;
+    }
+    sum = wave_sum(sum);
+    ties = wave_sum(ties);
+    if (lane == 0) {
+      sh.sums[s] = sum;
+      sh.ties[s] = ties;
+    }
+  });
+  __syncthreads();
+  if (wave != 0) return;
+  // By the first wave: the spans' sums with their kept ties, then the span that the draw falls in.
+  u64 total = 0, ties_before = 0;
+  for (int base = 0; base < n_spans; base += 64) {
+    const int s = base + lane;
+    const u64 ties = by_ties && s < n_spans ? sh.ties[s] : 0;
+    const u64 tie_at = ties_before + wave_inclusive(ties, lane) - ties;
+    const u64 mine_kept = tie_at >= keep ? 0 : (keep - tie_at < ties ? keep - tie_at : ties);
+    const u64 sum = s < n_spans ? sh.sums[s] + mine_kept * tie_w : 0;
+    if (s < n_spans) sh.sums[s] = sum;
+    total += wave_sum(sum);
+    ties_before += wave_sum(ties);
+  }
+  u64 target = any ? 0 : (u64)((double)(u < 1.f ? u : 1.f) * (double)total);
   if (target >= total) target = total - 1;
-  const int token = find(kept, target);
-  if (tid == 0) p.tokens[row] = token;
+  u64 before = 0, rank = 0;
+  int span = -1;
+  for (int base = 0; base < n_spans && span < 0; base += 64) {
+    const int s = base + lane;
+    const u64 sum = s < n_spans ? sh.sums[s] : 0, ties = by_ties && s < n_spans ? sh.ties[s] : 0;
+    const u64 run = wave_inclusive(sum, lane), tie_run = wave_inclusive(ties, lane);
+    const u64 hit = __ballot(before + run > target);
+    const int at = hit != 0 ? __builtin_ctzll(hit) : 63;
+    // (Up to the span, or past all 64.)
+    before += __shfl(run, at, 64) - (hit != 0 ? __shfl(sum, at, 64) : 0);
+    rank += __shfl(tie_run, at, 64) - (hit != 0 ? __shfl(ties, at, 64) : 0);
+    if (hit != 0) span = base + at;
+  }
+  row.spans(span, span + 1, lane, [&](int, int i0, const float(&v)[VEC]) {
+    u64 w[VEC], sum = 0;
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) ties += by_ties && v[e] == border ? 1 : 0;
+    u64 r = rank + wave_inclusive(ties, lane) - ties;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const bool tie = by_ties && v[e] == border;
+      const bool in = v[e] > border || (tie && r < keep) || (!by_ties && v[e] == border && v[e] > -INFINITY);
+      r += tie ? 1 : 0;
+      w[e] = in ? kept(v[e]) : 0;
+      sum += w[e];
+    }
+    u64 run = before + wave_inclusive(sum, lane) - sum;
+    const u64 hit = __ballot(run + sum > target);
+    if (hit == 0 || lane != __builtin_ctzll(hit)) return;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (run <= target && run + w[e] > target) p.tokens[b] = i0 + e;
+      run += w[e];
+    }
+  });
 }
 
 }  // namespace
@@ -280,7 +628,7 @@ extern "C" int cdx_sample_tokens(const void* logits, int32_t logits_fp32, int64_
   p.logits = logits;
   p.ld = ld;
   p.V = (int32_t)V;
-  p.shift = 62 - bits;
+  p.shift = 62 - bits < 51 ? 62 - bits : 51;
   p.uniforms = uniforms;
   p.temperature = temperature;
   p.top_k = top_k;

@@ -178,15 +178,19 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u == 0x80000000u ? 0x80000000u : (u & 0x80000000u ? ~u : u | 0x80000000u);
 }
 
+__device__ __forceinline__ int wave_inclusive(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(v, d, 64);
+    if (lane >= d) v += up;
+  }
+  return v;
+}
+
 // Exclusive sum over the block of a count per thread, and the block's total.
 __device__ __forceinline__ int block_exclusive(int v, int* lds, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(x, d, 64);
-    if (lane >= d) x += up;
-  }
+  const int x = wave_inclusive(v, lane);
   __syncthreads();
   if (lane == 63) lds[wave] = x;
   __syncthreads();
@@ -200,6 +204,8 @@ __device__ __forceinline__ int block_exclusive(int v, int* lds, int& total) {
   return before + x - v;
 }
 
+// PER: slots that a thread holds in registers (capacity <= 512 PER), or 0: every pass reads them.
+template <int PER>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const EvictParams p) {
   __shared__ int hist[256];
   __shared__ int sums[kSelectThreads / 64];
@@ -222,11 +228,40 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
     return;
   }
   const int64_t first_recent = (int64_t)p.positions[b] - p.recent + 1;
-  auto is_recent = [&](int i) { return (int64_t)sp[i] >= first_recent; };
+
+  uint32_t key[PER > 0 ? PER : 1];
+  uint32_t recent_bits = 0;
+  if constexpr (PER > 0) {
+    float wv[PER];
+    int32_t sv[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int i = u * kSelectThreads + tid;
+      wv[u] = i < len ? w[i] : 0.f;
+      sv[u] = i < len ? sp[i] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      key[u] = weight_key(wv[u]);
+      recent_bits |= (int64_t)sv[u] >= first_recent ? 1u << u : 0u;
+    }
+  }
+  // f(slot, key, recent) of every slot in use, the block's 512 threads on neighbouring ones.
+  auto each = [&](auto f) {
+    if constexpr (PER > 0) {
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const int i = u * kSelectThreads + tid;
+        if (i < len) f(i, key[u], (recent_bits >> u & 1) != 0);
+      }
+    } else {
+      for (int i = tid; i < len; i += kSelectThreads) f(i, weight_key(w[i]), (int64_t)sp[i] >= first_recent);
+    }
+  };
 
   // The recent tokens are kept before any other.
   int mine = 0, n_recent;
-  for (int i = tid; i < len; i += kSelectThreads) mine += is_recent(i) ? 1 : 0;
+  each([&](int, uint32_t, bool recent) { mine += recent ? 1 : 0; });
   block_exclusive(mine, sums, n_recent);
   const bool among_recent = n_recent > p.keep;  // (positions given twice: the tokens then rank by weight)
   int need = among_recent ? p.keep : p.keep - n_recent;
@@ -237,19 +272,25 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   while (shift > 0 && !all) {
     shift -= 8;
     __syncthreads();
-    for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
+    if (tid < 256) hist[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < len; i += kSelectThreads) {
-      const uint32_t key = weight_key(w[i]);
-      if (is_recent(i) == among_recent && (shift == 24 || key >> (shift + 8) == prefix))
-        atomicAdd(&hist[(key >> shift) & 255], 1);
-    }
+    each([&](int, uint32_t k, bool recent) {
+      const bool in = recent == among_recent && (shift == 24 || k >> (shift + 8) == prefix);
+      if (in) atomicAdd(&hist[(k >> shift) & 255], 1);
+    });
     __syncthreads();
-    if (tid == 0) {
-      int above = 0, d = 255;
-      while (d > 0 && above + hist[d] < need) above += hist[d--];
-      pick[0] = d;
-      pick[1] = above;
+    if (tid < 64) {
+      // The digit from above at which the counts reach `need`: four to a lane.
+      int n[4], lane_sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lane_sum += n[i] = hist[255 - 4 * tid - i];
+      int above = wave_inclusive(lane_sum, tid) - lane_sum;
+      if (above < need && above + lane_sum >= need) {  // (one lane)
+        int i = 0;
+        while (i < 3 && above + n[i] < need) above += n[i++];
+        pick[0] = 255 - 4 * tid - i;
+        pick[1] = above;
+      }
     }
     __syncthreads();
     prefix = prefix << 8 | (uint32_t)pick[0];
@@ -262,69 +303,86 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   int32_t* holes = p.moves + row * 2 * p.max_moves;
   int32_t* movers = holes + p.max_moves;
   int ties = 0, n_holes = 0, n_movers = 0;
-  for (int base = 0; base < len; base += kSelectThreads) {
-    const int i = base + tid;
+  auto order = [&](int i, uint32_t k, bool recent) {
     bool kept = false, tie = false;
     if (i < len) {
-      const bool rec = is_recent(i);
-      if (rec != among_recent) {
-        kept = rec;
-      } else if (!none) {
-        const uint32_t key = shift == 32 ? 0u : weight_key(w[i]) >> shift;
-        kept = key > prefix;
-        tie = key == prefix;
-      }
+      kept = recent != among_recent ? recent : !none && k >> (shift & 31) > prefix;
+      tie = recent == among_recent && !none && k >> (shift & 31) == prefix;
     }
-    int total;
-    const int before = block_exclusive(tie ? 1 : 0, sums, total);
-    if (tie && ties + before < need) kept = true;
-    ties += total;
+    int total, before = 0;
+    if (!all) {  // (else every tie is kept)
+      before = block_exclusive(tie ? 1 : 0, sums, total);
+      tie = tie && ties + before < need;
+      ties += total;
+    }
+    kept = kept || tie;
     const bool hole = i < len && i < p.keep && !kept, mover = i >= p.keep && kept;
-    const int hb = block_exclusive(hole ? 1 : 0, sums, total);
-    if (hole) holes[n_holes + hb] = i;
-    n_holes += total;
-    const int mb = block_exclusive(mover ? 1 : 0, sums, total);
-    if (mover) movers[n_movers + mb] = i;
-    n_movers += total;
+    // (Both counts in one word: at most 512 of each.)
+    const int both = block_exclusive((hole ? 1 : 0) | (mover ? 1 << 16 : 0), sums, total);
+    if (hole) holes[n_holes + (both & 0xffff)] = i;
+    if (mover) movers[n_movers + (both >> 16)] = i;
+    n_holes += total & 0xffff;
+    n_movers += total >> 16;
+    if (i < p.cap && !hole) {
+      nw[i] = i < p.keep ? w[i] : 0.f;
+      np[i] = i < p.keep ? sp[i] : -1;
+    }
+  };
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+      if (u * kSelectThreads < p.cap) order(u * kSelectThreads + tid, key[u], (recent_bits >> u & 1) != 0);
+  } else {
+    for (int base = 0; base < p.cap; base += kSelectThreads) {
+      const int i = base + tid;
+      order(i, i < len ? weight_key(w[i]) : 0u, i < len && (int64_t)sp[i] >= first_recent);
+    }
   }
   __syncthreads();  // the lists are whole, and this block's own stores are seen by all of it
   if (tid == 0) p.count[row] = n_holes;
-  // (n_holes == n_movers: keep slots are kept, keep lie below `keep`.)
-  for (int i = tid; i < p.cap; i += kSelectThreads) {
-    nw[i] = i < p.keep ? w[i] : 0.f;
-    np[i] = i < p.keep ? sp[i] : -1;
-  }
-  __syncthreads();
+  // (n_holes == n_movers: keep slots are kept, and every hole below `keep` stands for one at or above it.)
   for (int i = tid; i < n_holes; i += kSelectThreads) {
     nw[holes[i]] = w[movers[i]];
     np[holes[i]] = sp[movers[i]];
   }
 }
 
-constexpr int kMovePieces = 4;
+constexpr int kMoves = 4;                 // rows that a group of 16 lanes moves, of K and of V
+constexpr int kMoveBlock = 16 * kMoves;   // and a block
 
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictParams p, uint32_t blocks) {
   const int64_t row = blockIdx.x / blocks;
-  const int cpr = p.D / 8;
-  const int64_t n = (int64_t)p.count[row] * cpr;
-  const int64_t i0 = (int64_t)(blockIdx.x - (uint32_t)row * blocks) * (256 * kMovePieces) + threadIdx.x;
-  if (i0 >= n) return;
+  const int n = p.count[row], c = threadIdx.x & 15, cpr = p.D / 8;
+  const int m0 = (int)(blockIdx.x - (uint32_t)row * blocks) * kMoveBlock + (threadIdx.x >> 4);
+  if (m0 >= n || c >= cpr) return;
   const int h = (int)(row % p.nkv);
   const int64_t slab = row / p.nkv, b = slab % p.B, layer = slab / p.B;
   const int32_t* holes = p.moves + row * 2 * p.max_moves;
   const int32_t* movers = holes + p.max_moves;
-  uint4* k = reinterpret_cast<uint4*>(p.k_pages) + layer * p.layer_rows * cpr;
-  uint4* v = reinterpret_cast<uint4*>(p.v_pages) + layer * p.layer_rows * cpr;
+  typedef __attribute__((ext_vector_type(4))) unsigned int piece_t;
+  piece_t* k = reinterpret_cast<piece_t*>(p.k_pages) + layer * p.layer_rows * cpr;
+  piece_t* v = reinterpret_cast<piece_t*>(p.v_pages) + layer * p.layer_rows * cpr;
+  // Every piece is on its way before the first is stored (the moves are disjoint).
+  int64_t to[kMoves], from[kMoves];
+  piece_t x[kMoves], y[kMoves];
 #pragma unroll
-  for (int u = 0; u < kMovePieces; ++u) {
-    const int64_t i = i0 + u * 256;
-    if (i >= n) return;
-    const int32_t m = (int32_t)(i / cpr);
-    const int c = (int)(i - (int64_t)m * cpr);
-    const int64_t to = p.t.row(b, h, p.nkv, holes[m]), from = p.t.row(b, h, p.nkv, movers[m]);
-    if (to < 0 || from < 0) continue;
-    k[to * cpr + c] = k[from * cpr + c];
-    v[to * cpr + c] = v[from * cpr + c];
+  for (int u = 0; u < kMoves; ++u) {
+    const int m = min(m0 + 16 * u, n - 1);
+    to[u] = p.t.row(b, h, p.nkv, holes[m]);
+    from[u] = p.t.row(b, h, p.nkv, movers[m]);
+  }
+#pragma unroll
+  for (int u = 0; u < kMoves; ++u) {
+    if (from[u] < 0 || m0 + 16 * u >= n) to[u] = -1;
+    const int64_t at = max(from[u], (int64_t)0) * cpr + c;  // (row 0 of the pool stands in for a missing one)
+    x[u] = k[at];
+    y[u] = v[at];
+  }
+#pragma unroll
+  for (int u = 0; u < kMoves; ++u) {
+    if (to[u] < 0) continue;
+    k[to[u] * cpr + c] = x[u];
+    v[to[u] * cpr + c] = y[u];
   }
 }
 
@@ -436,7 +494,7 @@ extern "C" int cdx_paged_evict(int64_t layers, int64_t B, int32_t nkv, int32_t h
                 (long long)recent);
   if (layers == 0 || B == 0 || width == 0 || num_pages == 0) return CDX_OK;
   const int64_t cap = width * page_size, rows = layers * B * nkv, moves = evict_max_moves(cap, keep);
-  const int64_t blocks = (moves * (hd / 8) + 256 * kMovePieces - 1) / (256 * kMovePieces);
+  const int64_t blocks = (moves + kMoveBlock - 1) / kMoveBlock;
   if (layers > 65535 || rows > INT32_MAX || (blocks > 0 && rows > INT32_MAX / blocks))
     return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
   if (!lengths || !positions || !table || !k_pages || !v_pages || !weights || !slot_positions || !new_lengths ||
@@ -470,7 +528,13 @@ extern "C" int cdx_paged_evict(int64_t layers, int64_t B, int32_t nkv, int32_t h
   p.k_pages = k_pages;
   p.v_pages = v_pages;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  evict_select_kernel<<<dim3((unsigned)rows), dim3(kSelectThreads), 0, s>>>(p);
+  const dim3 grid((unsigned)rows), block(kSelectThreads);
+  if (cap <= 4 * kSelectThreads)
+    evict_select_kernel<4><<<grid, block, 0, s>>>(p);
+  else if (cap <= 16 * kSelectThreads)
+    evict_select_kernel<16><<<grid, block, 0, s>>>(p);
+  else
+    evict_select_kernel<0><<<grid, block, 0, s>>>(p);
   if (int rc = check_launch(name)) return rc;
   if (blocks == 0) return CDX_OK;
   evict_move_kernel<<<dim3((unsigned)(rows * blocks)), dim3(256), 0, s>>>(p, (uint32_t)blocks);

@@ -254,65 +254,106 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
 
 constexpr int kJoinThreads = 256;
 constexpr int kJoinSlots = 1024;  // slots of the weights that a block adds up
+constexpr int kMaxSplits = 256;
 
-// Blocks [0, B * nkv * chunks): chunk 0 joins the splits of one (sequence, KV head); with
-// weights every chunk adds the softmax weights of its slots, over the heads of the group.
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttnParams p, int chunks) {
-  const int chunk = blockIdx.x % chunks;
-  const uint32_t slab = blockIdx.x / chunks;
-  const int b = slab / p.nkv, h = slab - b * p.nkv;
-  const int32_t cap = p.t.capacity(), len = min(p.lengths[b], cap);
-  const int64_t row0 = (int64_t)b * p.nq + h * p.group, step = (int64_t)p.B * p.nq;
-  auto statistics = [&](int64_t row, float& M, float& L) {
-    M = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[s * step + row].x);
-    const float ref = M == -INFINITY ? 0.f : M;
-    L = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float2 ml = p.part_ml[s * step + row];
-      L = __builtin_fmaf(__builtin_amdgcn_exp2f(ml.x - ref), ml.y, L);
-    }
-    M = ref;
-  };
-  if (chunk == 0 && p.splits > 1) {
-    for (int i = threadIdx.x; i < p.group * (p.D / 4); i += kJoinThreads) {
-      const int hd = i / (p.D / 4), d = (i - hd * (p.D / 4)) * 4;
-      float M, L, o[4] = {0.f, 0.f, 0.f, 0.f};
-      statistics(row0 + hd, M, L);
-      for (int s = 0; s < p.splits; ++s) {
-        const int64_t at = s * step + row0 + hd;
-        const float f = __builtin_amdgcn_exp2f(p.part_ml[at].x - M);
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * p.D + d);
-        o[0] = __builtin_fmaf(f, x.x, o[0]), o[1] = __builtin_fmaf(f, x.y, o[1]);
-        o[2] = __builtin_fmaf(f, x.z, o[2]), o[3] = __builtin_fmaf(f, x.w, o[3]);
-      }
-      const float inv = len > 0 ? 1.f / L : 0.f;
+// Maximum (log2 units, 0 where there is none) and sum of a row of scores from its splits' own, by
+// a whole wave, returned to every lane.
+__device__ __forceinline__ float2 join_statistics(const PagedAttnParams& p, int64_t row, int lane) {
+  const int64_t step = (int64_t)p.B * p.nq;
+  float2 ml[kMaxSplits / 64];
+  float M = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= inv;
-      head_store4(p.out + (row0 + hd) * p.D + d, o);
-    }
+  for (int i = 0; i < kMaxSplits / 64; ++i) {
+    const int s = i * 64 + lane;
+    ml[i] = s < p.splits ? p.part_ml[s * step + row] : make_float2(-INFINITY, 0.f);
   }
-  if (p.scores == nullptr) return;
-  const int32_t s0 = chunk * kJoinSlots;
-  float w[kJoinSlots / kJoinThreads];
 #pragma unroll
-  for (int u = 0; u < kJoinSlots / kJoinThreads; ++u) {
-    const int32_t s = s0 + u * kJoinThreads + threadIdx.x;
+  for (int i = 0; i < kMaxSplits / 64; ++i) M = fmaxf(M, ml[i].x);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  const float ref = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 64; ++i) L = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[i].x - ref), ml[i].y, L);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) L += __shfl_xor(L, d, 64);
+  return make_float2(ref, L);
+}
+
+// The first `rows` blocks (none without splits) join the splits of one row each, 256 threads over
+// splits and columns.  The others add up the softmax weights of 1024 slots of one (sequence,
+// KV head), over the heads of its group.
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttnParams p, uint32_t rows, int chunks) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t step = (int64_t)p.B * p.nq;
+  const int32_t cap = p.t.capacity();
+  if (blockIdx.x < rows) {
+    __shared__ float4 part[kJoinThreads];
+    const int64_t row = blockIdx.x;
+    const int cols = p.D / 4, groups = min(kJoinThreads / cols, 16);
+    const int sg = tid / cols, d = (tid - sg * cols) * 4;
+    const float2 ml = join_statistics(p, row, lane);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (sg < groups) {
+#pragma unroll 4
+      for (int s = sg; s < p.splits; s += groups) {
+        const int64_t at = s * step + row;
+        const float f = __builtin_amdgcn_exp2f(p.part_ml[at].x - ml.x);
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * p.D + d);
+        o.x = __builtin_fmaf(f, x.x, o.x), o.y = __builtin_fmaf(f, x.y, o.y);
+        o.z = __builtin_fmaf(f, x.z, o.z), o.w = __builtin_fmaf(f, x.w, o.w);
+      }
+    }
+    part[tid] = o;
+    __syncthreads();
+    if (tid >= cols) return;
+    for (int g = 1; g < groups; ++g) {
+      const float4 x = part[g * cols + tid];
+      o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+    }
+    const float inv = p.lengths[row / p.nq] > 0 ? 1.f / ml.y : 0.f;
+    const float f[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    head_store4(p.out + row * p.D + d, f);
+    return;
+  }
+  constexpr int PER = kJoinSlots / kJoinThreads;
+  __shared__ float2 stats[kHeads];
+  const uint32_t block = blockIdx.x - rows, slab = block / chunks;
+  const int32_t s0 = (int32_t)(block - slab * chunks) * kJoinSlots + tid;
+  const int b = slab / p.nkv, h = slab - b * p.nkv;
+  const int32_t len = min(p.lengths[b], cap);
+  float w[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int32_t s = s0 + u * kJoinThreads;
     w[u] = s < cap ? p.w_in[(int64_t)slab * cap + s] : 0.f;
   }
-  for (int hd = 0; hd < p.group && s0 < len; ++hd) {
-    float M, L;
-    statistics(row0 + hd, M, L);
-    const float inv = 1.f / L;
+  if (s0 - tid < len) {
+    for (int h0 = 0; h0 < p.group; h0 += kHeads) {
+      const int heads = min(kHeads, p.group - h0);
+      const int64_t row0 = (int64_t)b * p.nq + h * p.group + h0;
+      __syncthreads();
+      for (int i = wave; i < heads; i += kJoinThreads / 64) {
+        const float2 ml = join_statistics(p, row0 + i, lane);
+        if (lane == 0) stats[i] = make_float2(ml.x, 1.f / ml.y);
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int i = 0; i < heads; ++i) {
 #pragma unroll
-    for (int u = 0; u < kJoinSlots / kJoinThreads; ++u) {
-      const int32_t s = s0 + u * kJoinThreads + threadIdx.x;
-      if (s < len) w[u] = __builtin_fmaf(__builtin_amdgcn_exp2f(p.scores[(row0 + hd) * cap + s] - M), inv, w[u]);
+        for (int u = 0; u < PER; ++u) {
+          const int32_t s = s0 + u * kJoinThreads;
+          if (s < len) {
+            const float e = __builtin_amdgcn_exp2f(p.scores[(row0 + i) * cap + s] - stats[i].x);
+            w[u] = __builtin_fmaf(e, stats[i].y, w[u]);
+          }
+        }
+      }
     }
   }
 #pragma unroll
-  for (int u = 0; u < kJoinSlots / kJoinThreads; ++u) {
-    const int32_t s = s0 + u * kJoinThreads + threadIdx.x;
+  for (int u = 0; u < PER; ++u) {
+    const int32_t s = s0 + u * kJoinThreads;
     if (s < cap) p.w_out[(int64_t)slab * cap + s] = w[u];
   }
 }
@@ -322,7 +363,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAtt
 int paged_splits(int64_t blocks, int64_t cap) {
   const int64_t want = (4 * (int64_t)device_cu_count() + blocks - 1) / blocks;
   const int64_t most = (cap + 2 * kWaves * kTile - 1) / (2 * kWaves * kTile);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 256}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
@@ -368,9 +409,9 @@ extern "C" int cdx_paged_attention_fwd(const uint16_t* q, int64_t B, int32_t nq,
   if (B == 0) return CDX_OK;
   const int64_t cap = width * page_size, group = nq / nkv, head_tiles = (group + kHeads - 1) / kHeads;
   const int64_t blocks = B * nkv * head_tiles;
-  const int64_t chunks = weights_in ? (cap + kJoinSlots - 1) / kJoinSlots : 1;
+  const int64_t chunks = weights_in ? (cap + kJoinSlots - 1) / kJoinSlots : 0;
   const int splits = paged_splits(blocks, cap);
-  if (B * nq > INT32_MAX / 1024 || blocks * splits > INT32_MAX || B * nkv * chunks > INT32_MAX)
+  if (B * nq > INT32_MAX / 1024 || blocks * splits > INT32_MAX || B * (nkv * chunks + nq) > INT32_MAX)
     return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
   if (!q || !k_pages || !v_pages || !table || !lengths || !out) return fail(CDX_EINVAL, "%s: null pointer", name);
   const PagedWork ws = paged_work(B, nq, hd, cap, splits, weights_in != nullptr);
@@ -409,6 +450,8 @@ extern "C" int cdx_paged_attention_fwd(const uint16_t* q, int64_t B, int32_t nq,
     paged_attn_kernel<4, 8><<<grid, block, 0, s>>>(p);
   if (int rc = check_launch(name)) return rc;
   if (splits == 1 && !weights_in) return CDX_OK;
-  paged_join_kernel<<<dim3((unsigned)(B * nkv * chunks)), dim3(kJoinThreads), 0, s>>>(p, (int)chunks);
+  const int64_t rows = splits > 1 ? B * nq : 0;
+  paged_join_kernel<<<dim3((unsigned)(rows + B * nkv * chunks)), dim3(kJoinThreads), 0, s>>>(
+      p, (uint32_t)rows, (int)std::max<int64_t>(chunks, 1));
   return check_launch(name);
 }

@@ -76,6 +76,12 @@ def paged_qkv_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     ``positions`` [B] of the fp32 table ``cos_sin`` [n_pos, D/2, 2] (RotaryEmbedding.cos_sin_table; a
     position outside it gives NaN).  k and v go to slot ``lengths - 1``: the lengths count the
     new token already.  Replaces the torch.cat and the norms of core/attention.py:138-161."""
+    fast = nat.host()
+    if fast is not None:
+        q = fast.paged_append(qkv, k_pages, v_pages, block_table, lengths, positions, num_heads, cos_sin, q_norm_w,
+                              k_norm_w, eps)
+        if q is not None:
+            return q
     what = "paged_qkv_append"
     forward_only(what, qkv, k_pages, v_pages, q_norm_w, k_norm_w)
     nat.require_device(k_pages, v_pages, q_norm_w, k_norm_w, what=what)
@@ -107,8 +113,8 @@ def paged_qkv_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
         nat.check(nat.lib().cdx_paged_append_fwd(
             qkv.data_ptr(), qkv.dtype == torch.float32, ld, B, num_heads, nkv, D, nat.ptr(q_norm_w), nat.ptr(k_norm_w),
             float(eps), cos_sin.data_ptr(), cos_sin.shape[0], lengths.data_ptr(), positions.data_ptr(),
-            table.data_ptr(), _ld(table), table.shape[1], pages, page, k_pages.data_ptr(), v_pages.data_ptr(), q.data_ptr(),
-            nat.stream_of(qkv)), "cdx_paged_append_fwd")
+            table.data_ptr(), _ld(table), table.shape[1], pages, page, k_pages.data_ptr(), v_pages.data_ptr(),
+            q.data_ptr(), nat.stream_of(qkv)), "cdx_paged_append_fwd")
     return q
 
 
@@ -116,6 +122,9 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
                 block_table: torch.Tensor, lengths: torch.Tensor) -> None:
     """Prompts' k and v [B, nkv, S, D] (normalised and rotated: mu_qkv_rope's, qkv_cache's) into the
     pages: rows t < lengths[b] (all S of them at most) to slot t."""
+    fast = nat.host()
+    if fast is not None and fast.paged_write(k, v, k_pages, v_pages, block_table, lengths):
+        return
     what = "paged_write"
     forward_only(what, k, v, k_pages, v_pages)
     nat.require_device(k, v, k_pages, v_pages, what=what)
@@ -143,6 +152,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     With ``weights`` [B, nkv, capacity] fp32, returns (out, weights + what each slot received,
     summed over the query heads of its group); ``weights_out`` may name the result's memory,
     ``weights`` itself among others."""
+    if scale is None:
+        scale = max(1, k_pages.shape[-1]) ** -0.5
+    fast = nat.host()
+    if fast is not None:
+        done = fast.paged_attention(q, k_pages, v_pages, block_table, lengths, scale, weights, weights_out)
+        if done is not None:
+            return done if weights is not None else done[0]
     what = "paged_attention"
     forward_only(what, q, k_pages, v_pages, weights)
     nat.require_device(q, k_pages, v_pages, what=what)
@@ -175,7 +191,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     with nat.on_device(q), nat.launch_region("paged_attention", q.device, B=B, nq=nq, nkv=nkv, D=D):
         nat.check(lib.cdx_paged_attention_fwd(
             q.data_ptr(), B, nq, nkv, D, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), _ld(table),
-            table.shape[1], pages, page, lengths.data_ptr(), float(D ** -0.5 if scale is None else scale),
+            table.shape[1], pages, page, lengths.data_ptr(), float(scale),
             out.data_ptr(), nat.ptr(weights), nat.ptr(weights_out), nat.ptr(work), ws, nat.stream_of(q)),
             "cdx_paged_attention_fwd")
     return out if weights is None else (out, weights_out)
@@ -193,6 +209,11 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     tokens.  Kept rows from slot ``keep`` on move into the evicted slots below it, in the pages;
     returns the new (lengths, weights, slot_positions), with 0 and -1 past the lengths.  The pages
     of a sequence that is cut must not be another's too."""
+    fast = nat.host()
+    if fast is not None and type(keep) is int and type(recent) is int:
+        new = fast.paged_evict(k_pages, v_pages, block_table, lengths, positions, weights, slot_positions, keep, recent)
+        if new is not None:
+            return new
     what = "paged_evict"
     forward_only(what, k_pages, v_pages, weights)
     nat.require_device(k_pages, v_pages, what=what)

@@ -51,6 +51,11 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     others).  temperature 0 takes the first maximum; top_k 0, top_p 1 and min_p 0 cut nothing.  In
     a tensor, a temperature or top_k below 0 counts as 0, top_p outside [0, 1] as the nearer end,
     min_p above 1 as 1.  A NaN logit counts as -inf; a row of -inf alone gives -1."""
+    fast = nat.host()
+    if fast is not None:
+        tokens = fast.sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p)
+        if tokens is not None:
+            return tokens
     what = "sample_tokens"
     nat.require_device(logits, uniforms, dtype=None, what=what)
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):

@@ -15,6 +15,7 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -453,6 +454,180 @@ std::optional<std::tuple<Tensor, Tensor, OptTensor>> block_step(
   return std::make_tuple(k, v, mu_out);
 }
 
+// ---- paged generation -------------------------------------------------------
+
+// A paged cache's tensors as the C-ABI takes them.  dims 5: with a leading layer dimension.
+struct Pages {
+  int64_t layers = 1, pages = 0, nkv = 0, page = 0, D = 0, B = 0, width = 0, ld = 0;
+  uint16_t *k = nullptr, *v = nullptr;
+  const int32_t* table = nullptr;
+  int64_t capacity() const { return width * page; }
+};
+
+inline bool no_grad(const Tensor& t) { return !(at::GradMode::is_enabled() && t.requires_grad()); }
+
+bool paged_cache(const Tensor& k, const Tensor& v, const Tensor& table, int64_t dims, Pages* c) {
+  if (!dense(k) || !dense(v) || !no_grad(k) || !no_grad(v) || k.dim() != dims || v.sizes() != k.sizes() ||
+      k.numel() == 0 || !plain(table, at::kInt) || table.dim() != 2 || table.size(0) == 0 || table.size(1) == 0 ||
+      table.stride(1) != 1)
+    return false;
+  c->layers = dims == 5 ? k.size(0) : 1;
+  c->pages = k.size(-4);
+  c->nkv = k.size(-3);
+  c->page = k.size(-2);
+  c->D = k.size(-1);
+  c->B = table.size(0);
+  c->width = table.size(1);
+  c->ld = c->B > 1 ? table.stride(0) : c->width;
+  c->k = w16(k);
+  c->v = w16(v);
+  c->table = table.data_ptr<int32_t>();
+  const bool page_ok = c->page >= 16 && c->page <= 256 && (c->page & (c->page - 1)) == 0;
+  return page_ok && c->ld >= c->width && c->D % 8 == 0 && c->D <= 128 && c->nkv <= 65535;
+}
+
+// A plain contiguous int32 tensor with one value per sequence.
+inline bool per_sequence(const Tensor& t, int64_t B) {
+  return plain(t, at::kInt) && t.is_contiguous() && t.dim() == 1 && t.size(0) == B;
+}
+
+OptTensor paged_append(const Tensor& qkv, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths,
+                       const Tensor& positions, int64_t nq, const Tensor& cos_sin, const OptTensor& qn,
+                       const OptTensor& kn, double eps) {
+  Pages c;
+  const bool fp32 = qkv.defined() && qkv.scalar_type() == at::kFloat;
+  if (!paged_cache(k, v, table, 4, &c) || !dense(qkv, fp32 ? at::kFloat : at::kBFloat16) || !no_grad(qkv) ||
+      !per_sequence(lengths, c.B) || !per_sequence(positions, c.B) || nq <= 0 || nq > 65535 || nq % c.nkv != 0 ||
+      qkv.dim() != 2 || qkv.size(0) != c.B || qkv.size(1) != (nq + 2 * c.nkv) * c.D || !dense(cos_sin, at::kFloat) ||
+      cos_sin.dim() != 3 || cos_sin.size(0) == 0 || cos_sin.size(1) != c.D / 2 || cos_sin.size(2) != 2 ||
+      qn.has_value() != kn.has_value() || !(eps >= 0))
+    return {};
+  if (qn && (!dense(*qn) || !dense(*kn) || qn->numel() != c.D || kn->numel() != c.D || !no_grad(*qn) || !no_grad(*kn)))
+    return {};
+  Tensor q = like(k, {c.B, nq, c.D});
+  check(cdx_paged_append_fwd(qkv.data_ptr(), fp32, qkv.size(1), c.B, (int32_t)nq, (int32_t)c.nkv, (int32_t)c.D,
+                             u16(qn), u16(kn), (float)eps, cos_sin.data_ptr<float>(), cos_sin.size(0),
+                             lengths.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), c.table, c.ld, c.width,
+                             c.pages, (int32_t)c.page, c.k, c.v, w16(q), stream()),
+        "cdx_paged_append_fwd");
+  return q;
+}
+
+bool paged_write(const Tensor& k_new, const Tensor& v_new, const Tensor& k, const Tensor& v, const Tensor& table,
+                 const Tensor& lengths) {
+  Pages c;
+  if (!paged_cache(k, v, table, 4, &c) || !dense(k_new) || !dense(v_new) || !no_grad(k_new) || !no_grad(v_new) ||
+      k_new.dim() != 4 || k_new.sizes() != v_new.sizes() || k_new.size(0) != c.B || k_new.size(1) != c.nkv ||
+      k_new.size(3) != c.D || k_new.size(2) == 0 || !per_sequence(lengths, c.B))
+    return false;
+  check(cdx_paged_write(u16(k_new), u16(v_new), c.B, (int32_t)c.nkv, k_new.size(2), (int32_t)c.D,
+                        lengths.data_ptr<int32_t>(), c.table, c.ld, c.width, c.pages, (int32_t)c.page, c.k, c.v,
+                        stream()),
+        "cdx_paged_write");
+  return true;
+}
+
+// (out, new weights or None)
+std::optional<std::tuple<Tensor, OptTensor>> paged_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                             const Tensor& table, const Tensor& lengths, double scale,
+                                                             const OptTensor& weights, const OptTensor& weights_out) {
+  Pages c;
+  if (!paged_cache(k, v, table, 4, &c) || !dense(q) || !no_grad(q) || q.dim() != 3 || q.size(0) != c.B ||
+      q.size(2) != c.D || q.size(1) == 0 || q.size(1) > 65535 || q.size(1) % c.nkv != 0 ||
+      !per_sequence(lengths, c.B) || (weights_out && !weights))
+    return {};
+  auto rows = [&](const Tensor& t) {
+    return plain(t, at::kFloat) && t.is_contiguous() && no_grad(t) && t.dim() == 3 && t.size(0) == c.B &&
+           t.size(1) == c.nkv && t.size(2) == c.capacity();
+  };
+  if ((weights && !rows(*weights)) || (weights_out && !rows(*weights_out))) return {};
+  const int64_t nq = q.size(1);
+  Tensor out = like(q, {c.B, nq * c.D});
+  OptTensor w_out = weights_out;
+  if (weights && !w_out) w_out = like(*weights, weights->sizes());
+  const size_t bytes = cdx_paged_attention_workspace_bytes(c.B, (int32_t)nq, (int32_t)c.nkv, (int32_t)c.D,
+                                                           c.capacity(), weights.has_value());
+  Tensor work;
+  if (bytes) work = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte).requires_grad(false));
+  check(cdx_paged_attention_fwd(u16(q), c.B, (int32_t)nq, (int32_t)c.nkv, (int32_t)c.D, c.k, c.v, c.table, c.ld,
+                                c.width, c.pages, (int32_t)c.page, lengths.data_ptr<int32_t>(), (float)scale, w16(out),
+                                weights ? weights->data_ptr<float>() : nullptr,
+                                w_out ? w_out->data_ptr<float>() : nullptr, bytes ? work.data_ptr() : nullptr, bytes,
+                                stream()),
+        "cdx_paged_attention_fwd");
+  return std::make_tuple(out, w_out);
+}
+
+// (lengths, weights, slot positions)
+std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(const Tensor& k, const Tensor& v, const Tensor& table,
+                                                              const Tensor& lengths, const Tensor& positions,
+                                                              const Tensor& weights, const Tensor& slot_positions,
+                                                              int64_t keep, int64_t recent) {
+  Pages c;
+  if (!k.defined() || !paged_cache(k, v, table, k.dim() == 5 ? 5 : 4, &c) || !per_sequence(lengths, c.B) ||
+      !per_sequence(positions, c.B) || keep <= 0 || recent < 0 || recent > keep)
+    return {};
+  std::vector<int64_t> shape{c.B, c.nkv, c.capacity()};
+  if (k.dim() == 5) shape.insert(shape.begin(), c.layers);
+  if (!plain(weights, at::kFloat) || !plain(slot_positions, at::kInt) || !weights.is_contiguous() ||
+      !slot_positions.is_contiguous() || !no_grad(weights) || weights.sizes() != at::IntArrayRef(shape) ||
+      slot_positions.sizes() != at::IntArrayRef(shape))
+    return {};
+  Tensor new_len = ints(lengths, {c.B}), new_w = like(weights, shape), new_pos = ints(slot_positions, shape);
+  const size_t bytes = cdx_paged_evict_workspace_bytes(c.layers, c.B, (int32_t)c.nkv, c.capacity(), keep);
+  Tensor work = at::empty({(int64_t)bytes}, k.options().dtype(at::kByte).requires_grad(false));
+  check(cdx_paged_evict(c.layers, c.B, (int32_t)c.nkv, (int32_t)c.D, lengths.data_ptr<int32_t>(),
+                        positions.data_ptr<int32_t>(), c.table, c.ld, c.width, c.pages, (int32_t)c.page, c.k, c.v,
+                        weights.data_ptr<float>(), slot_positions.data_ptr<int32_t>(), keep, recent,
+                        new_len.data_ptr<int32_t>(), new_w.data_ptr<float>(), new_pos.data_ptr<int32_t>(),
+                        work.data_ptr(), bytes, stream()),
+        "cdx_paged_evict");
+  return std::make_tuple(new_len, new_w, new_pos);
+}
+
+// A setting of sample_tokens: a number within 0 .. top, or one value per row.
+struct Setting {
+  const void* rows = nullptr;
+  double value = 0;
+  bool ok = false;
+};
+Setting setting(const py::object& o, at::ScalarType dtype, int64_t B, double top) {
+  Setting s;
+  if (THPVariable_Check(o.ptr())) {
+    const Tensor& t = THPVariable_Unpack(o.ptr());
+    s.ok = plain(t, dtype) && t.is_contiguous() && t.dim() == 1 && t.size(0) == B;
+    if (s.ok) s.rows = t.data_ptr();
+  } else if (PyFloat_Check(o.ptr()) || PyLong_Check(o.ptr())) {
+    s.value = PyFloat_AsDouble(o.ptr());
+    if (s.value == -1.0 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return s;
+    }
+    s.ok = s.value >= 0 && s.value <= top && (dtype != at::kInt || s.value == std::floor(s.value));
+  }
+  return s;
+}
+
+OptTensor sample_tokens(const Tensor& logits, const Tensor& uniforms, const py::object& temperature,
+                        const py::object& top_k, const py::object& top_p, const py::object& min_p) {
+  const bool fp32 = logits.defined() && logits.scalar_type() == at::kFloat;
+  if (!plain(logits, fp32 ? at::kFloat : at::kBFloat16) || logits.dim() != 2 || logits.numel() == 0 ||
+      !plain(uniforms, at::kFloat) || !uniforms.is_contiguous() || uniforms.dim() != 1)
+    return {};
+  const int64_t B = logits.size(0), V = logits.size(1), ld = B > 1 ? logits.stride(0) : V;
+  if (uniforms.size(0) != B || V > (1 << 20) || ld < V || (V > 1 && logits.stride(1) != 1)) return {};
+  const Setting t = setting(temperature, at::kFloat, B, 3e38), k = setting(top_k, at::kInt, B, 1e9);
+  const Setting p = setting(top_p, at::kFloat, B, 1.0), m = setting(min_p, at::kFloat, B, 1.0);
+  if (!t.ok || !k.ok || !p.ok || !m.ok) return {};
+  Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong).requires_grad(false));
+  check(cdx_sample_tokens(logits.data_ptr(), fp32, ld, B, V, uniforms.data_ptr<float>(),
+                          static_cast<const float*>(t.rows), (float)t.value, static_cast<const int32_t*>(k.rows),
+                          (int32_t)k.value, static_cast<const float*>(p.rows), (float)p.value,
+                          static_cast<const float*>(m.rows), (float)m.value, tokens.data_ptr<int64_t>(), stream()),
+        "cdx_sample_tokens");
+  return tokens;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -469,4 +644,9 @@ PYBIND11_MODULE(_host, m) {
   m.def("swiglu_cggr", &swiglu_cggr);
   m.def("attention", &attention);
   m.def("block_step", &block_step);
+  m.def("paged_append", &paged_append);
+  m.def("paged_write", &paged_write);
+  m.def("paged_attention", &paged_attention);
+  m.def("paged_evict", &paged_evict);
+  m.def("sample_tokens", &sample_tokens);
 }

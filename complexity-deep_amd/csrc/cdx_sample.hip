@@ -23,10 +23,14 @@
 //     2048 bins of x (of counts for top-k, of weights for top-p), whose border bin is then
 //     resolved by a radix descent over its few tokens; the draw sums the kept weights by span.
 //     Those passes are paced by the exponentials, about 20 instructions in 64 bits a token.
+#include <float.h>
+
 #include "cdx_common.h"
 
 namespace cdx {
 namespace {
+
+typedef unsigned long long u64;
 
 constexpr int kThreads = 1024;
 constexpr int kSampleWaves = kThreads / 64;
@@ -35,8 +39,6 @@ constexpr int kListWave = 256;                // tokens that a wave can list
 constexpr int kLane = kListWave / 64;
 constexpr int kList = kListWave * kSampleWaves;
 constexpr int kBins = 2048;
-
-typedef unsigned long long u64;
 
 struct SampleParams {
   const void* logits;  // [B] rows of V at stride ld
@@ -63,20 +65,32 @@ __device__ __forceinline__ float key_logit(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-  return v;
+// Sum over the lanes up to this one (DPP: no LDS round trips).  The last lane has the wave's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp(u64 v) {
+  return (u64)(uint32_t)dpp<CTRL, ROWS>((int)(v >> 32)) << 32 | (uint32_t)dpp<CTRL, ROWS>((int)v);
 }
 template <typename T>
-__device__ __forceinline__ T wave_inclusive(T v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T up = __shfl_up(v, d, 64);
-    if (lane >= d) v += up;
-  }
+__device__ __forceinline__ T wave_inclusive(T v) {
+  v += dpp<0x111, 0xf>(v);  // from 1, 2, 4 and 8 lanes below in the row of 16
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v);  // the row before's last lane, then the first half's
+  v += dpp<0x143, 0xc>(v);
   return v;
+}
+__device__ __forceinline__ int read_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ u64 read_lane(u64 v, int lane) {
+  return (u64)(uint32_t)read_lane((int)(v >> 32), lane) << 32 | (uint32_t)read_lane((int)v, lane);
+}
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+  return read_lane(wave_inclusive(v), 63);
 }
 
 // One row, in pieces of 16 bytes at 16-byte addresses: piece c holds tokens c * VEC - head ..
@@ -84,94 +98,106 @@ __device__ __forceinline__ T wave_inclusive(T v, int lane) {
 template <typename TIn>
 struct Row {
   static constexpr int VEC = 16 / sizeof(TIn);
+  typedef __attribute__((ext_vector_type(4))) unsigned int piece_t;
   const TIn* x;  // of token -head (not read before token 0)
   int V, head, pieces;
+  int lo, hi;  // the pieces that lie inside the row
 
   __device__ __forceinline__ Row(const TIn* row, int V_) : V(V_) {
     head = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(TIn));
     x = row - head;
     pieces = (head + V + VEC - 1) / VEC;
+    lo = head > 0 ? 1 : 0;
+    hi = (head + V) / VEC - 1;
   }
   static __device__ __forceinline__ float value(const float* p) { return *p; }
   static __device__ __forceinline__ float value(const uint16_t* p) { return bf16_bits_to_f32(*p); }
-  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
-    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
-  }
-  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) { unpack8(v, f); }
-  __device__ __forceinline__ bool whole(int c) const { return (c > 0 || head == 0) && (c + 1) * VEC - head <= V; }
-  __device__ __forceinline__ void load(int c, float (&f)[VEC]) const {
-    if (whole(c)) {
-      unpack(*reinterpret_cast<const uint4*>(x + (int64_t)c * VEC), f);
-      return;
-    }
+  static __device__ __forceinline__ void unpack(const piece_t& v, float (&f)[4]) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int i = c * VEC + e - head;
-      f[e] = i >= 0 && i < V ? value(x + c * VEC + e) : -INFINITY;
+    for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
+  }
+  static __device__ __forceinline__ void unpack(const piece_t& v, float (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[2 * e] = __uint_as_float(v[e] << 16);
+      f[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
     }
   }
-  // f(span, first token, values) over the spans s0 <= span < s1, four loads ahead.
+  // f(span, first token, values) over the spans s0 <= span < s1.  AHEAD loads are on their way
+  // together: a piece that does not lie inside the row loads one that does and is then taken
+  // token by token.
   template <typename F>
   __device__ __forceinline__ void spans(int s0, int s1, int lane, F f) const {
     constexpr int AHEAD = 4;
     for (int s = s0; s < s1; s += AHEAD) {
-      float v[AHEAD][VEC];
+      piece_t raw[AHEAD];
+      if (lo <= hi) {
 #pragma unroll
-      for (int a = 0; a < AHEAD; ++a) {
-        const int c = (s + a) * 64 + lane;
-        if (s + a < s1 && c < pieces) {
-          load(c, v[a]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) v[a][e] = -INFINITY;
+        for (int a = 0; a < AHEAD; ++a) {
+          const int c = max(lo, min(hi, (s + a) * 64 + lane));
+          raw[a] = *reinterpret_cast<const piece_t*>(x + (int64_t)c * VEC);
         }
       }
 #pragma unroll
-      for (int a = 0; a < AHEAD; ++a)
-        if (s + a < s1) f(s + a, ((s + a) * 64 + lane) * VEC - head, v[a]);
+      for (int a = 0; a < AHEAD; ++a) {
+        if (s + a >= s1) break;
+        const int c = (s + a) * 64 + lane;
+        float v[VEC];
+        unpack(raw[a], v);
+        if (c < lo || c > hi) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const int i = c * VEC + e - head;
+            v[e] = i >= 0 && i < V ? value(x + c * VEC + e) : -INFINITY;
+          }
+        }
+        f(s + a, c * VEC - head, v);
+      }
     }
   }
 };
 
-// exp((x - top) / T) and its integer.
+// exp((x - top) / T) and its integer, in about 20 instructions.
 struct Weights {
-  double top, per_t, unit;  // unit: 2^shift
+  double top, per_t, unit;  // per_t: log2(e) / T; unit: 2^shift
 
-  // 2^t for t <= 0 as p 2^n, 2^-0.5 <= p <= 2^0.5: the series of 2^r = exp(r ln 2) to r^11, whose
-  // remainder is below 0.35^12 / 12! = 7e-15.
-  static __device__ __forceinline__ double mantissa(double t, int& n) {
-    const double k = __builtin_rint(t), r = t - k;
-    n = (int)k;
-    double p = 4.44553827187081e-10;               // ln2^11 / 11!
-    p = __builtin_fma(p, r, 7.054911620801121e-09);  // ln2^10 / 10!
-    p = __builtin_fma(p, r, 1.0178086009239699e-07);
-    p = __builtin_fma(p, r, 1.3215486790144309e-06);
-    p = __builtin_fma(p, r, 1.5252733804059841e-05);
-    p = __builtin_fma(p, r, 0.0001540353039338161);
-    p = __builtin_fma(p, r, 0.0013333558146428441);
-    p = __builtin_fma(p, r, 0.009618129107628477);
-    p = __builtin_fma(p, r, 0.055504108664821576);
-    p = __builtin_fma(p, r, 0.24022650695910072);
-    p = __builtin_fma(p, r, 0.6931471805599453);
-    return __builtin_fma(p, r, 1.0);
-  }
-  // (x - top) log2(e) / T, no lower than -256; a logit of -inf, and any other beside a top of
-  // +inf, is as low (also at a temperature without bounds).
-  __device__ __forceinline__ double exponent(float x) const {
-    const double t = ((double)x - top) * per_t;
-    return t >= -256.0 ? t : (x == top ? 0.0 : -256.0);
-  }
+  __device__ __forceinline__ Weights(float top_x, float T, int shift)
+      : top((double)fminf(top_x, FLT_MAX)), per_t(1.4426950408889634 / (double)T), unit((double)(1ull << shift)) {}
+
+  // 2^t = p 2^n, n the nearest integer to t (the low bits of t + 1.5 2^52), p = 1 + r q(r) with q
+  // the interpolation of (2^r - 1) / r at the nine Chebyshev nodes of |r| <= 1/2: 2^r to 3.7e-14 of it.
+  // A logit of -inf (whatever the temperature) and one far below the top weigh less than half a
+  // unit: the exponent stops at -100.  Beside a top of +inf only +inf itself is asked for.
   __device__ __forceinline__ double fraction(float x) const {
-    int n;
-    const double p = mantissa(exponent(x), n);
-    return __builtin_ldexp(p, n);
+    const double t = fmax(((double)fminf(x, FLT_MAX) - top) * per_t, -100.0);
+    const double k = t + 6755399441055744.0, r = t - (k - 6755399441055744.0);
+    double p = 1.0203121294744093e-07;
+    p = __builtin_fma(p, r, 1.3255224885642954e-06);
+    p = __builtin_fma(p, r, 1.5252686845242518e-05);
+    p = __builtin_fma(p, r, 0.00015403455852420133);
+    p = __builtin_fma(p, r, 0.0013333558179044413);
+    p = __builtin_fma(p, r, 0.009618129159402609);
+    p = __builtin_fma(p, r, 0.05550410866476042);
+    p = __builtin_fma(p, r, 0.2402265069581299);
+    p = __builtin_fma(p, r, 0.6931471805599453);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_bit_cast(double, __builtin_bit_cast(u64, p) + ((u64)(uint32_t)__builtin_bit_cast(u64, k) << 52));
   }
-  static __device__ __forceinline__ u64 round_units(double w) {
-    // w < 2^52: its integer is the low part of w + 2^52.
-    return __builtin_bit_cast(u64, w + 4503599627370496.0) & 0xfffffffffffffull;
+  // The bits of w 2^shift + 2^52 (below 2^53): kRaw and, in the low bits, the integer.  Sums of them
+  // wrap, and are right after as many kRaw are taken off.
+  static constexpr u64 kRaw = 0x4330000000000000ull;
+  __device__ __forceinline__ u64 raw(double w) const {
+    return __builtin_bit_cast(u64, __builtin_fma(w, unit, 4503599627370496.0));
   }
-  __device__ __forceinline__ u64 units(float x) const { return round_units(fraction(x) * unit); }
+  __device__ __forceinline__ u64 units(double w) const { return raw(w) - kRaw; }
+  __device__ __forceinline__ u64 units(float x) const { return units(fraction(x)); }
 };
+
+// Whether exp((x - top) / T) is above 0 at all in 64 bits, for the key of x (rare: u == 0).
+__device__ __forceinline__ bool any_weight(uint32_t key, float top, float T) {
+  const float x = key_logit(key);
+  return x > -INFINITY && top < INFINITY && exp(((double)x - (double)top) / (double)T) > 0.0;
+}
 
 struct Shared {
   u64 bins[kBins];
@@ -181,6 +207,7 @@ struct Shared {
   int list_index[kList];
   u64 red[kSampleWaves];
   u64 pick[3];
+  uint32_t range[2];
   int count[kSampleWaves];
   int total;
 };
@@ -206,7 +233,7 @@ __device__ __forceinline__ void pick_bin(Shared& sh, int n, u64 above, u64 limit
     const int d = lane * per + i;
     mine += sh.bins[descending ? n - 1 - d : d];
   }
-  u64 before = above + wave_inclusive(mine, lane) - mine;
+  u64 before = above + wave_inclusive(mine) - mine;
   int last = -1;
   u64 at = 0;
   for (int i = 0; i < per && before <= limit; ++i) {
@@ -296,18 +323,42 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     if (tid == 0) p.tokens[b] = first;
     return;
   }
-  const Weights wt{(double)top, 1.4426950408889634 / (double)T, (double)(1ull << p.shift)};
+  const Weights wt(top, T, p.shift);
   if (top_k >= p.V) top_k = 0;
   if (!(top_p < 1.f)) top_p = 1.f;
   if (top_p < 0.f) top_p = 0.f;
   const bool cut_p = top_p < 1.f;
 
-  // A logit below `bound` is not kept, whatever the others are.
-  float bound = -INFINITY;
+  // A logit below `bound` is not kept, whatever the others are.  (Beside +inf nothing else weighs.)
+  float bound = top == INFINITY ? INFINITY : -FLT_MAX;
   if (top_k > 0 && top_k <= min(row.pieces, kThreads)) {
-    // (A thread without tokens has -inf, which bounds nothing.)
-    u64 above = 0;
-    bound = key_logit(descend(sh, above, (u64)top_k - 1, [&](auto f) { f(logit_key(mine), 1); }));
+    // The high half of the k-th largest key among the threads' maxima, by the first wave, which
+    // halves the range between the least and the largest.  (A thread without tokens has -inf.)
+    sh.list_key[tid] = logit_key(mine) >> 16;
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t key[kThreads / 64], lo = ~0u, hi = logit_key(top) >> 16;
+#pragma unroll
+      for (int i = 0; i < kThreads / 64; ++i) {
+        key[i] = sh.list_key[i * 64 + lane];
+        lo = min(lo, key[i]);
+      }
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) lo = min(lo, (uint32_t)__shfl_xor((int)lo, d, 64));
+      while (lo < hi) {  // at least k keys reach lo, fewer hi + 1
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 64; ++i) n += key[i] >= mid ? 1 : 0;
+        if (wave_sum(n) >= top_k)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      if (lane == 0) sh.range[0] = lo << 16;
+    }
+    __syncthreads();
+    if (sh.range[0] > logit_key(-FLT_MAX)) bound = fmaxf(bound, key_logit(sh.range[0]));
   }
   if (min_p > 0.f && !cut_p) {
     // x >= top + T ln(min_p), less what the rounding of a weight (far below 1e-9 of it), and here of
@@ -315,37 +366,151 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     const double low = (double)top + (double)T * (log((double)(min_p < 1.f ? min_p : 1.f)) - 1e-9);
     bound = fmaxf(bound, (float)(low - 1e-6 * (fabs((double)top) + fabs(low))));
   }
-  const bool bounded = bound > -INFINITY || row.pieces * VEC <= kList;
+  const bool bounded = bound > -FLT_MAX || row.pieces * VEC <= kList;
 
   // The tokens that pass, in order, by wave; more than the list holds: count only.
   int listed = kListWave + 1;
   if (bounded) {
     listed = 0;
     row.spans(s0, s1, lane, [&](int, int i0, const float(&v)[VEC]) {
+      float most = v[0];
+#pragma unroll
+      for (int e = 1; e < VEC; ++e) most = fmaxf(most, v[e]);
+      if (__ballot(most >= bound) == 0) return;
       int n = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) n += v[e] >= bound && v[e] > -INFINITY ? 1 : 0;
-      if (__ballot(n > 0) == 0) return;
-      const int incl = wave_inclusive(n, lane);
+      for (int e = 0; e < VEC; ++e) n += v[e] >= bound ? 1 : 0;
+      const int incl = wave_inclusive(n);
       int at = listed + incl - n;
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (v[e] >= bound && v[e] > -INFINITY) {
+        if (v[e] >= bound) {
           if (at < kListWave) {
             sh.list_key[wave * kListWave + at] = logit_key(v[e]);
             sh.list_index[wave * kListWave + at] = i0 + e;
           }
           ++at;
         }
-      listed += __builtin_amdgcn_readlane(incl, 63);
+      listed += read_lane(incl, 63);
     });
   }
   __syncthreads();
   if (lane == 0) sh.count[wave] = listed;
   __syncthreads();
   bool fits = true;
+  int listed_all = 0;
 #pragma unroll
-  for (int w = 0; w < kSampleWaves; ++w) fits = fits && sh.count[w] <= kListWave;
+  for (int w = 0; w < kSampleWaves; ++w) {
+    fits = fits && sh.count[w] <= kListWave;
+    listed_all += sh.count[w];
+  }
+
+  if (fits && listed_all <= kListWave) {
+    // Few tokens: all that follows by one wave, without barriers.
+    if (wave != 0) return;
+    constexpr int SHIFT = sizeof(TIn) == 2 ? 16 : 0;  // (the other bits of a bf16 logit's key follow from these)
+    uint32_t key[kLane];
+    int index[kLane];
+    u64 w[kLane];
+    double wf[kLane];
+    bool on[kLane];
+#pragma unroll
+    for (int r = 0; r < kLane; ++r) {
+      int i = r * 64 + lane, from = 0;
+      on[r] = i < listed_all;
+      for (int v = 0; v < kSampleWaves - 1; ++v) {
+        const bool past = from == v && i >= sh.count[v];
+        i -= past ? sh.count[v] : 0;
+        from += past ? 1 : 0;
+      }
+      const int at = on[r] ? from * kListWave + i : 0;
+      key[r] = on[r] ? sh.list_key[at] >> SHIFT : 0u;
+      index[r] = sh.list_index[at];
+      wf[r] = on[r] ? wt.fraction(key_logit(sh.list_key[at])) : 0.0;
+      w[r] = on[r] ? wt.units(wf[r]) : 0;
+    }
+    uint32_t least = ~0u;
+#pragma unroll
+    for (int r = 0; r < kLane; ++r) least = on[r] ? min(least, key[r]) : least;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
+    const uint32_t most = logit_key(top) >> SHIFT;
+    if (top_k > 0) {
+      // The smallest key that fewer than k keys exceed.
+      uint32_t lo = least, hi = most;
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        int n = 0;
+#pragma unroll
+        for (int r = 0; r < kLane; ++r) n += __popcll(__ballot(on[r] && key[r] > mid));
+        if (n < top_k)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      least = lo;
+#pragma unroll
+      for (int r = 0; r < kLane; ++r) on[r] = on[r] && key[r] >= lo;
+    }
+    if (cut_p) {
+      // The smallest key whose larger ones weigh no more than p of the sum; ties by index.
+      u64 s = 0;
+#pragma unroll
+      for (int r = 0; r < kLane; ++r) s += on[r] ? w[r] : 0;
+      const u64 limit = (u64)((double)top_p * (double)wave_sum(s));
+      uint32_t lo = least, hi = most;
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        u64 above = 0;
+#pragma unroll
+        for (int r = 0; r < kLane; ++r) above += on[r] && key[r] > mid ? w[r] : 0;
+        if (wave_sum(above) <= limit)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      u64 above = 0, each = 0;
+#pragma unroll
+      for (int r = 0; r < kLane; ++r) {
+        above += on[r] && key[r] > lo ? w[r] : 0;
+        const u64 tie = __ballot(on[r] && key[r] == lo);
+        if (tie != 0) each = read_lane(w[r], __builtin_ctzll(tie));
+      }
+      const u64 keep = each != 0 ? (limit - wave_sum(above)) / each + 1 : ~0ull;
+      u64 before = 0;
+#pragma unroll
+      for (int r = 0; r < kLane; ++r) {
+        const u64 tie = __ballot(on[r] && key[r] == lo);
+        on[r] = on[r] && (key[r] > lo || (key[r] == lo && before + __popcll(tie & ((1ull << lane) - 1)) < keep));
+        before += __popcll(tie);
+      }
+    }
+    u64 s = 0;
+#pragma unroll
+    for (int r = 0; r < kLane; ++r) {
+      const bool is_top = key[r] == most;
+      on[r] = on[r] && (!(min_p > 0.f) || is_top || wf[r] >= (double)min_p);
+      // u == 0: the first kept token of any weight, also of one that rounds to no unit.
+      if (!(u > 0.f)) w[r] = is_top || any_weight(key[r] << SHIFT, top, T) ? 1 : 0;
+      w[r] = on[r] ? w[r] : 0;
+      s += w[r];
+    }
+    const u64 total = wave_sum(s);
+    u64 target = u > 0.f ? (u64)((double)(u < 1.f ? u : 1.f) * (double)total) : 0;
+    if (target >= total) target = total - 1;
+    u64 before = 0;
+#pragma unroll
+    for (int r = 0; r < kLane; ++r) {
+      const u64 run = before + wave_inclusive(w[r]);
+      const u64 hit = __ballot(run > target);
+      if (hit != 0) {
+        if (lane == __builtin_ctzll(hit)) p.tokens[b] = index[r];
+        return;
+      }
+      before = read_lane(run, 63);
+    }
+    return;
+  }
 
   if (fits) {
     uint32_t key[kLane];
@@ -373,7 +538,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
 #pragma unroll
     for (int r = 0; r < kLane; ++r) {
       wf[r] = on[r] ? wt.fraction(key_logit(key[r])) : 0.0;
-      w[r] = on[r] ? Weights::round_units(wf[r] * wt.unit) : 0;
+      w[r] = on[r] ? wt.units(wf[r]) : 0;
     }
     if (cut_p) {
       u64 s = 0;
@@ -411,7 +576,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
       const bool is_top = key_logit(key[r]) == top;
       on[r] = on[r] && (!(min_p > 0.f) || is_top || wf[r] >= (double)min_p);
       // u == 0: the first kept token of any weight, also of one that rounds to no unit.
-      if (!(u > 0.f)) w[r] = on[r] && (is_top || exp(((double)key_logit(key[r]) - wt.top) / (double)T) > 0.0) ? 1 : 0;
+      if (!(u > 0.f)) w[r] = is_top || any_weight(key[r], top, T) ? 1 : 0;
       w[r] = on[r] ? w[r] : 0;
       s += w[r];
     }
@@ -423,13 +588,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     if (target < before || target >= before + sh.red[wave]) return;  // another wave's
 #pragma unroll
     for (int r = 0; r < kLane; ++r) {
-      const u64 run = before + wave_inclusive(w[r], lane);
+      const u64 run = before + wave_inclusive(w[r]);
       const u64 hit = __ballot(run > target);
       if (hit != 0) {
         if (lane == __builtin_ctzll(hit)) p.tokens[b] = index[r];
         return;
       }
-      before = __shfl(run, 63, 64);
+      before = read_lane(run, 63);
     }
     return;
   }
@@ -448,7 +613,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const u64 w = v[e] > -INFINITY ? weight(v[e]) : 0;
+        const u64 w = v[e] >= -FLT_MAX ? weight(v[e]) : 0;
         if (w != 0) atomicAdd(&sh.bins[bin(v[e])], w);
       }
     });
@@ -461,10 +626,32 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     __syncthreads();
     const int chosen = (int)sh.pick[0];
     above = sh.pick[1];
+    // The logits of that bin are an interval: its ends by halving the range of keys.
+    if (tid < 2) {
+      uint32_t lo = logit_key(-FLT_MAX), hi = logit_key(top);
+      while (lo < hi) {  // lane 0: the first key at or below the bin; lane 1: the last at or above it
+        const uint32_t mid = lo + (hi - lo + tid) / 2;
+        const int at = bin(key_logit(mid));
+        if (tid == 0) {
+          if (at <= chosen)
+            hi = mid;
+          else
+            lo = mid + 1;
+        } else {
+          if (at >= chosen)
+            lo = mid;
+          else
+            hi = mid - 1;
+        }
+      }
+      sh.range[tid] = lo;
+    }
+    __syncthreads();
+    const float from = key_logit(sh.range[0]), to = key_logit(sh.range[1]);
     row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (v[e] > -INFINITY && bin(v[e]) == chosen) {
+        if (v[e] >= from && v[e] <= to) {
           const int at = atomicAdd(&sh.total, 1);
           if (at < kList) sh.list_key[at] = logit_key(v[e]);
         }
@@ -481,7 +668,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
         row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
-            if (v[e] > -INFINITY && bin(v[e]) == chosen) {
+            if (v[e] >= from && v[e] <= to) {
               const u64 w = weight(v[e]);
               if (w != 0) f(logit_key(v[e]), w);
             }
@@ -496,7 +683,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     return key;
   };
 
-  float low = -INFINITY;
+  float low = top == INFINITY ? INFINITY : -FLT_MAX;  // the least logit that top-k keeps
   if (top_k > 0) {
     // Bins over four times the spread of the threads' maxima.
     float least = mine > -INFINITY ? mine : top;
@@ -509,8 +696,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     for (int w = 0; w < kSampleWaves; ++w) least = fminf(least, __uint_as_float((uint32_t)sh.red[w]));
     const float spread = top - least;
     const float per_x = spread > 0.f && spread < INFINITY ? (float)(kBins / 4) / spread : 0.f;
-    low = key_logit(border_of(per_x, 0, [&](u64 n) { return (u64)top_k - 1 < n ? (u64)top_k - 1 : n - 1; },
-                              [](float) -> u64 { return 1; }));
+    const float kth = key_logit(border_of(per_x, 0, [&](u64 n) { return (u64)top_k - 1 < n ? (u64)top_k - 1 : n - 1; },
+                                          [](float) -> u64 { return 1; }));
+    low = fmaxf(low, kth);
   }
   float border = low;
   u64 keep = ~0ull, tie_w = 0;
@@ -523,32 +711,50 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     keep = (sh.pick[2] - sh.pick[1]) / tie_w + 1;
   }
   // Kept weights by span, the ties at the border counted apart.
-  const bool any = !(u > 0.f);
+  const bool any = !(u > 0.f), by_ties = keep != ~0ull;
   auto kept = [&](float x) -> u64 {
     if (x == top) return any ? 1 : wt.units(x);
     const double w = wt.fraction(x);
     if (min_p > 0.f && !(w >= (double)min_p)) return 0;
-    if (any) return exp(((double)x - wt.top) / (double)T) > 0.0 ? 1 : 0;
-    return Weights::round_units(w * wt.unit);
+    return any ? (any_weight(logit_key(x), top, T) ? 1 : 0) : wt.units(w);
   };
-  const bool by_ties = keep != ~0ull;
+  // What is summed as it is: the logits above the border, or without ties from it on.
+  const float least = by_ties ? key_logit(logit_key(border) + 1) : border;
   tie_w = by_ties ? kept(border) : 0;
   __syncthreads();
-  row.spans(s0, s1, lane, [&](int s, int, const float(&v)[VEC]) {
-    u64 sum = 0;
-    int ties = 0;
+  if (any || min_p > 0.f) {
+    row.spans(s0, s1, lane, [&](int s, int, const float(&v)[VEC]) {
+      u64 sum = 0;
+      int ties = 0;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (v[e] > border || (!by_ties && v[e] == border && v[e] > -INFINITY)) sum += kept(v[e]);
-      ties += by_ties && v[e] == border ? 1 : 0;
-    }
-    sum = wave_sum(sum);
-    ties = wave_sum(ties);
-    if (lane == 0) {
-      sh.sums[s] = sum;
-      sh.ties[s] = ties;
-    }
-  });
+      for (int e = 0; e < VEC; ++e) {
+        if (v[e] >= least) sum += kept(v[e]);
+        ties += by_ties && v[e] == border ? 1 : 0;
+      }
+      sum = wave_sum(sum);
+      ties = wave_sum(ties);
+      if (lane == 0) {
+        sh.sums[s] = sum;
+        sh.ties[s] = ties;
+      }
+    });
+  } else {
+    row.spans(s0, s1, lane, [&](int s, int, const float(&v)[VEC]) {
+      u64 sum = 0;
+      int ties = 0;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        sum += wt.raw(wt.fraction(v[e] >= least ? v[e] : -INFINITY));
+        ties += v[e] == border ? 1 : 0;
+      }
+      sum = wave_sum(sum - VEC * Weights::kRaw);
+      ties = wave_sum(ties);
+      if (lane == 0) {
+        sh.sums[s] = sum;
+        sh.ties[s] = ties;
+      }
+    });
+  }
   __syncthreads();
   if (wave != 0) return;
   // By the first wave: the spans' sums with their kept ties, then the span that the draw falls in.
@@ -556,7 +762,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
   for (int base = 0; base < n_spans; base += 64) {
     const int s = base + lane;
     const u64 ties = by_ties && s < n_spans ? sh.ties[s] : 0;
-    const u64 tie_at = ties_before + wave_inclusive(ties, lane) - ties;
+    const u64 tie_at = ties_before + wave_inclusive(ties) - ties;
     const u64 mine_kept = tie_at >= keep ? 0 : (keep - tie_at < ties ? keep - tie_at : ties);
     const u64 sum = s < n_spans ? sh.sums[s] + mine_kept * tie_w : 0;
     if (s < n_spans) sh.sums[s] = sum;
@@ -570,12 +776,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
   for (int base = 0; base < n_spans && span < 0; base += 64) {
     const int s = base + lane;
     const u64 sum = s < n_spans ? sh.sums[s] : 0, ties = by_ties && s < n_spans ? sh.ties[s] : 0;
-    const u64 run = wave_inclusive(sum, lane), tie_run = wave_inclusive(ties, lane);
+    const u64 run = wave_inclusive(sum), tie_run = wave_inclusive(ties);
     const u64 hit = __ballot(before + run > target);
     const int at = hit != 0 ? __builtin_ctzll(hit) : 63;
     // (Up to the span, or past all 64.)
-    before += __shfl(run, at, 64) - (hit != 0 ? __shfl(sum, at, 64) : 0);
-    rank += __shfl(tie_run, at, 64) - (hit != 0 ? __shfl(ties, at, 64) : 0);
+    before += read_lane(run, at) - (hit != 0 ? read_lane(sum, at) : 0);
+    rank += read_lane(tie_run, at) - (hit != 0 ? read_lane(ties, at) : 0);
     if (hit != 0) span = base + at;
   }
   row.spans(span, span + 1, lane, [&](int, int i0, const float(&v)[VEC]) {
@@ -583,16 +789,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     int ties = 0;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) ties += by_ties && v[e] == border ? 1 : 0;
-    u64 r = rank + wave_inclusive(ties, lane) - ties;
+    u64 r = rank + wave_inclusive(ties) - ties;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       const bool tie = by_ties && v[e] == border;
-      const bool in = v[e] > border || (tie && r < keep) || (!by_ties && v[e] == border && v[e] > -INFINITY);
+      const bool in = v[e] >= least || (tie && r < keep);
       r += tie ? 1 : 0;
       w[e] = in ? kept(v[e]) : 0;
       sum += w[e];
     }
-    u64 run = before + wave_inclusive(sum, lane) - sum;
+    u64 run = before + wave_inclusive(sum) - sum;
     const u64 hit = __ballot(run + sum > target);
     if (hit == 0 || lane != __builtin_ctzll(hit)) return;
 #pragma unroll

@@ -10,7 +10,8 @@ sort_tokens_by_expert, sort_tokens_by_expert_fast, cggr_grouped_gemm (also as
 grouped_gemm_pytorch and persistent_cggr_gemm), persistent_swiglu_cggr,
 fused_swiglu_triton, fused_swiglu_simple, fused_mu_qkv_projection.  Beyond the
 reference: the operators of a paged generation, paged_qkv_append, paged_write,
-paged_attention, paged_evict and sample_tokens.
+paged_attention, paged_evict and sample_tokens, and PagedKVCache, which ties them to a
+model (ComplexityModel.forward and generate_paged).
 
 The hot path (routing, MoE grouped SwiGLU GEMM, mu-QKV GEMM, add+RMSNorm) runs only
 on the kernels in libcdx.so; the forward is inference-only (no backward).
@@ -23,7 +24,7 @@ from .modeling import (CausalLMOutput, ComplexityConfig, ComplexityModel, Graphe
                        count_parameters, create_complexity_model)
 from .normalization import (FusedResidualRMSNorm, RMSNorm, fused_add_rmsnorm_inplace, fused_residual_rmsnorm,
                             fused_rmsnorm)
-from .paged import paged_attention, paged_evict, paged_qkv_append, paged_write
+from .paged import PagedKVCache, paged_attention, paged_evict, paged_qkv_append, paged_write
 from .rotary import RotaryEmbedding, apply_rotary_pos_emb
 from .sampling import sample_tokens
 from .token_routed_mlp import (RoutePlan, TokenRoutedMLP, cggr_grouped_gemm, cggr_grouped_gemm_triton,
@@ -43,4 +44,5 @@ __all__ = [
     "fused_swiglu_simple", "route_plan", "route_plans", "RoutePlan",
     "fused_mu_qkv_projection", "FusedMuQKVProjection",
     "paged_qkv_append", "paged_write", "paged_attention", "paged_evict", "sample_tokens",
+    "PagedKVCache",
 ]

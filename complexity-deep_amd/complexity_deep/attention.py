@@ -41,6 +41,7 @@ import torch.nn.functional as F
 from . import _native as nat
 from ._grad import forward_only
 from .linear import few_rows, linear, linear_accumulate_
+from .paged import PagedLayer, paged_attention, paged_qkv_append, paged_write
 from .rotary import RotaryEmbedding, apply_rotary_pos_emb
 
 
@@ -574,6 +575,38 @@ class ComplexityAttention(nn.Module):
             attn = cache_attention(q, k, v)
         return self._out_proj(attn, residual), (k, v) if use_cache else None
 
+    def _paged_attention(self, x: torch.Tensor, mu: Optional[torch.Tensor], layer: PagedLayer, attention_mask,
+                         residual: Optional[torch.Tensor]) -> torch.Tensor:
+        """The attention with a layer of a PagedKVCache, whose ``begin`` has counted x's tokens:
+        prompts attend among themselves and are then written into the pages; one new token per
+        sequence is appended and attends to every slot in use."""
+        if attention_mask is not None:
+            raise ValueError("ComplexityAttention: a paged cache takes no mask (ragged prompts have lengths)")
+        if not (self.fused_prologue or self.other_head_dim) or (self.training and self.attention_dropout > 0):
+            raise NotImplementedError("ComplexityAttention: a paged cache needs the module's own norms and rotary "
+                                      "embedding, heads of a multiple of 8 up to 128, and no dropout")
+        cache = layer.cache
+        B, S, _ = x.shape
+        D, nq, nkv = self.head_dim, self.num_heads, self.num_kv_heads
+        k_pages, v_pages, weights = cache.layer(layer.index)
+        if (B, nkv, D) != (cache.batch_size, k_pages.shape[1], k_pages.shape[3]) or (S != 1 and not cache.prompt):
+            raise ValueError(f"ComplexityAttention: input {tuple(x.shape)} with {nkv} KV heads of {D} does not match "
+                             "the paged cache")
+        if cache.prompt:
+            out, (k, v) = self.forward(x, use_cache=True, mu_prev=mu, residual=residual)
+            paged_write(k, v, k_pages, v_pages, cache.block_table, cache.lengths)
+            return out
+        w_x, w_mu = self.qkv_weights()
+        qkv = mu_qkv_project(x, mu, w_x, self.hidden_size, w_mu=w_mu)
+        qn = (self.q_norm.weight, self.k_norm.weight) if self.use_qk_norm else (None, None)
+        q = paged_qkv_append(qkv.view(B, -1), k_pages, v_pages, cache.block_table, cache.lengths, cache.positions, nq,
+                             self.rotary_emb.cos_sin_table(cache.newest, x.device), *qn,
+                             self.q_norm.eps if self.use_qk_norm else 0.0)
+        attn = paged_attention(q, k_pages, v_pages, cache.block_table, cache.lengths, weights=weights,
+                               weights_out=weights)
+        attn = attn if weights is None else attn[0]
+        return self._out_proj(attn.view(B, 1, -1), residual)
+
     def _out_proj(self, attn: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
         """o_proj(attn), or with ``residual``: residual + o_proj(attn) written into residual
         (one GEMM with beta = 1, the block's residual add of core/layer.py:174).  o_proj is
@@ -604,6 +637,8 @@ class ComplexityAttention(nn.Module):
         """Returns (o_proj(attention), new_kv); with ``residual`` (the block input h,
         contiguous) the output is added to it in place and residual is returned."""
         forward_only("ComplexityAttention", hidden_states, mu_prev, residual, module=self)
+        if type(past_key_value) is PagedLayer:
+            return self._paged_attention(hidden_states, mu_prev, past_key_value, attention_mask, residual), None
         B, S, _ = hidden_states.shape
         D = self.head_dim
         past_len = past_key_value[0].shape[2] if past_key_value is not None else 0

@@ -39,6 +39,8 @@ from ._grad import forward_only
 from .layer import TransformerBlock
 from .linear import embedding, linear
 from .normalization import RMSNorm, rms_norm
+from .paged import PagedKVCache
+from .sampling import sample_tokens
 from .token_routed_mlp import RoutePlan, TokenRoutedMLP, route_plans
 
 
@@ -214,19 +216,31 @@ class ComplexityModel(nn.Module):
     def forward(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                 labels: Optional[torch.Tensor] = None,
                 past_key_values: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None,
-                use_cache: bool = False) -> CausalLMOutput:
+                use_cache: bool = False, prompt_lengths: Optional[torch.Tensor] = None) -> CausalLMOutput:
+        """``past_key_values`` may be a PagedKVCache, which the call extends in place and returns: the
+        prompts first (right-padded ones with ``prompt_lengths`` [B]), then one token per sequence."""
         forward_only("ComplexityModel", module=self)
         B, S = input_ids.shape
+        paged = isinstance(past_key_values, PagedKVCache)
+        if paged:
+            if attention_mask is not None:
+                raise ValueError("ComplexityModel: a paged cache takes no mask (ragged prompts have prompt_lengths)")
+            if len(past_key_values) != len(self.layers):
+                raise ValueError(f"ComplexityModel: a paged cache of {len(past_key_values)} layers for "
+                                 f"{len(self.layers)}")
+            past_key_values.begin(B, S, prompt_lengths)
+        elif prompt_lengths is not None:
+            raise ValueError("ComplexityModel: prompt_lengths without a paged cache")
         h = embedding(input_ids, self.embed_tokens.weight)
         mu_prev = self.mu_init.expand(B, S, -1) if self.config.use_mu_guidance else None
         plans = self.route_plans(input_ids)
-        new_kvs = [] if use_cache else None
+        new_kvs = past_key_values if paged else ([] if use_cache else None)
         layers = list(self.layers)
         n_layers = len(layers)
         # A generation step of a few rows runs block by block through TransformerBlock.step,
         # which takes h itself (its norms are folded); other calls hand each block its
         # normalised input, produced by the block before.
-        steps = attention_mask is None and 0 < B * S <= 8
+        steps = attention_mask is None and 0 < B * S <= 8 and not paged
         normed = None
         # Layers 1.. read their normalised input and mu side by side from one [B, S, 2H]
         # buffer, written by the layer before (one K = 2H operand for the projection).
@@ -250,7 +264,7 @@ class ComplexityModel(nn.Module):
                     want_mu=not last, pair=None if last else pair)
             if mu is not None:
                 mu_prev = mu  # clamped to [-2, 2] inside the mu-guidance kernel
-            if use_cache:
+            if use_cache and not paged:
                 new_kvs.append(new_kv)
         if normed is None:
             normed = rms_norm(h, self.norm.weight, self.norm.eps)
@@ -297,6 +311,53 @@ class ComplexityModel(nn.Module):
             if (nxt == eos_token_id).all():
                 break
         return input_ids
+
+    @torch.no_grad()
+    def generate_paged(self, input_ids: torch.Tensor, max_new_tokens: int = 100, *, temperature: float = 1.0,
+                       top_k: int = 50, top_p: float = 0.9, min_p: float = 0.0, eos_token_id: Optional[int] = None,
+                       prompt_lengths: Optional[torch.Tensor] = None, uniforms: Optional[torch.Tensor] = None,
+                       cache: Optional[PagedKVCache] = None) -> torch.Tensor:
+        """The new tokens [B, n <= max_new_tokens] after the prompts ``input_ids`` [B, S], of
+        ``prompt_lengths`` [B] tokens each (at least 1) where they are right-padded, on a paged cache: unlike
+        ``generate``, whose cached steps keep the reference's top-left mask, every token attends
+        to all before it.
+
+        Tokens come from sample_tokens (settings as there; temperature 0 is greedy) with
+        ``uniforms`` [B, max_new_tokens], or with torch's random numbers.  A sequence that has
+        produced ``eos_token_id`` (the configuration's by default) repeats it; the generation ends when
+        all have.  ``cache`` (emptied first) may bound the memory (PagedKVCache's keep); by default it
+        has room for every token."""
+        B, S = input_ids.shape
+        eos = self.config.eos_token_id if eos_token_id is None else eos_token_id
+        dev = input_ids.device
+        if uniforms is None:
+            uniforms = torch.rand(B, max_new_tokens, device=dev)
+        elif tuple(uniforms.shape) != (B, max_new_tokens):
+            raise ValueError(f"generate_paged: uniforms must be [{B}, {max_new_tokens}], got {tuple(uniforms.shape)}")
+        if cache is None:
+            cache = PagedKVCache(self.config, B, S + max(1, max_new_tokens), device=dev)
+        else:
+            cache.reset()
+        columns = uniforms.t().contiguous()
+        tokens = torch.full((max_new_tokens, B), eos, dtype=torch.int64, device=dev)
+        done = torch.zeros(B, dtype=torch.bool, device=dev)
+        n = 0
+        while n < max_new_tokens:
+            if n == 0:
+                logits = self.forward(input_ids, past_key_values=cache, prompt_lengths=prompt_lengths).logits
+                logits = logits[:, -1] if prompt_lengths is None else \
+                    logits[torch.arange(B, device=dev), cache.positions.long().clamp(min=0)]
+            else:
+                logits = self.forward(tokens[n - 1].view(B, 1), past_key_values=cache).logits[:, -1]
+            new = sample_tokens(logits, columns[n], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            torch.where(done, tokens[n], new, out=tokens[n])
+            done |= tokens[n] == eos
+            n += 1
+            if n % 16 == 0 and bool(done.all()):  # (the host looks every 16 tokens)
+                break
+        ended = (tokens[:n] == eos).cummax(0).values.all(1)
+        last = int(ended.int().argmax()) + 1 if n and bool(ended.any()) else n
+        return tokens[:last].t().contiguous()
 
     # ---- utilities (modeling.py:296-318) --------------------------------------------
     def num_parameters(self, trainable_only: bool = True) -> int:

@@ -10,6 +10,7 @@ sequence, and a step's one token attends to every slot in use:
   paged_qkv_append  a step's projection: QK norm, RoPE, k and v appended  (cdx_paged_append_fwd)
   paged_attention   softmax(scale q k^T) v over the slots in use         (cdx_paged_attention_fwd)
   paged_evict       the slots with the least accumulated weight go       (cdx_paged_evict)
+  PagedKVCache      all of it for a model: ComplexityModel.forward takes one as past_key_values
 
 ``block_table`` [B, width] and ``lengths`` [B] are int32 tensors on the device and no call waits
 for their values: a slot past a sequence's capacity (width * page_size) or on a page outside the
@@ -19,7 +20,7 @@ is an empty sequence.  All of it can be captured into a HIP graph.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -246,3 +247,133 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
             int(keep), int(recent), *(t.data_ptr() for t in new), work.data_ptr(), ws, nat.stream_of(k_pages)),
             "cdx_paged_evict")
     return new
+
+
+class PagedLayer(NamedTuple):
+    """One layer of a PagedKVCache, as ComplexityAttention takes it for past_key_value."""
+    cache: "PagedKVCache"
+    index: int
+
+
+class PagedKVCache:
+    """The KV cache of ``batch_size`` sequences of a ComplexityModel, in pages:
+    ``model(ids, past_key_values=cache)`` first takes the prompts, [B, S], then one token per
+    sequence and call, [B, 1], and every token attends to all before it (a list of k and v keeps
+    the reference's top-left mask instead).
+
+    Each sequence has room for ``max_length`` tokens (rounded up to whole pages).  When the
+    longest is full, a call raises, or with ``keep`` first cuts every longer sequence to ``keep``
+    slots (paged_evict): the ``recent`` newest tokens (half of ``keep`` by default) stay, and those
+    that the steps so far attended to most.  Positions go on counting.
+
+    ``lengths`` and ``positions`` (of the newest tokens) live on the device and nothing waits for
+    them; ``longest`` and ``newest`` are the host's bounds.  One call at a time may use a cache."""
+
+    def __init__(self, config, batch_size: int, max_length: int, *, page_size: int = 64, keep: Optional[int] = None,
+                 recent: Optional[int] = None, device="cuda"):
+        nkv, D = config.num_key_value_heads, config.hidden_size // config.num_attention_heads
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"PagedKVCache: page size {page_size} is not one of {PAGE_SIZES}")
+        if D % 8 != 0 or D > 128 or config.hidden_size % 64 != 0:
+            raise ValueError(f"PagedKVCache: heads of {D} in a hidden size of {config.hidden_size} (multiples of 8 up "
+                             "to 128, and of 64, are supported)")
+        if batch_size <= 0 or max_length <= 0:
+            raise ValueError(f"PagedKVCache: bad size {batch_size} x {max_length}")
+        recent = recent if recent is not None else (keep // 2 if keep is not None else 0)
+        if keep is not None and not (0 < keep < max_length and 0 <= recent <= keep):
+            raise ValueError(f"PagedKVCache: keep={keep} must lie in 1 .. max_length - 1, recent={recent} in 0 .. keep")
+        self.batch_size, self.page_size, self.keep, self.recent = batch_size, page_size, keep, recent
+        width = -(-max_length // page_size)
+        self.capacity = width * page_size
+        shape = (config.num_hidden_layers, batch_size * width, nkv, page_size, D)
+        self.k_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        self.v_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        device = self.k_pages.device
+        self.block_table = torch.arange(batch_size * width, dtype=torch.int32, device=device).view(batch_size, width)
+        self._counts = torch.zeros(2, batch_size, dtype=torch.int32, device=device)
+        self.weights = self.slot_positions = None
+        if keep is not None:
+            shape = (shape[0], batch_size, nkv, self.capacity)
+            self.weights = torch.zeros(shape, dtype=torch.float32, device=device)
+            self.slot_positions = torch.empty(shape, dtype=torch.int32, device=device)
+        self.reset()
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        return self._counts[0]
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._counts[1]
+
+    def __len__(self) -> int:
+        return self.k_pages.shape[0]
+
+    def __getitem__(self, i: int) -> PagedLayer:
+        if not 0 <= i < len(self):
+            raise IndexError(f"PagedKVCache: layer {i} of {len(self)}")
+        return PagedLayer(self, i)
+
+    def layer(self, i: int) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+        """(k_pages, v_pages, weights) of layer i."""
+        return self.k_pages[i], self.v_pages[i], self.weights[i] if self.weights is not None else None
+
+    def reset(self) -> None:
+        """Empty every sequence."""
+        self._counts[0].zero_()
+        self._counts[1].fill_(-1)
+        if self.weights is not None:
+            self.weights.zero_()
+            self.slot_positions.fill_(-1)
+        self.longest = self.newest = 0  # no sequence has more slots, or has seen more tokens
+        self.prompt = True              # what the call at hand brings
+
+    def evict(self) -> None:
+        """Cut every sequence of more than ``keep`` slots to ``keep``."""
+        if self.keep is None:
+            raise ValueError("PagedKVCache: made without keep")
+        if self.longest <= self.keep:
+            return
+        new = paged_evict(self.k_pages, self.v_pages, self.block_table, self.lengths, self.positions, self.weights,
+                          self.slot_positions, self.keep, self.recent)
+        for t, n in zip((self.lengths, self.weights, self.slot_positions), new):
+            t.copy_(n)
+        self.longest = self.keep
+
+    def begin(self, batch_size: int, tokens: int, prompt_lengths: Optional[torch.Tensor] = None) -> None:
+        """Make room for a call's tokens and count them: the prompts (of ``prompt_lengths`` tokens
+        each, or all of them) of an empty cache, then one token per sequence."""
+        if batch_size != self.batch_size:
+            raise ValueError(f"PagedKVCache: {batch_size} sequences in a cache of {self.batch_size}")
+        if self.newest == 0:
+            if not 0 < tokens <= self.capacity:
+                raise ValueError(f"PagedKVCache: prompts of {tokens} tokens in a cache of {self.capacity}")
+            if prompt_lengths is None:
+                self._counts[0].fill_(tokens)
+            else:
+                if prompt_lengths.shape != (batch_size,) or prompt_lengths.is_floating_point():
+                    raise ValueError(f"PagedKVCache: prompt_lengths must be {batch_size} integers, got "
+                                     f"{prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
+                self._counts[0].copy_(prompt_lengths.clamp(0, tokens))
+            torch.sub(self._counts[0], 1, out=self._counts[1])
+            if self.slot_positions is not None:
+                at = torch.arange(self.capacity, dtype=torch.int32, device=self.slot_positions.device)
+                self.slot_positions.copy_(torch.where(at < self.lengths.view(-1, 1, 1), at, -1))
+            self.longest = self.newest = tokens
+            self.prompt = True
+            return
+        if tokens != 1 or prompt_lengths is not None:
+            raise ValueError("PagedKVCache: after the prompts a call takes one token per sequence (reset() empties the "
+                             "cache)")
+        if self.longest >= self.capacity:
+            if self.keep is None:
+                raise ValueError(f"PagedKVCache: full ({self.capacity} tokens)")
+            self.evict()
+        self._counts.add_(1)
+        if self.slot_positions is not None:
+            shape = (*self.slot_positions.shape[:-1], 1)
+            slot = (self.lengths.long() - 1).view(-1, 1, 1).expand(shape)
+            self.slot_positions.scatter_(-1, slot, self.positions.view(-1, 1, 1).expand(shape))
+        self.longest += 1
+        self.newest += 1
+        self.prompt = False

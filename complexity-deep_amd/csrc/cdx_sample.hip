@@ -19,10 +19,12 @@
 //     needs the sum over the tokens below it).
 //   * Few tokens pass a bound: a second pass lists them, in order, in LDS, and everything else
 //     (the exact k-th, top-p, the draw) happens among at most 256 a wave, four to a lane.
-//   * Without a bound, or with more than the lists hold, thresholds come from a histogram over
-//     2048 bins of x (of counts for top-k, of weights for top-p), whose border bin is then
-//     resolved by a radix descent over its few tokens; the draw sums the kept weights by span.
-//     Those passes are paced by the exponentials, about 20 instructions in 64 bits a token.
+//   * Without a bound, or with more than the lists hold, thresholds come from a histogram, and the
+//     draw sums the kept weights by span.  bf16 logits take few values: those within reach of the
+//     top are counted one by one, and a table in LDS holds their weights, one exponential each.
+//     fp32 logits are summed in 2048 bins of x (of counts for top-k, of weights for top-p), whose
+//     border bin is then resolved by a radix descent over its few tokens; their passes are paced
+//     by the exponentials, about 20 instructions in 64 bits a token.
 #include <float.h>
 
 #include "cdx_common.h"
@@ -199,12 +201,34 @@ __device__ __forceinline__ bool any_weight(uint32_t key, float top, float T) {
   return x > -INFINITY && top < INFINITY && exp(((double)x - (double)top) / (double)T) > 0.0;
 }
 
+constexpr int kTable = 8192;  // values of bf16 logits
+
+// bf16 values in order, 0 apart and those below 2^-24 in magnitude as one (+-1): 128 a binade.
+constexpr int kTinyBits = 0x337f;  // the largest bf16 below 2^-24
+__device__ __forceinline__ int value_step(float x) {
+  const int u = (int)__float_as_uint(x), m = (u >> 16) & 0x7fff, sign = u >> 31;
+  const int mm = m == 0 ? 0 : max(m, kTinyBits) - (kTinyBits - 1);
+  return (mm ^ sign) - sign;
+}
+__device__ __forceinline__ float step_value(int s) {  // (of a step other than +-1)
+  const uint32_t m = s == 0 ? 0u : (uint32_t)(abs(s) + kTinyBits - 1) << 16;
+  return __uint_as_float(s < 0 ? m | 0x80000000u : m);
+}
+
+template <typename TIn>
 struct Shared {
+  static constexpr int kSpans = (int)(kMaxVocab * sizeof(TIn) / 1024) + 1;
   u64 bins[kBins];
-  u64 sums[kMaxVocab / 256 + 1];  // by span: at most 2^20 / 256 + 1 of them
-  int ties[kMaxVocab / 256 + 1];
-  uint32_t list_key[kList];
-  int list_index[kList];
+  u64 sums[kSpans];
+  int ties[kSpans];
+  union {
+    struct {
+      uint32_t list_key[kList];
+      int list_index[kList];
+    };
+    uint32_t counts[kTable];
+  };
+  u64 table[sizeof(TIn) == 2 ? kTable : 1];
   u64 red[kSampleWaves];
   u64 pick[3];
   uint32_t range[2];
@@ -212,8 +236,27 @@ struct Shared {
   int total;
 };
 
+// Sum over the threads before this one, and over the block.
+template <typename T, typename Sh>
+__device__ __forceinline__ T block_exclusive(T v, Sh& sh, T& total) {
+  const int wave = threadIdx.x >> 6;
+  const T run = wave_inclusive(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) sh.red[wave] = (u64)run;
+  __syncthreads();
+  T before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSampleWaves; ++w) {
+    before += w < wave ? (T)sh.red[w] : 0;
+    total += (T)sh.red[w];
+  }
+  return before + run - v;
+}
+
 // Sum over the block, returned to every thread.
-__device__ __forceinline__ u64 block_sum(u64 v, Shared& sh) {
+template <typename Sh>
+__device__ __forceinline__ u64 block_sum(u64 v, Sh& sh) {
   v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
@@ -226,7 +269,8 @@ __device__ __forceinline__ u64 block_sum(u64 v, Shared& sh) {
 
 // By wave 0: the last of n bins, from the highest down, that holds something and before which
 // the sum is within the limit: (bin, that sum) into pick.
-__device__ __forceinline__ void pick_bin(Shared& sh, int n, u64 above, u64 limit, bool descending) {
+template <typename Sh>
+__device__ __forceinline__ void pick_bin(Sh& sh, int n, u64 above, u64 limit, bool descending) {
   const int lane = threadIdx.x, per = n / 64;
   u64 mine = 0;
   for (int i = 0; i < per; ++i) {
@@ -254,8 +298,8 @@ __device__ __forceinline__ void pick_bin(Shared& sh, int n, u64 above, u64 limit
 
 // The smallest key before which the items of larger keys weigh no more than the limit, and that
 // weight.  each(f) calls f(key, weight) for the thread's items.  A byte at a time.
-template <typename Each>
-__device__ uint32_t descend(Shared& sh, u64& above, u64 limit, Each each) {
+template <typename Sh, typename Each>
+__device__ uint32_t descend(Sh& sh, u64& above, u64 limit, Each each) {
   uint32_t prefix = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
@@ -275,7 +319,7 @@ __device__ uint32_t descend(Shared& sh, u64& above, u64 limit, Each each) {
 
 template <typename TIn>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
-  __shared__ Shared sh;
+  __shared__ Shared<TIn> sh;
   constexpr int VEC = Row<TIn>::VEC;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t b = blockIdx.x;
@@ -683,35 +727,119 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     return key;
   };
 
-  float low = top == INFINITY ? INFINITY : -FLT_MAX;  // the least logit that top-k keeps
-  if (top_k > 0) {
-    // Bins over four times the spread of the threads' maxima.
-    float least = mine > -INFINITY ? mine : top;
+  const bool any = !(u > 0.f);
+  float border = -FLT_MAX;   // the least logit kept
+  u64 keep = ~0ull;          // of those that equal it: so many by index, or all
+  bool tabled = false;       // whether the weights of the values lie in the table
+  int top_step = 0;
+  if constexpr (sizeof(TIn) == 2) {
+    // Logits below `cutoff` weigh less than 2^-64.
+    const float cutoff = top - 45.f * T;
+    top_step = value_step(top);
+    const int steps = top_step - value_step(cutoff) + 2;  // (cutoff, cut to 16 bits, may round up a step)
+    tabled = !any && top < INFINITY && cutoff > -FLT_MAX && steps < kTable;
+    if (tabled && (top_k > 0 || cut_p)) {
+      __syncthreads();
+      for (int i = tid; i < kTable; i += kThreads) sh.counts[i] = 0;
+      if (tid == 0) sh.total = 0;
+      __syncthreads();
+      row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
+        bool tiny = false;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) least = fminf(least, __shfl_xor(least, d, 64));
-    __syncthreads();
-    if (lane == 0) sh.red[wave] = __float_as_uint(least);
-    __syncthreads();
+        for (int e = 0; e < VEC; ++e) {
+          const int step = value_step(v[e]);
+          tiny = tiny || step * step == 1;
+          atomicAdd(&sh.counts[v[e] >= cutoff ? top_step - step : kTable - 1], 1u);  // (the last one: not counted)
+        }
+        if (__ballot(tiny) != 0) sh.total = 1;
+      });
+      __syncthreads();
+      tabled = sh.total == 0;  // (different values that share a step: by bins)
+    }
+    if (tabled) {
+      constexpr int PER = kTable / kThreads;
+      const int i0 = tid * PER;
+      const bool counted = top_k > 0 || cut_p;
+      uint32_t n[PER];
+      u64 w[PER];
+      int last = steps;  // the step (from the top) of the k-th largest logit
 #pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) least = fminf(least, __uint_as_float((uint32_t)sh.red[w]));
-    const float spread = top - least;
-    const float per_x = spread > 0.f && spread < INFINITY ? (float)(kBins / 4) / spread : 0.f;
-    const float kth = key_logit(border_of(per_x, 0, [&](u64 n) { return (u64)top_k - 1 < n ? (u64)top_k - 1 : n - 1; },
-                                          [](float) -> u64 { return 1; }));
-    low = fmaxf(low, kth);
+      for (int i = 0; i < PER; ++i) n[i] = counted ? sh.counts[i0 + i] : 0;
+      if (top_k > 0) {
+        int mine_n = 0, all_n;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) mine_n += (int)n[i];
+        int before = block_exclusive(mine_n, sh, all_n);
+        if (tid == 0) sh.range[0] = (uint32_t)steps;
+        __syncthreads();
+        if (before < top_k && before + mine_n >= top_k)  // (one thread, or none: fewer lie above the cutoff)
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            if (before < top_k && before + (int)n[i] >= top_k) sh.range[0] = (uint32_t)(i0 + i);
+            before += (int)n[i];
+          }
+        __syncthreads();
+        last = (int)sh.range[0];
+      }
+      border = last < steps ? step_value(top_step - last) : cutoff;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float x = step_value(top_step - i0 - i);
+        const bool in = i0 + i <= last && i0 + i < steps && x >= cutoff;
+        const double f = in ? wt.fraction(x) : 0.0;
+        w[i] = in ? wt.units(f) : 0;
+        sh.table[i0 + i] = i0 + i == 0 || !(min_p > 0.f) || f >= (double)min_p ? w[i] : 0;
+      }
+      if (cut_p) {
+        u64 mass = 0, total;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) mass += n[i] * w[i];
+        u64 before = block_exclusive(mass, sh, total);
+        const u64 limit = (u64)((double)top_p * (double)total);
+        if (before <= limit && before + mass > limit)  // (one thread)
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const u64 m = n[i] * w[i];
+            if (before <= limit && before + m > limit) {
+              sh.pick[0] = (u64)(i0 + i);
+              sh.pick[1] = (limit - before) / w[i] + 1;
+            }
+            before += m;
+          }
+        __syncthreads();
+        border = step_value(top_step - (int)sh.pick[0]);
+        keep = sh.pick[1];
+      }
+    }
   }
-  float border = low;
-  u64 keep = ~0ull, tie_w = 0;
-  if (cut_p) {
-    // A weight past 2^-64 is no unit: bins over that many times T ln 2.
-    const float range = 44.4f * T, per_x = range < 1e30f && range > 1e-30f ? (float)kBins / range : 0.f;
-    border = key_logit(border_of(per_x, 0, [&](u64 n) { return (u64)((double)top_p * (double)n); },
-                                 [&](float x) -> u64 { return x >= low ? wt.units(x) : 0; }));
-    tie_w = wt.units(border);
-    keep = (sh.pick[2] - sh.pick[1]) / tie_w + 1;
+  if (!tabled) {
+    float low = top == INFINITY ? INFINITY : -FLT_MAX;  // the least logit that top-k keeps
+    if (top_k > 0) {
+      // Bins over four times the spread of the threads' maxima.
+      float least = mine > -INFINITY ? mine : top;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) least = fminf(least, __shfl_xor(least, d, 64));
+      __syncthreads();
+      if (lane == 0) sh.red[wave] = __float_as_uint(least);
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kSampleWaves; ++w) least = fminf(least, __uint_as_float((uint32_t)sh.red[w]));
+      const float spread = top - least;
+      const float per_x = spread > 0.f && spread < INFINITY ? (float)(kBins / 4) / spread : 0.f;
+      auto limit = [&](u64 n) { return (u64)top_k - 1 < n ? (u64)top_k - 1 : n - 1; };
+      low = fmaxf(low, key_logit(border_of(per_x, 0, limit, [](float) -> u64 { return 1; })));
+    }
+    border = low;
+    if (cut_p) {
+      // A weight past 2^-64 is no unit: bins over that many times T ln 2.
+      const float range = 44.4f * T, per_x = range < 1e30f && range > 1e-30f ? (float)kBins / range : 0.f;
+      border = key_logit(border_of(per_x, 0, [&](u64 n) { return (u64)((double)top_p * (double)n); },
+                                   [&](float x) -> u64 { return x >= low ? wt.units(x) : 0; }));
+      keep = (sh.pick[2] - sh.pick[1]) / wt.units(border) + 1;
+    }
   }
   // Kept weights by span, the ties at the border counted apart.
-  const bool any = !(u > 0.f), by_ties = keep != ~0ull;
+  const bool by_ties = keep != ~0ull;
   auto kept = [&](float x) -> u64 {
     if (x == top) return any ? 1 : wt.units(x);
     const double w = wt.fraction(x);
@@ -720,9 +848,33 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
   };
   // What is summed as it is: the logits above the border, or without ties from it on.
   const float least = by_ties ? key_logit(logit_key(border) + 1) : border;
-  tie_w = by_ties ? kept(border) : 0;
+  const u64 tie_w = by_ties ? kept(border) : 0;
   __syncthreads();
-  if (any || min_p > 0.f) {
+  if (tabled) {
+    row.spans(s0, s1, lane, [&](int s, int, const float(&v)[VEC]) {
+      u64 sum = 0;
+      int ties = 0;
+      bool tiny = false;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int step = value_step(v[e]);
+        tiny = tiny || step * step == 1;
+        sum += sh.table[v[e] >= least ? top_step - step : kTable - 1];  // (the last one is 0)
+        ties += v[e] == border ? 1 : 0;
+      }
+      if (__ballot(tiny) != 0) {  // values that share a step: one by one
+        sum = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum += v[e] >= least ? kept(v[e]) : 0;
+      }
+      sum = wave_sum(sum);
+      ties = wave_sum(ties);
+      if (lane == 0) {
+        sh.sums[s] = sum;
+        sh.ties[s] = ties;
+      }
+    });
+  } else if (any || min_p > 0.f) {
     row.spans(s0, s1, lane, [&](int s, int, const float(&v)[VEC]) {
       u64 sum = 0;
       int ties = 0;

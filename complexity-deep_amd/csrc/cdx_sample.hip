@@ -112,8 +112,6 @@ struct Row {
     lo = head > 0 ? 1 : 0;
     hi = (head + V) / VEC - 1;
   }
-  static __device__ __forceinline__ float value(const float* p) { return *p; }
-  static __device__ __forceinline__ float value(const uint16_t* p) { return bf16_bits_to_f32(*p); }
   static __device__ __forceinline__ void unpack(const piece_t& v, float (&f)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
@@ -125,11 +123,27 @@ struct Row {
       f[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
     }
   }
-  // f(span, first token, values) over the spans s0 <= span < s1.  AHEAD loads are on their way
-  // together: a piece that does not lie inside the row loads one that does and is then taken
-  // token by token.
+  // A piece that does not lie inside the row, token by token.
+  __device__ __forceinline__ piece_t edge(int c) const {
+    piece_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = sizeof(TIn) == 2 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int i = c * VEC + e - head;
+      if (i < 0 || i >= V) continue;
+      if constexpr (sizeof(TIn) == 2)
+        v[e / 2] = e & 1 ? (v[e / 2] & 0xffffu) | (uint32_t)x[c * VEC + e] << 16
+                         : (v[e / 2] & 0xffff0000u) | (uint32_t)x[c * VEC + e];
+      else
+        v[e] = __float_as_uint(x[c * VEC + e]);
+    }
+    return v;
+  }
+  // f(span, first token, piece) over the spans s0 <= span < s1.  AHEAD loads are on their way
+  // together (a piece that does not lie inside the row loads one that does, in its place).
   template <typename F>
-  __device__ __forceinline__ void spans(int s0, int s1, int lane, F f) const {
+  __device__ __forceinline__ void each_piece(int s0, int s1, int lane, F f) const {
     constexpr int AHEAD = 4;
     for (int s = s0; s < s1; s += AHEAD) {
       piece_t raw[AHEAD];
@@ -144,18 +158,19 @@ struct Row {
       for (int a = 0; a < AHEAD; ++a) {
         if (s + a >= s1) break;
         const int c = (s + a) * 64 + lane;
-        float v[VEC];
-        unpack(raw[a], v);
-        if (c < lo || c > hi) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int i = c * VEC + e - head;
-            v[e] = i >= 0 && i < V ? value(x + c * VEC + e) : -INFINITY;
-          }
-        }
-        f(s + a, c * VEC - head, v);
+        if (c < lo || c > hi) raw[a] = edge(c);
+        f(s + a, c * VEC - head, raw[a]);
       }
     }
+  }
+  // As values.
+  template <typename F>
+  __device__ __forceinline__ void spans(int s0, int s1, int lane, F f) const {
+    each_piece(s0, s1, lane, [&](int s, int i0, const piece_t& raw) {
+      float v[VEC];
+      unpack(raw, v);
+      f(s, i0, v);
+    });
   }
 };
 
@@ -203,16 +218,37 @@ __device__ __forceinline__ bool any_weight(uint32_t key, float top, float T) {
 
 constexpr int kTable = 8192;  // values of bf16 logits
 
-// bf16 values in order, 0 apart and those below 2^-24 in magnitude as one (+-1): 128 a binade.
-constexpr int kTinyBits = 0x337f;  // the largest bf16 below 2^-24
+// bf16 values in order: from 2^-24 in magnitude on 128 steps a binade, positive and negative; those
+// nearer to 0 share step 0.
+constexpr int kLeastBits = 0x3380;  // 2^-24
 __device__ __forceinline__ int value_step(float x) {
-  const int u = (int)__float_as_uint(x), m = (u >> 16) & 0x7fff, sign = u >> 31;
-  const int mm = m == 0 ? 0 : max(m, kTinyBits) - (kTinyBits - 1);
-  return (mm ^ sign) - sign;
+  const int u = (int)__float_as_uint(x), m = max((u >> 16) & 0x7fff, kLeastBits - 1) - (kLeastBits - 1);
+  return u < 0 ? -m : m;
 }
-__device__ __forceinline__ float step_value(int s) {  // (of a step other than +-1)
-  const uint32_t m = s == 0 ? 0u : (uint32_t)(abs(s) + kTinyBits - 1) << 16;
+__device__ __forceinline__ float step_value(int s) {
+  const uint32_t m = s == 0 ? 0u : (uint32_t)(abs(s) + kLeastBits - 1) << 16;
   return __uint_as_float(s < 0 ? m | 0x80000000u : m);
+}
+// For each of a piece's values: how many steps below the top it lies, at most `most` (also a NaN
+// and -inf; one of step 0 gives any number up to that).
+struct StepsBelow {
+  int plus, minus;
+  uint32_t most;
+  __device__ __forceinline__ StepsBelow(int top_step, int most_)
+      : plus(top_step + kLeastBits - 1), minus(top_step - kLeastBits + 1 + 32768), most((uint32_t)most_) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t word, bool high) const {
+    const int t = high ? (int)word >> 16 : (int)(word << 16) >> 16;  // negative: its magnitude - 2^15
+    return min((uint32_t)(t < 0 ? minus + t : plus - t), most);
+  }
+};
+// Whether a piece holds a value of step 0.
+template <typename P>
+__device__ __forceinline__ bool has_tiny(const P& v) {
+  typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+  u16x2 least = __builtin_bit_cast(u16x2, v[0] & 0x7fff7fffu);
+#pragma unroll
+  for (int e = 1; e < 4; ++e) least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2, v[e] & 0x7fff7fffu));
+  return min(least[0], least[1]) < kLeastBits;
 }
 
 template <typename TIn>
@@ -321,6 +357,7 @@ template <typename TIn>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
   __shared__ Shared<TIn> sh;
   constexpr int VEC = Row<TIn>::VEC;
+  typedef typename Row<TIn>::piece_t piece_t;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t b = blockIdx.x;
   const Row<TIn> row(static_cast<const TIn*>(p.logits) + b * p.ld, p.V);
@@ -732,29 +769,47 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
   u64 keep = ~0ull;          // of those that equal it: so many by index, or all
   bool tabled = false;       // whether the weights of the values lie in the table
   int top_step = 0;
+  const float cutoff = top - 45.f * T;  // logits below it weigh less than 2^-64
   if constexpr (sizeof(TIn) == 2) {
-    // Logits below `cutoff` weigh less than 2^-64.
-    const float cutoff = top - 45.f * T;
     top_step = value_step(top);
     const int steps = top_step - value_step(cutoff) + 2;  // (cutoff, cut to 16 bits, may round up a step)
-    tabled = !any && top < INFINITY && cutoff > -FLT_MAX && steps < kTable;
+    const bool stepped = fabsf(top) >= 0x1p-24f;
+    tabled = stepped && !any && top < INFINITY && cutoff > -FLT_MAX && steps < kTable;
     if (tabled && (top_k > 0 || cut_p)) {
       __syncthreads();
       for (int i = tid; i < kTable; i += kThreads) sh.counts[i] = 0;
-      if (tid == 0) sh.total = 0;
+      if (tid == 0) {
+        sh.total = 0;
+        sh.pick[2] = 0;
+      }
       __syncthreads();
-      row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
-        bool tiny = false;
+      const StepsBelow below(top_step, steps);
+      row.each_piece(s0, s1, lane, [&](int, int, const piece_t& v) {
+        // (What lies below the cutoff goes to a count of its own.)
+        if (__ballot(has_tiny(v)) == 0) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) atomicAdd(&sh.counts[below(v[e / 2], e & 1)], 1u);
+          return;
+        }
+        // Step 0: counted together, weighed one by one.
+        float f[VEC];
+        row.unpack(v, f);
+        u64 mass = 0;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const int step = value_step(v[e]);
-          tiny = tiny || step * step == 1;
-          atomicAdd(&sh.counts[v[e] >= cutoff ? top_step - step : kTable - 1], 1u);  // (the last one: not counted)
+          const bool tiny = fabsf(f[e]) < 0x1p-24f;
+          if (!tiny) {
+            atomicAdd(&sh.counts[below(v[e / 2], e & 1)], 1u);
+          } else if (f[e] >= cutoff) {
+            atomicAdd(&sh.counts[top_step], 1u);
+            mass += wt.units(f[e]);
+            if (f[e] != 0.f) sh.total = 1;  // (other values among them)
+          }
         }
-        if (__ballot(tiny) != 0) sh.total = 1;
+        mass = wave_sum(mass);
+        if (lane == 0) atomicAdd(&sh.pick[2], mass);
       });
       __syncthreads();
-      tabled = sh.total == 0;  // (different values that share a step: by bins)
     }
     if (tabled) {
       constexpr int PER = kTable / kThreads;
@@ -762,9 +817,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
       const bool counted = top_k > 0 || cut_p;
       uint32_t n[PER];
       u64 w[PER];
+      const u64 step0_mass = sh.pick[2];
+      const int mixed = counted && sh.total != 0 ? top_step : -1;  // where different values are counted as one
       int last = steps;  // the step (from the top) of the k-th largest logit
 #pragma unroll
-      for (int i = 0; i < PER; ++i) n[i] = counted ? sh.counts[i0 + i] : 0;
+      for (int i = 0; i < PER; ++i) n[i] = counted && i0 + i < steps ? sh.counts[i0 + i] : 0;
       if (top_k > 0) {
         int mine_n = 0, all_n;
 #pragma unroll
@@ -793,13 +850,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
       if (cut_p) {
         u64 mass = 0, total;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) mass += n[i] * w[i];
+        for (int i = 0; i < PER; ++i) mass += i0 + i == mixed && mixed <= last ? step0_mass : n[i] * w[i];
         u64 before = block_exclusive(mass, sh, total);
         const u64 limit = (u64)((double)top_p * (double)total);
         if (before <= limit && before + mass > limit)  // (one thread)
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
-            const u64 m = n[i] * w[i];
+            const u64 m = i0 + i == mixed && mixed <= last ? step0_mass : n[i] * w[i];
             if (before <= limit && before + m > limit) {
               sh.pick[0] = (u64)(i0 + i);
               sh.pick[1] = (limit - before) / w[i] + 1;
@@ -807,9 +864,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
             before += m;
           }
         __syncthreads();
-        border = step_value(top_step - (int)sh.pick[0]);
+        last = (int)sh.pick[0];
+        border = step_value(top_step - last);
         keep = sh.pick[1];
       }
+      tabled = last != mixed;  // (a border among different values: by bins)
     }
   }
   if (!tabled) {
@@ -851,29 +910,41 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
   const u64 tie_w = by_ties ? kept(border) : 0;
   __syncthreads();
   if (tabled) {
-    row.spans(s0, s1, lane, [&](int s, int, const float(&v)[VEC]) {
-      u64 sum = 0;
-      int ties = 0;
-      bool tiny = false;
+    if constexpr (sizeof(TIn) == 2) {
+      // Entries past the border are not looked at, its own counts the ties instead (in the high bits).
+      constexpr int TIE = 56;
+      const int last = top_step - value_step(border) + (by_ties || border != cutoff ? 0 : 1);
+      if (tid == 0) {
+        if (by_ties) sh.table[last] = 1ull << TIE;
+        sh.table[last + 1] = 0;
+      }
+      __syncthreads();
+      const StepsBelow below(top_step, last + 1);
+      row.each_piece(s0, s1, lane, [&](int s, int, const piece_t& raw) {
+        u64 sum = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int step = value_step(v[e]);
-        tiny = tiny || step * step == 1;
-        sum += sh.table[v[e] >= least ? top_step - step : kTable - 1];  // (the last one is 0)
-        ties += v[e] == border ? 1 : 0;
-      }
-      if (__ballot(tiny) != 0) {  // values that share a step: one by one
-        sum = 0;
+        for (int e = 0; e < VEC; ++e) sum += sh.table[below(raw[e / 2], e & 1)];
+        int ties = (int)(sum >> TIE);
+        sum &= (1ull << TIE) - 1;
+        if (__ballot(has_tiny(raw)) != 0) {  // one by one
+          float v[VEC];
+          row.unpack(raw, v);
+          sum = 0;
+          ties = 0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum += v[e] >= least ? kept(v[e]) : 0;
-      }
-      sum = wave_sum(sum);
-      ties = wave_sum(ties);
-      if (lane == 0) {
-        sh.sums[s] = sum;
-        sh.ties[s] = ties;
-      }
-    });
+          for (int e = 0; e < VEC; ++e) {
+            sum += v[e] >= least ? kept(v[e]) : 0;
+            ties += by_ties && v[e] == border ? 1 : 0;
+          }
+        }
+        sum = wave_sum(sum);
+        if (by_ties) ties = wave_sum(ties);
+        if (lane == 0) {
+          sh.sums[s] = sum;
+          sh.ties[s] = ties;
+        }
+      });
+    }
   } else if (any || min_p > 0.f) {
     row.spans(s0, s1, lane, [&](int s, int, const float(&v)[VEC]) {
       u64 sum = 0;

@@ -22,7 +22,7 @@
 //   * Without a bound, or with more than the lists hold, thresholds come from a histogram, and the
 //     draw sums the kept weights by span.  bf16 logits take few values: those within reach of the
 //     top are counted one by one, and a table in LDS holds their weights, one exponential each.
-//     fp32 logits are summed in 2048 bins of x (of counts for top-k, of weights for top-p), whose
+//     fp32 logits are summed in 8192 bins of x (of counts for top-k, of weights for top-p), whose
 //     border bin is then resolved by a radix descent over its few tokens; their passes are paced
 //     by the exponentials, about 20 instructions in 64 bits a token.
 #include <float.h>
@@ -40,7 +40,7 @@ constexpr int64_t kMaxVocab = 1 << 20;
 constexpr int kListWave = 256;                // tokens that a wave can list
 constexpr int kLane = kListWave / 64;
 constexpr int kList = kListWave * kSampleWaves;
-constexpr int kBins = 2048;
+constexpr int kBins = 8192;
 
 struct SampleParams {
   const void* logits;  // [B] rows of V at stride ld
@@ -216,7 +216,7 @@ __device__ __forceinline__ bool any_weight(uint32_t key, float top, float T) {
   return x > -INFINITY && top < INFINITY && exp(((double)x - (double)top) / (double)T) > 0.0;
 }
 
-constexpr int kTable = 8192;  // values of bf16 logits
+constexpr int kTable = kBins;  // values of bf16 logits
 
 // bf16 values in order: from 2^-24 in magnitude on 128 steps a binade, positive and negative; those
 // nearer to 0 share step 0.
@@ -254,7 +254,10 @@ __device__ __forceinline__ bool has_tiny(const P& v) {
 template <typename TIn>
 struct Shared {
   static constexpr int kSpans = (int)(kMaxVocab * sizeof(TIn) / 1024) + 1;
-  u64 bins[kBins];
+  union {
+    u64 bins[kBins];
+    u64 table[kTable];
+  };
   u64 sums[kSpans];
   int ties[kSpans];
   union {
@@ -264,7 +267,6 @@ struct Shared {
     };
     uint32_t counts[kTable];
   };
-  u64 table[sizeof(TIn) == 2 ? kTable : 1];
   u64 red[kSampleWaves];
   u64 pick[3];
   uint32_t range[2];
@@ -303,31 +305,27 @@ __device__ __forceinline__ u64 block_sum(u64 v, Sh& sh) {
   return t;
 }
 
-// By wave 0: the last of n bins, from the highest down, that holds something and before which
-// the sum is within the limit: (bin, that sum) into pick.
+// By wave 0: the last of 256 bins, from the highest down, that holds something and before which the
+// sum is within the limit: (bin, that sum) into pick.
 template <typename Sh>
-__device__ __forceinline__ void pick_bin(Sh& sh, int n, u64 above, u64 limit, bool descending) {
-  const int lane = threadIdx.x, per = n / 64;
-  u64 mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int d = lane * per + i;
-    mine += sh.bins[descending ? n - 1 - d : d];
-  }
-  u64 before = above + wave_inclusive(mine) - mine;
+__device__ __forceinline__ void pick_digit(Sh& sh, u64 above, u64 limit) {
+  const int lane = threadIdx.x;
+  u64 v[4], mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mine += v[i] = sh.bins[255 - 4 * lane - i];
+  u64 before = above + wave_inclusive(mine) - mine, at = 0;
   int last = -1;
-  u64 at = 0;
-  for (int i = 0; i < per && before <= limit; ++i) {
-    const int d = lane * per + i;
-    const u64 v = sh.bins[descending ? n - 1 - d : d];
-    if (v != 0) {
-      last = d;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (v[i] != 0 && before <= limit) {
+      last = 255 - 4 * lane - i;
       at = before;
     }
-    before += v;
+    before += v[i];
   }
   const u64 lanes = __ballot(last >= 0);
   if (lanes != 0 && lane == 63 - __builtin_clzll(lanes)) {
-    sh.pick[0] = (u64)(descending ? n - 1 - last : last);
+    sh.pick[0] = (u64)last;
     sh.pick[1] = at;
   }
 }
@@ -345,7 +343,7 @@ __device__ uint32_t descend(Sh& sh, u64& above, u64 limit, Each each) {
       if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&sh.bins[(key >> shift) & 255], w);
     });
     __syncthreads();
-    if (threadIdx.x < 64) pick_bin(sh, 256, above, limit, true);
+    if (threadIdx.x < 64) pick_digit(sh, above, limit);
     __syncthreads();
     prefix = prefix << 8 | (uint32_t)sh.pick[0];
     above = sh.pick[1];
@@ -682,7 +680,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
 
   // Whole rows.  The border of a sum over the row (of counts or of weights), from the highest logit
   // down: by bins of equal width, then among the tokens of the border bin.
-  auto border_of = [&](float per_x, u64 above, auto limit_of, auto weight) -> uint32_t {
+  auto border_of = [&](float per_x, auto limit_of, auto weight) -> uint32_t {
     // Bins count down from the top; those past the last one are the last one.
     auto bin = [&](float x) -> int {
       const float d = (top - x) * per_x;
@@ -693,16 +691,24 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     __syncthreads();
     row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const u64 w = v[e] >= -FLT_MAX ? weight(v[e]) : 0;
-        if (w != 0) atomicAdd(&sh.bins[bin(v[e])], w);
-      }
+      for (int e = 0; e < VEC; ++e) atomicAdd(&sh.bins[bin(v[e])], weight(v[e]));
     });
     __syncthreads();
-    u64 t = 0;
-    for (int i = tid; i < kBins; i += kThreads) t += sh.bins[i];
-    const u64 limit = limit_of(block_sum(t, sh));
-    if (tid < 64) pick_bin(sh, kBins, above, limit, false);
+    constexpr int PER = kBins / kThreads;
+    u64 w[PER], mass = 0, total;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mass += w[i] = sh.bins[tid * PER + i];
+    u64 above = block_exclusive(mass, sh, total);
+    const u64 limit = limit_of(total);
+    if (above <= limit && above + mass > limit)  // (one thread)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (above <= limit && above + w[i] > limit) {
+          sh.pick[0] = (u64)(tid * PER + i);
+          sh.pick[1] = above;
+        }
+        above += w[i];
+      }
     if (tid == 0) sh.total = 0;
     __syncthreads();
     const int chosen = (int)sh.pick[0];
@@ -742,17 +748,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     const uint32_t key = descend(sh, above, limit, [&](auto f) {
       if (n <= kList) {
         for (int i = tid; i < n; i += kThreads) {
-          const u64 w = weight(key_logit(sh.list_key[i]));
-          if (w != 0) f(sh.list_key[i], w);
+          f(sh.list_key[i], weight(key_logit(sh.list_key[i])));
         }
       } else {
         row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
-            if (v[e] >= from && v[e] <= to) {
-              const u64 w = weight(v[e]);
-              if (w != 0) f(logit_key(v[e]), w);
-            }
+            if (v[e] >= from && v[e] <= to) f(logit_key(v[e]), weight(v[e]));
         });
       }
     });
@@ -886,14 +888,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
       const float spread = top - least;
       const float per_x = spread > 0.f && spread < INFINITY ? (float)(kBins / 4) / spread : 0.f;
       auto limit = [&](u64 n) { return (u64)top_k - 1 < n ? (u64)top_k - 1 : n - 1; };
-      low = fmaxf(low, key_logit(border_of(per_x, 0, limit, [](float) -> u64 { return 1; })));
+      auto one = [](float x) -> u64 { return x >= -FLT_MAX ? 1 : 0; };
+      low = fmaxf(low, key_logit(border_of(per_x, limit, one)));
     }
     border = low;
     if (cut_p) {
-      // A weight past 2^-64 is no unit: bins over that many times T ln 2.
+      // A weight below 2^-64 is no unit: bins over that many times T ln 2.
       const float range = 44.4f * T, per_x = range < 1e30f && range > 1e-30f ? (float)kBins / range : 0.f;
-      border = key_logit(border_of(per_x, 0, [&](u64 n) { return (u64)((double)top_p * (double)n); },
-                                   [&](float x) -> u64 { return x >= low ? wt.units(x) : 0; }));
+      border = key_logit(border_of(per_x, [&](u64 n) { return (u64)((double)top_p * (double)n); },
+                                   [&](float x) -> u64 { return wt.units(x >= low ? x : -INFINITY); }));
       keep = (sh.pick[2] - sh.pick[1]) / wt.units(border) + 1;
     }
   }

@@ -25,6 +25,9 @@ def _logits(B, V, seed, dtype, kind="model"):
     if kind == "masked":
         x = torch.where(torch.rand(B, V, generator=g) < 0.9, -math.inf, x)
         x[:, V // 2] = 0.5
+    if kind == "tiny":  # values around 0 among others, too many for the lists at the larger sizes
+        pool = torch.tensor([0.0, -0.0, 1e-9, -1e-9, 3e-8, -5e-8, 2.0 ** -24, -2.0 ** -24, 2.0 ** -23])
+        x = torch.where(torch.rand(B, V, generator=g) < 0.3, pool[torch.randint(0, 9, (B, V), generator=g)], x)
     if kind == "odd":
         pool = torch.tensor([math.nan, -math.inf, 0.0, -0.0, 1.0, -1.0, 1e-30, -3e38])
         x = pool[torch.randint(0, len(pool), (B, V), generator=g)]
@@ -48,7 +51,7 @@ SETTINGS = [{}, {"temperature": 0.0}, {"temperature": 0.7, "top_k": 50, "top_p":
             {"min_p": 1.0}, {"temperature": 1e-3}, {"temperature": 1e30, "top_p": 0.95}, {"top_k": 1000, "top_p": 0.99}]
 
 
-@pytest.mark.parametrize("kind", ["model", "ties", "flat", "masked", "odd"])
+@pytest.mark.parametrize("kind", ["model", "ties", "flat", "masked", "tiny", "odd"])
 @pytest.mark.parametrize("V,dtype", [(1, bf16), (2, torch.float32), (50, bf16), (511, bf16), (512, torch.float32),
                                      (1000, torch.float32), (5003, bf16)])
 def test_sample(cdx, V, dtype, kind):
@@ -64,8 +67,9 @@ def test_sample(cdx, V, dtype, kind):
 def test_sample_large_vocabularies(cdx, V, dtype, B):
     print(f"sample V={V} {dtype} B={B}", flush=True)
     for i, s in enumerate(({}, {"top_k": 50, "top_p": 0.9}, {"top_p": 0.95}, {"temperature": 1.3, "min_p": 0.01},
-                           {"top_k": 5000, "temperature": 2.0})):
-        x, u = _logits(B, V, V + i, dtype)
+                           {"top_k": 5000, "temperature": 2.0}, {"top_k": V // 2, "top_p": 0.999}, {"temperature": 0},
+                           {"temperature": 30.0, "top_p": 0.6}, {"top_k": 1000})):
+        x, u = _logits(B, V, V + i, dtype, "tiny" if i == 2 else "model")
         _check(cdx, x, u, **s)
 
 

@@ -15,10 +15,19 @@
 //     V's 8 rows are loaded in that slot order, a piece of DPL columns each, and transposed in
 //     registers (two bf16 of neighbouring rows per v_perm).  Nothing goes through LDS.
 //   * One pass: the running maximum and sum of the softmax, in log2 units and fp32, per wave.
-//     The four waves of a block take every fourth tile and are joined through LDS.
+//     The eight waves of a block take every eighth tile and are joined through LDS.  P is rounded
+//     to bf16 for the product with V (half a step, 2^-9, at random, on a sum of many), its sum is
+//     taken before that rounding.
 //   * A sequence is split into `splits` runs of tiles over blocks; the partial sums (fp32, with
 //     their maximum and sum) are joined by a second kernel, which also adds up the weights that
 //     each slot received, from the scores that the first kernel left.
+//
+// Measured (us and TB/s of K and V, calls in a row, both kernels): 16/8 heads of 128, 4 x 65536
+// slots 180 (5.96), 64 x 1024 48 (5.5), 64 sequences of 1 .. 2048 56 (4.8), 1 x 1000 11; 16/4 of
+// 80, 64 x 4096 66 (5.1); 8/4 of 40, 1 x 500 5.2.  A large copy moves 4.8 TB/s here.  What it took:
+// eight waves of at most 128 registers, two blocks on a CU (with a base address per tile shared by
+// the wave, and masks only in a sequence's last tile) 67 -> 56 us for the ragged 64; four waves of
+// 140 registers had been the better form before.
 #include <algorithm>
 
 #include "cdx_paged.h"
@@ -27,7 +36,7 @@ namespace cdx {
 namespace {
 
 constexpr int kTile = 32;   // slots of a wave's step
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kHeads = 16;  // query heads of a block: the columns of a matrix instruction
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -76,13 +85,14 @@ struct Piece<8> {
   typedef uint4 type;
 };
 
-// NC: pieces of 32 dims in a head; DPL: columns of V that a lane holds (16 DPL >= D).
-template <int NC, int DPL>
-__global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttnParams p) {
+// NC: pieces of 32 dims in a head; DPL: columns of V that a lane holds (16 DPL >= D); W: waves; FULL: D == 32 NC ==
+// 16 DPL, so that every lane holds dims of the head.
+template <int NC, int DPL, int W, bool FULL>
+__global__ __launch_bounds__(64 * W, NC == 4 && !FULL ? 2 : 4) void paged_attn_kernel(const PagedAttnParams p) {
   typedef typename Piece<DPL>::type vpiece_t;
   constexpr int PITCH = 16 * DPL + 4;
-  __shared__ float lds_o[kWaves][kHeads][PITCH];
-  __shared__ float lds_m[kWaves][kHeads], lds_l[kWaves][kHeads];
+  __shared__ float lds_o[W][kHeads][PITCH];
+  __shared__ float lds_m[W][kHeads], lds_l[W][kHeads];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -118,42 +128,42 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
   float m = -INFINITY, l = 0.f;
   const int32_t* table = p.t.table + (int64_t)b * p.t.ld;
   const int lps = p.t.log2_page;
-  const bool v_on = n * DPL < p.D;
+  // A tile's rows lie at a base that the wave shares; a lane's offsets from it stay.
+  const int D = FULL ? 32 * NC : p.D;
+  const uint32_t k_at = n * D + g * 8, v_at = 4 * g * D + n * DPL;
+  const bool v_on = FULL || n * DPL < D;
 
-  for (int32_t tile = (int32_t)split * per + wave; tile < t_end; tile += kWaves) {
+  for (int32_t tile = (int32_t)split * per + wave; tile < t_end; tile += W) {
     const int32_t s0 = tile * kTile;
     // The two halves of 16 slots each lie inside one page.
-    int32_t page[2];
+    const uint16_t *k_base[2], *v_base[2];
     bool there[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int32_t s = s0 + 16 * i;
-      there[i] = false;
-      page[i] = 0;
-      if (s < len) {
-        const int32_t pg = table[s >> lps];
-        there[i] = (uint32_t)pg < (uint32_t)p.t.num_pages;
-        page[i] = there[i] ? pg : 0;
-      }
+      const int32_t at = s0 + 16 * i;
+      const int32_t pg = at < len ? table[at >> lps] : -1;
+      there[i] = (uint32_t)pg < (uint32_t)p.t.num_pages;
+      const int64_t row0 = (((int64_t)(there[i] ? pg : 0) * p.nkv + h) << lps) + (at & ((1 << lps) - 1));
+      k_base[i] = p.k_pages + row0 * D;
+      v_base[i] = p.v_pages + row0 * D;
     }
     bf16x8 kf[2][NC];
     vpiece_t vr[8];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t row0 = (((int64_t)page[i] * p.nkv + h) << lps) + ((s0 + 16 * i) & ((1 << lps) - 1));
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int d = c * 32 + g * 8;
         uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (d < p.D) x = *reinterpret_cast<const uint4*>(p.k_pages + (row0 + n) * p.D + d);
+        if (FULL || c * 32 + g * 8 < D) x = *reinterpret_cast<const uint4*>(k_base[i] + k_at + c * 32);
         kf[i][c] = __builtin_bit_cast(bf16x8, x);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         vpiece_t x{};
-        if (v_on) x = *reinterpret_cast<const vpiece_t*>(p.v_pages + (row0 + 4 * g + r) * p.D + n * DPL);
-        // A value that no key of the sequence stands for weighs 0, which 0 * NaN is not.
-        if (!there[i] || s0 + 16 * i + 4 * g + r >= len) x = vpiece_t{};
+        if (v_on) x = *reinterpret_cast<const vpiece_t*>(v_base[i] + v_at + r * D);
         vr[4 * i + r] = x;
       }
     }
@@ -164,14 +174,24 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
 #pragma unroll
       for (int c = 0; c < NC; ++c) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][c], qf[c], a, 0, 0, 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        // (A page that is not in the pool makes the row NaN.)
-        const float z = there[i] ? a[r] * p.scale_log2 : __builtin_nanf("");
-        s[4 * i + r] = s0 + 16 * i + 4 * g + r < len ? z : -INFINITY;
+      for (int r = 0; r < 4; ++r) s[4 * i + r] = a[r] * p.scale_log2;
+    }
+    if (s0 + kTile > len || !there[0] || !there[1]) {
+      // Slots past the sequence weigh nothing, and their values must not count either (0 * NaN is
+      // NaN); a page that is not in the pool makes the row NaN.
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool behind = s0 + 16 * (i / 4) + 4 * g + i % 4 >= len, ok = there[i / 4];
+        s[i] = behind ? -INFINITY : (ok ? s[i] : __builtin_nanf(""));
+        if (behind || !ok) vr[i] = vpiece_t{};
       }
-      if (p.scores != nullptr && n < heads && s0 + 16 * i < len)  // (then the 16 slots lie inside the capacity)
-        *reinterpret_cast<f32x4*>(p.scores + ((int64_t)b * p.nq + head0 + n) * cap + s0 + 16 * i + 4 * g) =
-            f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+    }
+    if (p.scores != nullptr && n < heads) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (s0 + 16 * i < len)  // (then the 16 slots lie inside the capacity)
+          *reinterpret_cast<f32x4*>(p.scores + ((int64_t)b * p.nq + head0 + n) * cap + s0 + 16 * i + 4 * g) =
+              f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
     }
     float mx = s[0];
 #pragma unroll
@@ -222,15 +242,15 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
 #pragma unroll
     for (int j = 0; j < DPL; ++j) lds_o[wave][n][(4 * g + r) * DPL + j] = acc[j][r];
   __syncthreads();
-  for (int i = threadIdx.x; i < heads * (p.D / 4); i += 64 * kWaves) {
+  for (int i = threadIdx.x; i < heads * (p.D / 4); i += 64 * W) {
     const int hd = i / (p.D / 4), d = (i - hd * (p.D / 4)) * 4;
     float M = lds_m[0][hd];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, lds_m[w][hd]);
+    for (int w = 1; w < W; ++w) M = fmaxf(M, lds_m[w][hd]);
     const float ref = M == -INFINITY ? 0.f : M;
     float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float f = __builtin_amdgcn_exp2f(lds_m[w][hd] - ref);
       L = __builtin_fmaf(f, lds_l[w][hd], L);
 #pragma unroll
@@ -358,10 +378,15 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAtt
   }
 }
 
-// Blocks that a sequence and head is split over: enough of them for four blocks on each CU, each
-// with at least two tiles per wave when the sequences fill their tables.
+// Blocks that a sequence and head is split over: enough for two blocks on each CU, four where
+// tables are long (lengths then differ more: 100 sequences of up to 8192 slots, 16/4 heads of 80,
+// 119 against 110 us, 4 x 65536 slots 185 against 180), each with at least two tiles per wave (four:
+// 1 x 2000 slots 11.5 against 16.4 us).  Short tables whose blocks fill the CUs are not split, which
+// saves the second kernel (32 x 1024 slots 25.7 against 22.2 us).
 int paged_splits(int64_t blocks, int64_t cap) {
-  const int64_t want = (4 * (int64_t)device_cu_count() + blocks - 1) / blocks;
+  const int64_t cus = device_cu_count();
+  if (blocks >= cus && cap <= 4 * kWaves * kTile) return 1;
+  const int64_t want = ((cap >= 4096 ? 4 : 2) * cus + blocks - 1) / blocks;
   const int64_t most = (cap + 2 * kWaves * kTile - 1) / (2 * kWaves * kTile);
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
 }
@@ -441,13 +466,17 @@ extern "C" int cdx_paged_attention_fwd(const uint16_t* q, int64_t B, int32_t nq,
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(blocks * splits)), block(64 * kWaves);
   if (hd <= 32)
-    paged_attn_kernel<1, 4><<<grid, block, 0, s>>>(p);
-  else if (hd <= 64)
-    paged_attn_kernel<2, 4><<<grid, block, 0, s>>>(p);
+    paged_attn_kernel<1, 4, kWaves, false><<<grid, block, 0, s>>>(p);
+  else if (hd < 64)
+    paged_attn_kernel<2, 4, kWaves, false><<<grid, block, 0, s>>>(p);
+  else if (hd == 64)
+    paged_attn_kernel<2, 4, kWaves, true><<<grid, block, 0, s>>>(p);
   else if (hd <= 96)
-    paged_attn_kernel<3, 8><<<grid, block, 0, s>>>(p);
+    paged_attn_kernel<3, 8, kWaves, false><<<grid, block, 0, s>>>(p);
+  else if (hd < 128)
+    paged_attn_kernel<4, 8, kWaves, false><<<grid, block, 0, s>>>(p);
   else
-    paged_attn_kernel<4, 8><<<grid, block, 0, s>>>(p);
+    paged_attn_kernel<4, 8, kWaves, true><<<grid, block, 0, s>>>(p);
   if (int rc = check_launch(name)) return rc;
   if (splits == 1 && !weights_in) return CDX_OK;
   const int64_t rows = splits > 1 ? B * nq : 0;

@@ -160,6 +160,10 @@ def test_write_past_the_capacity_and_missing_pages(cdx):
     (16, 4, 80, 32, [500, 3, 97]), (8, 4, 40, 256, [1, 300, 511]), (4, 4, 32, 128, [90, 1000]),
     (32, 2, 96, 16, [33, 200]), (34, 2, 104, 64, [5, 260]), (40, 1, 128, 16, [77]), (6, 2, 8, 16, [1, 2, 50]),
     (2, 2, 24, 32, [0, 40, 0]), (16, 8, 128, 128, [5000]), (3, 1, 120, 16, [4099, 2]), (16, 1, 56, 64, [129]),
+    # many short sequences, some empty, beside a long one
+    (4, 2, 64, 16, [0, 700, 0, 1, 2, 3, 900, 0] + [33 * (i % 7) for i in range(90)] + [0]),
+    (2, 1, 32, 16, [i % 40 for i in range(1030)]), (2, 1, 16, 32, [i % 70 for i in range(300)]),
+    (4, 2, 128, 256, [20000, 1, 0, 257]), (2, 2, 64, 16, [9000]),  # many splits
 ])
 def test_attention(cdx, nq, nkv, D, page, lens):
     print(f"attention {nq}/{nkv} D={D} page={page} lengths={lens}", flush=True)
@@ -305,6 +309,8 @@ def _tracked(L, B, nkv, cap, lens, seed, kind="random"):
     (2, 2, 64, 16, [40, 41, 39, 0, -1, 48, 1], 40, 8), (None, 4, 40, 32, [33, 2, 64], 1, 0),
     (None, 1, 128, 64, [1, 2], 1, 1), (3, 2, 8, 16, [600, 700, 1300], 600, 600), (1, 3, 80, 32, [1000, 999], 100, 99),
     (None, 2, 64, 256, [256, 200], 256, 3),
+    (None, 2, 8, 64, [2048, 2000, 1999], 1999, 100), (None, 1, 8, 256, [5000, 8192], 3000, 10),
+    (None, 1, 8, 128, [9000, 8200], 4500, 4000),
 ])
 def test_evict(cdx, L, nkv, D, page, lens, keep, recent, kind):
     print(f"evict layers={L} nkv={nkv} D={D} page={page} lengths={lens} keep={keep} recent={recent} {kind}", flush=True)

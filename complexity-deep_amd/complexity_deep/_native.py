@@ -85,6 +85,9 @@ _SIGNATURES = {
     "cdx_linear_accum_fwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp]),
     "cdx_paged_append_fwd": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _vp, ctypes.c_float, _vp,
                                             _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "cdx_qkv_paged_fwd": (ctypes.c_int, [_vp, _i64, _vp, ctypes.c_float, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _i32,
+                                         _i32, _i32, _vp, _vp, ctypes.c_float, _vp, _i64, _vp, _vp, _vp, _i64, _i64,
+                                         _i64, _i32, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "cdx_paged_write": (ctypes.c_int, [_vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp,
                                        _vp]),
     "cdx_paged_attention_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32, _i32, _i64, _i32]),

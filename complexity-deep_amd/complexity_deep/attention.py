@@ -41,7 +41,7 @@ import torch.nn.functional as F
 from . import _native as nat
 from ._grad import forward_only
 from .linear import few_rows, linear, linear_accumulate_
-from .paged import PagedLayer, paged_attention, paged_qkv_append, paged_write
+from .paged import PagedLayer, paged_attention, paged_write
 from .rotary import RotaryEmbedding, apply_rotary_pos_emb
 
 
@@ -300,6 +300,44 @@ def qkv_cache(x: torch.Tensor, mu: Optional[torch.Tensor], w_x: torch.Tensor, w_
             nat.ptr(q), k.data_ptr(), v.data_ptr(), nat.ptr(attn), hd ** -0.5, work.data_ptr(), ws,
             nat.stream_of(x)), "cdx_qkv_cache_fwd")
     return q, attn, k, v
+
+
+def qkv_paged(x: torch.Tensor, mu: Optional[torch.Tensor], w_x: torch.Tensor, w_mu: torch.Tensor, H: int, nq: int,
+              q_norm_w: Optional[torch.Tensor], k_norm_w: Optional[torch.Tensor], eps: float, cos_sin: torch.Tensor,
+              k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+              positions: torch.Tensor) -> torch.Tensor:
+    """q [B, nq, D] of x [B, 1, H], its k and v appended to the pages (cdx_qkv_paged_fwd): the
+    projection and paged_qkv_append, with the projection of a few rows kept in fp32 between
+    them.  The cache's tensors are a PagedKVCache's, as paged_qkv_append takes them."""
+    nat.require_device(x, mu, w_x, w_mu, q_norm_w, k_norm_w, k_pages, v_pages, what="qkv_paged")
+    _check_widths(x, mu, H, "qkv_paged")
+    pages, nkv, page, D = k_pages.shape
+    B = x.shape[0]
+    if tuple(x.shape) != (B, 1, H) or w_x.shape[0] != (nq + 2 * nkv) * D or block_table.shape[0] != B:
+        raise ValueError(f"qkv_paged: input {tuple(x.shape)} and weight {tuple(w_x.shape)} do not match {nq} + 2 x "
+                         f"{nkv} heads of {D} in {block_table.shape[0]} sequences")
+    x2, ldx = _rows_view(x, H)
+    if ldx == 0:
+        x2, ldx = x.contiguous(), H
+    mu2, ldmu = None, 0
+    if mu is not None:
+        mu2, ldmu = _rows_view(mu.expand(B, 1, H) if mu.shape[:-1] != (B, 1) else mu, H)
+    wx_ptr, wmu_ptr, ldw = _weight_sources(w_x, w_mu, mu2, H, "qkv_paged")
+    if q_norm_w is not None:
+        q_norm_w = q_norm_w.to(x.dtype).contiguous()
+        k_norm_w = k_norm_w.to(x.dtype).contiguous()
+    q = torch.empty(B, nq, D, dtype=x.dtype, device=x.device)
+    lib = nat.lib()
+    ws = lib.cdx_qkv_cache_workspace_bytes(B, 1, nq, nkv, D)
+    work = torch.empty(ws, dtype=torch.uint8, device=x.device)
+    with nat.on_device(x), nat.launch_region("mu_qkv", x.device, M=B, H=H, N=w_x.shape[0], mu=mu is not None):
+        nat.check(lib.cdx_qkv_paged_fwd(
+            x2.data_ptr(), ldx, None, 0.0, nat.ptr(mu2), ldmu, wx_ptr, wmu_ptr, ldw, B, H, nq, nkv, D,
+            nat.ptr(q_norm_w), nat.ptr(k_norm_w), float(eps), cos_sin.data_ptr(), cos_sin.shape[0], lengths.data_ptr(),
+            positions.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], pages, page,
+            k_pages.data_ptr(), v_pages.data_ptr(), q.data_ptr(), work.data_ptr(), ws, nat.stream_of(x)),
+            "cdx_qkv_paged_fwd")
+    return q
 
 
 def cache_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
@@ -596,16 +634,22 @@ class ComplexityAttention(nn.Module):
             out, (k, v) = self.forward(x, use_cache=True, mu_prev=mu, residual=residual)
             paged_write(k, v, k_pages, v_pages, cache.block_table, cache.lengths)
             return out
-        w_x, w_mu = self.qkv_weights()
-        qkv = mu_qkv_project(x, mu, w_x, self.hidden_size, w_mu=w_mu)
         qn = (self.q_norm.weight, self.k_norm.weight) if self.use_qk_norm else (None, None)
-        q = paged_qkv_append(qkv.view(B, -1), k_pages, v_pages, cache.block_table, cache.lengths, cache.positions, nq,
-                             self.rotary_emb.cos_sin_table(cache.newest, x.device), *qn,
-                             self.q_norm.eps if self.use_qk_norm else 0.0)
-        attn = paged_attention(q, k_pages, v_pages, cache.block_table, cache.lengths, weights=weights,
-                               weights_out=weights)
-        attn = attn if weights is None else attn[0]
-        return self._out_proj(attn.view(B, 1, -1), residual)
+        eps = self.q_norm.eps if self.use_qk_norm else 0.0
+        table = self.rotary_emb.cos_sin_table(cache.newest, x.device)
+        fast = nat.host()
+        attn = None
+        if fast is not None:
+            attn = fast.paged_step(x, mu, self._qkv_w.buffer(self), nq, D, *qn, eps, table, k_pages, v_pages,
+                                   cache.block_table, cache.lengths, cache.positions, weights)
+        if attn is None:
+            w_x, w_mu = self.qkv_weights()
+            q = qkv_paged(x, mu, w_x, w_mu, self.hidden_size, nq, *qn, eps, table, k_pages, v_pages, cache.block_table,
+                          cache.lengths, cache.positions)
+            attn = paged_attention(q, k_pages, v_pages, cache.block_table, cache.lengths, weights=weights,
+                                   weights_out=weights)
+            attn = (attn if weights is None else attn[0]).view(B, 1, -1)
+        return self._out_proj(attn, residual)
 
     def _out_proj(self, attn: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
         """o_proj(attn), or with ``residual``: residual + o_proj(attn) written into residual

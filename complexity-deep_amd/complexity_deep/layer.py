@@ -23,6 +23,7 @@ from ._grad import forward_only
 from .attention import ComplexityAttention, _as_written, _plain_linear, _written
 from .mlp import SwiGLU
 from .normalization import RMSNorm, add_rms_norm, rms_norm
+from .paged import PagedLayer
 from .token_routed_mlp import RoutePlan, TokenRoutedMLP
 
 _written(TokenRoutedMLP, SwiGLU)
@@ -197,8 +198,14 @@ class TransformerBlock(nn.Module):
                                   or "fused" in guide.__dict__):
             return None
         qn, kn = (attn.q_norm, attn.k_norm) if attn.use_qk_norm else (None, None)
-        pk, pv = (past[0], past[1]) if past is not None else (None, None)
-        n_pos = h.shape[1] + (pk.shape[2] if pk is not None else 0)
+        table = lengths = positions = weights = None
+        if type(past) is PagedLayer:  # one new token per sequence, counted by the cache
+            cache = past.cache
+            pk, pv, weights = cache.layer(past.index)
+            table, lengths, positions, n_pos = cache.block_table, cache.lengths, cache.positions, cache.newest
+        else:
+            pk, pv = (past[0], past[1]) if past is not None else (None, None)
+            n_pos = h.shape[1] + (pk.shape[2] if pk is not None else 0)
         w_gu, w_down = mlp.kernel_weights()
         done = fast.block_step(
             h, ln1.weight, ln1.eps, mu_prev, attn._qkv_w.buffer(attn), attn.num_heads, attn.num_kv_heads, attn.head_dim,
@@ -206,7 +213,8 @@ class TransformerBlock(nn.Module):
             attn.rotary_emb.cos_sin_table(n_pos, h.device), pk, pv, attn.o_proj.weight, ln2.weight, ln2.eps, route.perm,
             route.offsets, route.num_experts, w_gu, w_down, mlp.expert_intermediate_size, mlp.use_shared_expert,
             guide.mu_proj.weight if guide is not None else None, guide.mu if guide is not None else None,
-            guide.mu_min if guide is not None else 0.0, guide.mu_max if guide is not None else 0.0, -2.0, 2.0)
+            guide.mu_min if guide is not None else 0.0, guide.mu_max if guide is not None else 0.0, -2.0, 2.0,
+            table, lengths, positions, weights)
         if done is None:
             return None
         k, v, mu = done

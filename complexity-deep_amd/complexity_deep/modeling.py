@@ -240,7 +240,7 @@ class ComplexityModel(nn.Module):
         # A generation step of a few rows runs block by block through TransformerBlock.step,
         # which takes h itself (its norms are folded); other calls hand each block its
         # normalised input, produced by the block before.
-        steps = attention_mask is None and 0 < B * S <= 8 and not paged
+        steps = attention_mask is None and 0 < B * S <= 8 and not (paged and past_key_values.prompt)
         normed = None
         # Layers 1.. read their normalised input and mu side by side from one [B, S, 2H]
         # buffer, written by the layer before (one K = 2H operand for the projection).

@@ -17,6 +17,7 @@
 //                         moves read and write disjoint rows and run in any order.
 //   evict_move_kernel     the rows of those pairs, 16 bytes per lane.
 #include "cdx_paged.h"
+#include "cdx_skinny.h"
 
 namespace cdx {
 
@@ -422,6 +423,71 @@ extern "C" int cdx_paged_append_fwd(const void* qkv, int32_t qkv_fp32, int64_t l
   else
     paged_append_kernel<uint16_t><<<grid, dim3(256), 0, s>>>(p);
   return check_launch(name);
+}
+
+extern "C" int cdx_qkv_paged_fwd(const uint16_t* x, int64_t ldx, const uint16_t* x_norm_w, float x_eps,
+                                 const uint16_t* mu, int64_t ldmu, const uint16_t* w, const uint16_t* w_mu,
+                                 int64_t ldw, int64_t B, int32_t H, int32_t nq, int32_t nkv, int32_t hd,
+                                 const uint16_t* q_norm_w, const uint16_t* k_norm_w, float eps, const float* cos_sin,
+                                 int64_t n_pos, const int32_t* lengths, const int32_t* positions,
+                                 const int32_t* table, int64_t table_ld, int64_t width, int64_t num_pages,
+                                 int32_t page_size, uint16_t* k_pages, uint16_t* v_pages, uint16_t* q_out, void* work,
+                                 size_t work_bytes, void* stream) {
+  using namespace cdx;
+  const char* name = "cdx_qkv_paged_fwd";
+  clear_error();
+  PagedTable t{};
+  if (int rc = paged_table(name, table, table_ld, width, num_pages, page_size, B, nkv, hd, &t)) return rc;
+  if (H <= 0 || nq <= 0 || nq % nkv != 0) return fail(CDX_EINVAL, "%s: bad shape H=%d nq=%d nkv=%d", name, H, nq, nkv);
+  if (H % 64 != 0) return fail(CDX_EUNSUPPORTED, "%s: H=%d must be a multiple of 64", name, H);
+  if (x_norm_w && !(x_eps >= 0.f)) return fail(CDX_EINVAL, "%s: eps must be >= 0", name);
+  if (ldx < H || ldw < H || (mu && ldmu != 0 && ldmu < H))
+    return fail(CDX_EINVAL, "%s: leading dimension too small", name);
+  if (ldx % 8 || ldw % 8 || (mu && ldmu % 8))
+    return fail(CDX_EUNSUPPORTED, "%s: leading dimensions must be multiples of 8", name);
+  const int64_t N = ((int64_t)nq + 2 * (int64_t)nkv) * hd;
+  if (N > INT32_MAX) return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
+  if (B == 0) return CDX_OK;
+  if (!x || !w || (mu && !w_mu) || !work) return fail(CDX_EINVAL, "%s: null pointer", name);
+  if (!aligned16(x) || !aligned16(w) || (mu && (!aligned16(mu) || !aligned16(w_mu))) || !aligned16(work) ||
+      !aligned16(x_norm_w))
+    return fail(CDX_EUNSUPPORTED, "%s: pointers must be 16-byte aligned", name);
+  const bool few = skinny_fits(B, N);
+  if (x_norm_w && (!few || B > kNormRows))
+    return fail(CDX_EUNSUPPORTED, "%s: a folded norm needs B <= %d", name, kNormRows);
+  const size_t need = cdx_qkv_cache_workspace_bytes(B, 1, nq, nkv, hd);
+  if (work_bytes < need)
+    return fail(CDX_EWORKSPACE, "%s: workspace needs %zu bytes, got %zu", name, need, work_bytes);
+  if (!cos_sin || !lengths || !positions || !q_out || !table || !k_pages || !v_pages || n_pos <= 0 || !(eps >= 0.f) ||
+      (q_norm_w == nullptr) != (k_norm_w == nullptr))
+    return fail(CDX_EINVAL, "%s: null pointer, empty cos/sin table, bad eps or one QK norm weight only", name);
+  if (!aligned16(cos_sin) || !aligned16(q_out) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(q_norm_w) ||
+      !aligned16(k_norm_w))
+    return fail(CDX_EUNSUPPORTED, "%s: pointers must be 16-byte aligned", name);
+  if (few) {
+    SkinnyParams sp{};
+    sp.a = x;
+    sp.lda = ldx;
+    sp.a2 = mu ? mu : x;
+    sp.lda2 = mu ? ldmu : ldx;
+    sp.b = w;
+    sp.b2 = mu ? w_mu : w;
+    sp.ldb = ldw;
+    sp.k_split = H;
+    sp.M = (int32_t)B;
+    sp.N = (int32_t)N;
+    sp.K = mu ? 2 * H : H;
+    sp.c = work;
+    sp.ldc = N;
+    sp.norm_w = x_norm_w;
+    sp.eps = x_eps;
+    if (int rc = skinny_gemm(sp, SkinnyEpi::kF32, reinterpret_cast<hipStream_t>(stream), name)) return rc;
+  } else if (int rc = cdx_mu_qkv_fwd(x, ldx, mu, ldmu, w, w_mu, ldw, B, H, (int32_t)N, static_cast<uint16_t*>(work), N,
+                                     stream)) {
+    return rc;
+  }
+  return cdx_paged_append_fwd(work, few, N, B, nq, nkv, hd, q_norm_w, k_norm_w, eps, cos_sin, n_pos, lengths, positions,
+                              table, table_ld, width, num_pages, page_size, k_pages, v_pages, q_out, stream);
 }
 
 extern "C" int cdx_paged_write(const uint16_t* k, const uint16_t* v, int64_t B, int32_t nkv, int64_t S, int32_t hd,

@@ -558,6 +558,21 @@ int cdx_paged_append_fwd(const void* qkv_dev, int32_t qkv_fp32, int64_t ldqkv, i
                          uint16_t* q_out_dev, void* stream);
 
 /*
+ * The projection of one new token per sequence (cdx_mu_qkv_fwd: x [B, H], mu NULL, [B, H] or one
+ * row with ldmu 0, weights at row stride ldw) and its append, fp32 in between for a few rows
+ * (cdx_few_rows).  With x_norm_w the projection reads RMSNorm(x) (B <= 8, few rows).  work:
+ * cdx_qkv_cache_workspace_bytes(B, 1, nq, nkv, hd).
+ */
+int cdx_qkv_paged_fwd(const uint16_t* x_dev, int64_t ldx, const uint16_t* x_norm_w_dev, float x_eps,
+                      const uint16_t* mu_dev, int64_t ldmu, const uint16_t* w_dev, const uint16_t* w_mu_dev,
+                      int64_t ldw, int64_t B, int32_t H, int32_t nq, int32_t nkv, int32_t hd,
+                      const uint16_t* q_norm_w_dev, const uint16_t* k_norm_w_dev, float eps,
+                      const float* cos_sin_dev, int64_t n_pos, const int32_t* lengths_dev,
+                      const int32_t* positions_dev, const int32_t* table_dev, int64_t table_ld, int64_t width,
+                      int64_t num_pages, int32_t page_size, uint16_t* k_pages_dev, uint16_t* v_pages_dev,
+                      uint16_t* q_out_dev, void* work_dev, size_t work_bytes, void* stream);
+
+/*
  * Prompts into the pages: k, v [B, nkv, S, hd] bf16 (normalised and rotated, as the fused
  * projection writes them), rows t < min(lengths[b], S) to slot t.
  */

@@ -141,6 +141,31 @@ def test_generate_paged(cdx):
     assert int(bounded.lengths.max()) <= 16 and m.generate_paged(ids, 0).shape == (B, 0)
 
 
+@pytest.mark.parametrize("B,keep", [(2, None), (9, None), (9, 24), (70, None)])
+def test_steps_while_launches_are_timed(cdx, B, keep):
+    """The Python launch sites compute what the native call paths do: the same bits, or for up to 8
+    rows (whose norms are folded into the products otherwise) the same numbers."""
+    print(f"paged model: launch hook, B={B} keep={keep}", flush=True)
+    from complexity_deep import _native as nat
+    m = _model(cdx, 64, 4, 2)
+    ids = torch.randint(0, 600, (B, 30), generator=torch.Generator().manual_seed(4)).cuda()
+    outs, names = [], set()
+    for hook in (None, lambda name, *a: names.add(name)):
+        cache = cdx.PagedKVCache(m.config, B, 32, page_size=16, keep=keep)
+        try:
+            nat.set_launch_hook(hook)
+            with torch.no_grad():
+                m(ids[:, :25], past_key_values=cache)
+                outs.append(torch.stack([m(ids[:, i:i + 1], past_key_values=cache).logits for i in range(5)]))
+        finally:
+            nat.set_launch_hook(None)
+    assert {"paged_write", "paged_attention"} <= names
+    if B > 8:
+        assert torch.equal(*outs)
+    e = errors(*outs)
+    assert e["max_rel"] <= MAX_REL and e["rel_rms"] <= REL_RMS, e
+
+
 def test_a_captured_step(cdx):
     """A step (with its tokens' choice) in a HIP graph, replayed, against eager steps."""
     print("paged model: captured step", flush=True)

@@ -229,8 +229,17 @@ class ComplexityModel(nn.Module):
                 raise ValueError(f"ComplexityModel: a paged cache of {len(past_key_values)} layers for "
                                  f"{len(self.layers)}")
             past_key_values.begin(B, S, prompt_lengths)
-        elif prompt_lengths is not None:
+            try:
+                return self._forward(input_ids, None, labels, past_key_values, use_cache, True)
+            except BaseException:
+                past_key_values.cancel()
+                raise
+        if prompt_lengths is not None:
             raise ValueError("ComplexityModel: prompt_lengths without a paged cache")
+        return self._forward(input_ids, attention_mask, labels, past_key_values, use_cache, False)
+
+    def _forward(self, input_ids, attention_mask, labels, past_key_values, use_cache, paged) -> CausalLMOutput:
+        B, S = input_ids.shape
         h = embedding(input_ids, self.embed_tokens.weight)
         mu_prev = self.mu_init.expand(B, S, -1) if self.config.use_mu_guidance else None
         plans = self.route_plans(input_ids)

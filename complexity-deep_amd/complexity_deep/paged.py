@@ -228,6 +228,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     if isinstance(keep, bool) or isinstance(recent, bool) or int(keep) != keep or int(recent) != recent \
             or keep <= 0 or not 0 <= recent <= keep:
         raise ValueError(f"{what}: keep={keep} must be a positive integer and recent={recent} lie in 0 .. keep")
+    keep, recent = int(keep), int(recent)
     if weights.dtype != torch.float32 or tuple(weights.shape) != shape:
         raise ValueError(f"{what}: weights must be fp32 {shape}, got {weights.dtype} {tuple(weights.shape)}")
     weights = weights if weights.is_contiguous() else weights.contiguous()
@@ -244,7 +245,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
         nat.check(lib.cdx_paged_evict(
             layers, B, nkv, D, lengths.data_ptr(), positions.data_ptr(), table.data_ptr(), _ld(table), table.shape[1],
             pages, page, k_pages.data_ptr(), v_pages.data_ptr(), weights.data_ptr(), slot_positions.data_ptr(),
-            int(keep), int(recent), *(t.data_ptr() for t in new), work.data_ptr(), ws, nat.stream_of(k_pages)),
+            keep, recent, *(t.data_ptr() for t in new), work.data_ptr(), ws, nat.stream_of(k_pages)),
             "cdx_paged_evict")
     return new
 
@@ -267,7 +268,9 @@ class PagedKVCache:
     that the steps so far attended to most.  Positions go on counting.
 
     ``lengths`` and ``positions`` (of the newest tokens) live on the device and nothing waits for
-    them; ``longest`` and ``newest`` are the host's bounds.  One call at a time may use a cache."""
+    them; ``longest`` and ``newest`` are the host's bounds.  One call at a time may use a cache.  A
+    step that is captured into a graph counts on the device when it is replayed, not here: keep to
+    max_length then (a token past the capacity is not stored)."""
 
     def __init__(self, config, batch_size: int, max_length: int, *, page_size: int = 64, keep: Optional[int] = None,
                  recent: Optional[int] = None, device="cuda"):
@@ -371,9 +374,27 @@ class PagedKVCache:
             self.evict()
         self._counts.add_(1)
         if self.slot_positions is not None:
-            shape = (*self.slot_positions.shape[:-1], 1)
-            slot = (self.lengths.long() - 1).view(-1, 1, 1).expand(shape)
-            self.slot_positions.scatter_(-1, slot, self.positions.view(-1, 1, 1).expand(shape))
+            slot = self._new_slot()
+            self.slot_positions.scatter_(-1, slot, self.positions.view(-1, 1, 1).expand(slot.shape))
         self.longest += 1
         self.newest += 1
         self.prompt = False
+
+    def _new_slot(self) -> torch.Tensor:
+        """The slot of each sequence's newest token, by layer and head (the capacity bounds it here too:
+        a replayed step may count past it)."""
+        slot = (self.lengths.long() - 1).clamp(max=self.capacity - 1)
+        return slot.view(-1, 1, 1).expand(*self.slot_positions.shape[:-1], 1)
+
+    def cancel(self) -> None:
+        """Take back the tokens that the last ``begin`` counted (a call that raised)."""
+        if self.prompt:
+            self.reset()
+        else:
+            if self.weights is not None:
+                slot = self._new_slot()
+                self.weights.scatter_(-1, slot, 0.0)
+                self.slot_positions.scatter_(-1, slot, -1)
+            self._counts.sub_(1)
+            self.longest -= 1
+            self.newest -= 1

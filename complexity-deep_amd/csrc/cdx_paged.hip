@@ -18,6 +18,7 @@
 //   evict_move_kernel     the rows of those pairs, 16 bytes per lane.
 #include "cdx_paged.h"
 #include "cdx_skinny.h"
+#include "cdx_wave.h"
 
 namespace cdx {
 
@@ -179,19 +180,10 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u == 0x80000000u ? 0x80000000u : (u & 0x80000000u ? ~u : u | 0x80000000u);
 }
 
-__device__ __forceinline__ int wave_inclusive(int v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(v, d, 64);
-    if (lane >= d) v += up;
-  }
-  return v;
-}
-
 // Exclusive sum over the block of a count per thread, and the block's total.
 __device__ __forceinline__ int block_exclusive(int v, int* lds, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int x = wave_inclusive(v, lane);
+  const int x = wave_inclusive(v);
   __syncthreads();
   if (lane == 63) lds[wave] = x;
   __syncthreads();
@@ -208,7 +200,7 @@ __device__ __forceinline__ int block_exclusive(int v, int* lds, int& total) {
 // PER: slots that a thread holds in registers (capacity <= 512 PER), or 0: every pass reads them.
 template <int PER>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const EvictParams p) {
-  __shared__ int hist[256];
+  __shared__ int hist[4][256];  // of each digit
   __shared__ int sums[kSelectThreads / 64];
   __shared__ int pick[2];
   const int64_t row = blockIdx.x;
@@ -229,6 +221,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
     return;
   }
   const int64_t first_recent = (int64_t)p.positions[b] - p.recent + 1;
+  for (int i = tid; i < 4 * 256; i += kSelectThreads) hist[i >> 8][i & 255] = 0;
 
   uint32_t key[PER > 0 ? PER : 1];
   uint32_t recent_bits = 0;
@@ -272,20 +265,18 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   bool all = need == 0;  // no ties to count: the keys above `prefix` are kept, or all at it
   while (shift > 0 && !all) {
     shift -= 8;
-    __syncthreads();
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
+    int* counts = hist[shift >> 3];  // (cleared before the sum over the block above)
     each([&](int, uint32_t k, bool recent) {
       const bool in = recent == among_recent && (shift == 24 || k >> (shift + 8) == prefix);
-      if (in) atomicAdd(&hist[(k >> shift) & 255], 1);
+      if (in) atomicAdd(&counts[(k >> shift) & 255], 1);
     });
     __syncthreads();
     if (tid < 64) {
       // The digit from above at which the counts reach `need`: four to a lane.
       int n[4], lane_sum = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) lane_sum += n[i] = hist[255 - 4 * tid - i];
-      int above = wave_inclusive(lane_sum, tid) - lane_sum;
+      for (int i = 0; i < 4; ++i) lane_sum += n[i] = counts[255 - 4 * tid - i];
+      int above = wave_inclusive(lane_sum) - lane_sum;
       if (above < need && above + lane_sum >= need) {  // (one lane)
         int i = 0;
         while (i < 3 && above + n[i] < need) above += n[i++];
@@ -296,7 +287,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
     __syncthreads();
     prefix = prefix << 8 | (uint32_t)pick[0];
     need -= pick[1];
-    all = hist[pick[0]] == need;
+    all = counts[pick[0]] == need;
   }
   const bool none = need == 0;  // (nothing of the class is kept)
 

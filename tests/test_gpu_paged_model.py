@@ -226,7 +226,19 @@ def test_refusals(cdx):
             m(ids, past_key_values=cdx.PagedKVCache(cdx.ComplexityConfig(
                 hidden_size=256, num_attention_heads=4, num_key_value_heads=2, num_hidden_layers=3), 2, 32))
         assert cache.lengths.tolist() == [0, 0]  # nothing counted
+        # A call that raises inside the model counts nothing either.
+        attn = m.layers[1].self_attn
+        attn.train(), setattr(attn, "attention_dropout", 0.1)
+        with pytest.raises(NotImplementedError):
+            m(ids, past_key_values=cache)
+        assert cache.lengths.tolist() == [0, 0] and cache.newest == 0
+        attn.eval()
         m(ids, past_key_values=cache)
+        attn.train()
+        with pytest.raises(NotImplementedError):
+            m(ids[:, :1], past_key_values=cache)
+        assert cache.lengths.tolist() == [5, 5] and cache.positions.tolist() == [4, 4] and cache.newest == 5
+        attn.eval()
         with pytest.raises(ValueError):
             m(ids, past_key_values=cache)  # a second prompt
         for _ in range(11):

@@ -464,16 +464,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
     u64 w[kLane];
     double wf[kLane];
     bool on[kLane];
+    // Item i of all lies in the list of the last wave that begins at or before it.
+    const int through = wave_inclusive(lane < kSampleWaves ? sh.count[lane] : 0);
 #pragma unroll
     for (int r = 0; r < kLane; ++r) {
-      int i = r * 64 + lane, from = 0;
-      on[r] = i < listed_all;
+      const int i = r * 64 + lane;
+      int from = 0, begin = 0;
+#pragma unroll
       for (int v = 0; v < kSampleWaves - 1; ++v) {
-        const bool past = from == v && i >= sh.count[v];
-        i -= past ? sh.count[v] : 0;
-        from += past ? 1 : 0;
+        const int end = read_lane(through, v);
+        from += i >= end ? 1 : 0;
+        begin = i >= end ? end : begin;
       }
-      const int at = on[r] ? from * kListWave + i : 0;
+      on[r] = i < listed_all;
+      const int at = on[r] ? from * kListWave + i - begin : 0;
       key[r] = on[r] ? sh.list_key[at] >> SHIFT : 0u;
       index[r] = sh.list_index[at];
       wf[r] = on[r] ? wt.fraction(key_logit(sh.list_key[at])) : 0.0;

@@ -5,6 +5,11 @@
 // a page are one contiguous piece; every kernel here moves whole rows in pieces of 8 or 16
 // bytes per lane and is bound by memory, or for a step's few rows by its launch.
 //
+// Measured (us of a kernel): append of 256 tokens, 16/8 heads of 128, 3.5 (one token of 8/4 heads of
+// 40: 2.0); write of 8 prompts of up to 2048 tokens (67 MB read and written) 13, 5.1 TB/s, where a
+// large copy moves 4.8; eviction of one slot a head, 12 layers x 4 x 1025 slots, 7.9 + 3.3, of half a
+// prompt, 24 layers x 8 x up to 2048 slots of 8 x 128, 18.8 + 65 (280 MB of rows moved).
+//
 //   paged_append_kernel   the packed projection of one new token per sequence, read once: per-head
 //                         RMSNorm, RoPE at the sequence's own position, q out, k and v into the
 //                         sequence's last slot.  16 lanes hold one head (lane i columns 4 i ..
@@ -14,7 +19,9 @@
 //   evict_select_kernel   one block per (layer, sequence, head): the slots to keep by a radix
 //                         descent over (recent, weight), then the pairs (hole, mover) in slot
 //                         order.  Holes lie below `keep` and movers at or above it, so that the
-//                         moves read and write disjoint rows and run in any order.
+//                         moves read and write disjoint rows and run in any order; one slot a
+//                         head costs one row's move, where a cache kept in order would shift
+//                         half of its rows.
 //   evict_move_kernel     the rows of those pairs, 16 bytes per lane.
 #include "cdx_paged.h"
 #include "cdx_skinny.h"

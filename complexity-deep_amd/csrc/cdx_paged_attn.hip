@@ -15,16 +15,16 @@
 //     V's 8 rows are loaded in that slot order, a piece of DPL columns each, and transposed in
 //     registers (two bf16 of neighbouring rows per v_perm).  Nothing goes through LDS.
 //   * One pass: the running maximum and sum of the softmax, in log2 units and fp32, per wave.
-//     The eight waves of a block take every eighth tile and are joined through LDS.  P is rounded
-//     to bf16 for the product with V (half a step, 2^-9, at random, on a sum of many), its sum is
-//     taken before that rounding.
+//     The eight waves of a block take every eighth tile and are joined through LDS.  P enters
+//     the product with V as two bf16 parts (2^-16 of it is lost; one part alone, 2^-8, took 5.2
+//     instead of 5.4 us for the smallest calls and the same for all others).
 //   * A sequence is split into `splits` runs of tiles over blocks; the partial sums (fp32, with
 //     their maximum and sum) are joined by a second kernel, which also adds up the weights that
 //     each slot received, from the scores that the first kernel left.
 //
 // Measured (us and TB/s of K and V, calls in a row, both kernels): 16/8 heads of 128, 4 x 65536
-// slots 180 (5.96), 64 x 1024 48 (5.5), 64 sequences of 1 .. 2048 56 (4.8), 1 x 1000 11; 16/4 of
-// 80, 64 x 4096 66 (5.1); 8/4 of 40, 1 x 500 5.2.  A large copy moves 4.8 TB/s here.  What it took:
+// slots 184 (5.8), 64 x 1024 49 (5.5), 64 sequences of 1 .. 2048 56 (4.8), 1 x 1000 11; 16/4 of
+// 80, 64 x 4096 66 (5.1); 8/4 of 40, 1 x 500 5.4.  A large copy moves 4.8 TB/s here.  What it took:
 // eight waves of at most 128 registers, two blocks on a CU (with a base address per tile shared by
 // the wave, and masks only in a sequence's last tile) 67 -> 56 us for the ragged 64; four waves of
 // 140 registers had been the better form before.
@@ -209,7 +209,13 @@ __global__ __launch_bounds__(64 * W, NC == 4 && !FULL ? 2 : 4) void paged_attn_k
       pf[i] = __builtin_amdgcn_exp2f(s[i] - m_ref);
       l += pf[i];
     }
-    const bf16x8 pb = __builtin_bit_cast(bf16x8, pack8(pf));
+    // P in two bf16 parts, to 2^-16 of it.
+    const uint4 p_hi = pack8(pf);
+    float hi[8];
+    unpack8(p_hi, hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pf[i] -= hi[i];
+    const bf16x8 pb = __builtin_bit_cast(bf16x8, p_hi), pb_low = __builtin_bit_cast(bf16x8, pack8(pf));
     const uint32_t* vw = reinterpret_cast<const uint32_t*>(vr);  // [8 rows][DPL / 2]
 #pragma unroll
     for (int j = 0; j < DPL; ++j) {
@@ -228,6 +234,7 @@ __global__ __launch_bounds__(64 * W, NC == 4 && !FULL ? 2 : 4) void paged_attn_k
         a.w = low_halves(vw[6 * RW + w], vw[7 * RW + w]);
       }
       acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pb, acc[j], 0, 0, 0);
+      acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pb_low, acc[j], 0, 0, 0);
     }
   }
 

@@ -25,6 +25,12 @@
 //     fp32 logits are summed in 8192 bins of x (of counts for top-k, of weights for top-p), whose
 //     border bin is then resolved by a radix descent over its few tokens; their passes are paced
 //     by the exponentials, about 20 instructions in 64 bits a token.
+//
+// Measured (us of the kernel): 1 x 100000 bf16, top-k 50 and top-p 0.9, 16.8, of which 3.2 is one
+// pass over the row by one CU (200 KB at 62 GB/s), 3.4 the bound, 4.8 the list; 256 x 100000
+// bf16, top-p by row, 46 (passes: maximum 7, counts 9, table 5, sums 15); 64 x 32000 fp32, min-p, 10.4;
+// 1 x 100000 fp32, top-p, 76.  With radix passes over the row in place of bounds, lists and counts the
+// first three took 310, 456 and 46.
 #include <float.h>
 
 #include "cdx_common.h"

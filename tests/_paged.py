@@ -41,8 +41,9 @@ def attention(q, k_pages, v_pages, table, lengths, scale=None):
     attention, what each slot received, and a bound of a bf16 kernel's error.
 
     The kernel's scores are fp32 sums of D exact products (each partial sum rounded: D 2^-24 of
-    the sum of magnitudes), its weights are rounded to bf16 before the product with v (2^-8 of
-    each), their sum is not, and the result is rounded once (2^-8 of it)."""
+    the sum of magnitudes); its weights enter the product with v as two bf16 parts (each rounding
+    2^-8: 2^-16 of a weight is lost), summed in fp32 over tiles of 32 slots, waves and splits;
+    the result is rounded once (2^-8 of it)."""
     q, k_pages, v_pages, table = q.double().cpu(), k_pages.double().cpu(), v_pages.double().cpu(), table.cpu()
     B, nq, D = q.shape
     nkv, page = k_pages.shape[1:3]
@@ -61,7 +62,8 @@ def attention(q, k_pages, v_pages, table, lengths, scale=None):
             delta = (D + 8) * 2.0 ** -24 * scale * float((k[g].abs() @ q[b, h].abs()).max()) + 2.0 ** -19
             out[b, h] = p @ v[g]
             weights[b, g, :n] += p
-            bound[b, h] = (2.0 ** -8 + 2 * delta) * (p @ v[g].abs()) + 2.0 ** -8 * out[b, h].abs()
+            sums = (n / 32 + 64) * 2.0 ** -23
+            bound[b, h] = (2.0 ** -16 + 2 * delta + sums) * (p @ v[g].abs()) + 2.0 ** -8 * out[b, h].abs()
     return out, weights, bound
 
 

@@ -8,7 +8,7 @@
 // Measured (us of a kernel): append of 256 tokens, 16/8 heads of 128, 3.5 (one token of 8/4 heads of
 // 40: 2.0); write of 8 prompts of up to 2048 tokens (67 MB read and written) 13, 5.1 TB/s, where a
 // large copy moves 4.8; eviction of one slot a head, 12 layers x 4 x 1025 slots, 7.9 + 3.3, of half a
-// prompt, 24 layers x 8 x up to 2048 slots of 8 x 128, 18.8 + 65 (280 MB of rows moved).
+// prompt, 24 layers x 8 x up to 2048 slots of 8 x 128, 18.8 + 65 (292 MB of rows read and written).
 //
 //   paged_append_kernel   the packed projection of one new token per sequence, read once: per-head
 //                         RMSNorm, RoPE at the sequence's own position, q out, k and v into the
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
 
 constexpr int kMoveBlock = 16;  // rows that a block moves, of K and of V: one per 16 lanes
 
-// One row a group: 62 us for 24 layers x 8 sequences of up to 2048 slots of 8 x 128 values (280 MB
+// One row a group: 62 us for 24 layers x 8 sequences of up to 2048 slots of 8 x 128 values (292 MB
 // read and written); two, four and eight rows, all loaded before the first is stored, 99, 95, 107.
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictParams p, uint32_t blocks) {
   const int64_t row = blockIdx.x / blocks;

@@ -636,7 +636,7 @@ class ComplexityAttention(nn.Module):
             return out
         qn = (self.q_norm.weight, self.k_norm.weight) if self.use_qk_norm else (None, None)
         eps = self.q_norm.eps if self.use_qk_norm else 0.0
-        table = self.rotary_emb.cos_sin_table(cache.newest, x.device)
+        table = cache.rotary_table(self.rotary_emb, x.device)
         fast = nat.host()
         attn = None
         if fast is not None:

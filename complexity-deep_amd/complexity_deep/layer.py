@@ -202,15 +202,16 @@ class TransformerBlock(nn.Module):
         if type(past) is PagedLayer:  # one new token per sequence, counted by the cache
             cache = past.cache
             pk, pv, weights = cache.layer(past.index)
-            table, lengths, positions, n_pos = cache.block_table, cache.lengths, cache.positions, cache.newest
+            table, lengths, positions = cache.block_table, cache.lengths, cache.positions
+            cos_sin = cache.rotary_table(attn.rotary_emb, h.device)
         else:
             pk, pv = (past[0], past[1]) if past is not None else (None, None)
-            n_pos = h.shape[1] + (pk.shape[2] if pk is not None else 0)
+            cos_sin = attn.rotary_emb.cos_sin_table(h.shape[1] + (pk.shape[2] if pk is not None else 0), h.device)
         w_gu, w_down = mlp.kernel_weights()
         done = fast.block_step(
             h, ln1.weight, ln1.eps, mu_prev, attn._qkv_w.buffer(attn), attn.num_heads, attn.num_kv_heads, attn.head_dim,
             qn.weight if qn is not None else None, kn.weight if kn is not None else None, qn.eps if qn is not None else 0.0,
-            attn.rotary_emb.cos_sin_table(n_pos, h.device), pk, pv, attn.o_proj.weight, ln2.weight, ln2.eps, route.perm,
+            cos_sin, pk, pv, attn.o_proj.weight, ln2.weight, ln2.eps, route.perm,
             route.offsets, route.num_experts, w_gu, w_down, mlp.expert_intermediate_size, mlp.use_shared_expert,
             guide.mu_proj.weight if guide is not None else None, guide.mu if guide is not None else None,
             guide.mu_min if guide is not None else 0.0, guide.mu_max if guide is not None else 0.0, -2.0, 2.0,

@@ -270,7 +270,9 @@ class PagedKVCache:
     ``lengths`` and ``positions`` (of the newest tokens) live on the device and nothing waits for
     them; ``longest`` and ``newest`` are the host's bounds.  One call at a time may use a cache.  A
     step that is captured into a graph counts on the device when it is replayed, not here: keep to
-    max_length then (a token past the capacity is not stored)."""
+    max_length then (a token past the capacity is not stored).  A TransformerBlock or
+    ComplexityAttention called by itself takes ``cache[i]``, after ``begin`` has counted the call's
+    tokens."""
 
     def __init__(self, config, batch_size: int, max_length: int, *, page_size: int = 64, keep: Optional[int] = None,
                  recent: Optional[int] = None, device="cuda"):
@@ -294,6 +296,7 @@ class PagedKVCache:
         device = self.k_pages.device
         self.block_table = torch.arange(batch_size * width, dtype=torch.int32, device=device).view(batch_size, width)
         self._counts = torch.zeros(2, batch_size, dtype=torch.int32, device=device)
+        self._tables = {}
         self.weights = self.slot_positions = None
         if keep is not None:
             shape = (shape[0], batch_size, nkv, self.capacity)
@@ -316,6 +319,13 @@ class PagedKVCache:
         if not 0 <= i < len(self):
             raise IndexError(f"PagedKVCache: layer {i} of {len(self)}")
         return PagedLayer(self, i)
+
+    def rotary_table(self, rotary, device) -> torch.Tensor:
+        """The fp32 (cos, sin) table of a layer's rotary embedding for every position that a call can
+        ask for, kept as long as the cache (a captured step reads it where it was)."""
+        table = rotary.cos_sin_table(max(self.newest, self.capacity), device)
+        self._tables[table.data_ptr()] = table
+        return table
 
     def layer(self, i: int) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
         """(k_pages, v_pages, weights) of layer i."""

@@ -551,7 +551,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
       const bool is_top = key[r] == most;
       on[r] = on[r] && (!(min_p > 0.f) || is_top || wf[r] >= (double)min_p);
       // u == 0: the first kept token of any weight, also of one that rounds to no unit.
-      if (!(u > 0.f)) w[r] = is_top || any_weight(key[r] << SHIFT, top, T) ? 1 : 0;
+      if (!(u > 0.f)) {
+        const uint32_t low_bits = SHIFT != 0 && key[r] < 0x8000u ? 0xffffu : 0u;  // (of a negative logit's key)
+        w[r] = is_top || any_weight(key[r] << SHIFT | low_bits, top, T) ? 1 : 0;
+      }
       w[r] = on[r] ? w[r] : 0;
       s += w[r];
     }

@@ -251,3 +251,41 @@ def test_refusals(cdx):
         m(ids, past_key_values=cache)
         with pytest.raises(ValueError):
             m.generate_paged(ids, 4, uniforms=torch.rand(2, 3, device="cuda"))
+
+
+def test_modules_by_themselves(cdx):
+    """An attention module and a block on one layer of a cache, after begin."""
+    print("paged model: modules by themselves", flush=True)
+    m = _model(cdx, 64, 4, 2, layers=1, use_mu_guidance=False)
+    B, S = 3, 12
+    x = torch.randn(B, S + 1, 256, device="cuda").to(bf16)
+    ids = torch.randint(0, 600, (B, S + 1), device="cuda")
+    for module, kw in ((m.layers[0].self_attn, {}), (m.layers[0], {"token_ids": True})):
+        args = lambda a, b: {k: ids[:, a:b].contiguous() for k in kw}  # noqa: E731
+        cache = cdx.PagedKVCache(m.config, B, S + 1, page_size=16)
+        with torch.no_grad():
+            whole = module(x, **args(0, S + 1))[0]
+            cache.begin(B, S)
+            first = module(x[:, :S].contiguous(), past_key_value=cache[0], **args(0, S))[0]
+            cache.begin(B, 1)
+            last = module(x[:, S:].contiguous(), past_key_value=cache[0], **args(S, S + 1))[0]
+        e = errors(torch.cat([first, last], 1), whole)
+        assert e["max_rel"] <= MAX_REL and e["rel_rms"] <= REL_RMS, e
+
+
+def test_a_cache_with_pages_of_its_own_order(cdx):
+    """A pool whose pages a server handed out in another order, one prefix shared."""
+    print("paged model: block table replaced", flush=True)
+    m = _model(cdx, 64, 4, 2, layers=2)
+    B, S = 2, 16
+    ids = torch.randint(0, 600, (1, S), device="cuda").expand(B, S).contiguous()
+    nxt = torch.randint(0, 600, (B, 6), device="cuda")
+    plain = cdx.PagedKVCache(m.config, B, 48, page_size=16)
+    mixed = cdx.PagedKVCache(m.config, B, 48, page_size=16)
+    mixed.block_table = torch.tensor([[5, 0, 3], [5, 4, 1]], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        a, b = (m(ids, past_key_values=c).logits for c in (plain, mixed))
+        assert torch.equal(a, b)
+        for i in range(6):
+            a, b = (m(nxt[:, i:i + 1], past_key_values=c).logits for c in (plain, mixed))
+            assert torch.equal(a, b)

@@ -187,7 +187,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         weights = weights if weights.is_contiguous() else weights.contiguous()
     out = torch.empty(B, nq * D, dtype=q.dtype, device=q.device)
     lib = nat.lib()
-    ws = lib.cdx_paged_attention_workspace_bytes(B, nq, nkv, D, cap, weights is not None)
+    with nat.on_device(q):  # (the splits, and so the size, go by the current device's CUs)
+        ws = lib.cdx_paged_attention_workspace_bytes(B, nq, nkv, D, cap, weights is not None)
     work = torch.empty(ws, dtype=torch.uint8, device=q.device) if ws else None
     with nat.on_device(q), nat.launch_region("paged_attention", q.device, B=B, nq=nq, nkv=nkv, D=D):
         nat.check(lib.cdx_paged_attention_fwd(

@@ -280,7 +280,7 @@ __global__ __launch_bounds__(64 * W, NC == 4 && !FULL ? 2 : 4) void paged_attn_k
 }
 
 constexpr int kJoinThreads = 256;
-constexpr int kJoinSlots = 1024;  // slots of the weights that a block adds up
+constexpr int kJoinSlots = 512;  // slots of the weights that a block adds up
 constexpr int kMaxSplits = 256;
 
 // Maximum (log2 units, 0 where there is none) and sum of a row of scores from its splits' own, by
@@ -308,7 +308,7 @@ __device__ __forceinline__ float2 join_statistics(const PagedAttnParams& p, int6
 }
 
 // The first `rows` blocks (none without splits) join the splits of one row each, 256 threads over
-// splits and columns.  The others add up the softmax weights of 1024 slots of one (sequence,
+// splits and columns.  The others add up the softmax weights of 512 slots of one (sequence,
 // KV head), over the heads of its group.
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttnParams p, uint32_t rows, int chunks) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;

@@ -45,6 +45,7 @@ constexpr int64_t kMaxVocab = 1 << 20;
 constexpr int kListWave = 256;                // tokens that a wave can list
 constexpr int kLane = kListWave / 64;
 constexpr int kList = kListWave * kSampleWaves;
+constexpr int kHeld = 13;                     // pieces of a row that a lane can hold
 constexpr int kBins = 8192;
 
 struct SampleParams {
@@ -138,6 +139,22 @@ struct Row {
         if (c < lo || c > hi) raw[a] = edge(c);
         f(s + a, c * VEC - head, raw[a]);
       }
+    }
+  }
+  // All pieces of the spans s0 <= span < s1 <= s0 + HELD, on their way together.
+  template <int HELD>
+  __device__ __forceinline__ void hold(int s0, int s1, int lane, piece_t (&held)[HELD]) const {
+    if (lo <= hi) {
+#pragma unroll
+      for (int a = 0; a < HELD; ++a) {
+        const int c = max(lo, min(hi, (s0 + a) * 64 + lane));
+        if (s0 + a < s1) held[a] = *reinterpret_cast<const piece_t*>(x + (int64_t)c * VEC);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < HELD; ++a) {
+      const int c = (s0 + a) * 64 + lane;
+      if (s0 + a < s1 && (c < lo || c > hi)) held[a] = edge(c);
     }
   }
   // As values.
@@ -344,9 +361,27 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
   float top_p = p.top_p ? p.top_p[b] : p.top_p1;
   int top_k = p.top_k ? p.top_k[b] : p.top_k1;
 
+  // A row of up to 16 x 13 spans (106496 bf16 logits) stays in registers.
+  piece_t held[kHeld];
+  const bool holds = per_wave <= kHeld;
+  auto each_span = [&](auto f) {
+    if (holds) {
+#pragma unroll
+      for (int a = 0; a < kHeld; ++a) {
+        if (s0 + a >= s1) break;
+        float v[VEC];
+        row.unpack(held[a], v);
+        f(s0 + a, ((s0 + a) * 64 + lane) * VEC - row.head, v);
+      }
+    } else {
+      row.spans(s0, s1, lane, f);
+    }
+  };
+  if (holds) row.hold(s0, s1, lane, held);
+
   // The largest logit (fmaxf passes over NaN), of the thread and of the row.
   float mine = -INFINITY;
-  row.spans(s0, s1, lane, [&](int, int, const float(&v)[VEC]) {
+  each_span([&](int, int, const float(&v)[VEC]) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) mine = fmaxf(mine, v[e]);
   });
@@ -428,7 +463,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
   int listed = kListWave + 1;
   if (bounded) {
     listed = 0;
-    row.spans(s0, s1, lane, [&](int, int i0, const float(&v)[VEC]) {
+    each_span([&](int, int i0, const float(&v)[VEC]) {
       float most = v[0];
 #pragma unroll
       for (int e = 1; e < VEC; ++e) most = fmaxf(most, v[e]);

@@ -26,11 +26,13 @@
 //     border bin is then resolved by a radix descent over its few tokens; their passes are paced
 //     by the exponentials, about 20 instructions in 64 bits a token.
 //
-// Measured (us of the kernel): 1 x 100000 bf16, top-k 50 and top-p 0.9, 16.8, of which 3.2 is one
-// pass over the row by one CU (200 KB at 62 GB/s), 3.4 the bound, 4.8 the list; 256 x 100000
-// bf16, top-p by row, 46 (passes: maximum 7, counts 9, table 5, sums 15); 64 x 32000 fp32, min-p, 10.4;
-// 1 x 100000 fp32, top-p, 76.  With radix passes over the row in place of bounds, lists and counts the
-// first three took 310, 456 and 46.
+// Measured (us of the kernel): 1 x 100000 bf16, top-k 50 and top-p 0.9, 16.1, of which 2.1 is the pass
+// over the row by one CU, 3.4 the bound, 3.6 the list, 4.7 the wave's choice; 256 x 100000 bf16, top-p by
+// row, 46 (passes: maximum 7, counts 9, table 5, sums 15); 64 x 32000 fp32, min-p, 10.5; 1 x 100000
+// fp32, top-p, 77.  With radix passes over the row in place of bounds, lists and counts the first three
+// took 310, 456 and 46.  A row held in registers for the counts and sums too spilled (256 rows 113), as
+// did eight loads ahead instead of four (64 x 32000 17); a bound by waves instead of by the block (the
+// least of the waves' own) listed too many (42).
 #include <float.h>
 
 #include "cdx_common.h"

@@ -291,18 +291,21 @@ class PagedKVCache:
         self.batch_size, self.page_size, self.keep, self.recent = batch_size, page_size, keep, recent
         width = -(-max_length // page_size)
         self.capacity = width * page_size
-        shape = (config.num_hidden_layers, batch_size * width, nkv, page_size, D)
-        self.k_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
-        self.v_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
-        device = self.k_pages.device
-        self.block_table = torch.arange(batch_size * width, dtype=torch.int32, device=device).view(batch_size, width)
-        self._counts = torch.zeros(2, batch_size, dtype=torch.int32, device=device)
-        self._tables = {}
-        self.weights = self.slot_positions = None
-        if keep is not None:
-            shape = (shape[0], batch_size, nkv, self.capacity)
-            self.weights = torch.zeros(shape, dtype=torch.float32, device=device)
-            self.slot_positions = torch.empty(shape, dtype=torch.int32, device=device)
+        # (Ordinary tensors also under inference_mode: they are written in place wherever the cache is used.)
+        with torch.inference_mode(False), torch.no_grad():
+            shape = (config.num_hidden_layers, batch_size * width, nkv, page_size, D)
+            self.k_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
+            self.v_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
+            device = self.k_pages.device
+            pages = torch.arange(batch_size * width, dtype=torch.int32, device=device)
+            self.block_table = pages.view(batch_size, width)
+            self._counts = torch.zeros(2, batch_size, dtype=torch.int32, device=device)
+            self._tables = {}
+            self.weights = self.slot_positions = None
+            if keep is not None:
+                shape = (shape[0], batch_size, nkv, self.capacity)
+                self.weights = torch.zeros(shape, dtype=torch.float32, device=device)
+                self.slot_positions = torch.empty(shape, dtype=torch.int32, device=device)
         self.reset()
 
     @property

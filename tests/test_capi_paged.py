@@ -200,3 +200,14 @@ def test_cache_counts():
     full.begin(1, 16)
     with pytest.raises(ValueError, match="full"):
         full.begin(1, 1)
+
+
+def test_a_cache_made_under_inference_mode():
+    import complexity_deep as cdx
+    with torch.inference_mode():
+        c = cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), 2, 20, page_size=16, keep=10, device="cpu")
+    c.begin(2, 5)
+    with torch.inference_mode():
+        c.begin(2, 1)
+    c.begin(2, 1)
+    assert c.lengths.tolist() == [7, 7] and not c.lengths.is_inference()

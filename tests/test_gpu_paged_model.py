@@ -120,6 +120,10 @@ def test_generate_paged(cdx):
     u = torch.rand(B, n, device="cuda")
     a = m.generate_paged(ids, n, uniforms=u, min_p=0.01, eos_token_id=-5, cache=cache)
     assert torch.equal(a, m.generate_paged(ids, n, uniforms=u, min_p=0.01, eos_token_id=-5, cache=cache))
+    with torch.inference_mode():
+        assert torch.equal(a, m.generate_paged(ids, n, uniforms=u, min_p=0.01, eos_token_id=-5))
+        made_inside = cdx.PagedKVCache(m.config, B, S + n)
+    assert torch.equal(a, m.generate_paged(ids, n, uniforms=u, min_p=0.01, eos_token_id=-5, cache=made_inside))
     # A right-padded prompt generates what it does on its own.
     lens = torch.tensor([S, 4, 6]).cuda()
     ragged = m.generate_paged(ids, n, temperature=0.0, prompt_lengths=lens, eos_token_id=-5)

@@ -861,6 +861,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
         __syncthreads();
         last = (int)sh.range[0];
       }
+      // A k-th largest logit among different values counted as one: which of them stay is told by
+      // the bins, and what top-p's total holds of them too.
+      const bool split = last == mixed;
       border = last < steps ? step_value(top_step - last) : cutoff;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -870,7 +873,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
         w[i] = in ? wt.units(f) : 0;
         sh.table[i0 + i] = i0 + i == 0 || !(min_p > 0.f) || f >= (double)min_p ? w[i] : 0;
       }
-      if (cut_p) {
+      if (cut_p && !split) {
         u64 mass = 0, total;
 #pragma unroll
         for (int i = 0; i < PER; ++i) mass += i0 + i == mixed && mixed <= last ? step0_mass : n[i] * w[i];
@@ -891,7 +894,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) 
         border = step_value(top_step - last);
         keep = sh.pick[1];
       }
-      tabled = last != mixed;  // (a border among different values: by bins)
+      tabled = !split && last != mixed;  // (a border among different values: by bins)
     }
   }
   if (!tabled) {

@@ -180,3 +180,18 @@ def test_sample_refusals(cdx):
         with pytest.raises((ValueError, RuntimeError)):
             cdx.sample_tokens(*args, **s)
     assert cdx.sample_tokens(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [bf16, torch.float32])
+def test_sample_top_k_that_ends_among_values_around_zero(cdx, dtype):
+    """The k-th largest logit lies among values of less than 2^-24, too many for the lists, and top-p
+    cuts above them: its total holds what top-k kept of them, and nothing else."""
+    print(f"sample: top-k ends around zero, {dtype}", flush=True)
+    V, B = 32768, 12
+    row = torch.tensor([1e-9, -1e-9]).repeat(V // 2)
+    row[1000:9000:1000] = 9 - torch.arange(8) / 16
+    x = row.to(dtype).expand(B, V).contiguous()
+    u = (torch.arange(B) + 0.5) / B
+    for s in ({"top_k": 1000, "top_p": 0.5}, {"top_k": 20000, "top_p": 0.5}, {"top_k": 1000, "top_p": 0.9},
+              {"top_k": 1000, "top_p": 0.5, "min_p": 0.7}, {"top_k": 1000, "top_p": 0.7, "temperature": 0.5}):
+        _check(cdx, x, u, **s)

@@ -41,7 +41,7 @@ import torch.nn.functional as F
 from . import _native as nat
 from ._grad import forward_only
 from .linear import few_rows, linear, linear_accumulate_
-from .paged import PagedLayer, paged_attention, paged_write
+from .paged import PagedLayer, _ints, _ld, _pages, _rotary, paged_attention, paged_write
 from .rotary import RotaryEmbedding, apply_rotary_pos_emb
 
 
@@ -309,20 +309,29 @@ def qkv_paged(x: torch.Tensor, mu: Optional[torch.Tensor], w_x: torch.Tensor, w_
     """q [B, nq, D] of x [B, 1, H], its k and v appended to the pages (cdx_qkv_paged_fwd): the
     projection and paged_qkv_append, with the projection of a few rows kept in fp32 between
     them.  The cache's tensors are a PagedKVCache's, as paged_qkv_append takes them."""
-    nat.require_device(x, mu, w_x, w_mu, q_norm_w, k_norm_w, k_pages, v_pages, what="qkv_paged")
-    _check_widths(x, mu, H, "qkv_paged")
+    what = "qkv_paged"
+    nat.require_device(x, mu, w_x, w_mu, q_norm_w, k_norm_w, k_pages, v_pages, what=what)
+    nat.require_device(x, block_table, lengths, positions, cos_sin, dtype=None, what=what)
+    _check_widths(x, mu, H, what)
+    table = _pages(k_pages, v_pages, block_table, 4, what)
     pages, nkv, page, D = k_pages.shape
     B = x.shape[0]
-    if tuple(x.shape) != (B, 1, H) or w_x.shape[0] != (nq + 2 * nkv) * D or block_table.shape[0] != B:
-        raise ValueError(f"qkv_paged: input {tuple(x.shape)} and weight {tuple(w_x.shape)} do not match {nq} + 2 x "
-                         f"{nkv} heads of {D} in {block_table.shape[0]} sequences")
+    if tuple(x.shape) != (B, 1, H) or w_x.shape[0] != (nq + 2 * nkv) * D or table.shape[0] != B:
+        raise ValueError(f"{what}: input {tuple(x.shape)} and weight {tuple(w_x.shape)} do not match {nq} + 2 x "
+                         f"{nkv} heads of {D} in {table.shape[0]} sequences")
+    lengths = _ints(lengths, (B,), x, f"{what}: lengths")
+    positions = _ints(positions, (B,), x, f"{what}: positions")
+    _rotary(cos_sin, D, what)
+    if (q_norm_w is None) != (k_norm_w is None) or \
+            (q_norm_w is not None and not q_norm_w.numel() == k_norm_w.numel() == D):
+        raise ValueError(f"{what}: the QK norm weights must have {D} elements, both or neither")
     x2, ldx = _rows_view(x, H)
     if ldx == 0:
         x2, ldx = x.contiguous(), H
     mu2, ldmu = None, 0
     if mu is not None:
         mu2, ldmu = _rows_view(mu.expand(B, 1, H) if mu.shape[:-1] != (B, 1) else mu, H)
-    wx_ptr, wmu_ptr, ldw = _weight_sources(w_x, w_mu, mu2, H, "qkv_paged")
+    wx_ptr, wmu_ptr, ldw = _weight_sources(w_x, w_mu, mu2, H, what)
     if q_norm_w is not None:
         q_norm_w = q_norm_w.to(x.dtype).contiguous()
         k_norm_w = k_norm_w.to(x.dtype).contiguous()
@@ -334,7 +343,7 @@ def qkv_paged(x: torch.Tensor, mu: Optional[torch.Tensor], w_x: torch.Tensor, w_
         nat.check(lib.cdx_qkv_paged_fwd(
             x2.data_ptr(), ldx, None, 0.0, nat.ptr(mu2), ldmu, wx_ptr, wmu_ptr, ldw, B, H, nq, nkv, D,
             nat.ptr(q_norm_w), nat.ptr(k_norm_w), float(eps), cos_sin.data_ptr(), cos_sin.shape[0], lengths.data_ptr(),
-            positions.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], pages, page,
+            positions.data_ptr(), table.data_ptr(), _ld(table), table.shape[1], pages, page,
             k_pages.data_ptr(), v_pages.data_ptr(), q.data_ptr(), work.data_ptr(), ws, nat.stream_of(x)),
             "cdx_qkv_paged_fwd")
     return q

@@ -60,6 +60,12 @@ def _ld(table: torch.Tensor) -> int:
     return max(table.shape[1], table.stride(0)) if table.shape[0] > 1 else table.shape[1]
 
 
+def _rotary(cos_sin: torch.Tensor, D: int, what: str) -> None:
+    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.dim() != 3 \
+            or tuple(cos_sin.shape[1:]) != (D // 2, 2) or cos_sin.shape[0] == 0:
+        raise ValueError(f"{what}: cos_sin must be a contiguous fp32 table [positions, {D // 2}, 2]")
+
+
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """t contiguous at a 16-byte address."""
     t = t if t.is_contiguous() else t.contiguous()
@@ -94,9 +100,7 @@ def paged_qkv_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
         raise ValueError(f"{what}: {num_heads} query heads over {nkv} KV heads")
     if qkv.dtype not in (torch.bfloat16, torch.float32) or tuple(qkv.shape) != (B, N):
         raise ValueError(f"{what}: qkv must be bf16 or fp32 [{B}, {N}], got {qkv.dtype} {tuple(qkv.shape)}")
-    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.dim() != 3 \
-            or tuple(cos_sin.shape[1:]) != (D // 2, 2) or cos_sin.shape[0] == 0:
-        raise ValueError(f"{what}: cos_sin must be a contiguous fp32 table [positions, {D // 2}, 2]")
+    _rotary(cos_sin, D, what)
     if (q_norm_w is None) != (k_norm_w is None):
         raise ValueError(f"{what}: pass both QK norm weights or neither")
     if q_norm_w is not None:

@@ -293,3 +293,66 @@ def test_a_cache_with_pages_of_its_own_order(cdx):
         for i in range(6):
             a, b = (m(nxt[:, i:i + 1], past_key_values=c).logits for c in (plain, mixed))
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B", [2, 9])
+def test_block_tables_of_any_stride(cdx, B):
+    """A block table whose columns are not neighbours in memory, as a view of a server's wider one."""
+    print(f"paged model: strided block table, B={B}", flush=True)
+    m = _model(cdx, 64, 4, 2, layers=2)
+    ids = torch.randint(0, 600, (B, 20), generator=torch.Generator().manual_seed(8)).cuda()
+    plain, strided = (cdx.PagedKVCache(m.config, B, 48, page_size=16) for _ in range(2))
+    wide = torch.zeros(B, 6, dtype=torch.int32, device="cuda")
+    wide[:, ::2] = plain.block_table
+    wide[:, 1::2] = plain.block_table.flip(0)  # (pages of the other sequences)
+    strided.block_table = wide[:, ::2]
+    with torch.no_grad():
+        a, b = (m(ids[:, :14], past_key_values=c).logits for c in (plain, strided))
+        assert torch.equal(a, b)
+        for i in range(14, 20):
+            a, b = (m(ids[:, i:i + 1], past_key_values=c).logits for c in (plain, strided))
+            e = errors(a, b)  # (the norms are folded, or not, by the call path)
+            assert e["max_rel"] <= MAX_REL and e["rel_rms"] <= REL_RMS, (i, e)
+    for r in range(B):
+        for i in range(2):
+            for x, y in zip(plain.layer(i)[:2], strided.layer(i)[:2]):
+                a, b = (ref.slots(t, plain.block_table, r, 20).float() for t in (x, y))
+                assert torch.equal(a[:, :14], b[:, :14])
+                assert float((a - b).abs().max()) <= MAX_REL * float(a.abs().max())
+
+
+def test_block_tables_of_other_types_are_refused(cdx):
+    """Before anything is written, in the native call path and in the other one."""
+    print("paged model: block tables of other types", flush=True)
+    from complexity_deep.attention import qkv_paged
+    m = _model(cdx, 64, 4, 2, layers=2)
+    ids = torch.randint(0, 600, (2, 8), generator=torch.Generator().manual_seed(8)).cuda()
+    cache = cdx.PagedKVCache(m.config, 2, 48, page_size=16)
+    table = cache.block_table
+    attn = m.layers[0].self_attn
+    with torch.no_grad():
+        m(ids[:, :5], past_key_values=cache)
+        before = [t.clone() for t in (cache.k_pages, cache.v_pages, cache._counts)]
+        for bad in (table.long(), table.cpu(), table.float(), table[:1], table[0]):
+            cache.block_table = bad
+            with pytest.raises((ValueError, RuntimeError)):
+                m(ids[:, 5:6], past_key_values=cache)
+        cache.block_table = table
+        x = torch.randn(2, 1, 256, device="cuda").to(bf16)
+        args = dict(x=x, mu=None, w_x=attn.qkv_weights()[0], w_mu=attn.qkv_weights()[1], H=256, nq=4, q_norm_w=None,
+                    k_norm_w=None, eps=1e-6, cos_sin=attn.rotary_emb.cos_sin_table(48, x.device),
+                    k_pages=cache.k_pages[0], v_pages=cache.v_pages[0], block_table=table, lengths=cache.lengths,
+                    positions=cache.positions)
+        for name, bad in (("lengths", cache.lengths.long()), ("lengths", cache.lengths[:1]),
+                          ("positions", cache.positions.cpu()), ("positions", cache.positions.float()),
+                          ("cos_sin", args["cos_sin"].double()), ("cos_sin", args["cos_sin"][:, :16]),
+                          ("q_norm_w", x[0, 0, :64]), ("k_pages", cache.k_pages[0].transpose(1, 2)),
+                          ("v_pages", cache.v_pages[0][:1])):
+            with pytest.raises((ValueError, RuntimeError)):
+                qkv_paged(**{**args, name: bad})
+        with pytest.raises(ValueError):
+            qkv_paged(**{**args, "q_norm_w": x[0, 0, :8], "k_norm_w": x[0, 0, :8]})
+        for t, b in zip((cache.k_pages, cache.v_pages, cache._counts), before):
+            assert torch.equal(*(x.view(torch.int16) if x.dtype == bf16 else x for x in (t, b)))
+        m(ids[:, 5:6], past_key_values=cache)
+        assert cache.lengths.tolist() == [6, 6]

@@ -73,6 +73,15 @@ __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
   return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
+// Both bf16 of a word, Inf and NaN as the largest finite value of their sign: as signed integers the
+// positive ones lie above it, as unsigned integers the negative ones.
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x) {
+  typedef __attribute__((ext_vector_type(2))) short i16x2;
+  typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+  const i16x2 i = __builtin_elementwise_min(__builtin_bit_cast(i16x2, x), i16x2{0x7f7f, 0x7f7f});
+  const u16x2 u = __builtin_elementwise_min(__builtin_bit_cast(u16x2, i), u16x2{0xff7f, 0xff7f});
+  return __builtin_bit_cast(uint32_t, u);
+}
 
 template <int DPL>
 struct Piece;
@@ -234,6 +243,10 @@ __global__ __launch_bounds__(64 * W, NC == 4 && !FULL ? 2 : 4) void paged_attn_k
         a.w = low_halves(vw[6 * RW + w], vw[7 * RW + w]);
       }
       acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pb, acc[j], 0, 0, 0);
+      // The low part is 0 or negative where the high part is exact or rounded up, and 0 Inf has no
+      // value: an infinite value counts once, by the high part, and is a finite one here (two
+      // packed minima a word: 1 x 500 slots 5.2 -> 5.3 us, 64 of 1 .. 2048 56.1 -> 56.5, 4 x 65536 none).
+      a = make_uint4(finite_halves(a.x), finite_halves(a.y), finite_halves(a.z), finite_halves(a.w));
       acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pb_low, acc[j], 0, 0, 0);
     }
   }

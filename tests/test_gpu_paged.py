@@ -511,3 +511,48 @@ def test_refusals(cdx):
         attend(q=q.clone().requires_grad_())
     with torch.no_grad():
         attend(q=q.clone().requires_grad_())
+
+
+# ---- values and sizes at the ends of their ranges --------------------------------
+
+@pytest.mark.parametrize("nq,nkv,D,page,lens", [(4, 2, 64, 16, [1, 2, 40, 700]), (16, 8, 128, 64, [1, 33, 5000]),
+                                                (8, 4, 40, 32, [1, 64, 300]), (16, 4, 80, 16, [3, 100])])
+def test_attention_over_infinite_values(cdx, nq, nkv, D, page, lens):
+    """An infinite value that has a weight makes its column infinite (both signs, or a NaN: NaN) and
+    leaves the others as they are."""
+    print(f"attention: infinite values, {nq}/{nkv} D={D} lengths={lens}", flush=True)
+    k, v, table = ref.cache(len(lens), nkv, D, page, -(-max(lens) // page))
+    q = torch.randn(len(lens), nq, D, device="cuda").to(bf16)
+    lengths = _ints(lens)
+    clean = cdx.paged_attention(q, k, v, table, lengths).view(len(lens), nq, D)
+    inf, want = math.inf, {3: math.inf, 5: -math.inf, 6: math.inf, 7: math.nan}
+    for at in (0, -1):  # the first slot in use, the last one
+        w = v.clone()
+        for b, n in enumerate(lens):
+            t = at % n
+            for col, value in want.items():
+                w[int(table[b, t // page]), :, t % page, col] = value
+            if n > 1:  # a second one: the sum of two signs has no value
+                t = n // 2 if at == 0 else 0
+                w[int(table[b, t // page]), :, t % page, 5:7] = torch.tensor([-inf, -inf], device="cuda").to(bf16)
+        out = cdx.paged_attention(q, k, w, table, lengths).view(len(lens), nq, D)
+        for b, n in enumerate(lens):
+            sixth = math.nan if n > 1 else inf
+            for col, value in {**want, 6: sixth}.items():
+                got = out[b, :, col].float()
+                assert bool(got.isnan().all() if math.isnan(value) else (got == value).all()), (b, n, col, got)
+        rest = [c for c in range(D) if c not in want]
+        assert torch.equal(out[..., rest], clean[..., rest])
+
+
+def test_attention_repeats_bit_for_bit(cdx):
+    """Long sequences over many splits, with other calls between."""
+    print("attention: repeated", flush=True)
+    k, v, table = ref.cache(4, 8, 128, 128, 65, spare=20)
+    g = torch.Generator().manual_seed(2)
+    q, other = ((1.5 * torch.randn(4, 16, 128, generator=g)).to(bf16).cuda() for _ in range(2))
+    lengths = _ints([8320, 8192, 8191, 4097])
+    first = cdx.paged_attention(q, k, v, table, lengths)
+    for _ in range(20):
+        cdx.paged_attention(other, k, v, table, lengths)
+        assert torch.equal(cdx.paged_attention(q, k, v, table, lengths), first)

@@ -356,3 +356,68 @@ def test_block_tables_of_other_types_are_refused(cdx):
             assert torch.equal(*(x.view(torch.int16) if x.dtype == bf16 else x for x in (t, b)))
         m(ids[:, 5:6], past_key_values=cache)
         assert cache.lengths.tolist() == [6, 6]
+
+
+@pytest.mark.parametrize("B", [2, 9])
+def test_a_step_that_raises_leaves_the_weights(cdx, B):
+    """A bounded cache after a step that raised in its second layer is what it was, and the step done
+    again gives what it gives on a cache that never saw it raise."""
+    print(f"paged model: raised steps, B={B}", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    ids = torch.randint(0, 600, (B, 40), generator=torch.Generator().manual_seed(6)).cuda()
+    caches = [cdx.PagedKVCache(m.config, B, 32, page_size=16, keep=20, recent=4) for _ in range(2)]
+
+    def interrupted(*a):
+        raise KeyboardInterrupt
+
+    with torch.no_grad():
+        for c in caches:
+            m(ids[:, :28], past_key_values=c)
+        for i in range(28, 40):  # (the cache is full, and cut, at the fifth of these)
+            before = [t.clone() for t in (caches[0].weights, caches[0].slot_positions, caches[0]._counts)]
+            cut = caches[0].longest == caches[0].capacity
+            attn = m.layers[1].self_attn
+            attn.train(), setattr(attn, "attention_dropout", 0.1)
+            with pytest.raises(NotImplementedError):
+                m(ids[:, i:i + 1], past_key_values=caches[0])
+            attn.eval()
+            hook = m.layers[1].mlp.register_forward_pre_hook(interrupted)
+            with pytest.raises(KeyboardInterrupt):
+                m(ids[:, i:i + 1], past_key_values=caches[0])
+            hook.remove()
+            if not cut:  # (a cut, which the step done again would make too, stays)
+                for t, s in zip((caches[0].weights, caches[0].slot_positions, caches[0]._counts), before):
+                    assert torch.equal(t, s), i
+            a, b = (m(ids[:, i:i + 1], past_key_values=c).logits for c in caches)
+            assert torch.equal(a, b), i
+            assert caches[0].longest == caches[1].longest and caches[0].newest == caches[1].newest
+            for name in ("weights", "slot_positions", "_counts"):
+                assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), (i, name)
+
+
+def test_a_captured_step_of_a_bounded_cache(cdx):
+    """Replayed, it leaves the weights and positions that eager steps leave."""
+    print("paged model: captured step, bounded cache", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    B, S, n = 2, 20, 8
+    ids = torch.randint(0, 600, (B, S + n), generator=torch.Generator().manual_seed(9)).cuda()
+    caches = [cdx.PagedKVCache(m.config, B, 64, page_size=16, keep=32) for _ in range(2)]
+    with torch.no_grad():
+        for c in caches:
+            m(ids[:, :S], past_key_values=c)
+        tok = ids[:, S:S + 1].clone()
+        state = ("_counts", "weights", "slot_positions")
+        before = [getattr(caches[1], name).clone() for name in state]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = m(tok, past_key_values=caches[1]).logits
+        for name, t in zip(state, before):
+            getattr(caches[1], name).copy_(t)
+        for i in range(n):
+            tok.copy_(ids[:, S + i:S + i + 1])
+            eager = m(tok, past_key_values=caches[0]).logits
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(logits, eager), i
+            for name in state:
+                assert torch.equal(*(getattr(c, name) for c in caches)), (i, name)

@@ -16,6 +16,9 @@ void clear_error();
 // Checks hipGetLastError() after a launch; returns CDX_OK or CDX_ELAUNCH.
 int check_launch(const char* what);
 
+// Blocks of so many threads that one launch can have: its threads are counted in 32 bits.
+constexpr int64_t max_blocks(int threads) { return (int64_t)UINT32_MAX / threads; }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Compute units of the current device (256 on MI355X, the fallback if the query fails),

@@ -163,7 +163,7 @@ constexpr int kSelectThreads = 512;
 
 struct EvictParams {
   int32_t B, nkv, D, cap, keep, recent, max_moves;
-  int64_t rows;                // layers x B x nkv
+  int64_t row0;                // of layers x B x nkv rows, the launch's first
   const int32_t* lengths;      // [B]
   const int32_t* positions;    // [B], of the newest tokens
   const float* weights;        // [rows][cap]
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   __shared__ int hist[4][256];  // of each digit
   __shared__ int sums[kSelectThreads / 64];
   __shared__ int pick[2];
-  const int64_t row = blockIdx.x;
+  const int64_t row = p.row0 + blockIdx.x;
   const int b = (int)(row / p.nkv % p.B);
   const int tid = threadIdx.x;
   const int len = max(0, min(p.lengths[b], p.cap));
@@ -352,9 +352,10 @@ constexpr int kMoveBlock = 16;  // rows that a block moves, of K and of V: one p
 // One row a group: 62 us for 24 layers x 8 sequences of up to 2048 slots of 8 x 128 values (292 MB
 // read and written); two, four and eight rows, all loaded before the first is stored, 99, 95, 107.
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictParams p, uint32_t blocks) {
-  const int64_t row = blockIdx.x / blocks;
+  const uint32_t r = blockIdx.x / blocks;
+  const int64_t row = p.row0 + r;
   const int n = p.count[row], c = threadIdx.x & 15, cpr = p.D / 8;
-  const int m = (int)(blockIdx.x - (uint32_t)row * blocks) * kMoveBlock + (threadIdx.x >> 4);
+  const int m = (int)(blockIdx.x - r * blocks) * kMoveBlock + (threadIdx.x >> 4);
   if (m >= n || c >= cpr) return;
   const int h = (int)(row % p.nkv);
   const int64_t slab = row / p.nkv, b = slab % p.B, layer = slab / p.B;
@@ -399,9 +400,7 @@ extern "C" int cdx_paged_append_fwd(const void* qkv, int32_t qkv_fp32, int64_t l
   if (!aligned16(qkv) || !aligned16(cos_sin) || !aligned16(q_out) || !aligned16(k_pages) || !aligned16(v_pages) ||
       !aligned16(q_norm_w) || !aligned16(k_norm_w))
     return fail(CDX_EUNSUPPORTED, "%s: pointers must be 16-byte aligned", name);
-  p.qkv = qkv;
   p.ld = ldqkv;
-  p.B = (int32_t)B;
   p.nq = nq;
   p.nkv = nkv;
   p.D = hd;
@@ -410,18 +409,26 @@ extern "C" int cdx_paged_append_fwd(const void* qkv, int32_t qkv_fp32, int64_t l
   p.eps = eps;
   p.cos_sin = cos_sin;
   p.n_pos = n_pos;
-  p.lengths = lengths;
-  p.positions = positions;
   p.k_pages = k_pages;
   p.v_pages = v_pages;
-  p.q = q_out;
-  const dim3 grid((unsigned)((B * heads + 15) / 16));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (qkv_fp32)
-    paged_append_kernel<float><<<grid, dim3(256), 0, s>>>(p);
-  else
-    paged_append_kernel<uint16_t><<<grid, dim3(256), 0, s>>>(p);
-  return check_launch(name);
+  const int64_t per = max_blocks(256) * 16 / heads;  // sequences of one launch
+  for (int64_t b0 = 0; b0 < B; b0 += per) {
+    const int64_t n = B - b0 < per ? B - b0 : per;
+    p.B = (int32_t)n;
+    p.qkv = static_cast<const char*>(qkv) + b0 * ldqkv * (qkv_fp32 ? 4 : 2);
+    p.lengths = lengths + b0;
+    p.positions = positions + b0;
+    p.t.table = table ? table + b0 * table_ld : nullptr;
+    p.q = q_out + b0 * nq * hd;
+    const dim3 grid((unsigned)((n * heads + 15) / 16));
+    if (qkv_fp32)
+      paged_append_kernel<float><<<grid, dim3(256), 0, s>>>(p);
+    else
+      paged_append_kernel<uint16_t><<<grid, dim3(256), 0, s>>>(p);
+    if (int rc = check_launch(name)) return rc;
+  }
+  return CDX_OK;
 }
 
 extern "C" int cdx_qkv_paged_fwd(const uint16_t* x, int64_t ldx, const uint16_t* x_norm_w, float x_eps,
@@ -501,7 +508,7 @@ extern "C" int cdx_paged_write(const uint16_t* k, const uint16_t* v, int64_t B, 
   if (S < 0) return fail(CDX_EINVAL, "%s: bad shape S=%lld", name, (long long)S);
   if (B == 0 || S == 0 || width == 0 || num_pages == 0) return CDX_OK;
   const int64_t pieces = S * (hd / 8), blocks = (pieces + 256 * kWritePieces - 1) / (256 * kWritePieces);
-  if (S > INT32_MAX || B * nkv * blocks > INT32_MAX) return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
+  if (S > INT32_MAX || B * nkv * blocks > max_blocks(256)) return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
   if (!k || !v || !lengths || !table || !k_pages || !v_pages) return fail(CDX_EINVAL, "%s: null pointer", name);
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages))
     return fail(CDX_EUNSUPPORTED, "%s: pointers must be 16-byte aligned", name);
@@ -542,7 +549,7 @@ extern "C" int cdx_paged_evict(int64_t layers, int64_t B, int32_t nkv, int32_t h
   if (layers == 0 || B == 0 || width == 0 || num_pages == 0) return CDX_OK;
   const int64_t cap = width * page_size, rows = layers * B * nkv, moves = evict_max_moves(cap, keep);
   const int64_t blocks = (moves + kMoveBlock - 1) / kMoveBlock;
-  if (layers > 65535 || rows > INT32_MAX || (blocks > 0 && rows > INT32_MAX / blocks))
+  if (layers > 65535 || rows > INT32_MAX || blocks > max_blocks(256))
     return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
   if (!lengths || !positions || !table || !k_pages || !v_pages || !weights || !slot_positions || !new_lengths ||
       !new_weights || !new_slot_positions || !work)
@@ -561,7 +568,6 @@ extern "C" int cdx_paged_evict(int64_t layers, int64_t B, int32_t nkv, int32_t h
   p.keep = (int32_t)(keep < cap ? keep : cap);
   p.recent = (int32_t)(recent < INT32_MAX ? recent : INT32_MAX);
   p.max_moves = (int32_t)moves;
-  p.rows = rows;
   p.lengths = lengths;
   p.positions = positions;
   p.weights = weights;
@@ -575,15 +581,23 @@ extern "C" int cdx_paged_evict(int64_t layers, int64_t B, int32_t nkv, int32_t h
   p.k_pages = k_pages;
   p.v_pages = v_pages;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)rows), block(kSelectThreads);
-  if (cap <= 4 * kSelectThreads)
-    evict_select_kernel<4><<<grid, block, 0, s>>>(p);
-  else if (cap <= 16 * kSelectThreads)
-    evict_select_kernel<16><<<grid, block, 0, s>>>(p);
-  else
-    evict_select_kernel<0><<<grid, block, 0, s>>>(p);
-  if (int rc = check_launch(name)) return rc;
+  const int64_t select = max_blocks(kSelectThreads);
+  for (p.row0 = 0; p.row0 < rows; p.row0 += select) {
+    const dim3 grid((unsigned)(rows - p.row0 < select ? rows - p.row0 : select)), block(kSelectThreads);
+    if (cap <= 4 * kSelectThreads)
+      evict_select_kernel<4><<<grid, block, 0, s>>>(p);
+    else if (cap <= 16 * kSelectThreads)
+      evict_select_kernel<16><<<grid, block, 0, s>>>(p);
+    else
+      evict_select_kernel<0><<<grid, block, 0, s>>>(p);
+    if (int rc = check_launch(name)) return rc;
+  }
   if (blocks == 0) return CDX_OK;
-  evict_move_kernel<<<dim3((unsigned)(rows * blocks)), dim3(256), 0, s>>>(p, (uint32_t)blocks);
-  return check_launch(name);
+  const int64_t per = max_blocks(256) / blocks;
+  for (p.row0 = 0; p.row0 < rows; p.row0 += per) {
+    const int64_t n = rows - p.row0 < per ? rows - p.row0 : per;
+    evict_move_kernel<<<dim3((unsigned)(n * blocks)), dim3(256), 0, s>>>(p, (uint32_t)blocks);
+    if (int rc = check_launch(name)) return rc;
+  }
+  return CDX_OK;
 }

@@ -456,7 +456,8 @@ extern "C" int cdx_paged_attention_fwd(const uint16_t* q, int64_t B, int32_t nq,
   const int64_t blocks = B * nkv * head_tiles;
   const int64_t chunks = weights_in ? (cap + kJoinSlots - 1) / kJoinSlots : 0;
   const int splits = paged_splits(blocks, cap);
-  if (B * nq > INT32_MAX / 1024 || blocks * splits > INT32_MAX || B * (nkv * chunks + nq) > INT32_MAX)
+  if (B * nq > INT32_MAX / 1024 || blocks * splits > max_blocks(64 * kWaves) ||
+      B * (nkv * chunks + nq) > max_blocks(kJoinThreads))
     return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
   if (!q || !k_pages || !v_pages || !table || !lengths || !out) return fail(CDX_EINVAL, "%s: null pointer", name);
   const PagedWork ws = paged_work(B, nq, hd, cap, splits, weights_in != nullptr);

@@ -35,6 +35,8 @@
 // least of the waves' own) listed too many (42).
 #include <float.h>
 
+#include <algorithm>
+
 #include "cdx_common.h"
 #include "cdx_wave.h"
 
@@ -1081,24 +1083,28 @@ extern "C" int cdx_sample_tokens(const void* logits, int32_t logits_fp32, int64_
   int bits = 0;
   while ((1ll << bits) < V) ++bits;
   SampleParams p{};
-  p.logits = logits;
   p.ld = ld;
   p.V = (int32_t)V;
   p.shift = 62 - bits < 51 ? 62 - bits : 51;
-  p.uniforms = uniforms;
-  p.temperature = temperature;
-  p.top_k = top_k;
-  p.top_p = top_p;
-  p.min_p = min_p;
   p.temperature1 = temperature1;
   p.top_p1 = top_p1;
   p.min_p1 = min_p1;
   p.top_k1 = top_k1;
-  p.tokens = tokens;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (logits_fp32)
-    sample_kernel<float><<<dim3((unsigned)B), dim3(kThreads), 0, s>>>(p);
-  else
-    sample_kernel<uint16_t><<<dim3((unsigned)B), dim3(kThreads), 0, s>>>(p);
-  return check_launch(name);
+  for (int64_t b0 = 0; b0 < B; b0 += max_blocks(kThreads)) {
+    p.logits = static_cast<const char*>(logits) + b0 * ld * (logits_fp32 ? 4 : 2);
+    p.uniforms = uniforms + b0;
+    p.temperature = temperature ? temperature + b0 : nullptr;
+    p.top_k = top_k ? top_k + b0 : nullptr;
+    p.top_p = top_p ? top_p + b0 : nullptr;
+    p.min_p = min_p ? min_p + b0 : nullptr;
+    p.tokens = tokens + b0;
+    const dim3 grid((unsigned)std::min<int64_t>(B - b0, max_blocks(kThreads)));
+    if (logits_fp32)
+      sample_kernel<float><<<grid, dim3(kThreads), 0, s>>>(p);
+    else
+      sample_kernel<uint16_t><<<grid, dim3(kThreads), 0, s>>>(p);
+    if (int rc = check_launch(name)) return rc;
+  }
+  return CDX_OK;
 }

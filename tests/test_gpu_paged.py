@@ -556,3 +556,46 @@ def test_attention_repeats_bit_for_bit(cdx):
     for _ in range(20):
         cdx.paged_attention(other, k, v, table, lengths)
         assert torch.equal(cdx.paged_attention(q, k, v, table, lengths), first)
+
+
+def test_evict_of_many_heads(cdx):
+    """More heads than one launch has threads for."""
+    print("evict: 9 x 2^20 heads of 64 slots", flush=True)
+    L, B, nkv, D, page, cap, keep = 9, 1 << 17, 8, 8, 64, 64, 32
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k = torch.empty(L, B, nkv, page, D, dtype=bf16, device="cuda")
+    k.view(torch.int16).random_(0, 1 << 14, generator=g)
+    v = k + 1
+    table = torch.arange(B, dtype=torch.int32, device="cuda").view(B, 1)
+    lengths = torch.full((B,), cap, dtype=torch.int32, device="cuda")
+    # Half of the slots, and always the upper half of every second sequence, weigh more than the others.
+    heavy = torch.rand(L, B, nkv, cap, generator=g, device="cuda").argsort(-1) < keep
+    heavy[:, ::2] = torch.arange(cap, device="cuda") >= keep
+    pos = torch.arange(cap, dtype=torch.int32, device="cuda").expand(L, B, nkv, cap).contiguous()
+    k0 = k.clone()
+    n, w, p = cdx.paged_evict(k, v, table, lengths, lengths - 1, heavy.float(), pos, keep, 0)
+    assert bool((n == keep).all()) and bool((w[..., :keep] == 1).all()) and bool((w[..., keep:] == 0).all())
+    assert bool((p[..., keep:] == -1).all())
+    held = p[..., :keep].long()
+    assert bool(torch.gather(heavy, -1, held).all()) and bool((held.sort(-1).values.diff(dim=-1) > 0).all())
+    for l in range(L):  # the rows moved with their positions
+        for pages, start in ((k, k0), (v, k0 + 1)):
+            want = torch.gather(start[l], 2, held[l].unsqueeze(-1).expand(B, nkv, keep, D))
+            assert torch.equal(pages[l, :, :, :keep], want)
+
+
+def test_append_of_many_sequences(cdx):
+    """More heads than one launch has threads for: what two calls of half of them give."""
+    print("append: 2^20 sequences of 256 heads", flush=True)
+    B, nq, nkv, D, page = 1 << 20, 254, 1, 8, 16
+    k = torch.zeros(B, nkv, page, D, dtype=bf16, device="cuda")
+    v = torch.zeros_like(k)
+    qkv = torch.empty(B, (nq + 2 * nkv) * D, dtype=bf16, device="cuda").uniform_(-1, 1)
+    at = torch.arange(B, dtype=torch.int32, device="cuda")
+    table, lengths, positions, cs = at.flip(0).view(B, 1), at % page + 1, at % 40, _table(40, D)
+    q = cdx.paged_qkv_append(qkv, k, v, table, lengths, positions, nq, cs)
+    k2, v2 = torch.zeros_like(k), torch.zeros_like(v)
+    for part in (slice(0, B // 2), slice(B // 2, B)):
+        half = cdx.paged_qkv_append(qkv[part], k2, v2, table[part], lengths[part], positions[part], nq, cs)
+        assert torch.equal(q[part], half)
+    assert torch.equal(k, k2) and torch.equal(v, v2)

@@ -195,3 +195,23 @@ def test_sample_top_k_that_ends_among_values_around_zero(cdx, dtype):
     for s in ({"top_k": 1000, "top_p": 0.5}, {"top_k": 20000, "top_p": 0.5}, {"top_k": 1000, "top_p": 0.9},
               {"top_k": 1000, "top_p": 0.5, "min_p": 0.7}, {"top_k": 1000, "top_p": 0.7, "temperature": 0.5}):
         _check(cdx, x, u, **s)
+
+
+def test_sample_of_many_rows(cdx):
+    """More rows than one launch has threads for, with settings of each row."""
+    print("sample: 2^22 + 5 rows", flush=True)
+    B, V = (1 << 22) + 5, 9
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for dtype in (bf16, torch.float32):
+        x = torch.rand(B, V, generator=g, device="cuda").argsort(-1).to(dtype)  # (no ties)
+        u = torch.rand(B, generator=g, device="cuda")
+        best = x.argmax(-1)
+        zero, one = torch.zeros(B, device="cuda"), torch.ones(B, dtype=torch.int32, device="cuda")
+        assert torch.equal(cdx.sample_tokens(x, u, temperature=0), best)
+        assert torch.equal(cdx.sample_tokens(x, u, top_k=one), best)
+        assert torch.equal(cdx.sample_tokens(x, u, top_p=zero), best)
+        assert torch.equal(cdx.sample_tokens(x, u, min_p=zero + 1), best)
+        assert torch.equal(cdx.sample_tokens(x, u, temperature=zero), best)
+        some = cdx.sample_tokens(x, u)
+        for part in (slice(0, 1000), slice(B - 1000, B)):
+            assert torch.equal(cdx.sample_tokens(x[part], u[part]), some[part])

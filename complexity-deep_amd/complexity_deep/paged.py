@@ -272,8 +272,10 @@ class PagedKVCache:
     slots (paged_evict): the ``recent`` newest tokens (half of ``keep`` by default) stay, and those
     that the steps so far attended to most.  Positions go on counting.
 
-    ``lengths`` and ``positions`` (of the newest tokens) live on the device and nothing waits for
-    them; ``longest`` and ``newest`` are the host's bounds.  One call at a time may use a cache.  A
+    ``lengths`` and ``positions`` (of the newest tokens) live on the device; ``longest`` and ``newest``
+    are the host's bounds, and nothing waits for the device but the first call of a batch whose
+    bound, of right-padded prompts with prompt_lengths on the device, has reached the capacity: it reads
+    how long the longest is.  One call at a time may use a cache.  A
     step that is captured into a graph counts on the device when it is replayed, not here: keep to
     max_length then (a token past the capacity is not stored).  A TransformerBlock or
     ComplexityAttention called by itself takes ``cache[i]``, after ``begin`` has counted the call's
@@ -348,6 +350,7 @@ class PagedKVCache:
             self.weights.zero_()
             self.slot_positions.fill_(-1)
         self.longest = self.newest = 0  # no sequence has more slots, or has seen more tokens
+        self._exact = True              # whether one has as many slots
         self.prompt = True              # what the call at hand brings
         self._saved = False             # whether _weights_before holds the weights before it
 
@@ -383,11 +386,17 @@ class PagedKVCache:
                 at = torch.arange(self.capacity, dtype=torch.int32, device=self.slot_positions.device)
                 self.slot_positions.copy_(torch.where(at < self.lengths.view(-1, 1, 1), at, -1))
             self.longest = self.newest = tokens
+            self._exact = prompt_lengths is None
+            if prompt_lengths is not None and not prompt_lengths.is_cuda:
+                self._read_longest(prompt_lengths.clamp(0, tokens))
             self.prompt = True
             return
         if tokens != 1 or prompt_lengths is not None:
             raise ValueError("PagedKVCache: after the prompts a call takes one token per sequence (reset() empties the "
                              "cache)")
+        capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()
+        if self.longest >= self.capacity and not self._exact and not capturing:
+            self._read_longest(self.lengths)
         if self.longest >= self.capacity:
             if self.keep is None:
                 raise ValueError(f"PagedKVCache: full ({self.capacity} tokens)")
@@ -395,8 +404,7 @@ class PagedKVCache:
         # Every layer adds to the weights in place: a call that raises is taken back from a copy (1B preset, 32
         # sequences of 2048 slots: 14 us of a step of 2.4 ms).  A step that is captured runs as a whole or not
         # at all, and makes none.
-        self._saved = self.weights is not None and not (self.weights.is_cuda
-                                                        and torch.cuda.is_current_stream_capturing())
+        self._saved = self.weights is not None and not capturing
         if self._saved:
             self._weights_before.copy_(self.weights)
         self._counts.add_(1)
@@ -406,6 +414,9 @@ class PagedKVCache:
         self.longest += 1
         self.newest += 1
         self.prompt = False
+
+    def _read_longest(self, lengths: torch.Tensor) -> None:
+        self.longest, self._exact = int(lengths.max()), True
 
     def _new_slot(self) -> torch.Tensor:
         """The slot of each sequence's newest token, by layer and head (the capacity bounds it here too:

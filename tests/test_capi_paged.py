@@ -211,3 +211,19 @@ def test_a_cache_made_under_inference_mode():
         c.begin(2, 1)
     c.begin(2, 1)
     assert c.lengths.tolist() == [7, 7] and not c.lengths.is_inference()
+
+
+@pytest.mark.parametrize("keep", [None, 8])
+def test_a_cache_is_full_when_its_longest_sequence_is(keep):
+    """Not when the padded prompts and the steps after them are as long as the capacity."""
+    import complexity_deep as cdx
+    c = cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), 3, 16, page_size=16, keep=keep, device="cpu")
+    c.begin(3, 15, torch.tensor([3, 0, 6]))
+    assert (c.longest, c.newest) == (6, 15)
+    for i in range(10):
+        c.begin(3, 1)
+        assert c.lengths.tolist() == [4 + i, 1 + i, 7 + i] and c.longest == 7 + i
+    if keep is None:
+        with pytest.raises(ValueError, match="full"):
+            c.begin(3, 1)
+    assert c.lengths.tolist() == [13, 10, 16] and c.longest == 16

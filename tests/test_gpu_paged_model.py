@@ -421,3 +421,32 @@ def test_a_captured_step_of_a_bounded_cache(cdx):
             assert torch.equal(logits, eager), i
             for name in state:
                 assert torch.equal(*(getattr(c, name) for c in caches)), (i, name)
+
+
+@pytest.mark.parametrize("keep", [None, 12])
+def test_padding_takes_no_room(cdx, keep):
+    """Right-padded prompts whose padded length nearly fills the cache: each sequence has room for
+    its own tokens, and a bounded cache is cut when its longest sequence fills it."""
+    print(f"paged model: padded prompts in a small cache, keep={keep}", flush=True)
+    m = _model(cdx, 64, 4, 2, layers=2)
+    ids = torch.randint(0, 600, (2, 40), generator=torch.Generator().manual_seed(10)).cuda()
+    lens = torch.tensor([5, 3], device="cuda")
+    small, wide = (cdx.PagedKVCache(m.config, 2, n, page_size=16, keep=keep) for n in (16, 64))
+    with torch.no_grad():
+        for c in (small, wide):
+            m(ids[:, :15], past_key_values=c, prompt_lengths=lens)
+        for i in range(11):
+            a, b = (m(ids[:, 15 + i:16 + i], past_key_values=c).logits for c in (small, wide))
+            e = errors(a, b)  # (the split of a row's keys follows the capacity)
+            assert e["max_rel"] <= MAX_REL and e["rel_rms"] <= REL_RMS, (i, e)
+            assert small.lengths.tolist() == [6 + i, 4 + i]
+        assert small.longest == 16
+        if keep is None:
+            with pytest.raises(ValueError, match="full"):
+                m(ids[:, 26:27], past_key_values=small)
+            assert small.lengths.tolist() == [16, 14]
+        else:
+            for i in range(10):
+                m(ids[:, 26 + i:27 + i], past_key_values=small)
+                assert small.longest == int(small.lengths.max()) <= 16
+            assert small.lengths.tolist() == [14, 14]

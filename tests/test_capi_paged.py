@@ -227,3 +227,11 @@ def test_a_cache_is_full_when_its_longest_sequence_is(keep):
         with pytest.raises(ValueError, match="full"):
             c.begin(3, 1)
     assert c.lengths.tolist() == [13, 10, 16] and c.longest == 16
+
+
+@pytest.mark.parametrize("bad", [dict(keep=10.5), dict(keep=True), dict(keep=8, recent=2.5), dict(keep=8, recent=True)])
+def test_a_bound_that_is_no_integer_is_refused_at_once(bad):
+    """Not by the first cut, in the middle of a generation."""
+    import complexity_deep as cdx
+    with pytest.raises(ValueError, match="PagedKVCache"):
+        cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), 2, 40, device="cpu", **bad)

@@ -373,6 +373,9 @@ class PagedKVCache:
         each, or all of them) of an empty cache, then one token per sequence."""
         if batch_size != self.batch_size:
             raise ValueError(f"PagedKVCache: {batch_size} sequences in a cache of {self.batch_size}")
+        if self.block_table.shape[-1] * self.page_size < self.capacity:
+            raise ValueError(f"PagedKVCache: a block table {tuple(self.block_table.shape)} of pages of {self.page_size} "
+                             f"has no room for {self.capacity} tokens")
         if self.newest == 0:
             if not 0 < tokens <= self.capacity:
                 raise ValueError(f"PagedKVCache: prompts of {tokens} tokens in a cache of {self.capacity}")

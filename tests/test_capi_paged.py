@@ -235,3 +235,19 @@ def test_a_bound_that_is_no_integer_is_refused_at_once(bad):
     import complexity_deep as cdx
     with pytest.raises(ValueError, match="PagedKVCache"):
         cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), 2, 40, device="cpu", **bad)
+
+
+def test_a_narrower_block_table_is_refused():
+    """Tokens past its pages would be dropped, and nobody told."""
+    import complexity_deep as cdx
+    c = cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), 2, 40, page_size=16, device="cpu")
+    whole = c.block_table
+    c.block_table = whole[:, :2]
+    with pytest.raises(ValueError, match="block table"):
+        c.begin(2, 5)
+    c.block_table = torch.cat([whole, whole], 1)  # (a wider one is no harm)
+    c.begin(2, 5)
+    c.block_table = whole[:, :2]
+    with pytest.raises(ValueError, match="block table"):
+        c.begin(2, 1)
+    assert c.lengths.tolist() == [5, 5] and c.longest == 5

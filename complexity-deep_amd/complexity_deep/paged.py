@@ -291,8 +291,9 @@ class PagedKVCache:
                              "to 128, and of 64, are supported)")
         if batch_size <= 0 or max_length <= 0:
             raise ValueError(f"PagedKVCache: bad size {batch_size} x {max_length}")
-        if any(isinstance(n, bool) or not isinstance(n, int) for n in (keep, recent) if n is not None):
+        if any(isinstance(n, bool) or int(n) != n for n in (keep, recent) if n is not None):
             raise ValueError(f"PagedKVCache: keep={keep} and recent={recent} must be integers")
+        keep, recent = (None if n is None else int(n) for n in (keep, recent))
         recent = recent if recent is not None else (keep // 2 if keep is not None else 0)
         if keep is not None and not (0 < keep < max_length and 0 <= recent <= keep):
             raise ValueError(f"PagedKVCache: keep={keep} must lie in 1 .. max_length - 1, recent={recent} in 0 .. keep")

@@ -251,3 +251,11 @@ def test_a_narrower_block_table_is_refused():
     with pytest.raises(ValueError, match="block table"):
         c.begin(2, 1)
     assert c.lengths.tolist() == [5, 5] and c.longest == 5
+
+
+def test_whole_numbers_of_other_types_are_bounds():
+    import numpy as np
+    import complexity_deep as cdx
+    for keep, recent in ((np.int64(8), np.int32(3)), (8.0, 3.0)):
+        c = cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), 2, 40, keep=keep, recent=recent, device="cpu")
+        assert (c.keep, c.recent) == (8, 3) and type(c.keep) is type(c.recent) is int

@@ -5,10 +5,11 @@
 // a page are one contiguous piece; every kernel here moves whole rows in pieces of 8 or 16
 // bytes per lane and is bound by memory, or for a step's few rows by its launch.
 //
-// Measured (us of a kernel): append of 256 tokens, 16/8 heads of 128, 3.5 (one token of 8/4 heads of
-// 40: 2.0); write of 8 prompts of up to 2048 tokens (67 MB read and written) 13, 5.1 TB/s, where a
-// large copy moves 4.8; eviction of one slot a head, 12 layers x 4 x 1025 slots, 7.9 + 3.3, of half a
-// prompt, 24 layers x 8 x up to 2048 slots of 8 x 128, 18.8 + 65 (292 MB of rows read and written).
+// Measured (us of a kernel): append of 256 tokens, 16/8 heads of 128, 3.3 (one token of 8/4 heads of
+// 40: 2.2); write of 8 prompts of up to 2048 tokens (67 MB read and written) 12.9, 5.2 TB/s, where the
+// plainest copy of 64 MB moves 5.3 (of 512 MB 6.2); eviction of one slot a head, 12 layers x 4 x 1025
+// slots, 7.8 + 3.4, of half a prompt, 24 layers x 8 x up to 2048 slots of 8 x 128, 18.6 + 67 (292 MB of
+// rows read and written, 4.4 TB/s).
 //
 //   paged_append_kernel   the packed projection of one new token per sequence, read once: per-head
 //                         RMSNorm, RoPE at the sequence's own position, q out, k and v into the
@@ -205,7 +206,7 @@ __device__ __forceinline__ int block_exclusive(int v, int* lds, int& total) {
 }
 
 // PER: slots that a thread holds in registers (capacity <= 512 PER), or 0: every pass reads them (24
-// layers x 8 x 2048 slots: held 24.5 us, read again 38).
+// layers x 8 x 2048 slots: held 18.6 us, read again 24.3; 12 x 4 x 1088: 7.8, 10.0).
 template <int PER>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const EvictParams p) {
   __shared__ int hist[4][256];  // of each digit
@@ -349,8 +350,9 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
 
 constexpr int kMoveBlock = 16;  // rows that a block moves, of K and of V: one per 16 lanes
 
-// One row a group: 62 us for 24 layers x 8 sequences of up to 2048 slots of 8 x 128 values (292 MB
-// read and written); two, four and eight rows, all loaded before the first is stored, 99, 95, 107.
+// One row a group: 62 us, when it was tried, for 24 layers x 8 sequences of up to 2048 slots of 8 x 128
+// values (292 MB read and written); two, four and eight rows, all loaded before the first is stored,
+// 99, 95, 107.
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictParams p, uint32_t blocks) {
   const uint32_t r = blockIdx.x / blocks;
   const int64_t row = p.row0 + r;

@@ -16,15 +16,15 @@
 //     registers (two bf16 of neighbouring rows per v_perm).  Nothing goes through LDS.
 //   * One pass: the running maximum and sum of the softmax, in log2 units and fp32, per wave.
 //     The eight waves of a block take every eighth tile and are joined through LDS.  P enters
-//     the product with V as two bf16 parts (2^-16 of it is lost; one part alone, 2^-8, took 5.2
-//     instead of 5.4 us for the smallest calls and the same for all others).
+//     the product with V as two bf16 parts (2^-16 of it is lost; one part alone, 2^-8, takes 5.3
+//     instead of 5.6 us for 1 x 500 slots, 48.8 instead of 49.4 for 64 x 1024 and the same for long ones).
 //   * A sequence is split into `splits` runs of tiles over blocks; the partial sums (fp32, with
 //     their maximum and sum) are joined by a second kernel, which also adds up the weights that
 //     each slot received, from the scores that the first kernel left.
 //
 // Measured (us and TB/s of K and V, calls in a row, both kernels): 16/8 heads of 128, 4 x 65536
-// slots 184 (5.8), 64 x 1024 49 (5.5), 64 sequences of 1 .. 2048 56 (4.8), 1 x 1000 11; 16/4 of
-// 80, 64 x 4096 66 (5.1); 8/4 of 40, 1 x 500 5.4.  A large copy moves 4.8 TB/s here.  What it took:
+// slots 184 (5.8), 64 x 1024 49 (5.4), 64 sequences of 1 .. 2048 56.5 (4.8), 1 x 1000 11.5; 16/4 of
+// 80, 64 x 4096 67 (5.0); 8/4 of 40, 1 x 500 5.3-5.6.  The plainest kernel reads 6.3 TB/s here.  What it took:
 // eight waves of at most 128 registers, two blocks on a CU (with a base address per tile shared by
 // the wave, and masks only in a sequence's last tile) 67 -> 56 us for the ragged 64; four waves of
 // 140 registers had been the better form before.

@@ -26,10 +26,12 @@
 //     border bin is then resolved by a radix descent over its few tokens; their passes are paced
 //     by the exponentials, about 20 instructions in 64 bits a token.
 //
-// Measured (us of the kernel): 1 x 100000 bf16, top-k 50 and top-p 0.9, 16.1, of which 2.1 is the pass
-// over the row by one CU, 3.4 the bound, 3.6 the list, 4.7 the wave's choice; 256 x 100000 bf16, top-p by
-// row, 46 (passes: maximum 7, counts 9, table 5, sums 15); 64 x 32000 fp32, min-p, 10.5; 1 x 100000
-// fp32, top-p, 77.  With radix passes over the row in place of bounds, lists and counts the first three
+// Measured (us of the kernel): 1 x 100000 bf16, top-k 50 and top-p 0.9, 16.3, of which 2.2 is the pass
+// over the row by one CU, 3.4 the bound, 3.8 the list, 4.7 the wave's choice; 256 x 100000 bf16, top-p by
+// row, 46 (a block with a cut: maximum 3, counts 10, table and border 6, sums 14, draw 3, 36 in all; the
+// rest is the launch and the slowest rows); one row of those, 36; 64 x 32000 fp32, min-p, 10.5; fp32 with
+// top-p, 1 x 100000 78, 256 x 100000 105; the first maximum (T == 0) of 1 x 100000 bf16 7.5, of 256 12.9.
+// With radix passes over the row in place of bounds, lists and counts the first three
 // took 310, 456 and 46.  A row held in registers for the counts and sums too spilled (256 rows 113), as
 // did eight loads ahead instead of four (64 x 32000 17); a bound by waves instead of by the block (the
 // least of the waves' own) listed too many (42).
@@ -49,7 +51,11 @@ constexpr int64_t kMaxVocab = 1 << 20;
 constexpr int kListWave = 256;                // tokens that a wave can list
 constexpr int kLane = kListWave / 64;
 constexpr int kList = kListWave * kSampleWaves;
-constexpr int kHeld = 13;                     // pieces of a row that a lane can hold
+// Pieces of a row that a lane can hold.  bf16 rows gain by more of them, and the fp32 kernel spills them: 9
+// of its registers with 8 pieces, 56 with 13, 112 with 16 (us with 8, 13 and 16: top-k, 1 x 100000 bf16 17.3,
+// 16.4, 16.6, 1 x 131072 16.6, 16.5, 16.2; min-p at T = 1, 64 x 32000 fp32 12.5, 13.2, 17.2, 64 x 65536 17.3,
+// 17.6, 21.7).
+constexpr int kHeld = 13;
 constexpr int kBins = 8192;
 
 struct SampleParams {

@@ -259,3 +259,16 @@ def test_whole_numbers_of_other_types_are_bounds():
     for keep, recent in ((np.int64(8), np.int32(3)), (8.0, 3.0)):
         c = cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), 2, 40, keep=keep, recent=recent, device="cpu")
         assert (c.keep, c.recent) == (8, 3) and type(c.keep) is type(c.recent) is int
+
+
+def test_more_threads_than_a_launch_has_are_refused(lib):
+    """Where a call is not cut into several launches (operands of hundreds of gigabytes)."""
+    write = _call(lib.cdx_paged_write,
+                  "k v B nkv S hd lengths table table_ld width num_pages page k_pages v_pages stream",
+                  [16, 16, 100000, 2, 1 << 20, 64, 16, 16, 4, 4, 9, 16, 16, 16, None])
+    assert write() == CDX_EUNSUPPORTED
+    attend = _call(lib.cdx_paged_attention_fwd,
+                   "q B nq nkv hd k_pages v_pages table table_ld width num_pages page lengths scale out w_in w_out work "
+                   "work_bytes stream",
+                   [16, 100000, 4, 2, 64, 16, 16, 16, 4096, 4096, 9, 16, 16, 0.125, 16, 16, 16, 16, 1 << 60, None])
+    assert attend() == CDX_EUNSUPPORTED

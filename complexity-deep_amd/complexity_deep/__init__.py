@@ -24,7 +24,8 @@ from .modeling import (CausalLMOutput, ComplexityConfig, ComplexityModel, Graphe
                        count_parameters, create_complexity_model)
 from .normalization import (FusedResidualRMSNorm, RMSNorm, fused_add_rmsnorm_inplace, fused_residual_rmsnorm,
                             fused_rmsnorm)
-from .paged import PagedKVCache, paged_attention, paged_evict, paged_qkv_append, paged_write
+from .paged import (PagedKVCache, PagedRows, paged_attention, paged_chunk_append, paged_chunk_attention, paged_evict,
+                    paged_qkv_append, paged_reserve, paged_truncate, paged_write)
 from .rotary import RotaryEmbedding, apply_rotary_pos_emb
 from .sampling import sample_tokens
 from .token_routed_mlp import (RoutePlan, TokenRoutedMLP, cggr_grouped_gemm, cggr_grouped_gemm_triton,
@@ -44,5 +45,6 @@ __all__ = [
     "fused_swiglu_simple", "route_plan", "route_plans", "RoutePlan",
     "fused_mu_qkv_projection", "FusedMuQKVProjection",
     "paged_qkv_append", "paged_write", "paged_attention", "paged_evict", "sample_tokens",
-    "PagedKVCache",
+    "paged_reserve", "paged_truncate", "paged_chunk_append", "paged_chunk_attention",
+    "PagedKVCache", "PagedRows",
 ]

@@ -96,6 +96,16 @@ _SIGNATURES = {
     "cdx_paged_evict_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i32, _i64, _i64]),
     "cdx_paged_evict": (ctypes.c_int, [_i64, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp,
                                        _vp, _i64, _i64, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "cdx_paged_reserve": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _vp,
+                                         _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cdx_paged_truncate": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _vp, _vp,
+                                          _vp]),
+    "cdx_paged_chunk_append_fwd": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _vp, ctypes.c_float, _vp,
+                                                  _i64, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "cdx_paged_chunk_attention_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i32, _i32, _i32, _i64, _i64]),
+    "cdx_paged_chunk_attention_fwd": (ctypes.c_int, [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64,
+                                                     _i32, _vp, _vp, _vp, _i64, ctypes.c_float, _vp, _vp,
+                                                     ctypes.c_size_t, _vp]),
     "cdx_sample_tokens": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _i32, _vp,
                                          ctypes.c_float, _vp, ctypes.c_float, _vp, _vp]),
     "cdx_hbm_probe": (ctypes.c_int, [_i32, _vp, _vp, _i64, _vp]),

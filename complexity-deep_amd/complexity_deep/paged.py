@@ -37,8 +37,7 @@ def _ints(t: torch.Tensor, shape: Tuple[int, ...], like: torch.Tensor, what: str
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, dims: int, what: str) -> torch.Tensor:
-    """The block table with unit stride, after checks of the cache's tensors."""
+def _page_shapes(k_pages: torch.Tensor, v_pages: torch.Tensor, dims: int, what: str) -> None:
     if k_pages.dim() != dims or v_pages.shape != k_pages.shape:
         raise ValueError(f"{what}: k_pages and v_pages must share one shape of {dims} dimensions, got "
                          f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
@@ -49,6 +48,11 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, di
         raise ValueError(f"{what}: page size {page} is not one of {PAGE_SIZES}")
     if D % 8 != 0 or not 0 < D <= 128:
         raise ValueError(f"{what}: head dim {D} must be a multiple of 8 up to 128")
+
+
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, dims: int, what: str) -> torch.Tensor:
+    """The block table with unit stride, after checks of the cache's tensors."""
+    _page_shapes(k_pages, v_pages, dims, what)
     if table.dtype != torch.int32 or table.dim() != 2 or table.device != k_pages.device:
         raise ValueError(f"{what}: block_table must be an int32 tensor [sequences, pages] on {k_pages.device}, got "
                          f"{table.dtype} {tuple(table.shape)} on {table.device}")
@@ -253,6 +257,223 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
             keep, recent, *(t.data_ptr() for t in new), work.data_ptr(), ws, nat.stream_of(k_pages)),
             "cdx_paged_evict")
     return new
+
+
+class PagedRows(NamedTuple):
+    """What ``paged_reserve`` says of a call's rows; all on the device."""
+    starts: torch.Tensor                # [B] int32: the first row of each sequence
+    counts: torch.Tensor                # [B] int32: its new tokens, 0 where they were refused
+    lengths: torch.Tensor               # [B] int32: its slots in use, the new ones' counted
+    positions: torch.Tensor             # [B] int32: of its newest token
+    free_count: Optional[torch.Tensor]  # [1] int32: pages left in the pool
+    row_slots: torch.Tensor             # [rows] int64: page * page_size + row in the page, or -1
+    row_positions: torch.Tensor         # [rows] int32, or -1
+
+
+def _pool(free_pages: torch.Tensor, free_count: torch.Tensor, like: torch.Tensor, what: str) -> None:
+    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous() \
+            or free_pages.device != like.device:
+        raise ValueError(f"{what}: free_pages must be a contiguous int32 list on {like.device}, got {free_pages.dtype} "
+                         f"{tuple(free_pages.shape)} on {free_pages.device}")
+    if free_count.dtype != torch.int32 or tuple(free_count.shape) != (1,) or free_count.device != like.device:
+        raise ValueError(f"{what}: free_count must be one int32 on {like.device}, got {free_count.dtype} "
+                         f"{tuple(free_count.shape)} on {free_count.device}")
+
+
+def _table_rows(table: torch.Tensor, page_size: int, what: str, written: bool) -> None:
+    """Checks of a block table that is taken without its pages."""
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"{what}: page size {page_size} is not one of {PAGE_SIZES}")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] == 0:
+        raise ValueError(f"{what}: block_table must be an int32 tensor [sequences, pages], got {table.dtype} "
+                         f"{tuple(table.shape)}")
+    if written and not (table.shape[1] <= 1 or table.stride(1) == 1) or \
+            written and table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError(f"{what}: block_table needs rows of its own with unit stride (it is written in place), got "
+                         f"strides {table.stride()}")
+
+
+def paged_reserve(counts: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
+                  page_size: int, rows: int, *, stride: Optional[int] = None,
+                  free_pages: Optional[torch.Tensor] = None, free_count: Optional[torch.Tensor] = None) -> PagedRows:
+    """Room for ``counts`` [B] new tokens of each sequence behind its ``lengths`` [B] slots, and where each of
+    a call's ``rows`` rows goes.  The rows lie one sequence behind the other, or with ``stride`` those of
+    sequence b from row b * stride on (a padded batch).
+
+    With a pool, the pages that a sequence lacks are taken from the end of ``free_pages``, a list whose
+    first ``free_count`` [1] entries are pages that nobody has, and written into ``block_table``; without
+    one the table names every page already.  A sequence gets all of its tokens or none: none if
+    its rows or its capacity do not suffice, or if fewer pages are left than it and the sequences
+    before it ask for (one that needs no page is served all the same).
+
+    Nothing but the table is changed: the returned lengths, positions (of the newest tokens) and free_count
+    are the new ones, and a call that goes on with the old ones has undone it."""
+    fast = nat.host()
+    if fast is not None and type(page_size) is int and type(rows) is int and (stride is None or type(stride) is int):
+        done = fast.paged_reserve(counts, lengths, positions, block_table, page_size, rows, stride, free_pages,
+                                  free_count)
+        if done is not None:
+            return PagedRows(*done)
+    what = "paged_reserve"
+    nat.require_device(block_table, counts, lengths, positions, free_pages, free_count, dtype=None, what=what)
+    _table_rows(block_table, page_size, what, True)
+    B, width = block_table.shape
+    if rows < 0 or rows >= 2 ** 31 - 4096:
+        raise ValueError(f"{what}: rows={rows} is out of range")
+    if stride is not None and not 0 < stride < 2 ** 31:
+        raise ValueError(f"{what}: stride={stride} must be positive (None: rows one behind the other)")
+    if (free_pages is None) != (free_count is None):
+        raise ValueError(f"{what}: pass both free_pages and free_count or neither")
+    if free_pages is not None:
+        _pool(free_pages, free_count, block_table, what)
+    counts, lengths, positions = (_ints(t, (B,), block_table, f"{what}: {n}") for t, n in
+                                  ((counts, "counts"), (lengths, "lengths"), (positions, "positions")))
+    dev = block_table.device
+    small = torch.empty(4 * B + 1, dtype=torch.int32, device=dev)
+    starts, new_counts = small[:B], small[B:2 * B]
+    new_lengths, new_positions, new_free = small[2 * B:3 * B], small[3 * B:4 * B], small[4 * B:]
+    row_slots = torch.empty(rows, dtype=torch.int64, device=dev)
+    row_positions = torch.empty(rows, dtype=torch.int32, device=dev)
+    pool = free_pages is not None
+    with nat.on_device(block_table), nat.launch_region("paged_reserve", dev, B=B, rows=rows):
+        nat.check(nat.lib().cdx_paged_reserve(
+            counts.data_ptr(), lengths.data_ptr(), positions.data_ptr(), B, stride or 0, rows, block_table.data_ptr(),
+            _ld(block_table), width, page_size, nat.ptr(free_pages), free_pages.numel() if pool else 0,
+            nat.ptr(free_count), starts.data_ptr(), new_counts.data_ptr(), new_lengths.data_ptr(),
+            new_positions.data_ptr(), new_free.data_ptr() if pool else None, row_slots.data_ptr(),
+            row_positions.data_ptr(), nat.stream_of(block_table)), "cdx_paged_reserve")
+    return PagedRows(starts, new_counts, new_lengths, new_positions, new_free if pool else None, row_slots,
+                     row_positions)
+
+
+def paged_truncate(to: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
+                   page_size: int, free_pages: torch.Tensor, free_count: torch.Tensor
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cut every sequence of more than ``to`` [B] slots to that many and give the pages behind them back to
+    the pool (``free_pages``, in place): 0 for a sequence that has ended, fewer tokens for one whose
+    speculated ones were not accepted.  Returns the new (lengths, positions, free_count).
+
+    The pages must be the sequence's own.  The table keeps its entries: those past the new length name
+    pages that may be another's from then on."""
+    fast = nat.host()
+    if fast is not None and type(page_size) is int:
+        done = fast.paged_truncate(to, lengths, positions, block_table, page_size, free_pages, free_count)
+        if done is not None:
+            return done
+    what = "paged_truncate"
+    nat.require_device(block_table, to, lengths, positions, free_pages, free_count, dtype=None, what=what)
+    _table_rows(block_table, page_size, what, False)
+    table = block_table if block_table.stride(-1) == 1 and (
+        block_table.shape[0] == 1 or block_table.stride(0) >= block_table.shape[1]) else block_table.contiguous()
+    B, width = table.shape
+    _pool(free_pages, free_count, table, what)
+    to, lengths, positions = (_ints(t, (B,), table, f"{what}: {n}") for t, n in
+                              ((to, "to"), (lengths, "lengths"), (positions, "positions")))
+    small = torch.empty(2 * B + 1, dtype=torch.int32, device=table.device)
+    new = small[:B], small[B:2 * B], small[2 * B:]
+    with nat.on_device(table), nat.launch_region("paged_truncate", table.device, B=B):
+        nat.check(nat.lib().cdx_paged_truncate(
+            to.data_ptr(), lengths.data_ptr(), positions.data_ptr(), B, table.data_ptr(), _ld(table), width, page_size,
+            free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), *(t.data_ptr() for t in new),
+            nat.stream_of(table)), "cdx_paged_truncate")
+    return new
+
+
+def paged_chunk_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, row_slots: torch.Tensor,
+                       row_positions: torch.Tensor, num_heads: int, cos_sin: torch.Tensor,
+                       q_norm_w: Optional[torch.Tensor] = None, k_norm_w: Optional[torch.Tensor] = None,
+                       eps: float = 1e-6) -> torch.Tensor:
+    """q [rows, num_heads, D] of a call's new tokens, their k and v written to the slots ``row_slots`` [rows] of
+    the pages (paged_reserve's): what paged_qkv_append does for one token per sequence, at the positions
+    ``row_positions`` [rows].  A row without a slot gives zeros and is not stored."""
+    fast = nat.host()
+    if fast is not None:
+        q = fast.paged_chunk_append(qkv, k_pages, v_pages, row_slots, row_positions, num_heads, cos_sin, q_norm_w,
+                                    k_norm_w, eps)
+        if q is not None:
+            return q
+    what = "paged_chunk_append"
+    forward_only(what, qkv, k_pages, v_pages, q_norm_w, k_norm_w)
+    nat.require_device(k_pages, v_pages, q_norm_w, k_norm_w, what=what)
+    nat.require_device(qkv, k_pages, row_slots, row_positions, cos_sin, dtype=None, what=what)
+    _page_shapes(k_pages, v_pages, 4, what)
+    pages, nkv, page, D = k_pages.shape
+    R, N = qkv.shape[0] if qkv.dim() == 2 else -1, (num_heads + 2 * nkv) * D
+    if num_heads <= 0 or nkv == 0 or num_heads % nkv != 0:
+        raise ValueError(f"{what}: {num_heads} query heads over {nkv} KV heads")
+    if qkv.dtype not in (torch.bfloat16, torch.float32) or qkv.dim() != 2 or qkv.shape[1] != N:
+        raise ValueError(f"{what}: qkv must be bf16 or fp32 [rows, {N}], got {qkv.dtype} {tuple(qkv.shape)}")
+    _rotary(cos_sin, D, what)
+    if (q_norm_w is None) != (k_norm_w is None):
+        raise ValueError(f"{what}: pass both QK norm weights or neither")
+    if q_norm_w is not None:
+        if q_norm_w.numel() != D or k_norm_w.numel() != D:
+            raise ValueError(f"{what}: the QK norm weights must have {D} elements")
+        q_norm_w, k_norm_w = _aligned(q_norm_w), _aligned(k_norm_w)
+    if row_slots.dtype != torch.int64 or tuple(row_slots.shape) != (R,):
+        raise ValueError(f"{what}: row_slots must be int64 [{R}], got {row_slots.dtype} {tuple(row_slots.shape)}")
+    row_slots = row_slots if row_slots.is_contiguous() else row_slots.contiguous()
+    row_positions = _ints(row_positions, (R,), qkv, f"{what}: row_positions")
+    ld = qkv.stride(0) if R > 1 else N
+    if qkv.stride(-1) != 1 or ld < N or ld % 8 != 0 or qkv.data_ptr() % 16 != 0:
+        qkv, ld = _aligned(qkv), N
+    cos_sin = _aligned(cos_sin)
+    q = torch.empty(R, num_heads, D, dtype=torch.bfloat16, device=qkv.device)
+    with nat.on_device(qkv), nat.launch_region("paged_chunk_append", qkv.device, rows=R, nq=num_heads, nkv=nkv, D=D):
+        nat.check(nat.lib().cdx_paged_chunk_append_fwd(
+            qkv.data_ptr(), qkv.dtype == torch.float32, ld, R, num_heads, nkv, D, nat.ptr(q_norm_w), nat.ptr(k_norm_w),
+            float(eps), cos_sin.data_ptr(), cos_sin.shape[0], row_slots.data_ptr(), row_positions.data_ptr(), pages,
+            page, k_pages.data_ptr(), v_pages.data_ptr(), q.data_ptr(), nat.stream_of(qkv)),
+            "cdx_paged_chunk_append_fwd")
+    return q
+
+
+def paged_chunk_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                          starts: torch.Tensor, counts: torch.Tensor, lengths: torch.Tensor,
+                          scale: Optional[float] = None, *, max_tokens: Optional[int] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v of any number of new tokens per sequence, each over the slots up to its own,
+    the heads merged: [rows, nq * D].  q [rows, nq, D] bf16: sequence b's ``counts[b]`` tokens, in the last of
+    its ``lengths[b]`` slots, are rows ``starts[b]`` on (paged_reserve's; the starts ascend).  scale defaults to
+    D ** -0.5.  Rows of no sequence, and tokens without slots, give zeros.
+
+    ``max_tokens``: no sequence brings more than so many, by which the kernels are chosen (the rows, if
+    it is not known)."""
+    if scale is None:
+        scale = max(1, k_pages.shape[-1]) ** -0.5
+    fast = nat.host()
+    if fast is not None and (max_tokens is None or type(max_tokens) is int):
+        out = fast.paged_chunk_attention(q, k_pages, v_pages, block_table, starts, counts, lengths, scale, max_tokens)
+        if out is not None:
+            return out
+    what = "paged_chunk_attention"
+    forward_only(what, q, k_pages, v_pages)
+    nat.require_device(q, k_pages, v_pages, what=what)
+    nat.require_device(q, block_table, starts, counts, lengths, dtype=None, what=what)
+    table = _pages(k_pages, v_pages, block_table, 4, what)
+    pages, nkv, page, D = k_pages.shape
+    B, cap = table.shape[0], table.shape[1] * page
+    if q.dim() != 3 or q.shape[2] != D or nkv == 0 or q.shape[1] == 0 or q.shape[1] % nkv != 0:
+        raise ValueError(f"{what}: q {tuple(q.shape)} does not match {nkv} KV heads of {D}")
+    R, nq = q.shape[:2]
+    if B == 0 or table.shape[1] == 0 or pages == 0:
+        raise ValueError(f"{what}: empty block table or pool")
+    if max_tokens is not None and max_tokens < 0:
+        raise ValueError(f"{what}: max_tokens={max_tokens} must not be negative")
+    most = R if max_tokens is None else min(R, max_tokens)
+    starts, counts, lengths = (_ints(t, (B,), q, f"{what}: {n}") for t, n in
+                               ((starts, "starts"), (counts, "counts"), (lengths, "lengths")))
+    q = _aligned(q)
+    out = torch.empty(R, nq * D, dtype=q.dtype, device=q.device)
+    lib = nat.lib()
+    with nat.on_device(q):  # (the splits, and so the size, go by the current device's CUs)
+        ws = lib.cdx_paged_chunk_attention_workspace_bytes(R, B, nq, nkv, D, cap, most)
+    work = torch.empty(ws, dtype=torch.uint8, device=q.device) if ws else None
+    with nat.on_device(q), nat.launch_region("paged_chunk_attention", q.device, rows=R, B=B, nq=nq, nkv=nkv, D=D):
+        nat.check(lib.cdx_paged_chunk_attention_fwd(
+            q.data_ptr(), R, B, nq, nkv, D, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), _ld(table),
+            table.shape[1], pages, page, starts.data_ptr(), counts.data_ptr(), lengths.data_ptr(), most, float(scale),
+            out.data_ptr(), nat.ptr(work), ws, nat.stream_of(q)), "cdx_paged_chunk_attention_fwd")
+    return out
 
 
 class PagedLayer(NamedTuple):

@@ -31,15 +31,27 @@
 // 140 registers had been the better form before.
 #include <algorithm>
 
-#include "cdx_paged.h"
+#include "cdx_paged_attn.h"
 
 namespace cdx {
+
+// Blocks that a sequence and head is split over: enough for two blocks on each CU, four where
+// tables are long (lengths then differ more: 100 sequences of up to 8192 slots, 16/4 heads of 80,
+// 119 against 110 us, 4 x 65536 slots 185 against 180), each with at least two tiles per wave (four:
+// 1 x 2000 slots 11.5 against 16.4 us).  Short tables whose blocks fill the CUs are not split, which
+// saves the second kernel (32 x 1024 slots 25.7 against 22.2 us).
+int paged_splits(int64_t blocks, int64_t cap) {
+  const int64_t cus = device_cu_count();
+  if (blocks >= cus && cap <= 4 * kPagedWaves * kPagedTile) return 1;
+  const int64_t want = ((cap >= 4096 ? 4 : 2) * cus + blocks - 1) / blocks;
+  const int64_t most = (cap + 2 * kPagedWaves * kPagedTile - 1) / (2 * kPagedWaves * kPagedTile);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kPagedMaxSplits}));
+}
+
 namespace {
 
-constexpr int kTile = 32;   // slots of a wave's step
-constexpr int kWaves = 8;
+constexpr int kTile = kPagedTile, kWaves = kPagedWaves;
 constexpr int kHeads = 16;  // query heads of a block: the columns of a matrix instruction
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct PagedAttnParams {
   const uint16_t* q;  // [B][nq][D]
@@ -55,44 +67,6 @@ struct PagedAttnParams {
   float* scores;      // [B][nq][cap] in log2 units, or nullptr
   const float* w_in;  // [B][nkv][cap]
   float* w_out;
-};
-
-// Both values that lanes l and l ^ 16 (l ^ 32) hold, reduced.
-__device__ __forceinline__ float max_over_groups(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
-}
-__device__ __forceinline__ float sum_over_groups(float x) {
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
-}
-
-// The low (high) halves of two words, side by side.
-__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {
-  return __builtin_amdgcn_perm(b, a, 0x05040100u);
-}
-__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
-  return __builtin_amdgcn_perm(b, a, 0x07060302u);
-}
-// Both bf16 of a word, Inf and NaN as the largest finite value of their sign: as signed integers the
-// positive ones lie above it, as unsigned integers the negative ones.
-__device__ __forceinline__ uint32_t finite_halves(uint32_t x) {
-  typedef __attribute__((ext_vector_type(2))) short i16x2;
-  typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
-  const i16x2 i = __builtin_elementwise_min(__builtin_bit_cast(i16x2, x), i16x2{0x7f7f, 0x7f7f});
-  const u16x2 u = __builtin_elementwise_min(__builtin_bit_cast(u16x2, i), u16x2{0xff7f, 0xff7f});
-  return __builtin_bit_cast(uint32_t, u);
-}
-
-template <int DPL>
-struct Piece;
-template <>
-struct Piece<4> {
-  typedef uint2 type;
-};
-template <>
-struct Piece<8> {
-  typedef uint4 type;
 };
 
 // NC: pieces of 32 dims in a head; DPL: columns of V that a lane holds (16 DPL >= D); W: waves; FULL: D == 32 NC ==
@@ -294,8 +268,8 @@ __global__ __launch_bounds__(64 * W, NC == 4 && !FULL ? 2 : 4) void paged_attn_k
 }
 
 constexpr int kJoinThreads = 256;
+constexpr int kMaxSplits = kPagedMaxSplits;
 constexpr int kJoinSlots = 512;  // slots of the weights that a block adds up
-constexpr int kMaxSplits = 256;
 
 // Maximum (log2 units, 0 where there is none) and sum of a row of scores from its splits' own, by
 // a whole wave, returned to every lane.
@@ -397,19 +371,6 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAtt
     const int32_t s = s0 + u * kJoinThreads;
     if (s < cap) p.w_out[(int64_t)slab * cap + s] = w[u];
   }
-}
-
-// Blocks that a sequence and head is split over: enough for two blocks on each CU, four where
-// tables are long (lengths then differ more: 100 sequences of up to 8192 slots, 16/4 heads of 80,
-// 119 against 110 us, 4 x 65536 slots 185 against 180), each with at least two tiles per wave (four:
-// 1 x 2000 slots 11.5 against 16.4 us).  Short tables whose blocks fill the CUs are not split, which
-// saves the second kernel (32 x 1024 slots 25.7 against 22.2 us).
-int paged_splits(int64_t blocks, int64_t cap) {
-  const int64_t cus = device_cu_count();
-  if (blocks >= cus && cap <= 4 * kWaves * kTile) return 1;
-  const int64_t want = ((cap >= 4096 ? 4 : 2) * cus + blocks - 1) / blocks;
-  const int64_t most = (cap + 2 * kWaves * kTile - 1) / (2 * kWaves * kTile);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }

@@ -501,6 +501,109 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(const Tensor& k, c
   return std::make_tuple(new_len, new_w, new_pos);
 }
 
+// A block table taken without its pages: int32 rows of unit stride, apart from each other.
+inline bool table_rows(const Tensor& t, int64_t page) {
+  return plain(t, at::kInt) && t.dim() == 2 && t.size(0) > 0 && t.size(1) > 0 && t.stride(1) == 1 &&
+         (t.size(0) == 1 || t.stride(0) >= t.size(1)) && page >= 16 && page <= 256 && (page & (page - 1)) == 0;
+}
+inline int64_t table_ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+inline bool page_list(const Tensor& pages, const Tensor& count) {
+  return plain(pages, at::kInt) && pages.dim() == 1 && pages.is_contiguous() && pages.numel() > 0 &&
+         per_sequence(count, 1);
+}
+
+// (starts, counts, lengths, positions, free count or None, row slots, row positions)
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor, Tensor, Tensor>> paged_reserve(
+    const Tensor& counts, const Tensor& lengths, const Tensor& positions, const Tensor& table, int64_t page,
+    int64_t rows, std::optional<int64_t> stride, const OptTensor& free_pages, const OptTensor& free_count) {
+  if (!table_rows(table, page) || rows < 0 || rows > INT32_MAX - 4096 ||
+      (stride && (*stride <= 0 || *stride > INT32_MAX)) || free_pages.has_value() != free_count.has_value())
+    return {};
+  const int64_t B = table.size(0);
+  if (!per_sequence(counts, B) || !per_sequence(lengths, B) || !per_sequence(positions, B) ||
+      (free_pages && !page_list(*free_pages, *free_count)))
+    return {};
+  Tensor small = ints(table, {4 * B + 1}), row_positions = ints(table, {rows});
+  Tensor row_slots = at::empty({rows}, table.options().dtype(at::kLong).requires_grad(false));
+  int32_t* out = small.data_ptr<int32_t>();
+  check(cdx_paged_reserve(counts.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), B,
+                          stride.value_or(0), rows, table.data_ptr<int32_t>(), table_ld(table), table.size(1),
+                          (int32_t)page, free_pages ? free_pages->data_ptr<int32_t>() : nullptr,
+                          free_pages ? free_pages->numel() : 0, free_count ? free_count->data_ptr<int32_t>() : nullptr,
+                          out, out + B, out + 2 * B, out + 3 * B, free_pages ? out + 4 * B : nullptr,
+                          row_slots.data_ptr<int64_t>(), row_positions.data_ptr<int32_t>(), stream()),
+        "cdx_paged_reserve");
+  OptTensor left;
+  if (free_pages) left = small.narrow(0, 4 * B, 1);
+  return std::make_tuple(small.narrow(0, 0, B), small.narrow(0, B, B), small.narrow(0, 2 * B, B),
+                         small.narrow(0, 3 * B, B), left, row_slots, row_positions);
+}
+
+std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_truncate(const Tensor& to, const Tensor& lengths,
+                                                                 const Tensor& positions, const Tensor& table,
+                                                                 int64_t page, const Tensor& free_pages,
+                                                                 const Tensor& free_count) {
+  if (!table_rows(table, page) || !page_list(free_pages, free_count)) return {};
+  const int64_t B = table.size(0);
+  if (!per_sequence(to, B) || !per_sequence(lengths, B) || !per_sequence(positions, B)) return {};
+  Tensor small = ints(table, {2 * B + 1});
+  int32_t* out = small.data_ptr<int32_t>();
+  check(cdx_paged_truncate(to.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), B,
+                           table.data_ptr<int32_t>(), table_ld(table), table.size(1), (int32_t)page,
+                           free_pages.data_ptr<int32_t>(), free_pages.numel(), free_count.data_ptr<int32_t>(), out,
+                           out + B, out + 2 * B, stream()),
+        "cdx_paged_truncate");
+  return std::make_tuple(small.narrow(0, 0, B), small.narrow(0, B, B), small.narrow(0, 2 * B, 1));
+}
+
+OptTensor paged_chunk_append(const Tensor& qkv, const Tensor& k, const Tensor& v, const Tensor& row_slots,
+                             const Tensor& row_positions, int64_t nq, const Tensor& cos_sin, const OptTensor& qn,
+                             const OptTensor& kn, double eps) {
+  const bool fp32 = qkv.defined() && qkv.scalar_type() == at::kFloat;
+  if (!dense(k) || !dense(v) || !no_grad(k) || !no_grad(v) || k.dim() != 4 || v.sizes() != k.sizes() || k.numel() == 0 ||
+      !dense(qkv, fp32 ? at::kFloat : at::kBFloat16) || !no_grad(qkv) || qkv.dim() != 2 || qkv.size(0) == 0)
+    return {};
+  const int64_t rows = qkv.size(0), nkv = k.size(1), page = k.size(2), D = k.size(3);
+  if (page < 16 || page > 256 || (page & (page - 1)) != 0 || D % 8 != 0 || D > 128 || nkv > 65535 || nq <= 0 ||
+      nq > 65535 || nq % nkv != 0 || qkv.size(1) != (nq + 2 * nkv) * D || !plain(row_slots, at::kLong) ||
+      !row_slots.is_contiguous() || row_slots.dim() != 1 || row_slots.size(0) != rows ||
+      !per_sequence(row_positions, rows) || !dense(cos_sin, at::kFloat) || cos_sin.dim() != 3 || cos_sin.size(0) == 0 ||
+      cos_sin.size(1) != D / 2 || cos_sin.size(2) != 2 || qn.has_value() != kn.has_value() || !(eps >= 0))
+    return {};
+  if (qn && (!dense(*qn) || !dense(*kn) || qn->numel() != D || kn->numel() != D || !no_grad(*qn) || !no_grad(*kn)))
+    return {};
+  Tensor q = like(k, {rows, nq, D});
+  check(cdx_paged_chunk_append_fwd(qkv.data_ptr(), fp32, qkv.size(1), rows, (int32_t)nq, (int32_t)nkv, (int32_t)D,
+                                   u16(qn), u16(kn), (float)eps, cos_sin.data_ptr<float>(), cos_sin.size(0),
+                                   row_slots.data_ptr<int64_t>(), row_positions.data_ptr<int32_t>(), k.size(0),
+                                   (int32_t)page, w16(k), w16(v), w16(q), stream()),
+        "cdx_paged_chunk_append_fwd");
+  return q;
+}
+
+OptTensor paged_chunk_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table,
+                                const Tensor& starts, const Tensor& counts, const Tensor& lengths, double scale,
+                                std::optional<int64_t> max_tokens) {
+  Pages c;
+  if (!paged_cache(k, v, table, 4, &c) || !dense(q) || !no_grad(q) || q.dim() != 3 || q.size(0) == 0 ||
+      q.size(2) != c.D || q.size(1) == 0 || q.size(1) > 65535 || q.size(1) % c.nkv != 0 ||
+      !per_sequence(starts, c.B) || !per_sequence(counts, c.B) || !per_sequence(lengths, c.B) ||
+      (max_tokens && *max_tokens < 0))
+    return {};
+  const int64_t rows = q.size(0), nq = q.size(1), most = std::min(rows, max_tokens.value_or(rows));
+  Tensor out = like(q, {rows, nq * c.D});
+  const size_t bytes = cdx_paged_chunk_attention_workspace_bytes(rows, c.B, (int32_t)nq, (int32_t)c.nkv, (int32_t)c.D,
+                                                                 c.capacity(), most);
+  Tensor work;
+  if (bytes) work = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte).requires_grad(false));
+  check(cdx_paged_chunk_attention_fwd(u16(q), rows, c.B, (int32_t)nq, (int32_t)c.nkv, (int32_t)c.D, c.k, c.v, c.table,
+                                      c.ld, c.width, c.pages, (int32_t)c.page, starts.data_ptr<int32_t>(),
+                                      counts.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), most, (float)scale,
+                                      w16(out), bytes ? work.data_ptr() : nullptr, bytes, stream()),
+        "cdx_paged_chunk_attention_fwd");
+  return out;
+}
+
 // The attention of one new token per sequence on a layer of a paged cache, up to o_proj: the
 // projection of x [B, 1, H] (of RMSNorm(x) with `norm`, B <= 8), its append and the attention, whose
 // weights go to `weights`.  w as in `attention`.
@@ -742,5 +845,9 @@ PYBIND11_MODULE(_host, m) {
   m.def("paged_write", &paged_write);
   m.def("paged_attention", &paged_attention);
   m.def("paged_evict", &paged_evict);
+  m.def("paged_reserve", &paged_reserve);
+  m.def("paged_truncate", &paged_truncate);
+  m.def("paged_chunk_append", &paged_chunk_append);
+  m.def("paged_chunk_attention", &paged_chunk_attention);
   m.def("sample_tokens", &sample_tokens);
 }

@@ -618,6 +618,79 @@ int cdx_paged_evict(int64_t layers, int64_t B, int32_t nkv, int32_t hd, const in
                     void* work_dev, size_t work_bytes, void* stream);
 
 /*
+ * Calls that bring any number of new tokens per sequence.  Their rows lie sequence by sequence in one
+ * array: counts[b] rows from row starts[b] on, one sequence behind the other or each in a field of
+ * its own.
+ *
+ * cdx_paged_reserve: the pages for counts[b] tokens more (< 0 counts as 0) behind the lengths[b] (< 0
+ * as 0) that sequence b has, and the map of the call's rows.
+ *   stride        0: sequences one behind the other; else sequence b's rows begin at b * stride
+ *   free_pages    the pool's list: its first *free_count entries are pages that nobody has.  In order of
+ *                 b, the pages ceil(lengths / page_size) .. of a sequence are taken from the end of
+ *                 the list and written into its row of the table.  free_count NULL: no pool, the
+ *                 table names every page already.
+ * A sequence gets all of its tokens or none: none if its rows end past `rows` (or its stride), if its
+ * capacity is too small, or if its pages and those asked for by the sequences before it are more than
+ * the list has (a sequence that needs no page is not refused for that).
+ *   starts, new_counts, new_lengths, new_positions [B], new_free_count [1]: as they are after the call,
+ *                 refused sequences with 0 tokens and unchanged (positions: of the newest tokens).  The
+ *                 list itself stays as it is; with the old counts the call is undone.
+ *   row_slots, row_positions [rows]: page * page_size + row in the page, and the position, of every row's
+ *                 token; -1 for rows without one (and a slot of -1 where the page is negative).
+ * cdx_paged_truncate: sequences of more than to[b] slots cut to that many (< 0 counts as 0), their
+ * positions by as much, and the pages behind ceil(to / page_size) put back at the end of the list, the
+ * first sequence's first page last: what reserve took it finds again.  Table entries past the new length
+ * stay as they are and name pages that may be another's.  Pages that come back must be the
+ * sequence's own; past free_capacity, the list's room, they are dropped.
+ *
+ * No counterpart in the reference, which has one cache tensor per batch.
+ */
+int cdx_paged_reserve(const int32_t* counts_dev, const int32_t* lengths_dev, const int32_t* positions_dev, int64_t B,
+                      int64_t stride, int64_t rows, int32_t* table_dev, int64_t table_ld, int64_t width,
+                      int32_t page_size, const int32_t* free_pages_dev, int64_t free_capacity,
+                      const int32_t* free_count_dev, int32_t* starts_dev, int32_t* new_counts_dev,
+                      int32_t* new_lengths_dev, int32_t* new_positions_dev, int32_t* new_free_count_dev,
+                      int64_t* row_slots_dev, int32_t* row_positions_dev, void* stream);
+int cdx_paged_truncate(const int32_t* to_dev, const int32_t* lengths_dev, const int32_t* positions_dev, int64_t B,
+                       const int32_t* table_dev, int64_t table_ld, int64_t width, int32_t page_size,
+                       int32_t* free_pages_dev, int64_t free_capacity, const int32_t* free_count_dev,
+                       int32_t* new_lengths_dev, int32_t* new_positions_dev, int32_t* new_free_count_dev,
+                       void* stream);
+
+/*
+ * The append of such a call's rows from their packed projections, as cdx_paged_append_fwd does it for
+ * one token per sequence: q normalised and rotated to q_out [rows, nq, hd], k and v to slot
+ * row_slots[r].  A row without a slot (< 0, or not of the pool) gives zeros in q_out and is not stored;
+ * two rows must not have the same slot.
+ */
+int cdx_paged_chunk_append_fwd(const void* qkv_dev, int32_t qkv_fp32, int64_t ldqkv, int64_t rows, int32_t nq,
+                               int32_t nkv, int32_t hd, const uint16_t* q_norm_w_dev, const uint16_t* k_norm_w_dev,
+                               float eps, const float* cos_sin_dev, int64_t n_pos, const int64_t* row_slots_dev,
+                               const int32_t* row_positions_dev, int64_t num_pages, int32_t page_size,
+                               uint16_t* k_pages_dev, uint16_t* v_pages_dev, uint16_t* q_out_dev, void* stream);
+
+/*
+ * Attention of such a call's rows.  Row starts[b] + i, i < counts[b], is the token in slot
+ * lengths[b] - counts[b] + i (the lengths count the new tokens) and attends to the slots up to its own.
+ * q, out [rows, nq, hd] bf16; starts ascend, each sequence's rows ending before the next one's begin.
+ * (A count below 0 counts as 0.)  Rows that belong to no sequence, and tokens without a slot up to their own, give zeros; a page outside
+ * the pool gives NaN in the rows that attend to it.  Infinite values and NaN in slots that a row does not
+ * attend to do not reach it.
+ *   max_tokens   no sequence brings more tokens (a hint by which the kernel is chosen; `rows` if unknown)
+ * work: cdx_paged_chunk_attention_workspace_bytes bytes (may be 0), used until the call's work is done.
+ *
+ * No counterpart in the reference, whose cached calls keep the top-left mask (core/attention.py:170-175).
+ */
+size_t cdx_paged_chunk_attention_workspace_bytes(int64_t rows, int64_t B, int32_t nq, int32_t nkv, int32_t hd,
+                                                 int64_t capacity, int64_t max_tokens);
+int cdx_paged_chunk_attention_fwd(const uint16_t* q_dev, int64_t rows, int64_t B, int32_t nq, int32_t nkv, int32_t hd,
+                                  const uint16_t* k_pages_dev, const uint16_t* v_pages_dev, const int32_t* table_dev,
+                                  int64_t table_ld, int64_t width, int64_t num_pages, int32_t page_size,
+                                  const int32_t* starts_dev, const int32_t* counts_dev, const int32_t* lengths_dev,
+                                  int64_t max_tokens, float scale, uint16_t* out_dev, void* work_dev,
+                                  size_t work_bytes, void* stream);
+
+/*
  * tokens[b] from logits [B, V] at stride ld (bf16, or fp32 with logits_fp32) and uniforms[b] in
  * [0, 1): w_i = exp((x_i - max) / T), cut by top-k (all that tie with the k-th stay), then top-p
  * (descending, equal ones by index: a token stays while the sum before it is <= p * total), then

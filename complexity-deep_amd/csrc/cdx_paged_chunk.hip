@@ -180,6 +180,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
   const int D = FULL ? 32 * NC : p.D;
   const uint32_t k_at = n * D + g * 8, v_at = 4 * g * D + n * DPL;
   const bool v_on = FULL || n * DPL < D;
+  int32_t wild = INT32_MAX;  // the first tile whose infinite values and NaN were left out
 
   for (int32_t tile = (int32_t)split * per + wave; tile < t_end; tile += W) {
     const int32_t s0 = tile * kPagedTile;
@@ -239,9 +240,9 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
 #pragma unroll
         for (int w = 0; w < RW; ++w) special = special || (slot >= min_seen && any_special(vw[i * RW + w]));
       }
-      // Infinite values and NaN of a slot that some queries see and others do not: added one by one.
-      special = __builtin_amdgcn_ballot_w64(special) != 0;
-      if (special) {
+      // Infinite values and NaN of a slot that some queries see and others do not are added at the end.
+      if (__builtin_amdgcn_ballot_w64(special) != 0) {
+        wild = min(wild, tile);
 #pragma unroll
         for (int w = 0; w < 8 * RW; ++w) vw[w] = without_special(vw[w]);
       }
@@ -261,27 +262,6 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
     for (int i = 0; i < 8; ++i) {
       pf[i] = __builtin_amdgcn_exp2f(s[i] - m_ref);
       l += pf[i];
-    }
-    if (special) {
-#pragma unroll 1
-      for (int slot = 0; slot < kPagedTile; ++slot) {
-        if (s0 + slot >= max_seen || !there[slot >> 4]) continue;
-        // Query n's weight of the slot lies with the lanes of group (slot % 16) / 4.
-        float w = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w = i == 4 * (slot >> 4) + (slot & 3) ? pf[i] : w;
-        w = __shfl(w, n + 4 * (slot & 12), 64);
-        if (s0 + slot >= seen) continue;
-        const uint16_t* v_row = v_base[slot >> 4] + (slot & 15) * D;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int j = 0; j < DPL; ++j) {
-            const int d = (4 * g + r) * DPL + j;
-            const uint32_t x = d < D ? v_row[d] : 0u;
-            if ((x & 0x7f80u) == 0x7f80u) acc[j][r] = __builtin_fmaf(w, bf16_bits_to_f32(x), acc[j][r]);
-          }
-      }
     }
     // P in two bf16 parts, to 2^-16 of it.
     const uint4 p_hi = pack8(pf);
@@ -310,6 +290,24 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
       // value: an infinite value counts once, by the high part, and is a finite one here.
       a = make_uint4(finite_halves(a.x), finite_halves(a.y), finite_halves(a.z), finite_halves(a.w));
       acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pb_low, acc[j], 0, 0, 0);
+    }
+  }
+
+  // An infinite value or NaN makes the column so of each query that sees it, whatever its weight: added as
+  // it is (twice is once where a product has added it already).
+  for (int32_t tile = wild; tile < t_end; tile += W) {
+#pragma unroll 1
+    for (int32_t slot = tile * kPagedTile; slot < min(tile * kPagedTile + kPagedTile, max_seen); ++slot) {
+      const int64_t row = p.t.row(ct.b, h, p.nkv, slot);
+      if (row < 0 || slot >= seen) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) {
+          const int d = (4 * g + r) * DPL + j;
+          const uint32_t x = d < D ? p.v_pages[row * D + d] : 0u;
+          if ((x & 0x7f80u) == 0x7f80u) acc[j][r] += bf16_bits_to_f32(x);
+        }
     }
   }
 
@@ -434,6 +432,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
 
   f32x16 o[RB][NDB];
   float m_run[RB], m_ref[RB], l_run[RB], mx[RB];
+  int32_t wild = INT32_MAX;  // the first tile whose infinite values and NaN were left out
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     m_run[rb] = -INFINITY, m_ref[rb] = 0.f, l_run[rb] = 0.f, mx[rb] = -INFINITY;
@@ -493,7 +492,11 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
       const int32_t s = (t0 + t) * kKeys + wave * 16;
       const int64_t row = (((int64_t)max(pg, 0) * p.nkv + h) << lp) + (s & ((1 << lp) - 1));
       const int32_t rows = pg < 0 ? 0 : min(max(block_seen - s, 0), 16);
-      const __amdgpu_buffer_rsrc_t rs = make_rsrc(pages + row * D, (uint32_t)(rows * D * 2));
+      // (The whole wave's: said so, as a descriptor that the compiler takes for a lane's costs a loop over lanes.)
+      const uint64_t base = (uint64_t)(pages + row * D);
+      const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), up = __builtin_amdgcn_readfirstlane(base >> 32);
+      const uint32_t bytes = __builtin_amdgcn_readfirstlane(rows * D * 2);
+      const __amdgpu_buffer_rsrc_t rs = make_rsrc((const void*)((uint64_t)up << 32 | lo), bytes);
 #pragma unroll
       for (int j = 0; j < DMAS; ++j) buf_dma16(rs, off[j], 0u, dst + (wave * DMAS + j) * 1024);
     };
@@ -552,13 +555,20 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
     // ---- softmax -------------------------------------------------------------------
     // Score v of key block kb in a lane is key 32 kb + 8 (v / 4) + 4 hi + v % 4 of query r32.
     // What tile t's queries see of it, and their maxima in log2 units.
-    auto row_max = [&](int set, int32_t t, bool mask) __attribute__((always_inline)) {
-      if (mask) {
-        uint32_t gone = 0;  // bit w: keys 16 w .. of the tile lie on a page that is not there
+    auto row_max = [&](int set, int32_t t, bool bad) __attribute__((always_inline)) {
+      if (__builtin_expect(bad, 0)) {
+#pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const int64_t key = (int64_t)(t0 + t) * kKeys + 16 * w;
-          if (key < block_seen && (uint32_t)table[key >> lp] >= (uint32_t)p.t.num_pages) gone |= 1u << w;
+          const int32_t key = (t0 + t) * kKeys + 16 * w;
+          if (key < block_seen && (uint32_t)table[key >> lp] >= (uint32_t)p.t.num_pages)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+              for (int v = 0; v < 16; ++v)
+                if (v / 8 == (w & 1)) s[set][rb][w >> 1][v] = __builtin_nanf("");
         }
+      }
+      if (t >= full || bad) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           const int32_t lim = seen[rb] - (t0 + t) * kKeys - 4 * hi;
@@ -567,8 +577,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
               const int c = kb * 32 + 8 * (v >> 2) + (v & 3);
-              const float x = gone >> (c / 16) & 1 ? __builtin_nanf("") : s[set][rb][kb][v];
-              s[set][rb][kb][v] = c >= lim ? -INFINITY : x;
+              s[set][rb][kb][v] = c >= lim ? -INFINITY : s[set][rb][kb][v];
             }
         }
       }
@@ -617,8 +626,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
       reinterpret_cast<uint32_t*>(&pf[rb][sl])[j] = w;
     };
     // Infinite values and NaN in a tile that some queries do not see whole (0 of P times them has no
-    // value): they leave a slab's V^T here, and once its products are done they are added one by
-    // one, where they are seen.
+    // value) leave V^T, slab by slab, and are added at the end.
     auto tame = [&](int sl) __attribute__((always_inline)) {
       typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
       uint32_t* w = reinterpret_cast<uint32_t*>(vfr[sl & 1]);
@@ -631,36 +639,6 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
       for (int i = 0; i < 4 * NDB; ++i) w[i] = without_special(w[i]);
       return true;
     };
-    auto add_specials = [&](int buf, int32_t t) __attribute__((always_inline)) {
-#pragma unroll 1
-      for (int row = 0; row < kKeys; ++row) {
-        // The key's weight lies with the lanes of half row / 4 % 2, as value row % 4 + 4 (row / 8 % 2) of its slab.
-        const int from = r32 + 32 * (row >> 2 & 1), word = 4 * (row >> 4) + 2 * (row >> 3 & 1) + (row >> 1 & 1);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          uint32_t pair = 0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pair = i == word ? reinterpret_cast<const uint32_t*>(&pf[rb][i / 4])[i % 4] : pair;
-          pair = (uint32_t)__shfl((int)pair, from, 64);
-          const float weight = __uint_as_float(row & 1 ? pair & 0xffff0000u : pair << 16);
-          if ((t0 + t) * kKeys + row >= seen[rb]) continue;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int c = (4 * db + g) ^ (CPR > 4 ? 4 * (row / RPL % (CPR / 4)) : 0);
-              const uint2 x =
-                  *reinterpret_cast<const uint2*>(lds + 2 * TILE + buf * TILE + row * ROWB + c * 16 + hi * 8);
-              const uint32_t e[4] = {x.x & 0xffffu, x.x >> 16, x.y & 0xffffu, x.y >> 16};
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if ((e[i] & 0x7f80u) == 0x7f80u)
-                  o[rb][db][4 * g + i] = __builtin_fmaf(weight, bf16_bits_to_f32(e[i]), o[rb][db][4 * g + i]);
-            }
-        }
-      }
-    };
-
     // ---- pipeline --------------------------------------------------------------------
     // Tile t's softmax and O += V(t)^T P(t), with the QK products of tile t + 1 between.  Its DMAs, issued
     // behind its barrier, fetch K(t + 2) into the buffer of K(t) and V(t + 1) into that of V(t - 1); both
@@ -683,7 +661,6 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
       constexpr int QK = next ? RB * 2 * NKD : 0, PV = RB * NDB, PAIRS = 16 * RB;
       constexpr int SPAN = QK + 3 * PV;  // products before the last slab's
       const bool masked = t >= full || bad_next;  // (bad_next: of tile t until sync has gone on)
-      bool wild = false;
       sync(t, cur);
       if constexpr (next) {
 #pragma unroll
@@ -708,14 +685,13 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
           const int sl = (i - QK) / PV, at = (i - QK) % PV;
           if (at == 0) {
             if (sl < 3) v_read(cur, sl + 1);
-            if (__builtin_expect(masked, 0)) wild |= tame(sl);
+            if (__builtin_expect(masked, 0) && tame(sl)) wild = min(wild, t);
           }
           pv(sl, at);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (__builtin_expect(wild, 0)) add_specials(cur, t);
-      if constexpr (next) row_max(nxt, t + 1, t + 1 >= full || bad_next);
+      if constexpr (next) row_max(nxt, t + 1, bad_next);
     };
 
     look_up();
@@ -738,7 +714,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
         if (i % RB == 0 && i / RB + KRING - 1 < 2 * NKD) k_read(0, i / RB + KRING - 1);
         qk(0, i);
       }
-      row_max(0, 0, 0 >= full || bad_next);
+      row_max(0, 0, bad_next);
     }
     // Every wave passes sync(t) once for each t < nt, in order, so the barriers pair up.
     int32_t t = 0;
@@ -758,6 +734,22 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
       ++t;
     }
     for (; t < nt; ++t) sync(t, t & 1);
+  }
+
+  // As in the few kernel: added as they are, whatever their weights.
+  for (int32_t slot = wild < ntw ? (t0 + wild) * kKeys : INT32_MAX; slot < min((t0 + ntw) * kKeys, wave_seen); ++slot) {
+    const int64_t row = p.t.row(ct.b, h, p.nkv, slot);
+    if (row < 0) continue;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int d = 32 * db + 8 * (v >> 2) + 4 * hi + (v & 3);
+          const uint32_t x = !GEN || d < D ? p.v_pages[row * D + d] : 0u;
+          if (slot < seen[rb] && (x & 0x7f80u) == 0x7f80u) o[rb][db][v] += bf16_bits_to_f32(x);
+        }
   }
 
   // ---- O^T / l ---------------------------------------------------------------------
@@ -931,7 +923,7 @@ ChunkPlan chunk_plan(int64_t rows, int64_t B, int64_t nq, int64_t nkv, int64_t h
   }
   if (c.tile) {
     c.tiles = rows * group / 128 + B;
-    c.splits = tile_splits(c.tiles * nkv, cap);
+    c.splits = tile_splits(((rows * group + 127) / 128 + (B - 1) / 2) * nkv, cap);
     c.rows = rows * nq;
     if (c.splits > 1) {
       c.o = round16((size_t)(c.splits * c.rows * hd) * sizeof(float));

@@ -5,13 +5,15 @@
 // t(r) = length[b] - count[b] + i being the slot of row r, the i-th new token of sequence b: it attends to
 // everything before it and to itself.  Sequences bring different numbers of rows, which only the
 // device knows.  The (row, query head) pairs of one (sequence, KV head) are its queries, row by
-// row, so that a tile of queries shares K and V over the heads of the group as well as over rows;
-// tiles are numbered so that a block finds its sequence from the first rows alone (chunk_tile).
+// row, so that a tile of queries shares K and V over the heads of the group as well as over rows.
 //
-//   paged_chunk_few_kernel  16 queries a block: the cache's bytes bound it.  paged_attn_kernel's walk of the
-//                           pages with the columns of the matrix instruction taken by queries of several rows.
+//   paged_chunk_tile_kernel  tiles of 128 queries, K and V through LDS.
+//   paged_chunk_few_kernel   for calls of few keys and queries, which wait for latency: 16 queries a block,
+//                            paged_attn_kernel's walk of the pages with the columns of the matrix
+//                            instruction taken by queries of several rows.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "cdx_gemm.h"
 #include "cdx_paged_attn.h"
@@ -27,16 +29,15 @@ struct ChunkParams {
   const int32_t* starts;   // [B], ascending
   const int32_t* counts;   // [B]
   const int32_t* lengths;  // [B], the new tokens counted
-  int32_t B, rows, nq, nkv, D, group, splits;
-  int32_t few;       // sequences of so many queries are the few kernel's (0: none)
-  bool by_sequence;  // the few kernel takes those sequences alone, a block each and head
-  uint32_t tiles;    // numbers that a tile may have
+  int32_t B, rows, nq, nkv, D, group;
+  int32_t splits;   // of a tile's slots, at most
+  int32_t piece;    // of the tile kernel: tiles of keys of a split
+  uint32_t tiles;   // of the tile kernel: numbers that a tile may have
   float scale_log2;
   uint16_t* out;    // [rows][nq][D]
-  // Of each split, by (row, head), or by sequence [B][nkv][kFew]:
-  int64_t part_rows;
-  float* part_o;    // [splits][part_rows][D], unnormalised
-  float2* part_ml;  // [splits][part_rows]: maximum (log2 units) and sum; a sum of -1: no key at all
+  // Partial sums by split, row and head.
+  float* part_o;    // [splits][rows][nq][D], unnormalised
+  float2* part_ml;  // maximum (log2 units) and sum; a sum of -1: no key at all
 };
 
 constexpr int kFew = 16;  // queries of a block: the columns of a matrix instruction
@@ -52,7 +53,7 @@ struct ChunkTile {
   // The token that query m belongs to; outside 0 .. count - 1: none.
   __device__ __forceinline__ int32_t token(int32_t m, int group) const { return begin + m / group - first; }
   __device__ __forceinline__ int32_t slots_of(int32_t token, int32_t cap) const {
-    return min(max(before + token + 1, 0), cap);
+    return (int32_t)min(max((int64_t)before + token + 1, (int64_t)0), (int64_t)cap);
   }
   // Slots that query m sees; 0: a row without a token, or a token without slots.
   __device__ __forceinline__ int32_t seen(int32_t m, int group, int32_t cap) const {
@@ -60,42 +61,35 @@ struct ChunkTile {
     const int32_t i = token(m, group);
     return (uint32_t)i < (uint32_t)count ? slots_of(i, cap) : 0;
   }
+  // Slots that any of queries m .. to - 1 sees.
+  __device__ __forceinline__ int32_t most_seen(int32_t m, int32_t to, int group, int32_t cap) const {
+    const int32_t from = max(token(m, group), 0), last = min(token(to - 1, group), count - 1);
+    return m < to && from <= last ? slots_of(last, cap) : 0;
+  }
 };
 
-__device__ __forceinline__ ChunkTile chunk_sequence(const ChunkParams& p, int b) {
-  ChunkTile t;
-  t.b = b;
-  t.first = p.starts[b];
-  t.count = max(p.counts[b], 0);
-  t.before = (int32_t)min(max((int64_t)p.lengths[b] - t.count, (int64_t)INT32_MIN / 2), (int64_t)INT32_MAX / 2);
-  t.begin = b == 0 ? 0 : min(max(t.first, 0), p.rows);
-  const int32_t end = b + 1 < p.B ? min(max(p.starts[b + 1], t.begin), p.rows) : p.rows;
-  t.queries = (end - t.begin) * p.group;  // (rows * nq fits 31 bits)
-  t.m0 = 0;
-  return t;
-}
-
-// The last sequence whose number is at most x, by the whole wave: 64 of them are looked at a time.
-template <typename F>
-__device__ __forceinline__ int last_sequence(int B, int64_t x, int lane, F number) {
-  int lo = 0, n = B;
+// Sequence b's tiles begin at number first_row * group / BM + b: ascending, and at least as far apart
+// as the tiles of the rows between.  The whole wave looks at 64 sequences at a time.
+template <int BM>
+__device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t tile, int lane) {
+  auto number = [&](int b) { return (int64_t)p.starts[b] * p.group / BM + b; };
+  int lo = 0, n = p.B;
   while (n > 1) {
     const int step = (n + 63) >> 6, b = lo + lane * step;
-    const bool upto = lane == 0 || (b < lo + n && number(b) <= x);
+    const bool upto = lane == 0 || (b < lo + n && number(b) <= tile);
     const int at = (__popcll(__ballot(upto)) - 1) * step;
     lo += at;
     n = min(step, n - at);
   }
-  return __builtin_amdgcn_readfirstlane(lo);
-}
-
-// Sequence b's tiles begin at number first_row * group / BM + b: ascending, and at least as far apart as
-// the tiles of the rows between.
-template <int BM>
-__device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t tile, int lane) {
-  auto number = [&](int b) { return (int64_t)p.starts[b] * p.group / BM + b; };
-  const int b = last_sequence(p.B, tile, lane, number);
-  ChunkTile t = chunk_sequence(p, b);
+  const int b = __builtin_amdgcn_readfirstlane(lo);
+  ChunkTile t;
+  t.b = b;
+  t.first = p.starts[b];
+  t.count = max(p.counts[b], 0);
+  t.before = (int32_t)max((int64_t)p.lengths[b] - t.count, (int64_t)INT32_MIN);
+  t.begin = b == 0 ? 0 : min(max(t.first, 0), p.rows);
+  const int32_t end = b + 1 < p.B ? min(max(p.starts[b + 1], t.begin), p.rows) : p.rows;
+  t.queries = (end - t.begin) * p.group;  // (rows * nq fits 31 bits)
   const int64_t at = b == 0 ? tile : tile - number(b);
   t.m0 = at < 0 || at * BM >= t.queries ? t.queries : (int32_t)at * BM;
   return t;
@@ -128,16 +122,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
   const uint32_t split = blockIdx.x % p.splits;
   const uint32_t rest = blockIdx.x / p.splits;
   const int h = rest % p.nkv;
-  ChunkTile ct;
-  if (p.by_sequence) {
-    ct = chunk_sequence(p, rest / p.nkv);
-    if ((int64_t)ct.count * p.group > kFew || ct.first < ct.begin) return;
-    const int64_t m0 = (int64_t)(ct.first - ct.begin) * p.group;
-    ct.m0 = m0 < ct.queries ? (int32_t)m0 : ct.queries;
-    ct.queries = min(ct.queries, ct.m0 + ct.count * p.group);
-  } else {
-    ct = chunk_tile<kFew>(p, rest / p.nkv, lane);
-  }
+  const ChunkTile ct = chunk_tile<kFew>(p, rest / p.nkv, lane);
   if (!ct.any()) return;
   const int queries = min(kFew, ct.queries - ct.m0);
   const int32_t cap = p.t.capacity();
@@ -339,7 +324,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
     const int64_t row = query(c);
     const bool sees = ct.seen(ct.m0 + c, p.group, cap) > 0;
     if (p.splits > 1) {
-      const int64_t at = split * p.part_rows + (p.by_sequence ? ((int64_t)ct.b * p.nkv + h) * kFew + c : row);
+      const int64_t at = (int64_t)split * p.rows * p.nq + row;
       if (d == 0) p.part_ml[at] = make_float2(M, sees ? L : -1.f);
       *reinterpret_cast<float4*>(p.part_o + at * p.D + d) = make_float4(o[0], o[1], o[2], o[3]);
     } else {
@@ -370,11 +355,21 @@ __device__ __forceinline__ float sum_of_halves(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// f(0) .. f(N - 1) with the numbers as constants.
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+constexpr int kTileM = 128;  // queries of a tile
+
 // HD: dims of a row in LDS; NKD: steps of 16 dims (16 NKD >= D); GEN: D < HD, and the dims past D are zeros.
-// RB: blocks of 32 queries of a wave, four waves a block.
-template <int HD, int NKD, bool GEN, int RB>
-__global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(const ChunkParams p) {
-  constexpr int BM = 128 * RB;
+template <int HD, int NKD, bool GEN>
+__global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkParams p) {
   constexpr int ROWB = HD * 2;            // bytes of a K or V row
   constexpr int CPR = HD / 8;             // 16-byte chunks of it
   constexpr int RPL = 256 / ROWB;         // rows in 256 bytes: all banks once
@@ -385,81 +380,61 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
   static_assert(HD == 32 || HD == 64 || HD == 128, "rows of 64, 128 or 256 bytes");
   static_assert(DMAS * DMA_ROWS == 16, "a wave fetches 16 rows, which lie in one page");
   const int D = GEN ? p.D : HD;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];  // two K tiles, two V tiles
+  // Two K tiles, two V tiles, each an object of its own: the compiler waits for DMAs into what a transposing
+  // read may alias.
+  __shared__ __attribute__((aligned(1024))) uint8_t lds_k0[TILE], lds_k1[TILE], lds_v0[TILE], lds_v1[TILE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hi = lane >> 5, r32 = lane & 31;
   // KV heads run fastest: with eight of them each XCD reads the cache of one.  The last tiles of a
-  // sequence, which see most, come first.
+  // sequence, which see most, come first.  Splits run slowest: the later ones of short tiles have nothing to
+  // do, and blocks go to XCDs and CUs in turn, so that every second one with nothing leaves half of the chip
+  // idle (16 sequences of up to 4099, heads of 80, two splits: 145 us so, ... with the splits side by side).
   const int h = blockIdx.x % p.nkv;
-  uint32_t rest = blockIdx.x / p.nkv;
-  const int split = rest % p.splits;
-  const ChunkTile ct = chunk_tile<BM>(p, p.tiles - 1 - rest / p.splits, lane);
+  const uint32_t rest = blockIdx.x / p.nkv;
+  const int split = rest / p.tiles;
+  const ChunkTile ct = chunk_tile<kTileM>(p, p.tiles - 1 - rest % p.tiles, lane);
   if (!ct.any()) return;
-  const int32_t cap = p.t.capacity(), group = p.group;
-  const int32_t end_m = min(ct.queries, ct.m0 + BM);  // past the tile's last query
+  const int32_t cap = p.t.capacity(), group = p.group, b = ct.b;
+  const int32_t m0 = ct.m0, end_m = min(ct.queries, m0 + kTileM);  // past the tile's last query
   auto row_of = [&](int32_t m) { return (int64_t)(ct.begin + m / group) * p.nq + h * group + m % group; };
-  if ((int64_t)ct.count * group <= p.few) {
-    // The other kernel's sequence: only the rows without a token are left, up to the next one's.
-    if (split != 0) return;
-    const int cpr = D / 8;
-    for (int i = threadIdx.x; i < (end_m - ct.m0) * cpr; i += 256) {
-      const int32_t m = ct.m0 + i / cpr;
-      if ((uint32_t)ct.token(m, group) >= (uint32_t)ct.count)
-        *reinterpret_cast<uint4*>(p.out + row_of(m) * D + i % cpr * 8) = make_uint4(0u, 0u, 0u, 0u);
-    }
-    return;
-  }
-  // Slots seen by any of queries [m, to), and by the first token among them.
-  auto most_seen = [&](int32_t m, int32_t to) {
-    const int32_t first = max(ct.token(m, group), 0), last = min(ct.token(to - 1, group), ct.count - 1);
-    return m < to && first <= last ? ct.slots_of(last, cap) : 0;
-  };
-  const int32_t block_seen = __builtin_amdgcn_readfirstlane(most_seen(ct.m0, end_m));
-  const int32_t all_tiles = (block_seen + kKeys - 1) / kKeys, per = (all_tiles + p.splits - 1) / p.splits;
-  const int32_t t0 = split * per, nt = max(min(all_tiles, t0 + per) - t0, 0);
-  const int32_t mw = ct.m0 + wave * 32 * RB;
-  const int32_t wave_seen = __builtin_amdgcn_readfirstlane(most_seen(mw, min(end_m, mw + 32 * RB)));
+  // What the block's, and the wave's, queries see at most; of these, tiles t0 .. t0 + nt - 1 of keys are at hand.
+  const int32_t block_seen = __builtin_amdgcn_readfirstlane(ct.most_seen(m0, end_m, group, cap));
+  const int32_t all_tiles = (block_seen + kKeys - 1) / kKeys;
+  const int32_t t0 = split * p.piece, nt = min(all_tiles - t0, p.piece);
+  if (nt <= 0 && split > 0) return;
+  const bool whole = all_tiles <= p.piece;
+  const int32_t mw = m0 + wave * 32;
+  const int32_t wave_seen = __builtin_amdgcn_readfirstlane(ct.most_seen(mw, min(end_m, mw + 32), group, cap));
   // Tiles of this wave, and the first one that some of its queries do not see whole.
   const int32_t ntw = max(min((wave_seen + kKeys - 1) / kKeys - t0, nt), 0);
   const int32_t full = __builtin_amdgcn_readfirstlane(ct.slots_of(max(ct.token(mw, group), 0), cap)) / kKeys - t0;
-  int32_t seen[RB];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int32_t m = mw + rb * 32 + r32;
-    seen[rb] = m < end_m ? ct.seen(m, group, cap) : 0;
-  }
+  const int32_t m = mw + r32;
+  const int32_t seen = m < end_m ? ct.seen(m, group, cap) : 0;
 
-  f32x16 o[RB][NDB];
-  float m_run[RB], m_ref[RB], l_run[RB], mx[RB];
+  f32x16 o[NDB];
+  float m_run = -INFINITY, m_ref = 0.f, l_run = 0.f, mx = -INFINITY;
   int32_t wild = INT32_MAX;  // the first tile whose infinite values and NaN were left out
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    m_run[rb] = -INFINITY, m_ref[rb] = 0.f, l_run[rb] = 0.f, mx[rb] = -INFINITY;
+  for (int db = 0; db < NDB; ++db)
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) o[rb][db][v] = 0.f;
-  }
+    for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
 
   if (nt > 0) {
-    // Q fragments: the B operand, query r32 of a block, dims 16 k + 8 hi .. + 8.
-    bf16x8 qf[RB][NKD];
+    // Q fragments: the B operand, query r32 of the wave's, dims 16 k + 8 hi .. + 8.
+    bf16x8 qf[NKD];
+    const uint16_t* q_row = p.q + (seen > 0 ? row_of(m) * D : 0) + 8 * hi;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const uint16_t* q_row = p.q + (seen[rb] > 0 ? row_of(mw + rb * 32 + r32) * D : 0) + 8 * hi;
-#pragma unroll
-      for (int k = 0; k < NKD; ++k) {
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (seen[rb] > 0 && (!GEN || 16 * k + 8 * hi < D)) x = *reinterpret_cast<const uint4*>(q_row + 16 * k);
-        qf[rb][k] = __builtin_bit_cast(bf16x8, x);
-      }
+    for (int k = 0; k < NKD; ++k) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (seen > 0 && (!GEN || 16 * k + 8 * hi < D)) x = *reinterpret_cast<const uint4*>(q_row + 16 * k);
+      qf[k] = __builtin_bit_cast(bf16x8, x);
     }
 
     // ---- pages -------------------------------------------------------------------
     // Lane i knows the page of this wave's 16 rows of tile window + i; a page's number is read off
     // when its tile is fetched.  missing: bit i for a tile with a page that is not in the pool.
-    const int32_t* table = p.t.table + (int64_t)ct.b * p.t.ld;
+    const int32_t* table = p.t.table + (int64_t)b * p.t.ld;
     const int lp = p.t.log2_page;
     int32_t page_ids = 0, window = t0;
     uint64_t missing = 0;
@@ -526,30 +501,29 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
       const int c = 4 * db + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
       vf_off[db] = v_key * ROWB + ((c ^ (CPR > 4 ? 4 * (v_key / RPL % (CPR / 4)) : 0)) << 4) + (lane & 1) * 8;
     }
-    constexpr int KRING = RB == 1 ? 3 : 4;
-    bf16x8 kfr[KRING], vfr[2][NDB], pf[RB][4];
-    f32x16 s[2][RB][2];  // S^T of two tiles: the one in the softmax and the next one
+    constexpr int KRING = 3;
+    bf16x8 kfr[KRING], vfr[2][NDB], pf[4];
+    f32x16 s[2][2];  // S^T of two tiles: the one in the softmax and the next one
     auto k_read = [&](int buf, int j) __attribute__((always_inline)) {
-      kfr[j % KRING] = *reinterpret_cast<const bf16x8*>(lds + buf * TILE + kf_off[j % NKD] + (j / NKD) * 32 * ROWB);
+      kfr[j % KRING] = *reinterpret_cast<const bf16x8*>((buf ? lds_k1 : lds_k0) + kf_off[j % NKD] + (j / NKD) * 32 * ROWB);
     };
     auto qk = [&](int set, int i) __attribute__((always_inline)) {
-      const int j = i / RB, rb = i % RB, kb = j / NKD, k = j % NKD;
-      s[set][rb][kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[j % KRING], qf[rb][k],
-                                                              k == 0 ? f32x16{} : s[set][rb][kb], 0, 0, 0);
+      const int kb = i / NKD, k = i % NKD;
+      s[set][kb] =
+          __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[i % KRING], qf[k], k == 0 ? f32x16{} : s[set][kb], 0, 0, 0);
     };
     auto v_read = [&](int buf, int sl) __attribute__((always_inline)) {
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
-        const uint8_t* at = lds + 2 * TILE + buf * TILE + vf_off[db] + sl * 16 * ROWB;
+        const uint8_t* at = (buf ? lds_v1 : lds_v0) + vf_off[db] + sl * 16 * ROWB;
         typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
         const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
         const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * ROWB));
         vfr[sl & 1][db] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
       }
     };
-    auto pv = [&](int sl, int i) __attribute__((always_inline)) {
-      const int db = i / RB, rb = i % RB;
-      o[rb][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr[sl & 1][db], pf[rb][sl], o[rb][db], 0, 0, 0);
+    auto pv = [&](int sl, int db) __attribute__((always_inline)) {
+      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr[sl & 1][db], pf[sl], o[db], 0, 0, 0);
     };
 
     // ---- softmax -------------------------------------------------------------------
@@ -562,68 +536,54 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
           const int32_t key = (t0 + t) * kKeys + 16 * w;
           if (key < block_seen && (uint32_t)table[key >> lp] >= (uint32_t)p.t.num_pages)
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-              for (int v = 0; v < 16; ++v)
-                if (v / 8 == (w & 1)) s[set][rb][w >> 1][v] = __builtin_nanf("");
+            for (int v = 8 * (w & 1); v < 8 * (w & 1) + 8; ++v) s[set][w >> 1][v] = __builtin_nanf("");
         }
       }
       if (t >= full || bad) {
+        const int32_t lim = seen - (t0 + t) * kKeys - 4 * hi;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          const int32_t lim = seen[rb] - (t0 + t) * kKeys - 4 * hi;
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              const int c = kb * 32 + 8 * (v >> 2) + (v & 3);
-              s[set][rb][kb][v] = c >= lim ? -INFINITY : s[set][rb][kb][v];
-            }
-        }
+          for (int v = 0; v < 16; ++v) {
+            const int key = kb * 32 + 8 * (v >> 2) + (v & 3);
+            s[set][kb][v] = key >= lim ? -INFINITY : s[set][kb][v];
+          }
       }
+      float x[2];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        float x[2];
+      for (int kb = 0; kb < 2; ++kb) {
+        x[kb] = fmaxf(s[set][kb][0], s[set][kb][1]);
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          x[kb] = fmaxf(s[set][rb][kb][0], s[set][rb][kb][1]);
-#pragma unroll
-          for (int v = 2; v < 16; v += 2) x[kb] = fmaxf(fmaxf(x[kb], s[set][rb][kb][v]), s[set][rb][kb][v + 1]);
-        }
-        mx[rb] = max_of_halves(fmaxf(x[0], x[1])) * p.scale_log2;
+        for (int v = 2; v < 16; v += 2) x[kb] = fmaxf(fmaxf(x[kb], s[set][kb][v]), s[set][kb][v + 1]);
       }
+      mx = max_of_halves(fmaxf(x[0], x[1])) * p.scale_log2;
     };
     // The reference m_run moves only when a query's maximum passes it by more than kLazy; until then
     // P = 2^(t - m_run) <= 2^kLazy, which bf16 and fp32 hold, and the division by l cancels it.
     auto move_max = [&]() __attribute__((always_inline)) {
-      bool over = false;
+      if (__builtin_amdgcn_ballot_w64(mx > m_run + kLazy) != 0) {
+        const float m_new = fmaxf(m_run, mx);
+        m_ref = m_new == -INFINITY ? 0.f : m_new;  // scores of -inf weigh nothing, also the first ones
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
+        m_run = m_new;
+        l_run *= alpha;
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) over = over || mx[rb] > m_run[rb] + kLazy;
-      if (__builtin_amdgcn_ballot_w64(over) != 0) {
+        for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          const float m_new = fmaxf(m_run[rb], mx[rb]);
-          m_ref[rb] = m_new == -INFINITY ? 0.f : m_new;  // scores of -inf weigh nothing, also the first ones
-          const float alpha = __builtin_amdgcn_exp2f(m_run[rb] - m_ref[rb]);
-          m_run[rb] = m_new;
-          l_run[rb] *= alpha;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) o[rb][db][v] *= alpha;
-        }
+          for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
       }
     };
     // P of two neighbouring keys of slab sl, rounded to bf16 (the sum l is of the rounded ones, so that the
     // weights that V is multiplied by add up to 1), and its place among the slab's operand.
     auto p_pair = [&](int set, int u) __attribute__((always_inline)) {
-      const int sl = u / (4 * RB), rb = u / 4 % RB, j = u % 4, kb = sl >> 1, v = 8 * (sl & 1) + 2 * j;
-      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[set][rb][kb][v], p.scale_log2, -m_ref[rb]));
-      const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[set][rb][kb][v + 1], p.scale_log2, -m_ref[rb]));
-      const uint32_t w = pack_bf16x2(a, b);
-      l_run[rb] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w),
-                                                  __builtin_bit_cast(bf16x2_t, 0x3F803F80u), l_run[rb], false);
-      reinterpret_cast<uint32_t*>(&pf[rb][sl])[j] = w;
+      const int sl = u / 4, j = u % 4, kb = sl >> 1, v = 8 * (sl & 1) + 2 * j;
+      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[set][kb][v], p.scale_log2, -m_ref));
+      const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[set][kb][v + 1], p.scale_log2, -m_ref));
+      uint32_t w = pack_bf16x2(a, b);
+      asm volatile("" : "+v"(w));  // here, between the products, and not where the operand is used
+      l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w),
+                                                  __builtin_bit_cast(bf16x2_t, 0x3F803F80u), l_run, false);
+      reinterpret_cast<uint32_t*>(&pf[sl])[j] = w;
     };
     // Infinite values and NaN in a tile that some queries do not see whole (0 of P times them has no
     // value) leave V^T, slab by slab, and are added at the end.
@@ -649,16 +609,16 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
       const int32_t pg_next = pg_ahead;
       if (t + 2 < nt) {
         advance(t + 2);
-        fetch(p.k_pages, t + 2, pg_ahead, k_off, lds + cur * TILE);
+        fetch(p.k_pages, t + 2, pg_ahead, k_off, cur ? lds_k1 : lds_k0);
       } else {
         bad_next = bad_ahead;
       }
-      if (t + 1 < nt) fetch(p.v_pages, t + 1, pg_next, v_off, lds + 2 * TILE + (cur ^ 1) * TILE);
+      if (t + 1 < nt) fetch(p.v_pages, t + 1, pg_next, v_off, cur ? lds_v0 : lds_v1);
     };
     auto body = [&](int32_t t, auto par, auto more) __attribute__((always_inline)) {
       constexpr int cur = decltype(par)::value, nxt = cur ^ 1;
       constexpr bool next = decltype(more)::value;
-      constexpr int QK = next ? RB * 2 * NKD : 0, PV = RB * NDB, PAIRS = 16 * RB;
+      constexpr int QK = next ? 2 * NKD : 0, PV = NDB, PAIRS = 16;
       constexpr int SPAN = QK + 3 * PV;  // products before the last slab's
       const bool masked = t >= full || bad_next;  // (bad_next: of tile t until sync has gone on)
       sync(t, cur);
@@ -669,38 +629,37 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
         v_read(cur, 0);
       }
       move_max();
-#pragma unroll
-      for (int i = 0; i < QK + 4 * PV; ++i) {
+      each<QK + 4 * PV>([&](auto index) __attribute__((always_inline)) {
+        constexpr int i = decltype(index)::value;
         // The pairs of P are spread over the products before the last slab's, each slab's before its own.
-#pragma unroll
-        for (int u = 0; u < PAIRS; ++u) {
-          const int before = QK + u / (4 * RB) * PV, even = u * SPAN / PAIRS;
-          if ((even < before ? even : before) == i) p_pair(cur, u);
-        }
-        if (i < QK) {
-          if (i % RB == 0 && i / RB + KRING - 1 < 2 * NKD) k_read(nxt, i / RB + KRING - 1);
+        each<PAIRS>([&](auto pair) __attribute__((always_inline)) {
+          constexpr int u = decltype(pair)::value, before = QK + u / 4 * PV, even = u * SPAN / PAIRS;
+          if constexpr ((even < before ? even : before) == i) p_pair(cur, u);
+        });
+        if constexpr (i < QK) {
+          if constexpr (i + KRING - 1 < 2 * NKD) k_read(nxt, i + KRING - 1);
           qk(nxt, i);
-          if (i == (QK > 8 ? QK - 8 : 0)) v_read(cur, 0);
+          if constexpr (i == (QK > 8 ? QK - 8 : 0)) v_read(cur, 0);
         } else {
-          const int sl = (i - QK) / PV, at = (i - QK) % PV;
-          if (at == 0) {
-            if (sl < 3) v_read(cur, sl + 1);
+          constexpr int sl = (i - QK) / PV, at = (i - QK) % PV;
+          if constexpr (at == 0) {
+            if constexpr (sl < 3) v_read(cur, sl + 1);
             if (__builtin_expect(masked, 0) && tame(sl)) wild = min(wild, t);
           }
           pv(sl, at);
         }
         __builtin_amdgcn_sched_barrier(0);
-      }
+      });
       if constexpr (next) row_max(nxt, t + 1, bad_next);
     };
 
     look_up();
     advance(0);
-    fetch(p.k_pages, 0, pg_ahead, k_off, lds);
-    fetch(p.v_pages, 0, pg_ahead, v_off, lds + 2 * TILE);
+    fetch(p.k_pages, 0, pg_ahead, k_off, lds_k0);
+    fetch(p.v_pages, 0, pg_ahead, v_off, lds_v0);
     if (nt > 1) {
       advance(1);
-      fetch(p.k_pages, 1, pg_ahead, k_off, lds + TILE);
+      fetch(p.k_pages, 1, pg_ahead, k_off, lds_k1);
     } else {
       bad_next = bad_ahead;
     }
@@ -710,8 +669,8 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
 #pragma unroll
       for (int j = 0; j < KRING - 1 && j < 2 * NKD; ++j) k_read(0, j);
 #pragma unroll
-      for (int i = 0; i < RB * 2 * NKD; ++i) {
-        if (i % RB == 0 && i / RB + KRING - 1 < 2 * NKD) k_read(0, i / RB + KRING - 1);
+      for (int i = 0; i < 2 * NKD; ++i) {
+        if (i + KRING - 1 < 2 * NKD) k_read(0, i + KRING - 1);
         qk(0, i);
       }
       row_max(0, 0, bad_next);
@@ -733,110 +692,122 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void paged_chunk_tile_kernel(
         body(t, std::integral_constant<int, 0>{}, std::false_type{});
       ++t;
     }
-    for (; t < nt; ++t) sync(t, t & 1);
+    for (; t < nt; ++t) {
+      if (t & 1)
+        sync(t, 1);
+      else
+        sync(t, 0);
+    }
   }
 
   // As in the few kernel: added as they are, whatever their weights.
   for (int32_t slot = wild < ntw ? (t0 + wild) * kKeys : INT32_MAX; slot < min((t0 + ntw) * kKeys, wave_seen); ++slot) {
-    const int64_t row = p.t.row(ct.b, h, p.nkv, slot);
+    const int64_t row = p.t.row(b, h, p.nkv, slot);
     if (row < 0) continue;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int d = 32 * db + 8 * (v >> 2) + 4 * hi + (v & 3);
-          const uint32_t x = !GEN || d < D ? p.v_pages[row * D + d] : 0u;
-          if (slot < seen[rb] && (x & 0x7f80u) == 0x7f80u) o[rb][db][v] += bf16_bits_to_f32(x);
-        }
+      for (int v = 0; v < 16; ++v) {
+        const int d = 32 * db + 8 * (v >> 2) + 4 * hi + (v & 3);
+        const uint32_t x = !GEN || d < D ? p.v_pages[row * D + d] : 0u;
+        if (slot < seen && (x & 0x7f80u) == 0x7f80u) o[db][v] += bf16_bits_to_f32(x);
+      }
   }
 
   // ---- O^T / l ---------------------------------------------------------------------
+  l_run = sum_of_halves(l_run);
+  if (!whole) {
+    if (m < end_m) {
+      const int64_t at = (int64_t)split * p.rows * p.nq + row_of(m);
+      if (hi == 0) p.part_ml[at] = make_float2(m_run, seen > 0 ? l_run : -1.f);
+      if (ntw > 0) {  // (else a maximum of -inf: the sums are not read)
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) l_run[rb] = sum_of_halves(l_run[rb]);
-  if (p.splits > 1) {
-    const int64_t base = split * p.part_rows;
+        for (int db = 0; db < NDB; ++db)
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int32_t m = mw + rb * 32 + r32;
-      if (m >= end_m) continue;
-      const int64_t at = base + row_of(m);
-      if (hi == 0) p.part_ml[at] = make_float2(m_run[rb], seen[rb] > 0 ? l_run[rb] : -1.f);
-      if (ntw == 0) continue;  // (a maximum of -inf: the sums are not read)
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int d = 32 * db + 8 * g + 4 * hi;
-          if (!GEN || d < D)
-            *reinterpret_cast<float4*>(p.part_o + at * D + d) =
-                make_float4(o[rb][db][4 * g], o[rb][db][4 * g + 1], o[rb][db][4 * g + 2], o[rb][db][4 * g + 3]);
-        }
+          for (int g = 0; g < 4; ++g) {
+            const int d = 32 * db + 8 * g + 4 * hi;
+            if (!GEN || d < D)
+              *reinterpret_cast<float4*>(p.part_o + at * D + d) =
+                  make_float4(o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
+          }
+      }
     }
     return;
   }
   // A lane holds 8-byte pieces of one query: they are staged through LDS, 16-byte chunk c of row r at position
   // c ^ (r % CPR), and go out as whole rows.
-  static_assert(4 * 32 * RB * ROWB <= 4 * TILE, "output staging must fit the tiles");
+  static_assert(2 * 32 * ROWB == TILE, "a block of 32 queries of two waves fills a K tile");
   __syncthreads();
-  uint8_t* stage = lds + wave * 32 * RB * ROWB;
+  uint8_t* stage = (wave & 2 ? lds_k1 : lds_k0) + (wave & 1) * 32 * ROWB;
+  const float inv = 1.f / l_run;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const float inv = 1.f / l_run[rb];
-    const bool sees = seen[rb] > 0;
+  for (int db = 0; db < NDB; ++db)
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint2 w = make_uint2(pack_bf16x2(o[rb][db][4 * g] * inv, o[rb][db][4 * g + 1] * inv),
-                             pack_bf16x2(o[rb][db][4 * g + 2] * inv, o[rb][db][4 * g + 3] * inv));
-        if (!sees) w = make_uint2(0u, 0u);
-        const int ch = (db * 4 + g) ^ (r32 % CPR);
-        *reinterpret_cast<uint2*>(stage + (rb * 32 + r32) * ROWB + ch * 16 + hi * 8) = w;
-      }
-  }
+    for (int g = 0; g < 4; ++g) {
+      uint2 w = make_uint2(pack_bf16x2(o[db][4 * g] * inv, o[db][4 * g + 1] * inv),
+                           pack_bf16x2(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv));
+      if (seen <= 0) w = make_uint2(0u, 0u);
+      const int ch = (db * 4 + g) ^ (r32 % CPR);
+      *reinterpret_cast<uint2*>(stage + r32 * ROWB + ch * 16 + hi * 8) = w;
+    }
   // The wave's own LDS writes complete before its reads (and stay ahead of them).
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
   __builtin_amdgcn_wave_barrier();
   const int jc = lane % CPR;
-  if (GEN && jc * 8 >= D) return;
 #pragma unroll
-  for (int i = 0; i < 32 * RB * CPR / 64; ++i) {
+  for (int i = 0; i < CPR / 2; ++i) {
     const int r = i * (64 / CPR) + lane / CPR;
     const uint4 x = *reinterpret_cast<const uint4*>(stage + r * ROWB + ((jc ^ (r % CPR)) << 4));
-    if (mw + r < end_m) *reinterpret_cast<uint4*>(p.out + row_of(mw + r) * D + jc * 8) = x;
+    if (mw + r < end_m && (!GEN || jc * 8 < D)) *reinterpret_cast<uint4*>(p.out + row_of(mw + r) * D + jc * 8) = x;
   }
 }
 
 constexpr int kJoinThreads = 256;
 
-// One query a block: its splits' sums by 256 threads over splits and columns.  The first few_blocks are
-// queries of the few kernel's sequences (f), the others the (row, head) pairs of p's.
-__global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const ChunkParams f, uint32_t few_blocks,
-                                                                        const ChunkParams p) {
+// The sums of tiles that several splits took, by tile and KV head; the others are done.
+// parts: blocks that a tile's queries are joined by.
+__global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const ChunkParams p, int parts) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int part = blockIdx.x % parts, rest = blockIdx.x / parts, h = rest % p.nkv;
+  const ChunkTile ct = chunk_tile<kTileM>(p, rest / p.nkv, lane);
+  if (!ct.any()) return;
+  const int32_t end_m = min(ct.queries, ct.m0 + kTileM);
+  const int32_t seen = ct.most_seen(ct.m0, end_m, p.group, p.t.capacity());
+  const int pieces = ((seen + kKeys - 1) / kKeys + p.piece - 1) / p.piece;
+  if (pieces <= 1) return;
+  const int cols = p.D / 4;
+  const int64_t step = (int64_t)p.rows * p.nq;
+  for (int i = part * kJoinThreads + tid; i < (end_m - ct.m0) * cols; i += parts * kJoinThreads) {
+    const int32_t m = ct.m0 + i / cols, d = i % cols * 4;
+    const int64_t row = (int64_t)(ct.begin + m / p.group) * p.nq + h * p.group + m % p.group;
+    float M = -INFINITY, L = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    bool sees = true;
+#pragma unroll 4
+    for (int k = 0; k < pieces; ++k) {
+      const float2 ml = p.part_ml[k * step + row];
+      // (Where the maximum is -inf no sum was written, or one of nothing.)
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (ml.x != -INFINITY) y = *reinterpret_cast<const float4*>(p.part_o + (k * step + row) * p.D + d);
+      sees = ml.y != -1.f;
+      const float top = fmaxf(M, ml.x), ref = top == -INFINITY ? 0.f : top;
+      const float f = __builtin_amdgcn_exp2f(M - ref), g = __builtin_amdgcn_exp2f(ml.x - ref);
+      M = top;
+      L = __builtin_fmaf(L, f, g * ml.y);
+      o.x = __builtin_fmaf(o.x, f, g * y.x), o.y = __builtin_fmaf(o.y, f, g * y.y);
+      o.z = __builtin_fmaf(o.z, f, g * y.z), o.w = __builtin_fmaf(o.w, f, g * y.w);
+    }
+    const float inv = 1.f / L;
+    const float y[4] = {sees ? o.x * inv : 0.f, sees ? o.y * inv : 0.f, sees ? o.z * inv : 0.f, sees ? o.w * inv : 0.f};
+    head_store4(p.out + row * p.D + d, y);
+  }
+}
+
+// One (row, head) a block: its splits' sums by 256 threads over splits and columns.
+__global__ __launch_bounds__(kJoinThreads) void paged_chunk_few_join_kernel(const ChunkParams p) {
   __shared__ float4 part[kJoinThreads];
   const int tid = threadIdx.x, lane = tid & 63;
-  const bool of_few = blockIdx.x < few_blocks;
-  const int splits = of_few ? f.splits : p.splits;
-  const int64_t step = of_few ? f.part_rows : p.part_rows, at0 = of_few ? blockIdx.x : blockIdx.x - few_blocks;
-  const float* part_o = of_few ? f.part_o : p.part_o;
-  const float2* part_ml = of_few ? f.part_ml : p.part_ml;
-  int64_t row = at0;
-  if (of_few) {
-    const ChunkTile ct = chunk_sequence(f, (int)(at0 / (f.nkv * kFew)));
-    const int h = (int)(at0 / kFew % f.nkv), c = (int)(at0 % kFew);
-    const int64_t first = (int64_t)(ct.first - ct.begin) * f.group;
-    if ((int64_t)ct.count * f.group > kFew || c >= ct.count * f.group || ct.first < ct.begin || first + c >= ct.queries)
-      return;
-    row = ((int64_t)ct.first + c / f.group) * f.nq + h * f.group + c % f.group;
-  } else if (p.few > 0) {
-    // A token of the few kernel's sequences is joined above.
-    const int32_t r = (int32_t)(row / p.nq);
-    const int b = last_sequence(p.B, r, lane, [&](int i) { return (int64_t)p.starts[i]; });
-    const int32_t count = max(p.counts[b], 0);
-    if ((int64_t)count * p.group <= p.few) return;
-  }
+  const int64_t row = blockIdx.x, step = (int64_t)p.rows * p.nq;
   const int cols = p.D / 4, groups = min(kJoinThreads / cols, 16);
   const int sg = tid / cols, d = (tid - sg * cols) * 4;
   float2 ml[kPagedMaxSplits / 64];
@@ -844,7 +815,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const Ch
 #pragma unroll
   for (int i = 0; i < kPagedMaxSplits / 64; ++i) {
     const int s = i * 64 + lane;
-    ml[i] = s < splits ? part_ml[s * step + at0] : make_float2(-INFINITY, 0.f);
+    ml[i] = s < p.splits ? p.part_ml[s * step + row] : make_float2(-INFINITY, 0.f);
     M = fmaxf(M, ml[i].x);
   }
 #pragma unroll
@@ -859,12 +830,12 @@ __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const Ch
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (sg < groups) {
 #pragma unroll 4
-    for (int s = sg; s < splits; s += groups) {
-      const int64_t at = s * step + at0;
-      const float top = part_ml[at].x;
-      if (top == -INFINITY) continue;  // (no sum was written, or one of nothing)
+    for (int s = sg; s < p.splits; s += groups) {
+      const int64_t at = s * step + row;
+      const float top = p.part_ml[at].x;
+      if (top == -INFINITY) continue;  // (a sum of nothing)
       const float f = __builtin_amdgcn_exp2f(top - ref);
-      const float4 x = *reinterpret_cast<const float4*>(part_o + at * p.D + d);
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * p.D + d);
       o.x = __builtin_fmaf(f, x.x, o.x), o.y = __builtin_fmaf(f, x.y, o.y);
       o.z = __builtin_fmaf(f, x.z, o.z), o.w = __builtin_fmaf(f, x.w, o.w);
     }
@@ -877,25 +848,26 @@ __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const Ch
     o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
   }
   const float inv = 1.f / L;
-  const float x[4] = {sees ? o.x * inv : 0.f, sees ? o.y * inv : 0.f, sees ? o.z * inv : 0.f, sees ? o.w * inv : 0.f};
-  head_store4(p.out + row * p.D + d, x);
+  const float f[4] = {sees ? o.x * inv : 0.f, sees ? o.y * inv : 0.f, sees ? o.z * inv : 0.f, sees ? o.w * inv : 0.f};
+  head_store4(p.out + row * p.D + d, f);
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
-// What a call launches: the few kernel (over tiles, or a block per sequence beside the tile kernel), the tile
-// kernel, and a join where slots are split.
 struct ChunkPlan {
-  bool few, tile;
-  int64_t few_tiles, tiles;  // blocks a KV head and split
-  int few_splits, splits;
-  int64_t few_rows, rows;    // of their partial sums
-  size_t few_o, few_ml, o, ml;
-  size_t total() const { return few_o + few_ml + o + ml; }
+  bool few;
+  int64_t tiles;  // numbers that they may have
+  int splits, piece;
+  size_t o, ml;
+  size_t total() const { return o + ml; }
 };
 
+#ifndef FORCE_S
+#define FORCE_S 0
+#endif
 // Splits of a tile's slots: blocks come in turns of two a CU, and a turn costs what its slots cost.
 int tile_splits(int64_t blocks, int64_t cap) {
+  if (FORCE_S) return FORCE_S;
   const int64_t slots = 2 * device_cu_count();
   const int64_t most = std::min<int64_t>(kPagedMaxSplits, (cap + 8 * kKeys - 1) / (8 * kKeys));
   int best = 1;
@@ -910,25 +882,16 @@ int tile_splits(int64_t blocks, int64_t cap) {
 ChunkPlan chunk_plan(int64_t rows, int64_t B, int64_t nq, int64_t nkv, int64_t hd, int64_t cap, int64_t most) {
   ChunkPlan c{};
   const int64_t group = nq / nkv;
-  c.tile = std::min(most, rows) * group > kFew;
-  c.few = !c.tile || (B > 1 && group <= kFew);
-  if (c.few) {
-    c.few_tiles = c.tile ? B : rows * group / kFew + B;
-    c.few_splits = paged_splits(c.few_tiles * nkv, cap);
-    c.few_rows = c.tile ? B * nkv * kFew : rows * nq;
-    if (c.few_splits > 1) {
-      c.few_o = round16((size_t)(c.few_splits * c.few_rows * hd) * sizeof(float));
-      c.few_ml = round16((size_t)(c.few_splits * c.few_rows) * sizeof(float2));
-    }
-  }
-  if (c.tile) {
-    c.tiles = rows * group / 128 + B;
-    c.splits = tile_splits(((rows * group + 127) / 128 + (B - 1) / 2) * nkv, cap);
-    c.rows = rows * nq;
-    if (c.splits > 1) {
-      c.o = round16((size_t)(c.splits * c.rows * hd) * sizeof(float));
-      c.ml = round16((size_t)(c.splits * c.rows) * sizeof(float2));
-    }
+  c.few = std::min(most, rows) * group <= kFew;
+  const int64_t size = c.few ? kFew : kTileM;
+  c.tiles = rows * group / size + B;
+  const int64_t key_tiles = (cap + kKeys - 1) / kKeys;
+  c.splits = c.few ? paged_splits(c.tiles * nkv, cap)
+                   : tile_splits(((rows * group + kTileM - 1) / kTileM + (B - 1) / 2) * nkv, cap);
+  c.piece = (int)((key_tiles + c.splits - 1) / c.splits);
+  if (c.splits > 1) {
+    c.o = round16((size_t)(c.splits * rows * nq * hd) * sizeof(float));
+    c.ml = round16((size_t)(c.splits * rows * nq) * sizeof(float2));
   }
   return c;
 }
@@ -949,24 +912,23 @@ void launch_few(const ChunkParams& p, const dim3& grid, hipStream_t s) {
     paged_chunk_few_kernel<4, 8, true><<<grid, block, 0, s>>>(p);
 }
 
-template <int RB>
 void launch_tile(const ChunkParams& p, const dim3& grid, hipStream_t s) {
   const dim3 block(256);
   switch (p.D) {
-    case 32: return paged_chunk_tile_kernel<32, 2, false, RB><<<grid, block, 0, s>>>(p);
-    case 64: return paged_chunk_tile_kernel<64, 4, false, RB><<<grid, block, 0, s>>>(p);
-    case 128: return paged_chunk_tile_kernel<128, 8, false, RB><<<grid, block, 0, s>>>(p);
+    case 32: return paged_chunk_tile_kernel<32, 2, false><<<grid, block, 0, s>>>(p);
+    case 64: return paged_chunk_tile_kernel<64, 4, false><<<grid, block, 0, s>>>(p);
+    case 128: return paged_chunk_tile_kernel<128, 8, false><<<grid, block, 0, s>>>(p);
     default: break;
   }
   switch ((p.D + 15) / 16) {
     case 1:
-    case 2: return paged_chunk_tile_kernel<64, 2, true, RB><<<grid, block, 0, s>>>(p);
-    case 3: return paged_chunk_tile_kernel<64, 3, true, RB><<<grid, block, 0, s>>>(p);
-    case 4: return paged_chunk_tile_kernel<64, 4, true, RB><<<grid, block, 0, s>>>(p);
-    case 5: return paged_chunk_tile_kernel<128, 5, true, RB><<<grid, block, 0, s>>>(p);
-    case 6: return paged_chunk_tile_kernel<128, 6, true, RB><<<grid, block, 0, s>>>(p);
-    case 7: return paged_chunk_tile_kernel<128, 7, true, RB><<<grid, block, 0, s>>>(p);
-    default: return paged_chunk_tile_kernel<128, 8, true, RB><<<grid, block, 0, s>>>(p);
+    case 2: return paged_chunk_tile_kernel<64, 2, true><<<grid, block, 0, s>>>(p);
+    case 3: return paged_chunk_tile_kernel<64, 3, true><<<grid, block, 0, s>>>(p);
+    case 4: return paged_chunk_tile_kernel<64, 4, true><<<grid, block, 0, s>>>(p);
+    case 5: return paged_chunk_tile_kernel<128, 5, true><<<grid, block, 0, s>>>(p);
+    case 6: return paged_chunk_tile_kernel<128, 6, true><<<grid, block, 0, s>>>(p);
+    case 7: return paged_chunk_tile_kernel<128, 7, true><<<grid, block, 0, s>>>(p);
+    default: return paged_chunk_tile_kernel<128, 8, true><<<grid, block, 0, s>>>(p);
   }
 }
 
@@ -1002,11 +964,8 @@ extern "C" int cdx_paged_chunk_attention_fwd(const uint16_t* q, int64_t rows, in
   if (rows > INT32_MAX / 1024 || nq > 65535 || rows * nq > INT32_MAX)
     return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
   const ChunkPlan c = chunk_plan(rows, B, nq, nkv, hd, cap, max_tokens);
-  const int64_t few_blocks = c.few ? c.few_tiles * nkv * c.few_splits : 0;
-  const int64_t blocks = c.tile ? c.tiles * nkv * c.splits : 0;
-  const int64_t few_joins = c.few && c.few_splits > 1 ? c.few_rows : 0, joins = c.tile && c.splits > 1 ? c.rows : 0;
-  if (few_blocks > max_blocks(64 * kPagedWaves) || blocks > max_blocks(256) ||
-      few_joins + joins > max_blocks(kJoinThreads))
+  const int64_t blocks = c.tiles * nkv * c.splits;
+  if (blocks > max_blocks(64 * kPagedWaves) || rows * nq > max_blocks(kJoinThreads))
     return fail(CDX_EUNSUPPORTED, "%s: problem too large", name);
   if (!q || !k_pages || !v_pages || !table || !starts || !counts || !lengths || !out)
     return fail(CDX_EINVAL, "%s: null pointer", name);
@@ -1028,34 +987,24 @@ extern "C" int cdx_paged_chunk_attention_fwd(const uint16_t* q, int64_t rows, in
   p.group = (int32_t)group;
   p.scale_log2 = scale * kLog2e;
   p.out = out;
-  ChunkParams f = p;
-  char* at = static_cast<char*>(work);
-  f.by_sequence = c.tile;
-  f.splits = c.few_splits;
-  f.part_rows = c.few_rows;
-  f.part_o = reinterpret_cast<float*>(at);
-  f.part_ml = reinterpret_cast<float2*>(at + c.few_o);
-  at += c.few_o + c.few_ml;
-  p.few = c.few ? kFew : 0;
-  p.tiles = (uint32_t)c.tiles;
   p.splits = c.splits;
-  p.part_rows = c.rows;
-  p.part_o = reinterpret_cast<float*>(at);
-  p.part_ml = reinterpret_cast<float2*>(at + c.o);
+  p.piece = c.piece;
+  p.tiles = (uint32_t)c.tiles;
+  p.part_o = static_cast<float*>(work);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(work) + c.o);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (c.few) {
-    launch_few(f, dim3((unsigned)few_blocks), s);
-    if (int rc = check_launch(name)) return rc;
-  }
-  if (c.tile) {
-    launch_tile<1>(p, dim3((unsigned)blocks), s);
-    if (int rc = check_launch(name)) return rc;
-  }
-  if (few_joins + joins == 0) return CDX_OK;
-  // (Where the few kernel took every sequence, its sums lie by (row, head).)
-  if (!c.tile)
-    paged_chunk_join_kernel<<<dim3((unsigned)few_joins), dim3(kJoinThreads), 0, s>>>(f, 0, f);
+  const dim3 grid((unsigned)blocks), joiners(kJoinThreads);
+  if (c.few)
+    launch_few(p, grid, s);
   else
-    paged_chunk_join_kernel<<<dim3((unsigned)(few_joins + joins)), dim3(kJoinThreads), 0, s>>>(f, (uint32_t)few_joins, p);
+    launch_tile(p, grid, s);
+  if (int rc = check_launch(name)) return rc;
+  if (c.splits == 1) return CDX_OK;
+  if (c.few)
+    paged_chunk_few_join_kernel<<<dim3((unsigned)(rows * nq)), joiners, 0, s>>>(p);
+  else {
+    const int parts = (int)std::min<int64_t>(16, (4 * device_cu_count() + c.tiles * nkv - 1) / (c.tiles * nkv));
+    paged_chunk_join_kernel<<<dim3((unsigned)(c.tiles * nkv * parts)), joiners, 0, s>>>(p, parts);
+  }
   return check_launch(name);
 }

@@ -501,29 +501,28 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
       const int c = 4 * db + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
       vf_off[db] = v_key * ROWB + ((c ^ (CPR > 4 ? 4 * (v_key / RPL % (CPR / 4)) : 0)) << 4) + (lane & 1) * 8;
     }
-    constexpr int KRING = 3;
-    bf16x8 kfr[KRING], vfr[2][NDB], pf[4];
+    // Every product takes one operand from LDS, K's rows or V^T's: they are read RING - 1 products ahead.
+    constexpr int RING = 5;
+    bf16x8 fr[RING], pf[4];
     f32x16 s[2][2];  // S^T of two tiles: the one in the softmax and the next one
-    auto k_read = [&](int buf, int j) __attribute__((always_inline)) {
-      kfr[j % KRING] = *reinterpret_cast<const bf16x8*>((buf ? lds_k1 : lds_k0) + kf_off[j % NKD] + (j / NKD) * 32 * ROWB);
+    auto k_read = [&](int slot, int buf, int i) __attribute__((always_inline)) {
+      fr[slot] = *reinterpret_cast<const bf16x8*>((buf ? lds_k1 : lds_k0) + kf_off[i % NKD] + (i / NKD) * 32 * ROWB);
     };
-    auto qk = [&](int set, int i) __attribute__((always_inline)) {
+    auto qk = [&](int slot, int set, int i) __attribute__((always_inline)) {
       const int kb = i / NKD, k = i % NKD;
-      s[set][kb] =
-          __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[i % KRING], qf[k], k == 0 ? f32x16{} : s[set][kb], 0, 0, 0);
+      s[set][kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[slot], qf[k], k == 0 ? f32x16{} : s[set][kb], 0, 0, 0);
     };
-    auto v_read = [&](int buf, int sl) __attribute__((always_inline)) {
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const uint8_t* at = (buf ? lds_v1 : lds_v0) + vf_off[db] + sl * 16 * ROWB;
-        typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
-        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
-        const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * ROWB));
-        vfr[sl & 1][db] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
-      }
+    auto v_read = [&](int slot, int buf, int i) __attribute__((always_inline)) {
+      const int sl = i / NDB, db = i % NDB;
+      const uint8_t* at = (buf ? lds_v1 : lds_v0) + vf_off[db] + sl * 16 * ROWB;
+      typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+      const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * ROWB));
+      fr[slot] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto pv = [&](int sl, int db) __attribute__((always_inline)) {
-      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr[sl & 1][db], pf[sl], o[db], 0, 0, 0);
+    auto pv = [&](int slot, int i) __attribute__((always_inline)) {
+      const int sl = i / NDB, db = i % NDB;
+      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[slot], pf[sl], o[db], 0, 0, 0);
     };
 
     // ---- softmax -------------------------------------------------------------------
@@ -586,19 +585,19 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
       reinterpret_cast<uint32_t*>(&pf[sl])[j] = w;
     };
     // Infinite values and NaN in a tile that some queries do not see whole (0 of P times them has no
-    // value) leave V^T, slab by slab, and are added at the end.
-    auto tame = [&](int sl) __attribute__((always_inline)) {
+    // value) leave V^T, operand by operand, and are added at the end.
+    auto tame = [&](int slot) __attribute__((always_inline)) {
       typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
-      uint32_t* w = reinterpret_cast<uint32_t*>(vfr[sl & 1]);
+      uint32_t* w = reinterpret_cast<uint32_t*>(&fr[slot]);
       u16x2 top = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 4 * NDB; ++i)
-        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+      for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
       if (__builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= 0x7f80) == 0) return false;
 #pragma unroll
-      for (int i = 0; i < 4 * NDB; ++i) w[i] = without_special(w[i]);
+      for (int i = 0; i < 4; ++i) w[i] = without_special(w[i]);
       return true;
     };
+
     // ---- pipeline --------------------------------------------------------------------
     // Tile t's softmax and O += V(t)^T P(t), with the QK products of tile t + 1 between.  Its DMAs, issued
     // behind its barrier, fetch K(t + 2) into the buffer of K(t) and V(t + 1) into that of V(t - 1); both
@@ -622,31 +621,29 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
       constexpr int SPAN = QK + 3 * PV;  // products before the last slab's
       const bool masked = t >= full || bad_next;  // (bad_next: of tile t until sync has gone on)
       sync(t, cur);
-      if constexpr (next) {
-#pragma unroll
-        for (int j = 0; j < KRING - 1 && j < 2 * NKD; ++j) k_read(nxt, j);
-      } else {
-        v_read(cur, 0);
-      }
+      constexpr int ALL = QK + 4 * PV;
+      auto read = [&](auto index) __attribute__((always_inline)) {
+        constexpr int i = decltype(index)::value;
+        if constexpr (i < QK)
+          k_read(i % RING, nxt, i);
+        else if constexpr (i < ALL)
+          v_read(i % RING, cur, i - QK);
+      };
+      each<RING - 1>(read);
       move_max();
-      each<QK + 4 * PV>([&](auto index) __attribute__((always_inline)) {
+      each<ALL>([&](auto index) __attribute__((always_inline)) {
         constexpr int i = decltype(index)::value;
         // The pairs of P are spread over the products before the last slab's, each slab's before its own.
         each<PAIRS>([&](auto pair) __attribute__((always_inline)) {
           constexpr int u = decltype(pair)::value, before = QK + u / 4 * PV, even = u * SPAN / PAIRS;
           if constexpr ((even < before ? even : before) == i) p_pair(cur, u);
         });
+        read(std::integral_constant<int, i + RING - 1>{});
         if constexpr (i < QK) {
-          if constexpr (i + KRING - 1 < 2 * NKD) k_read(nxt, i + KRING - 1);
-          qk(nxt, i);
-          if constexpr (i == (QK > 8 ? QK - 8 : 0)) v_read(cur, 0);
+          qk(i % RING, nxt, i);
         } else {
-          constexpr int sl = (i - QK) / PV, at = (i - QK) % PV;
-          if constexpr (at == 0) {
-            if constexpr (sl < 3) v_read(cur, sl + 1);
-            if (__builtin_expect(masked, 0) && tame(sl)) wild = min(wild, t);
-          }
-          pv(sl, at);
+          if (__builtin_expect(masked, 0) && tame(i % RING)) wild = min(wild, t);
+          pv(i % RING, i - QK);
         }
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -666,13 +663,11 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
     __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 15));
     __syncthreads();
     if (ntw > 0) {
-#pragma unroll
-      for (int j = 0; j < KRING - 1 && j < 2 * NKD; ++j) k_read(0, j);
-#pragma unroll
-      for (int i = 0; i < 2 * NKD; ++i) {
-        if (i + KRING - 1 < 2 * NKD) k_read(0, i + KRING - 1);
-        qk(0, i);
-      }
+      each<2 * NKD + RING - 1>([&](auto index) __attribute__((always_inline)) {
+        constexpr int i = decltype(index)::value - (RING - 1);
+        if constexpr (i >= 0) qk(i % RING, 0, i);
+        if constexpr (i + RING - 1 < 2 * NKD) k_read((i + RING - 1) % RING, 0, i + RING - 1);
+      });
       row_max(0, 0, bad_next);
     }
     // Every wave passes sync(t) once for each t < nt, in order, so the barriers pair up.

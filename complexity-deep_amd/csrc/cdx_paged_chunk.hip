@@ -17,6 +17,7 @@
 
 #include "cdx_gemm.h"
 #include "cdx_paged_attn.h"
+#include "cdx_wave.h"
 
 namespace cdx {
 namespace {
@@ -42,12 +43,11 @@ struct ChunkParams {
 
 constexpr int kFew = 16;  // queries of a block: the columns of a matrix instruction
 
-// A tile of BM queries of one sequence.  Sequence b's own rows, with those that follow them up to the
-// next one's, are rows begin .. end - 1 of the call; row r is token r - first of the sequence.
+// A tile of queries of one sequence: rows begin .. of the call, row r being token r - first of the sequence.
 struct ChunkTile {
   int b;
   int32_t begin, first, count, before;  // before: slots in use ahead of the new tokens
-  int32_t m0, queries;                  // the tile's first query, and how many [begin, end) has
+  int32_t m0, queries;                  // the tile's first query, and how many the rows have
 
   __device__ __forceinline__ bool any() const { return m0 < queries; }
   // The token that query m belongs to; outside 0 .. count - 1: none.
@@ -68,11 +68,11 @@ struct ChunkTile {
   }
 };
 
-// Sequence b's tiles begin at number first_row * group / BM + b: ascending, and at least as far apart
-// as the tiles of the rows between.  The whole wave looks at 64 sequences at a time.
-template <int BM>
-__device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t tile, int lane) {
-  auto number = [&](int b) { return (int64_t)p.starts[b] * p.group / BM + b; };
+// The few kernel's tiles take the rows behind a sequence's, up to the next one's, along.  Sequence b's begin at
+// number first_row * group / kFew + b: ascending, and at least as far apart as the tiles of the rows
+// between.  The whole wave looks at 64 sequences at a time.
+__device__ __forceinline__ ChunkTile few_tile(const ChunkParams& p, uint32_t tile, int lane) {
+  auto number = [&](int b) { return (int64_t)p.starts[b] * p.group / kFew + b; };
   int lo = 0, n = p.B;
   while (n > 1) {
     const int step = (n + 63) >> 6, b = lo + lane * step;
@@ -91,7 +91,7 @@ __device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t t
   const int32_t end = b + 1 < p.B ? min(max(p.starts[b + 1], t.begin), p.rows) : p.rows;
   t.queries = (end - t.begin) * p.group;  // (rows * nq fits 31 bits)
   const int64_t at = b == 0 ? tile : tile - number(b);
-  t.m0 = at < 0 || at * BM >= t.queries ? t.queries : (int32_t)at * BM;
+  t.m0 = at < 0 || at * kFew >= t.queries ? t.queries : (int32_t)at * kFew;
   return t;
 }
 
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
   const uint32_t split = blockIdx.x % p.splits;
   const uint32_t rest = blockIdx.x / p.splits;
   const int h = rest % p.nkv;
-  const ChunkTile ct = chunk_tile<kFew>(p, rest / p.nkv, lane);
+  const ChunkTile ct = few_tile(p, rest / p.nkv, lane);
   if (!ct.any()) return;
   const int queries = min(kFew, ct.queries - ct.m0);
   const int32_t cap = p.t.capacity();
@@ -367,6 +367,49 @@ __device__ __forceinline__ void each(F&& f) {
 
 constexpr int kTileM = 128;  // queries of a tile
 
+// The tile kernel's tile of this number: what takes longest comes first, so that the blocks that are left at the
+// end are short ones.  Of 64 sequences each, by the keys of the last tile and the waves that its
+// queries occupy (a key costs one wave about half of what it costs four, the fetch being the same);
+// within a sequence the last tile first.  By a whole wave; without queries if there are fewer tiles.
+__device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t number, int lane) {
+  ChunkTile t{};
+  int64_t at = number;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const int n_seq = min(64, p.B - b0);
+    const int b = b0 + min(lane, n_seq - 1);
+    const int32_t first = p.starts[b], asked = max(p.counts[b], 0), length = p.lengths[b];
+    // (Rows outside the call's are dropped.)
+    const int32_t count = lane >= n_seq || first < 0 ? 0 : min(asked, max(p.rows - first, 0));
+    const int32_t queries = count * p.group, tiles = (queries + kTileM - 1) / kTileM;
+    const int64_t all = wave_sum((u64)tiles);
+    if (at >= all) {
+      at -= all;
+      continue;
+    }
+    // The place of each among the 64, and then the tiles of those in the first places.
+    const uint32_t keys = (uint32_t)min(max(length, 0), p.t.capacity()) / kKeys + 1;
+    const uint32_t cost = tiles > 0 ? keys * (uint32_t)(2 + (min(queries, kTileM) + 31) / 32) : 0;
+    int place = 0;
+    for (int i = 0; i < n_seq; ++i) {
+      const uint32_t other = (uint32_t)read_lane((int)cost, i);
+      place += other > cost || (other == cost && i < lane) ? 1 : 0;
+    }
+    if (lane >= n_seq) place = lane;
+    const int here = __builtin_amdgcn_ds_permute(place * 4, tiles << 6 | lane);
+    const int64_t upto = (int64_t)wave_inclusive((u64)(here >> 6));
+    const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
+    const int from = read_lane(here, i) & 63;
+    t.b = b0 + from;
+    t.begin = t.first = read_lane(first, from);
+    t.count = read_lane(count, from);
+    t.before = (int32_t)max((int64_t)read_lane(length, from) - read_lane(asked, from), (int64_t)INT32_MIN);
+    t.queries = t.count * p.group;
+    t.m0 = (int32_t)((int64_t)read_lane((u64)upto, i) - 1 - at) * kTileM;
+    return t;
+  }
+  return t;
+}
+
 // HD: dims of a row in LDS; NKD: steps of 16 dims (16 NKD >= D); GEN: D < HD, and the dims past D are zeros.
 template <int HD, int NKD, bool GEN>
 __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkParams p) {
@@ -386,14 +429,35 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hi = lane >> 5, r32 = lane & 31;
-  // KV heads run fastest: with eight of them each XCD reads the cache of one.  The last tiles of a
-  // sequence, which see most, come first.  Splits run slowest: the later ones of short tiles have nothing to
-  // do, and blocks go to XCDs and CUs in turn, so that every second one with nothing leaves half of the chip
-  // idle (16 sequences of up to 4099, heads of 80, two splits: 145 us so, ... with the splits side by side).
+  // KV heads run fastest: with eight of them each XCD reads the cache of one.  Splits run slowest: the later ones
+  // of short tiles have nothing to do, and blocks go to XCDs and CUs in turn, so that every second one
+  // with nothing leaves half of the chip idle (16 sequences of up to 4099, heads of 80, two splits: 145
+  // us so, 113 with the second ones behind the first).
   const int h = blockIdx.x % p.nkv;
-  const uint32_t rest = blockIdx.x / p.nkv;
+  const uint32_t rest = blockIdx.x / p.nkv, number = rest % p.tiles;
   const int split = rest / p.tiles;
-  const ChunkTile ct = chunk_tile<kTileM>(p, p.tiles - 1 - rest % p.tiles, lane);
+  if (split == 0) {
+    // Rows that belong to no sequence are zeros: those behind each one's up to the next one's.
+    auto zero = [&](int32_t from, int32_t to) {
+      for (int64_t r = (int64_t)from + number; r < to; r += p.tiles)
+        for (int c = lane; c < p.group * D / 8; c += 64)
+          reinterpret_cast<uint4*>(p.out + (r * p.nq + h * p.group) * D)[c] = make_uint4(0u, 0u, 0u, 0u);
+    };
+    for (int b0 = wave * 64; b0 < p.B; b0 += 256) {
+      const int b = b0 + lane;
+      int32_t from = 0, to = 0;
+      if (b < p.B) {
+        from = (int32_t)min(max((int64_t)p.starts[b] + max(p.counts[b], 0), (int64_t)0), (int64_t)p.rows);
+        to = b + 1 < p.B ? min(p.starts[b + 1], p.rows) : p.rows;
+      }
+      for (uint64_t left = __builtin_amdgcn_ballot_w64(from < to); left != 0; left &= left - 1) {
+        const int i = __builtin_ctzll(left);
+        zero(read_lane(from, i), read_lane(to, i));
+      }
+    }
+    if (wave == 0) zero(0, min(p.starts[0], p.rows));  // (and those ahead of the first)
+  }
+  const ChunkTile ct = chunk_tile(p, number, lane);
   if (!ct.any()) return;
   const int32_t cap = p.t.capacity(), group = p.group, b = ct.b;
   const int32_t m0 = ct.m0, end_m = min(ct.queries, m0 + kTileM);  // past the tile's last query
@@ -764,7 +828,7 @@ constexpr int kJoinThreads = 256;
 __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const ChunkParams p, int parts) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int part = blockIdx.x % parts, rest = blockIdx.x / parts, h = rest % p.nkv;
-  const ChunkTile ct = chunk_tile<kTileM>(p, rest / p.nkv, lane);
+  const ChunkTile ct = chunk_tile(p, rest / p.nkv, lane);
   if (!ct.any()) return;
   const int32_t end_m = min(ct.queries, ct.m0 + kTileM);
   const int32_t seen = ct.most_seen(ct.m0, end_m, p.group, p.t.capacity());

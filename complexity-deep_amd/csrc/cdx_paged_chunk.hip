@@ -95,10 +95,7 @@ __device__ __forceinline__ ChunkTile few_tile(const ChunkParams& p, uint32_t til
   return t;
 }
 
-// Whether one of a word's two bf16 is infinite or no number.
-__device__ __forceinline__ bool any_special(uint32_t x) {
-  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
-}
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 // Both bf16 of a word, Inf and NaN as 0.
 __device__ __forceinline__ uint32_t without_special(uint32_t x) {
   if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
@@ -212,7 +209,6 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
     }
     uint32_t* vw = reinterpret_cast<uint32_t*>(vr);  // [8 rows][DPL / 2]
     constexpr int RW = DPL / 2;
-    bool special = false;
     if (s0 + kPagedTile > min_seen || !there[0] || !there[1]) {
       // Slots past what a query sees weigh nothing, and values that no query sees must not count
       // either (0 * NaN is NaN); a page that is not in the pool makes a query that sees it NaN.
@@ -222,11 +218,12 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
         const bool ok = there[i / 4];
         s[i] = slot >= seen ? -INFINITY : (ok ? s[i] : __builtin_nanf(""));
         if (slot >= max_seen || !ok) vr[i] = vpiece_t{};
-#pragma unroll
-        for (int w = 0; w < RW; ++w) special = special || (slot >= min_seen && any_special(vw[i * RW + w]));
       }
-      // Infinite values and NaN of a slot that some queries see and others do not are added at the end.
-      if (__builtin_amdgcn_ballot_w64(special) != 0) {
+      // Infinite values and NaN that some queries may see and others not are added at the end.
+      u16x2_t top = {0, 0};
+#pragma unroll
+      for (int w = 0; w < 8 * RW; ++w) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, vw[w] & 0x7fff7fffu));
+      if (__builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= 0x7f80) != 0) {
         wild = min(wild, tile);
 #pragma unroll
         for (int w = 0; w < 8 * RW; ++w) vw[w] = without_special(vw[w]);
@@ -651,11 +648,10 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
     // Infinite values and NaN in a tile that some queries do not see whole (0 of P times them has no
     // value) leave V^T, operand by operand, and are added at the end.
     auto tame = [&](int slot) __attribute__((always_inline)) {
-      typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
       uint32_t* w = reinterpret_cast<uint32_t*>(&fr[slot]);
-      u16x2 top = {0, 0};
+      u16x2_t top = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+      for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
       if (__builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= 0x7f80) == 0) return false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = without_special(w[i]);

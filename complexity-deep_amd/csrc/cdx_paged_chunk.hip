@@ -917,19 +917,20 @@ struct ChunkPlan {
   size_t total() const { return o + ml; }
 };
 
-#ifndef FORCE_S
-#define FORCE_S 0
-#endif
-// Splits of a tile's slots: blocks come in turns of two a CU, and a turn costs what its slots cost.
-int tile_splits(int64_t blocks, int64_t cap) {
-  if (FORCE_S) return FORCE_S;
+// Splits of a tile's slots, for so many blocks of key_tiles tiles of keys: blocks come in turns of two a CU, and a
+// turn takes as long as its tiles and a beginning and end, which is about three; a second kernel takes as long
+// as three, and every block's sums, written and read at 5 TB/s, 0.02 (a tile of 128 queries and 64 keys:
+// 1.3 us).  4 x 512 tokens over 4096 of 12/4 heads of 64: one split 55 us, two 51, three 56; 64 over 8192
+// of 16/8 heads of 128: one split 137, two 77, four 45, eight 31; 2048 over 65536: one 1133, two 994, four 999.
+int tile_splits(int64_t blocks, int64_t key_tiles) {
   const int64_t slots = 2 * device_cu_count();
-  const int64_t most = std::min<int64_t>(kPagedMaxSplits, (cap + 8 * kKeys - 1) / (8 * kKeys));
   int best = 1;
   double cost = 1e30;
-  for (int64_t s = 1; s <= most && (s == 1 || blocks * (s - 1) < slots); ++s) {
-    const double c = (double)((blocks * s + slots - 1) / slots) / s + (s > 1 ? 0.02 * s : 0.0);
+  for (int64_t s = 1; s <= std::min<int64_t>(kPagedMaxSplits, key_tiles); ++s) {
+    const int64_t turns = (blocks * s + slots - 1) / slots, piece = (key_tiles + s - 1) / s;
+    const double c = (double)(turns * (piece + 3)) + (s > 1 ? 3.0 + 0.02 * (double)(blocks * s) : 0.0);
     if (c < cost) cost = c, best = (int)s;
+    if (turns > 4) break;
   }
   return best;
 }
@@ -942,7 +943,7 @@ ChunkPlan chunk_plan(int64_t rows, int64_t B, int64_t nq, int64_t nkv, int64_t h
   c.tiles = rows * group / size + B;
   const int64_t key_tiles = (cap + kKeys - 1) / kKeys;
   c.splits = c.few ? paged_splits(c.tiles * nkv, cap)
-                   : tile_splits(((rows * group + kTileM - 1) / kTileM + (B - 1) / 2) * nkv, cap);
+                   : tile_splits(((rows * group + kTileM - 1) / kTileM + (B - 1) / 2) * nkv, key_tiles);
   c.piece = (int)((key_tiles + c.splits - 1) / c.splits);
   if (c.splits > 1) {
     c.o = round16((size_t)(c.splits * rows * nq * hd) * sizeof(float));

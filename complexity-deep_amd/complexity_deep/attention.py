@@ -41,7 +41,8 @@ import torch.nn.functional as F
 from . import _native as nat
 from ._grad import forward_only
 from .linear import few_rows, linear, linear_accumulate_
-from .paged import PagedLayer, _ints, _ld, _pages, _rotary, paged_attention, paged_write
+from .paged import (PagedLayer, _ints, _ld, _pages, _rotary, paged_attention, paged_chunk_append,
+                    paged_chunk_attention, paged_write)
 from .rotary import RotaryEmbedding, apply_rotary_pos_emb
 
 
@@ -626,7 +627,8 @@ class ComplexityAttention(nn.Module):
                          residual: Optional[torch.Tensor]) -> torch.Tensor:
         """The attention with a layer of a PagedKVCache, whose ``begin`` has counted x's tokens:
         prompts attend among themselves and are then written into the pages; one new token per
-        sequence is appended and attends to every slot in use."""
+        sequence is appended and attends to every slot in use; the rows of a call with token_counts are
+        appended and attend to the slots up to their own."""
         if attention_mask is not None:
             raise ValueError("ComplexityAttention: a paged cache takes no mask (ragged prompts have lengths)")
         if not (self.fused_prologue or self.other_head_dim) or (self.training and self.attention_dropout > 0):
@@ -636,7 +638,10 @@ class ComplexityAttention(nn.Module):
         B, S, _ = x.shape
         D, nq, nkv = self.head_dim, self.num_heads, self.num_kv_heads
         k_pages, v_pages, weights = cache.layer(layer.index)
-        if (B, nkv, D) != (cache.batch_size, k_pages.shape[1], k_pages.shape[3]) or (S != 1 and not cache.prompt):
+        rows = cache.rows
+        if (nkv, D) != (k_pages.shape[1], k_pages.shape[3]) or (
+                B * S != rows.row_slots.numel() if rows is not None else
+                B != cache.batch_size or (S != 1 and not cache.prompt)):
             raise ValueError(f"ComplexityAttention: input {tuple(x.shape)} with {nkv} KV heads of {D} does not match "
                              "the paged cache")
         if cache.prompt:
@@ -646,6 +651,13 @@ class ComplexityAttention(nn.Module):
         qn = (self.q_norm.weight, self.k_norm.weight) if self.use_qk_norm else (None, None)
         eps = self.q_norm.eps if self.use_qk_norm else 0.0
         table = cache.rotary_table(self.rotary_emb, x.device)
+        if rows is not None:
+            qkv = self.project_qkv(x, mu)
+            q = paged_chunk_append(qkv.view(B * S, -1), k_pages, v_pages, rows.row_slots, rows.row_positions, nq, table,
+                                   *qn, eps)
+            attn = paged_chunk_attention(q, k_pages, v_pages, cache.block_table, rows.starts, rows.counts, rows.lengths,
+                                         max_tokens=cache.most)
+            return self._out_proj(attn.view(B, S, -1), residual)
         fast = nat.host()
         attn = None
         if fast is not None:

@@ -201,6 +201,8 @@ class TransformerBlock(nn.Module):
         table = lengths = positions = weights = None
         if type(past) is PagedLayer:  # one new token per sequence, counted by the cache
             cache = past.cache
+            if cache.rows is not None:
+                return None
             pk, pv, weights = cache.layer(past.index)
             table, lengths, positions = cache.block_table, cache.lengths, cache.positions
             cos_sin = cache.rotary_table(attn.rotary_emb, h.device)

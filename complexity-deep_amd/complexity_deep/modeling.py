@@ -216,24 +216,37 @@ class ComplexityModel(nn.Module):
     def forward(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                 labels: Optional[torch.Tensor] = None,
                 past_key_values: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None,
-                use_cache: bool = False, prompt_lengths: Optional[torch.Tensor] = None) -> CausalLMOutput:
+                use_cache: bool = False, prompt_lengths: Optional[torch.Tensor] = None,
+                token_counts=None) -> CausalLMOutput:
         """``past_key_values`` may be a PagedKVCache, which the call extends in place and returns: the
-        prompts first (right-padded ones with ``prompt_lengths`` [B]), then one token per sequence."""
+        prompts first (right-padded ones with ``prompt_lengths`` [B]), then one token per sequence; or with
+        ``token_counts`` (integers [B]) so many tokens of each sequence at any time, ids [B, S] right-padded or
+        [tokens] one sequence behind the other (logits [tokens, vocab] then)."""
         forward_only("ComplexityModel", module=self)
-        B, S = input_ids.shape
         paged = isinstance(past_key_values, PagedKVCache)
+        packed = input_ids.dim() == 1 and paged and token_counts is not None
+        if packed:
+            if labels is not None:
+                raise ValueError("ComplexityModel: labels with sequences one behind the other")
+            input_ids = input_ids.unsqueeze(0)
+        B, S = input_ids.shape
         if paged:
             if attention_mask is not None:
                 raise ValueError("ComplexityModel: a paged cache takes no mask (ragged prompts have prompt_lengths)")
             if len(past_key_values) != len(self.layers):
                 raise ValueError(f"ComplexityModel: a paged cache of {len(past_key_values)} layers for "
                                  f"{len(self.layers)}")
-            past_key_values.begin(B, S, prompt_lengths)
+            past_key_values.begin(past_key_values.batch_size if packed else B, S, prompt_lengths, token_counts, packed)
             try:
-                return self._forward(input_ids, None, labels, past_key_values, use_cache, True)
+                out = self._forward(input_ids, None, labels, past_key_values, use_cache, True)
             except BaseException:
                 past_key_values.cancel()
                 raise
+            if packed:
+                out.logits = out.logits[0]
+            return out
+        if token_counts is not None:
+            raise ValueError("ComplexityModel: token_counts without a paged cache")
         if prompt_lengths is not None:
             raise ValueError("ComplexityModel: prompt_lengths without a paged cache")
         return self._forward(input_ids, attention_mask, labels, past_key_values, use_cache, False)
@@ -249,7 +262,8 @@ class ComplexityModel(nn.Module):
         # A generation step of a few rows runs block by block through TransformerBlock.step,
         # which takes h itself (its norms are folded); other calls hand each block its
         # normalised input, produced by the block before.
-        steps = attention_mask is None and 0 < B * S <= 8 and not (paged and past_key_values.prompt)
+        steps = attention_mask is None and 0 < B * S <= 8 and \
+            not (paged and (past_key_values.prompt or past_key_values.rows is not None))
         normed = None
         # Layers 1.. read their normalised input and mu side by side from one [B, S, 2H]
         # buffer, written by the layer before (one K = 2H operand for the projection).
@@ -325,7 +339,7 @@ class ComplexityModel(nn.Module):
     def generate_paged(self, input_ids: torch.Tensor, max_new_tokens: int = 100, *, temperature: float = 1.0,
                        top_k: int = 50, top_p: float = 0.9, min_p: float = 0.0, eos_token_id: Optional[int] = None,
                        prompt_lengths: Optional[torch.Tensor] = None, uniforms: Optional[torch.Tensor] = None,
-                       cache: Optional[PagedKVCache] = None) -> torch.Tensor:
+                       cache: Optional[PagedKVCache] = None, chunk: Optional[int] = None) -> torch.Tensor:
         """The new tokens [B, n <= max_new_tokens] after the prompts ``input_ids`` [B, S], of
         ``prompt_lengths`` [B] tokens each (at least 1) where they are right-padded, on a paged cache: unlike
         ``generate``, whose cached steps keep the reference's top-left mask, every token attends
@@ -334,9 +348,12 @@ class ComplexityModel(nn.Module):
         Tokens come from sample_tokens (settings as there; temperature 0 is greedy) with
         ``uniforms`` [B, max_new_tokens], or with torch's random numbers.  A sequence that has
         produced ``eos_token_id`` (the configuration's by default) repeats it; the generation ends when
-        all have.  ``cache`` (emptied first) may bound the memory (PagedKVCache's keep); by default it
-        has room for every token."""
+        all have.  ``cache`` (emptied first) may bound the memory (PagedKVCache's keep, or its pages); by
+        default it has room for every token.  ``chunk`` takes the prompts in pieces of so many tokens each, which
+        bounds the activations and logits of long ones."""
         B, S = input_ids.shape
+        if chunk is not None and chunk <= 0:
+            raise ValueError(f"generate_paged: chunk={chunk} must be positive")
         eos = self.config.eos_token_id if eos_token_id is None else eos_token_id
         dev = input_ids.device
         if uniforms is None:
@@ -352,7 +369,9 @@ class ComplexityModel(nn.Module):
         done = torch.zeros(B, dtype=torch.bool, device=dev)
         n = 0
         while n < max_new_tokens:
-            if n == 0:
+            if n == 0 and chunk is not None:
+                logits = self._prompts_in_pieces(input_ids, prompt_lengths, cache, chunk)
+            elif n == 0:
                 logits = self.forward(input_ids, past_key_values=cache, prompt_lengths=prompt_lengths).logits
                 logits = logits[:, -1] if prompt_lengths is None else \
                     logits[torch.arange(B, device=dev), cache.positions.long().clamp(min=0)]
@@ -367,6 +386,22 @@ class ComplexityModel(nn.Module):
         ended = (tokens[:n] == eos).cummax(0).values.all(1)
         last = int(ended.int().argmax()) + 1 if n and bool(ended.any()) else n
         return tokens[:last].t().contiguous()
+
+    def _prompts_in_pieces(self, input_ids: torch.Tensor, prompt_lengths: Optional[torch.Tensor], cache: PagedKVCache,
+                           chunk: int) -> torch.Tensor:
+        """The logits [B, V] behind each prompt's last token, its tokens taken ``chunk`` at a time."""
+        B, S = input_ids.shape
+        n = prompt_lengths.clamp(0, S) if prompt_lengths is not None else torch.full((B,), S, dtype=torch.int64)
+        last = None
+        for at in range(0, S, chunk):
+            piece = input_ids[:, at:at + chunk]
+            counts = (n - at).clamp(0, piece.shape[1])
+            logits = self.forward(piece, past_key_values=cache, token_counts=counts).logits
+            end = (n - 1 - at).to(input_ids.device)
+            mine = logits[torch.arange(B, device=input_ids.device), end.clamp(0, piece.shape[1] - 1)]
+            here = ((end >= 0) & (end < piece.shape[1])).unsqueeze(1)
+            last = torch.where(here, mine, last if last is not None else torch.zeros_like(mine))
+        return last
 
     # ---- utilities (modeling.py:296-318) --------------------------------------------
     def num_parameters(self, trainable_only: bool = True) -> int:

@@ -10,6 +10,14 @@ sequence, and a step's one token attends to every slot in use:
   paged_qkv_append  a step's projection: QK norm, RoPE, k and v appended  (cdx_paged_append_fwd)
   paged_attention   softmax(scale q k^T) v over the slots in use         (cdx_paged_attention_fwd)
   paged_evict       the slots with the least accumulated weight go       (cdx_paged_evict)
+
+and, where a call brings any number of tokens of each sequence:
+
+  paged_reserve          pages from a pool, and the slots of the call's rows    (cdx_paged_reserve)
+  paged_truncate         sequences cut, pages back to the pool                  (cdx_paged_truncate)
+  paged_chunk_append     QK norm, RoPE, k and v into the slots                  (cdx_paged_chunk_append_fwd)
+  paged_chunk_attention  each token over the slots up to its own                (cdx_paged_chunk_attention_fwd)
+
   PagedKVCache      all of it for a model: ComplexityModel.forward takes one as past_key_values
 
 ``block_table`` [B, width] and ``lengths`` [B] are int32 tensors on the device and no call waits
@@ -20,6 +28,7 @@ is an empty sequence.  All of it can be captured into a HIP graph.
 
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -488,22 +497,30 @@ class PagedKVCache:
     sequence and call, [B, 1], and every token attends to all before it (a list of k and v keeps
     the reference's top-left mask instead).
 
-    Each sequence has room for ``max_length`` tokens (rounded up to whole pages).  When the
+    A call with ``token_counts`` brings any number of tokens of each sequence, none among them: second turns,
+    prompts in pieces, prompts of some beside steps of others, speculated tokens at once; ids [B, S],
+    right-padded, or [tokens], one sequence behind the other.  ``truncate`` takes tokens back,
+    ``release`` empties sequences, whose places others can take.
+
+    Each sequence has room for ``max_length`` tokens (rounded up to whole pages).  With ``pages`` the
+    sequences share a pool of so many pages, fewer than batch_size times that: a call takes what its
+    tokens need and raises if too few are left.  When the
     longest is full, a call raises, or with ``keep`` first cuts every longer sequence to ``keep``
     slots (paged_evict): the ``recent`` newest tokens (half of ``keep`` by default) stay, and those
-    that the steps so far attended to most.  Positions go on counting.
+    that the steps so far attended to most.  Positions go on counting.  A bounded cache takes its prompts and
+    then one token per sequence, and has no shared pool.
 
     ``lengths`` and ``positions`` (of the newest tokens) live on the device; ``longest`` and ``newest``
     are the host's bounds, and nothing waits for the device but the first call of a batch whose
     bound, of right-padded prompts with prompt_lengths on the device, has reached the capacity: it reads
-    how long the longest is.  One call at a time may use a cache.  A
+    how long the longest is; with token_counts on the device, or a pool, such a call reads all lengths.  One call at a time may use a cache.  A
     step that is captured into a graph counts on the device when it is replayed, not here: keep to
     max_length then (a token past the capacity is not stored).  A TransformerBlock or
     ComplexityAttention called by itself takes ``cache[i]``, after ``begin`` has counted the call's
     tokens."""
 
     def __init__(self, config, batch_size: int, max_length: int, *, page_size: int = 64, keep: Optional[int] = None,
-                 recent: Optional[int] = None, device="cuda"):
+                 recent: Optional[int] = None, pages: Optional[int] = None, device="cuda"):
         nkv, D = config.num_key_value_heads, config.hidden_size // config.num_attention_heads
         if page_size not in PAGE_SIZES:
             raise ValueError(f"PagedKVCache: page size {page_size} is not one of {PAGE_SIZES}")
@@ -518,18 +535,32 @@ class PagedKVCache:
         recent = recent if recent is not None else (keep // 2 if keep is not None else 0)
         if keep is not None and not (0 < keep < max_length and 0 <= recent <= keep):
             raise ValueError(f"PagedKVCache: keep={keep} must lie in 1 .. max_length - 1, recent={recent} in 0 .. keep")
+        if pages is not None and (isinstance(pages, bool) or int(pages) != pages or not 0 < pages < 2 ** 31):
+            raise ValueError(f"PagedKVCache: pages={pages} must be a positive integer")
+        if pages is not None and keep is not None:
+            raise ValueError("PagedKVCache: a bounded cache (keep) has pages of its own, not a pool's")
         self.batch_size, self.page_size, self.keep, self.recent = batch_size, page_size, keep, recent
+        self.pages = None if pages is None else int(pages)
         width = -(-max_length // page_size)
         self.capacity = width * page_size
         # (Ordinary tensors also under inference_mode: they are written in place wherever the cache is used.)
         with torch.inference_mode(False), torch.no_grad():
-            shape = (config.num_hidden_layers, batch_size * width, nkv, page_size, D)
+            shape = (config.num_hidden_layers, self.pages or batch_size * width, nkv, page_size, D)
             self.k_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
             self.v_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
             device = self.k_pages.device
-            pages = torch.arange(batch_size * width, dtype=torch.int32, device=device)
-            self.block_table = pages.view(batch_size, width)
-            self._counts = torch.zeros(2, batch_size, dtype=torch.int32, device=device)
+            own = torch.arange(batch_size * width, dtype=torch.int32, device=device).view(batch_size, width)
+            self.block_table = own if self.pages is None else torch.full_like(own, -1)
+            # The lengths, the positions, and the count of the pool's free pages, side by side as paged_reserve
+            # gives the new ones.
+            self._state = torch.zeros(2 * batch_size + 1, dtype=torch.int32, device=device)
+            self._counts = self._state[:2 * batch_size].view(2, batch_size)
+            self._undo = torch.empty_like(self._state)
+            self.free_pages = self.free_count = None
+            if self.pages is not None:
+                self.free_pages = torch.empty(self.pages, dtype=torch.int32, device=device)
+                self.free_count = self._state[2 * batch_size:]
+                self._ones = torch.ones(batch_size, dtype=torch.int32, device=device)
             self._tables = {}
             self.weights = self.slot_positions = self._weights_before = None
             if keep is not None:
@@ -570,12 +601,19 @@ class PagedKVCache:
         """Empty every sequence."""
         self._counts[0].zero_()
         self._counts[1].fill_(-1)
+        if self.pages is not None:
+            torch.arange(self.pages - 1, -1, -1, dtype=torch.int32, device=self.free_pages.device, out=self.free_pages)
+            self.free_count.fill_(self.pages)
         if self.weights is not None:
             self.weights.zero_()
             self.slot_positions.fill_(-1)
         self.longest = self.newest = 0  # no sequence has more slots, or has seen more tokens
         self._exact = True              # whether one has as many slots
+        self._lengths = [0] * self.batch_size  # the host's, or None if it does not know them
         self.prompt = True              # what the call at hand brings
+        self.rows = None                # (with token_counts: where its rows go
+        self.most = 0                   # and the most that a sequence has of them)
+        self._before = None             # what ``cancel`` goes back to after a call that took pages
         self._saved = False             # whether _weights_before holds the weights before it
 
     def evict(self) -> None:
@@ -588,26 +626,48 @@ class PagedKVCache:
                           self.slot_positions, self.keep, self.recent)
         for t, n in zip((self.lengths, self.weights, self.slot_positions), new):
             t.copy_(n)
-        self.longest = self.keep
+        self.longest, self._lengths = self.keep, None
 
-    def begin(self, batch_size: int, tokens: int, prompt_lengths: Optional[torch.Tensor] = None) -> None:
+    def begin(self, batch_size: int, tokens: int, prompt_lengths: Optional[torch.Tensor] = None,
+              token_counts=None, packed: bool = False) -> None:
         """Make room for a call's tokens and count them: the prompts (of ``prompt_lengths`` tokens
-        each, or all of them) of an empty cache, then one token per sequence."""
+        each, or all of them) of an empty cache, then one token per sequence; or with ``token_counts`` (integers
+        [B], on the device or the host) so many of each sequence, in rows of ``tokens`` each or, ``packed``,
+        one behind the other in ``tokens`` rows."""
         if batch_size != self.batch_size:
             raise ValueError(f"PagedKVCache: {batch_size} sequences in a cache of {self.batch_size}")
         if self.block_table.shape[-1] * self.page_size < self.capacity:
             raise ValueError(f"PagedKVCache: a block table {tuple(self.block_table.shape)} of pages of {self.page_size} "
                              f"has no room for {self.capacity} tokens")
+        self.rows = self._before = None
+        if token_counts is not None:
+            if self.keep is not None or prompt_lengths is not None or tokens <= 0:
+                raise ValueError("PagedKVCache: token_counts in a bounded cache, beside prompt_lengths, or without rows")
+            counts, known = self._integers(token_counts, "token_counts")
+            most = tokens if known is None else max(0, *known)
+            if known is not None and (min(known) < 0 or (sum(known) if packed else most) > tokens):
+                raise ValueError(f"PagedKVCache: token_counts {known} in {tokens} rows" + (" each" if not packed else ""))
+            self.rows = self._reserve(counts, known, most, tokens if packed else batch_size * tokens,
+                                      None if packed else tokens)
+            self.most, self.prompt = most, False
+            return
         if self.newest == 0:
             if not 0 < tokens <= self.capacity:
                 raise ValueError(f"PagedKVCache: prompts of {tokens} tokens in a cache of {self.capacity}")
-            if prompt_lengths is None:
+            if prompt_lengths is not None and (prompt_lengths.shape != (batch_size,)
+                                               or prompt_lengths.is_floating_point()):
+                raise ValueError(f"PagedKVCache: prompt_lengths must be {batch_size} integers, got "
+                                 f"{prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
+            n = None if prompt_lengths is None else prompt_lengths.clamp(0, tokens)
+            known = [tokens] * batch_size if n is None else (None if n.is_cuda else n.tolist())
+            if self.pages is not None:
+                n = torch.full_like(self.lengths, tokens) if n is None else n.to(self.lengths)
+                self._reserve(n, known, tokens, batch_size * tokens, tokens)
+            elif n is None:
                 self._counts[0].fill_(tokens)
             else:
-                if prompt_lengths.shape != (batch_size,) or prompt_lengths.is_floating_point():
-                    raise ValueError(f"PagedKVCache: prompt_lengths must be {batch_size} integers, got "
-                                     f"{prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
-                self._counts[0].copy_(prompt_lengths.clamp(0, tokens))
+                self._counts[0].copy_(n)
+            self._lengths = known
             torch.sub(self._counts[0], 1, out=self._counts[1])
             if self.slot_positions is not None:
                 at = torch.arange(self.capacity, dtype=torch.int32, device=self.slot_positions.device)
@@ -619,8 +679,12 @@ class PagedKVCache:
             self.prompt = True
             return
         if tokens != 1 or prompt_lengths is not None:
-            raise ValueError("PagedKVCache: after the prompts a call takes one token per sequence (reset() empties the "
-                             "cache)")
+            raise ValueError("PagedKVCache: after the prompts a call without token_counts takes one token per sequence "
+                             "(reset() empties the cache)")
+        if self.pages is not None:
+            self._reserve(self._ones, [1] * batch_size, 1, batch_size, None)
+            self.prompt = False
+            return
         capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()
         if self.longest >= self.capacity and not self._exact and not capturing:
             self._read_longest(self.lengths)
@@ -640,7 +704,85 @@ class PagedKVCache:
             self.slot_positions.scatter_(-1, slot, self.positions.view(-1, 1, 1).expand(slot.shape))
         self.longest += 1
         self.newest += 1
+        if self._lengths is not None:
+            self._lengths = [n + 1 for n in self._lengths]
         self.prompt = False
+
+    def _integers(self, values, name: str):
+        """(int32 [B] on the device, the same as a list if the host has them) of a tensor or a sequence."""
+        if not isinstance(values, torch.Tensor):
+            values = torch.tensor([operator.index(n) for n in values], dtype=torch.int64)
+        if values.shape != (self.batch_size,) or values.is_floating_point() or values.is_complex() \
+                or values.dtype == torch.bool:
+            raise ValueError(f"PagedKVCache: {name} must be {self.batch_size} integers, got {values.dtype} "
+                             f"{tuple(values.shape)}")
+        known = None if values.is_cuda else values.tolist()
+        return values.long().clamp(-2 ** 31, 2 ** 31 - 1).to(self.lengths.device, torch.int32), known
+
+    def _reserve(self, counts: torch.Tensor, known, most: int, rows: int, stride: Optional[int]) -> PagedRows:
+        """Pages and rows of ``counts`` tokens (on the host ``known``, or at most ``most`` each), which are counted.
+        Raises, with nothing changed, if the capacity or the pool does not suffice; a call that is being captured
+        is not looked at, and tokens that do not fit are then neither counted nor stored."""
+        capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()
+        before = (self.longest, self.newest, self._exact, self._lengths)
+        lengths = self._lengths
+        used = self.batch_size * -(-(self.longest + most) // self.page_size)
+        if not capturing and (self.longest + most > self.capacity or (self.pages is not None and used > self.pages)):
+            lengths = self.lengths.tolist() if lengths is None else lengths
+            known = [max(0, n) for n in counts.tolist()] if known is None else known
+            if any(c > 0 and n + c > self.capacity for n, c in zip(lengths, known)):
+                raise ValueError(f"PagedKVCache: full ({self.capacity} tokens)")
+            used, needed = (sum(-(-n // self.page_size) for n in ns)
+                            for ns in (lengths, [n + c for n, c in zip(lengths, known)]))
+            if self.pages is not None and needed > self.pages:
+                raise ValueError(f"PagedKVCache: {needed - used} pages are needed, and {self.pages - used} of "
+                                 f"{self.pages} are free")
+        new = paged_reserve(counts, self.lengths, self.positions, self.block_table, self.page_size, rows, stride=stride,
+                            free_pages=self.free_pages, free_count=self.free_count)
+        self._undo.copy_(self._state)
+        # (The new lengths, positions and count lie side by side.)
+        n = self._state.numel() if self.pages is not None else 2 * self.batch_size
+        self._state[:n].copy_(torch.as_strided(new.lengths, (n,), (1,)))
+        if lengths is not None and known is not None:
+            self._lengths = [n + c for n, c in zip(lengths, known)]
+            self.longest, self._exact = max(self._lengths), True
+        else:
+            self._lengths, self._exact = None, False
+            self.longest += most
+        self.newest = self.longest  # (without a bound by weight a token's position is its slot)
+        self._before = before
+        return new
+
+    def truncate(self, to) -> None:
+        """Cut every sequence of more than ``to`` [B] tokens (integers, on the device or the host) to its first so
+        many: speculated tokens that were not accepted, 0 for a sequence that has ended.  The pages
+        behind go back to the pool."""
+        if self.keep is not None:
+            raise ValueError("PagedKVCache: a bounded cache does not hold its tokens in order")
+        to, known = self._integers(to, "to")
+        if self.pages is not None:
+            new = paged_truncate(to, self.lengths, self.positions, self.block_table, self.page_size, self.free_pages,
+                                 self.free_count)
+            self._state.copy_(torch.as_strided(new[0], (self._state.numel(),), (1,)))
+        else:
+            gone = (self.lengths - to.clamp(min=0)).clamp(min=0)
+            self._counts.sub_(gone)
+        self.rows = self._before = None
+        if known is not None and (self._lengths is not None or max(known) <= 0):
+            self._lengths = [max(0, min(n, t)) for n, t in zip(self._lengths or known, known)]
+            self.longest, self._exact = max(self._lengths), True
+            self.newest = self.longest  # (0: as after reset())
+        else:
+            self._lengths, self._exact = None, False
+
+    def release(self, sequences) -> None:
+        """Empty these sequences (their numbers); the pages go back to the pool."""
+        to = [2 ** 31 - 1] * self.batch_size
+        for i in sequences:
+            if not 0 <= int(i) < self.batch_size:
+                raise IndexError(f"PagedKVCache: sequence {i} of {self.batch_size}")
+            to[int(i)] = 0
+        self.truncate(to)
 
     def _read_longest(self, lengths: torch.Tensor) -> None:
         self.longest, self._exact = int(lengths.max()), True
@@ -654,7 +796,12 @@ class PagedKVCache:
     def cancel(self) -> None:
         """Take back the tokens that the last ``begin`` counted, and the weights that they gave to others (a
         call that raised).  A cut that begin made stays: the call made again would make it too."""
-        if self.prompt:
+        if self.rows is not None or (self._before is not None and not self.prompt):
+            self._state.copy_(self._undo)
+            self.longest, self.newest, self._exact, self._lengths = self._before
+            self.rows = self._before = None
+            self.prompt = self.newest == 0
+        elif self.prompt:
             self.reset()
         else:
             if self.weights is not None:
@@ -664,3 +811,5 @@ class PagedKVCache:
             self._counts.sub_(1)
             self.longest -= 1
             self.newest -= 1
+            if self._lengths is not None:
+                self._lengths = [n - 1 for n in self._lengths]

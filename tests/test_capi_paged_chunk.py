@@ -105,3 +105,45 @@ def test_operators_refuse_cpu_tensors():
                                torch.zeros(3, **i32), 4, torch.zeros(8, 32, 2))
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         cdx.paged_chunk_attention(torch.zeros(3, 4, 64, dtype=torch.bfloat16), k, k, table, one, one, one)
+
+
+def test_cache_refuses_what_it_cannot_take():
+    """Before any memory is taken or a kernel called."""
+    import complexity_deep as cdx
+    cfg = cdx.ComplexityConfig.complexity_tiny()
+    for bad in (dict(pages=0), dict(pages=-3), dict(pages=2.5), dict(pages=True), dict(pages=8, keep=10)):
+        with pytest.raises(ValueError, match="PagedKVCache"):
+            cdx.PagedKVCache(cfg, 2, 40, device="cpu", **bad)
+    bounded = cdx.PagedKVCache(cfg, 2, 40, keep=10, device="cpu")
+    with pytest.raises(ValueError, match="bounded"):
+        bounded.begin(2, 3, token_counts=[3, 3])
+    with pytest.raises(ValueError, match="bounded"):
+        bounded.truncate([1, 1])
+    c = cdx.PagedKVCache(cfg, 2, 40, page_size=16, device="cpu")
+    for args in ((3, [1, 1], False), (2, [1, 1, 1], False), (2, [3, 1], False), (2, [-1, 1], False), (3, [2, 2], True),
+                 (0, [0, 0], False)):
+        with pytest.raises(ValueError, match="PagedKVCache"):
+            c.begin(args[0] if args[0] == 3 and not args[2] else 2, 3 if args[2] else min(args[0], 2),
+                    token_counts=args[1], packed=args[2])
+    with pytest.raises(ValueError, match="full"):
+        c.begin(2, 49, token_counts=[49, 1])
+    assert c.lengths.tolist() == [0, 0] and c.newest == 0
+
+
+def test_cache_without_a_pool_is_cut_anywhere():
+    import complexity_deep as cdx
+    c = cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), 3, 40, page_size=16, device="cpu")
+    c.begin(3, 9, torch.tensor([9, 4, 0]))
+    c.begin(3, 1)
+    c.truncate(torch.tensor([5, 50, 0]))
+    assert c.lengths.tolist() == [5, 5, 0] and c.positions.tolist() == [4, 4, -1] and c.longest == 5
+    c.begin(3, 1)
+    assert c.lengths.tolist() == [6, 6, 1] and c.longest == c.newest == 6
+    c.release([0])
+    assert c.lengths.tolist() == [0, 6, 1] and c.longest == 6
+    with pytest.raises(IndexError):
+        c.release([3])
+    c.release([1, 2])
+    assert c.lengths.tolist() == [0, 0, 0] and c.newest == 0 and c.positions.tolist() == [-1, -1, -1]
+    c.begin(3, 4)  # prompts again
+    assert c.lengths.tolist() == [4, 4, 4] and c.prompt

@@ -8,7 +8,7 @@
 //                    (the lists and counts that a call changes come out beside the old ones; a new
 //                    page's table entry is written by the row in its first slot, and read by
 //                    nobody), so that one launch without any wait between blocks does: every block sums
-//                    up the needs itself, 512 sequences at a time, and maps 2048 rows.
+//                    up the needs itself, 512 sequences at a time, and maps 512 rows.
 //   truncate_kernel  the pages past ceil(new length / page), put on the list so that the ones that
 //                    reserve took last come off it first: reserve and truncate undo each other.
 //   chunk_append_kernel  per row of the packed projection: per-head RMSNorm, RoPE, q out, k and v into the
@@ -20,7 +20,7 @@ namespace cdx {
 namespace {
 
 constexpr int kPlanThreads = 512;
-constexpr int kPlanRows = 4 * kPlanThreads;  // rows that a block maps
+constexpr int kPlanRows = kPlanThreads;  // rows that a block maps
 
 typedef long long i64;
 

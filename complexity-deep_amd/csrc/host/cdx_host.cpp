@@ -533,10 +533,9 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor, Tensor, Tens
                           out, out + B, out + 2 * B, out + 3 * B, free_pages ? out + 4 * B : nullptr,
                           row_slots.data_ptr<int64_t>(), row_positions.data_ptr<int32_t>(), stream()),
         "cdx_paged_reserve");
-  OptTensor left;
-  if (free_pages) left = small.narrow(0, 4 * B, 1);
-  return std::make_tuple(small.narrow(0, 0, B), small.narrow(0, B, B), small.narrow(0, 2 * B, B),
-                         small.narrow(0, 3 * B, B), left, row_slots, row_positions);
+  auto part = small.split_with_sizes({B, B, B, B, 1});
+  return std::make_tuple(part[0], part[1], part[2], part[3], free_pages ? OptTensor(part[4]) : OptTensor(), row_slots,
+                         row_positions);
 }
 
 std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_truncate(const Tensor& to, const Tensor& lengths,
@@ -553,7 +552,8 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_truncate(const Tensor& t
                            free_pages.data_ptr<int32_t>(), free_pages.numel(), free_count.data_ptr<int32_t>(), out,
                            out + B, out + 2 * B, stream()),
         "cdx_paged_truncate");
-  return std::make_tuple(small.narrow(0, 0, B), small.narrow(0, B, B), small.narrow(0, 2 * B, 1));
+  auto part = small.split_with_sizes({B, B, 1});
+  return std::make_tuple(part[0], part[1], part[2]);
 }
 
 OptTensor paged_chunk_append(const Tensor& qkv, const Tensor& k, const Tensor& v, const Tensor& row_slots,

@@ -691,6 +691,9 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
       };
       each<RING - 1>(read);
       move_max();
+      // Of the two waves of a SIMD the one among its products goes on with them (2048 tokens over 65536, heads of
+      // 128: 1015 -> 990 us, 4 x 512 over 4096 of 64: 51 -> 47; where the head is padded, heads of 80, 81 -> 84).
+      if constexpr (!GEN) __builtin_amdgcn_s_setprio(1);
       each<ALL>([&](auto index) __attribute__((always_inline)) {
         constexpr int i = decltype(index)::value;
         // The pairs of P are spread over the products before the last slab's, each slab's before its own.
@@ -707,6 +710,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
         }
         __builtin_amdgcn_sched_barrier(0);
       });
+      if constexpr (!GEN) __builtin_amdgcn_s_setprio(0);
       if constexpr (next) row_max(nxt, t + 1, bad_next);
     };
 

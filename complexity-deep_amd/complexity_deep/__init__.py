@@ -10,8 +10,9 @@ sort_tokens_by_expert, sort_tokens_by_expert_fast, cggr_grouped_gemm (also as
 grouped_gemm_pytorch and persistent_cggr_gemm), persistent_swiglu_cggr,
 fused_swiglu_triton, fused_swiglu_simple, fused_mu_qkv_projection.  Beyond the
 reference: the operators of a paged generation, paged_qkv_append, paged_write,
-paged_attention, paged_evict and sample_tokens, and PagedKVCache, which ties them to a
-model (ComplexityModel.forward and generate_paged).
+paged_attention, paged_evict and sample_tokens, those of any number of tokens per sequence
+and call, paged_reserve, paged_truncate, paged_chunk_append and paged_chunk_attention, and
+PagedKVCache, which ties them to a model (ComplexityModel.forward and generate_paged).
 
 The hot path (routing, MoE grouped SwiGLU GEMM, mu-QKV GEMM, add+RMSNorm) runs only
 on the kernels in libcdx.so; the forward is inference-only (no backward).

@@ -13,6 +13,11 @@
 //                    reserve took last come off it first: reserve and truncate undo each other.
 //   chunk_append_kernel  per row of the packed projection: per-head RMSNorm, RoPE, q out, k and v into the
 //                    row's slot; 16 lanes a head, as paged_append_kernel.
+//
+// Measured (us of a kernel): reserve 3.0 for one sequence, 4.5 for 256 with 8432 rows or 64 with 131072 (launch and two
+// rounds of loads); truncate 2.9 for 256 sequences, 5.0 for 1024 that give 32000 pages back; append of 8192 rows of
+// 16/8 heads of 128 25 (134 MB read and written, 5.4 TB/s, a plain copy's rate), of 5 rows 2.7.  Two heads a group of
+// lanes, loaded together, took as long.
 #include "cdx_paged.h"
 #include "cdx_wave.h"
 

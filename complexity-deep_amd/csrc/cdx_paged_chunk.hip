@@ -19,8 +19,8 @@
 //     columns of the matrix instruction taken by queries of several rows.
 //
 // Measured (us a call, issued back to back, and what of it bounds the call), 16/8 heads of 128 unless said: 2048 new tokens
-// over 65536 slots 1000 (1080 TFLOP/s), 8 x 1024 over 2048 118 (875), 8 prompts of 2048 163 (843); 4 chunks of 512
-// among 60 single tokens, up to 2048 slots, 53 (227 MB: 4.3 TB/s); 16 of 1 .. 777 over up to 4099, 16/4 of 80, 82
+// over 65536 slots 990 (1090 TFLOP/s), 8 x 1024 over 2048 113 (915), 8 prompts of 2048 156 (885); 4 chunks of 512
+// among 60 single tokens, up to 2048 slots, 50 (227 MB: 4.5 TB/s); 16 of 1 .. 777 over up to 4099, 16/4 of 80, 82
 // (590); 64 single tokens over 2049 94 (537 MB: 5.7 TB/s); 8 over 32768 31; 5 over 505, 8/4 of 40, 5.8.
 #include <algorithm>
 #include <type_traits>
@@ -376,12 +376,15 @@ __device__ __forceinline__ void each(F&& f) {
 constexpr int kTileM = 128;  // queries of a tile
 
 // The tile kernel's tile of this number: what takes longest comes first, so that the blocks that are left at the
-// end are short ones.  Of 64 sequences each, by the keys of the last tile and the waves that its
-// queries occupy (a key costs one wave about half of what it costs four, the fetch being the same);
-// within a sequence the last tile first.  By a whole wave; without queries if there are fewer tiles.
+// end are short ones (16 sequences of 1 .. 777 over up to 4099: 120 us by sequence, 82 so; 8 of 1024 over 2048:
+// 118 by sequence, the longest first, 113 so).  Of 64 sequences each, by the keys that a tile's last query
+// sees, in steps of 64; a sequence of fewer queries than a tile counts by the waves that they occupy (a
+// key costs one wave about half of what it costs four, the fetch being the same).  How many tiles there
+// are of so many keys or more is known for each sequence, so that the step of a number is found bit by
+// bit, and the tile among those of the step.  By a whole wave; without queries if there are fewer tiles.
 __device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t number, int lane) {
   ChunkTile t{};
-  int64_t at = number;
+  int32_t at = (int32_t)number;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     const int n_seq = min(64, p.B - b0);
     const int b = b0 + min(lane, n_seq - 1);
@@ -389,30 +392,38 @@ __device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t n
     // (Rows outside the call's are dropped.)
     const int32_t count = lane >= n_seq || first < 0 ? 0 : min(asked, max(p.rows - first, 0));
     const int32_t queries = count * p.group, tiles = (queries + kTileM - 1) / kTileM;
-    const int64_t all = wave_sum((u64)tiles);
+    const int32_t all = wave_sum(tiles);
     if (at >= all) {
       at -= all;
       continue;
     }
-    // The place of each among the 64, and then the tiles of those in the first places.
-    const uint32_t keys = (uint32_t)min(max(length, 0), p.t.capacity()) / kKeys + 1;
-    const uint32_t cost = tiles > 0 ? keys * (uint32_t)(2 + (min(queries, kTileM) + 31) / 32) : 0;
-    int place = 0;
-    for (int i = 0; i < n_seq; ++i) {
-      const uint32_t other = (uint32_t)read_lane((int)cost, i);
-      place += other > cost || (other == cost && i < lane) ? 1 : 0;
+    const int32_t before = min(max(length - asked, 0), p.t.capacity());
+    const int32_t top = (before + count) / kKeys + 1;
+    const int32_t only = top * (2 + (min(queries, kTileM) + 31) / 32) / 6;  // (of a sequence of one tile)
+    // Tiles of x steps or more: tile j sees before + (j + 1) kTileM / group keys.
+    auto from = [&](int32_t x) {
+      if (tiles <= 1) return only >= x ? tiles : 0;
+      const int64_t j = (((int64_t)kKeys * x - before) * p.group + kTileM - 1) / kTileM - 1;
+      return tiles - (int32_t)min(max(j, (int64_t)0), (int64_t)tiles);
+    };
+    int32_t above = 0, here = tiles;
+    if (n_seq > 1) {  // (one sequence's tiles go from the last to the first)
+      int32_t x = 0, most = top;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d, 64));
+      for (int bit = 31 - __builtin_clz(__builtin_amdgcn_readfirstlane(most)); bit >= 0; --bit)
+        if (wave_sum(from(x | 1 << bit)) > at) x |= 1 << bit;
+      above = from(x + 1), here = from(x) - above;
+      at -= wave_sum(above);
     }
-    if (lane >= n_seq) place = lane;
-    const int here = __builtin_amdgcn_ds_permute(place * 4, tiles << 6 | lane);
-    const int64_t upto = (int64_t)wave_inclusive((u64)(here >> 6));
+    const int32_t upto = wave_inclusive(here);
     const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
-    const int from = read_lane(here, i) & 63;
-    t.b = b0 + from;
-    t.begin = t.first = read_lane(first, from);
-    t.count = read_lane(count, from);
-    t.before = (int32_t)max((int64_t)read_lane(length, from) - read_lane(asked, from), (int64_t)INT32_MIN);
+    t.b = b0 + i;
+    t.begin = t.first = read_lane(first, i);
+    t.count = read_lane(count, i);
+    t.before = (int32_t)max((int64_t)read_lane(length, i) - read_lane(asked, i), (int64_t)INT32_MIN);
     t.queries = t.count * p.group;
-    t.m0 = (int32_t)((int64_t)read_lane((u64)upto, i) - 1 - at) * kTileM;
+    t.m0 = (read_lane(tiles - above + upto - here, i) - 1 - at) * kTileM;
     return t;
   }
   return t;

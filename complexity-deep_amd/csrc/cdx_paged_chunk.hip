@@ -398,9 +398,12 @@ __device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t n
       continue;
     }
     const int32_t before = min(max(length - asked, 0), p.t.capacity());
-    const int32_t top = (before + count) / kKeys + 1;
-    const int32_t only = top * (2 + (min(queries, kTileM) + 31) / 32) / 6;  // (of a sequence of one tile)
-    // Tiles of x steps or more: tile j sees before + (j + 1) kTileM / group keys.
+    // Steps of a sequence of one tile, and the most that a tile has (also a last one that is partly empty, as
+    // ``from`` counts it): tile j sees before + (j + 1) kTileM / group keys.
+    const int32_t steps = (int32_t)(((int64_t)before + count) / kKeys + 1);
+    const int32_t only = steps * (2 + (min(queries, kTileM) + 31) / 32) / 6;
+    const int32_t top = tiles <= 1 ? only : (int32_t)((before + (int64_t)tiles * kTileM / p.group) / kKeys);
+    // Tiles of x steps or more.
     auto from = [&](int32_t x) {
       if (tiles <= 1) return only >= x ? tiles : 0;
       const int64_t j = (((int64_t)kKeys * x - before) * p.group + kTileM - 1) / kTileM - 1;
@@ -408,7 +411,7 @@ __device__ __forceinline__ ChunkTile chunk_tile(const ChunkParams& p, uint32_t n
     };
     int32_t above = 0, here = tiles;
     if (n_seq > 1) {  // (one sequence's tiles go from the last to the first)
-      int32_t x = 0, most = top;
+      int32_t x = 0, most = max(top, 1);
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d, 64));
       for (int bit = 31 - __builtin_clz(__builtin_amdgcn_readfirstlane(most)); bit >= 0; --bit)

@@ -107,6 +107,16 @@ def test_reserve_and_truncate_random(cdx, seed):
     assert have.tolist() == (want[2] + [-5] * room)[:room]
 
 
+def test_a_pool_without_pages(cdx):
+    print("reserve: an empty list of free pages", flush=True)
+    free, count, table = _ints([]), _ints([0]), _ints([[3, -1], [4, -1]])
+    rows = cdx.paged_reserve(_ints([2, 1]), _ints([15, 3]), _ints([14, 2]), table, 16, 3, free_pages=free,
+                             free_count=count)
+    assert rows.counts.tolist() == [0, 1] and rows.row_slots.tolist() == [-1, -1, 67]
+    new = cdx.paged_truncate(_ints([0, 9]), rows.lengths, rows.positions, table, 16, free, rows.free_count)
+    assert [t.tolist() for t in new] == [[0, 4], [-1, 3], [0]]
+
+
 def test_truncate_undoes_reserve(cdx):
     print("truncate undoes reserve", flush=True)
     rng = random.Random(5)
@@ -399,6 +409,42 @@ def test_many_sequences(cdx):
         args = _case(B, 4, 2, 32, 16, before, counts, seed=B)
         want, bound = chunk.attention(*args)
         _check(_run(cdx, *args), want, bound)
+
+
+@pytest.mark.parametrize("nq,nkv,counts,before", [
+    (4, 4, [129, 129], [0, 0]), (4, 4, [129, 1, 193, 300], [0, 60, 0, 0]), (8, 4, [65, 64, 129], [0, 127, 0]),
+    (6, 2, [43, 43, 86], [62, 0, 20]), (4, 1, [33, 1, 65, 97, 2], [0, 255, 0, 31, 500]), (12, 4, [500], [0]),
+    (20, 1, [7, 40, 13], [0, 0, 64]), (128, 1, [1, 2, 3], [0, 9, 300]), (150, 1, [1, 2, 3], [0, 9, 300]),
+])
+def test_every_tile_once(cdx, nq, nkv, counts, before):
+    """Sequences whose tiles end past their tokens, at and around steps of the order that tiles are taken in."""
+    print(f"chunk attention: tiles {nq}/{nkv} {counts} over {before}", flush=True)
+    args = _case(len(counts), nq, nkv, 16, 16, before, counts, seed=nq)
+    want, bound = chunk.attention(*args)
+    _check(_run(cdx, *args, max_tokens=max(counts)), want, bound)
+    _check(_run(cdx, *args, max_tokens=0), want, bound)  # a wrong hint chooses another kernel, no other result
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_random_batches(cdx, seed):
+    rng = random.Random(seed)
+    nq, nkv = rng.choice([(4, 4), (4, 2), (6, 2), (8, 2), (16, 1), (3, 1)])
+    D, page = rng.choice([8, 32, 40, 64, 80, 128]), rng.choice([16, 32, 64, 128, 256])
+    B = rng.choice([1, 2, 5, 30, 64, 65, 130])
+    most, old = rng.choice([1, 4, 40, 300, 1000 // B + 1]), rng.choice([0, 1, 70, 600, 4000 // B])
+    counts = [rng.choice([0, 1, most, rng.randint(0, most)]) for _ in range(B)]
+    counts[rng.randrange(B)] = most
+    before = [rng.choice([0, old, rng.randint(0, old)]) for _ in range(B)]
+    gaps = [rng.choice([0, 0, 0, rng.randint(0, 9)]) for _ in range(B)]
+    print(f"chunk attention: random {nq}/{nkv} D={D} page={page} B={B} most={most} old={old}", flush=True)
+    args = _case(B, nq, nkv, D, page, before, counts, gaps=gaps, seed=seed)
+    want, bound = chunk.attention(*args, rounded_p=not _few(most, nq // nkv))
+    out = _run(cdx, *args, max_tokens=most)
+    _check(out, want, bound)
+    gap = torch.ones(out.shape[0], dtype=torch.bool)
+    for s, c in zip(args[4], counts):
+        gap[s:s + c] = False
+    assert not out[gap.cuda()].any()
 
 
 def test_strided_operands_and_streams(cdx):

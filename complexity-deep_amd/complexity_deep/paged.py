@@ -513,11 +513,12 @@ class PagedKVCache:
     ``lengths`` and ``positions`` (of the newest tokens) live on the device; ``longest`` and ``newest``
     are the host's bounds, and nothing waits for the device but the first call of a batch whose
     bound, of right-padded prompts with prompt_lengths on the device, has reached the capacity: it reads
-    how long the longest is; with token_counts on the device, or a pool, such a call reads all lengths.  One call at a time may use a cache.  A
-    step that is captured into a graph counts on the device when it is replayed, not here: keep to
-    max_length then (a token past the capacity is not stored).  A TransformerBlock or
-    ComplexityAttention called by itself takes ``cache[i]``, after ``begin`` has counted the call's
-    tokens."""
+    how long the longest is; with token_counts on the device, or a pool, such a call reads all lengths.  One
+    call at a time may use a cache.  A call that is captured into a graph counts on the device when it is
+    replayed, not here: keep to max_length then (a token past the capacity is not stored).  Calls with
+    token_counts, or of a pool, read the lengths first once a call of the cache was captured.  A
+    TransformerBlock or ComplexityAttention called by itself takes ``cache[i]``, after ``begin`` has
+    counted the call's tokens."""
 
     def __init__(self, config, batch_size: int, max_length: int, *, page_size: int = 64, keep: Optional[int] = None,
                  recent: Optional[int] = None, pages: Optional[int] = None, device="cuda"):
@@ -568,6 +569,7 @@ class PagedKVCache:
                 self.weights = torch.zeros(shape, dtype=torch.float32, device=device)
                 self._weights_before = torch.empty_like(self.weights)
                 self.slot_positions = torch.empty(shape, dtype=torch.int32, device=device)
+        self._replays = False  # whether a call was captured: its replays count on the device alone
         self.reset()
 
     @property
@@ -695,6 +697,7 @@ class PagedKVCache:
         # Every layer adds to the weights in place: a call that raises is taken back from a copy (1B preset, 32
         # sequences of 2048 slots: 14 us of a step of 2.4 ms).  A step that is captured runs as a whole or not
         # at all, and makes none.
+        self._replays |= capturing
         self._saved = self.weights is not None and not capturing
         if self._saved:
             self._weights_before.copy_(self.weights)
@@ -724,10 +727,12 @@ class PagedKVCache:
         Raises, with nothing changed, if the capacity or the pool does not suffice; a call that is being captured
         is not looked at, and tokens that do not fit are then neither counted nor stored."""
         capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()
+        self._replays |= capturing
         before = (self.longest, self.newest, self._exact, self._lengths)
-        lengths = self._lengths
+        lengths = self._lengths if not self._replays else None
         used = self.batch_size * -(-(self.longest + most) // self.page_size)
-        if not capturing and (self.longest + most > self.capacity or (self.pages is not None and used > self.pages)):
+        if not capturing and (self._replays or self.longest + most > self.capacity
+                              or (self.pages is not None and used > self.pages)):
             lengths = self.lengths.tolist() if lengths is None else lengths
             known = [max(0, n) for n in counts.tolist()] if known is None else known
             if any(c > 0 and n + c > self.capacity for n, c in zip(lengths, known)):
@@ -768,6 +773,8 @@ class PagedKVCache:
             gone = (self.lengths - to.clamp(min=0)).clamp(min=0)
             self._counts.sub_(gone)
         self.rows = self._before = None
+        if self._replays:
+            self._lengths = None
         if known is not None and (self._lengths is not None or max(known) <= 0):
             self._lengths = [max(0, min(n, t)) for n, t in zip(self._lengths or known, known)]
             self.longest, self._exact = max(self._lengths), True

@@ -237,6 +237,38 @@ def test_a_captured_call(cdx):
         assert torch.equal(caches[0]._state, caches[1]._state)
 
 
+@pytest.mark.parametrize("pages", [None, 12])
+def test_a_call_after_replayed_ones(cdx, pages):
+    """Replays count on the device alone: the calls after them go by its lengths."""
+    print(f"chunks: eager after replays, pages={pages}", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    cache = cdx.PagedKVCache(m.config, 2, 32, page_size=16, pages=pages)
+    ids = torch.randint(0, 600, (2, 1), generator=torch.Generator().manual_seed(3)).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.inference_mode(), torch.cuda.stream(side):
+        m(ids.expand(2, 18), past_key_values=cache, token_counts=[18, 18])
+        m(ids, past_key_values=cache)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.inference_mode(), torch.cuda.graph(graph):
+        m(ids, past_key_values=cache)
+    with torch.inference_mode():
+        for want in (22, 23, 24):
+            if want == 22:
+                for _ in range(3):
+                    graph.replay()
+            else:
+                graph.replay()
+            cache.truncate([want, want])
+            assert cache.lengths.tolist() == [want, want]
+            with pytest.raises(ValueError, match="full"):
+                m(ids.expand(2, 33 - want), past_key_values=cache, token_counts=[1, 33 - want])
+            assert cache.lengths.tolist() == [want, want]
+        m(ids.expand(2, 8), past_key_values=cache, token_counts=[8, 0])
+    assert cache.lengths.tolist() == [32, 24]
+
+
 def test_modules_by_themselves(cdx):
     print("chunks: an attention module by itself", flush=True)
     m = _model(cdx, 64, 4, 2)

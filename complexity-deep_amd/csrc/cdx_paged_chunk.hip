@@ -337,9 +337,10 @@ __global__ __launch_bounds__(64 * kPagedWaves, NC == 4 && !FULL ? 2 : 4) void pa
       *reinterpret_cast<float4*>(p.part_o + at * p.D + d) = make_float4(o[0], o[1], o[2], o[3]);
     } else {
       // No keys at all: zeros.  Keys whose scores are all -inf: 0 / 0, as softmax has it.
-      const float inv = sees ? 1.f / L : 0.f;
+      // (No product with 0: the sums of a column that sees nothing may hold infinite values.)
+      const float inv = 1.f / L;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= inv;
+      for (int e = 0; e < 4; ++e) o[e] = sees ? o[e] * inv : 0.f;
       head_store4(p.out + row * p.D + d, o);
     }
   }

@@ -332,6 +332,20 @@ def test_special_values_of_later_tokens_do_not_reach_earlier_ones(cdx, nq, nkv, 
         assert torch.equal(x[y.isinf()], y[y.isinf()])
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("slots,count,gap", [(64, 1, 3), (200, 5, 2), (3000, 2, 3), (90, 1, 200), (900, 150, 40)])
+def test_special_values_do_not_reach_rows_without_tokens(cdx, value, slots, count, gap):
+    """Rows behind a sequence's are taken along with its last ones; they stay zeros, whatever its cache holds."""
+    print(f"chunk attention: {value} in {slots} slots, {count} rows and {gap} without a token", flush=True)
+    args = _case(2, 4, 2, 64, 16, [slots - count, 0], [count, 0], gaps=[gap, gap], seed=slots)
+    q, k, v, table, starts, counts, lengths = args
+    for slot in (3, slots // 2):
+        v[int(table[0, slot // 16]), :, slot % 16, 5] = value
+    q[count:] = value
+    out = _run(cdx, *args, max_tokens=count)
+    assert not out[count:].any() and not bool(out[:count].view(count, 4, 64)[..., 5].isfinite().any())
+
+
 def test_missing_pages(cdx):
     print("chunk attention: pages outside the pool", flush=True)
     for count in (3, 100):

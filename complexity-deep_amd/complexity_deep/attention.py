@@ -662,12 +662,12 @@ class ComplexityAttention(nn.Module):
         attn = None
         if fast is not None:
             attn = fast.paged_step(x, mu, self._qkv_w.buffer(self), nq, D, *qn, eps, table, k_pages, v_pages,
-                                   cache.block_table, cache.lengths, cache.positions, weights)
+                                   cache.block_table, cache.step_lengths, cache.positions, weights)
         if attn is None:
             w_x, w_mu = self.qkv_weights()
             q = qkv_paged(x, mu, w_x, w_mu, self.hidden_size, nq, *qn, eps, table, k_pages, v_pages, cache.block_table,
-                          cache.lengths, cache.positions)
-            attn = paged_attention(q, k_pages, v_pages, cache.block_table, cache.lengths, weights=weights,
+                          cache.step_lengths, cache.positions)
+            attn = paged_attention(q, k_pages, v_pages, cache.block_table, cache.step_lengths, weights=weights,
                                    weights_out=weights)
             attn = (attn if weights is None else attn[0]).view(B, 1, -1)
         return self._out_proj(attn, residual)

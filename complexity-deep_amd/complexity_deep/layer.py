@@ -204,7 +204,7 @@ class TransformerBlock(nn.Module):
             if cache.rows is not None:
                 return None
             pk, pv, weights = cache.layer(past.index)
-            table, lengths, positions = cache.block_table, cache.lengths, cache.positions
+            table, lengths, positions = cache.block_table, cache.step_lengths, cache.positions
             cos_sin = cache.rotary_table(attn.rotary_emb, h.device)
         else:
             pk, pv = (past[0], past[1]) if past is not None else (None, None)

@@ -354,6 +354,8 @@ class ComplexityModel(nn.Module):
         B, S = input_ids.shape
         if chunk is not None and chunk <= 0:
             raise ValueError(f"generate_paged: chunk={chunk} must be positive")
+        if chunk is not None and S == 0:
+            raise ValueError("generate_paged: empty prompts")
         eos = self.config.eos_token_id if eos_token_id is None else eos_token_id
         dev = input_ids.device
         if uniforms is None:

@@ -580,6 +580,11 @@ class PagedKVCache:
     def positions(self) -> torch.Tensor:
         return self._counts[1]
 
+    @property
+    def step_lengths(self) -> torch.Tensor:
+        """What a step of one token per sequence takes for ``lengths``: 0 where the token has no slot."""
+        return self.lengths if self._step is None else self._step
+
     def __len__(self) -> int:
         return self.k_pages.shape[0]
 
@@ -613,6 +618,7 @@ class PagedKVCache:
         self._exact = True              # whether one has as many slots
         self._lengths = [0] * self.batch_size  # the host's, or None if it does not know them
         self.prompt = True              # what the call at hand brings
+        self._step = None
         self.rows = None                # (with token_counts: where its rows go
         self.most = 0                   # and the most that a sequence has of them)
         self._before = None             # what ``cancel`` goes back to after a call that took pages
@@ -684,7 +690,9 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: after the prompts a call without token_counts takes one token per sequence "
                              "(reset() empties the cache)")
         if self.pages is not None:
-            self._reserve(self._ones, [1] * batch_size, 1, batch_size, None)
+            rows = self._reserve(self._ones, [1] * batch_size, 1, batch_size, None)
+            # (A token that a replay finds no page for has no slot, and must not take the newest one's.)
+            self._step = rows.counts * rows.lengths if self._replays else None
             self.prompt = False
             return
         capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()

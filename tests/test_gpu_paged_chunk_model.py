@@ -204,6 +204,8 @@ def test_generation_with_prompts_in_pieces(cdx, oracle):
         assert new.shape == (B, 6) and cache.lengths.tolist() == (end + 5).tolist()
     with pytest.raises(ValueError):
         m.generate_paged(ids, 2, chunk=0)
+    with pytest.raises(ValueError):
+        m.generate_paged(ids[:, :0], 2, chunk=4)
 
 
 def test_a_captured_call(cdx):
@@ -267,6 +269,49 @@ def test_a_call_after_replayed_ones(cdx, pages):
             assert cache.lengths.tolist() == [want, want]
         m(ids.expand(2, 8), past_key_values=cache, token_counts=[8, 0])
     assert cache.lengths.tolist() == [32, 24]
+
+
+@pytest.mark.parametrize("B", [2, 12])
+def test_replayed_steps_of_a_pool_that_runs_out(cdx, B):
+    """A step that a replay finds no page for is neither counted nor stored, and leaves the tokens that are there."""
+    print(f"chunks: replayed steps of a pool that runs out, B={B}", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    cache = cdx.PagedKVCache(m.config, B, 64, page_size=16, pages=B + 1)
+    ids = torch.randint(0, 600, (B, 13), generator=torch.Generator().manual_seed(3)).cuda()
+    new = ids[:, :1].clone()
+    with torch.inference_mode():
+        m(ids, past_key_values=cache)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            m(new, past_key_values=cache)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = m(new, past_key_values=cache).logits
+        for _ in range(3):  # 14 -> 16, then the first sequence takes the page that is left
+            graph.replay()
+        assert cache.lengths.tolist() == [17] + [16] * (B - 1) and int(cache.free_count) == 0
+        table = cache.block_table[:, 0].long()
+        kept = [t[:, table].clone() for t in (cache.k_pages, cache.v_pages)]
+        for n in range(18, 22):
+            new.copy_(ids[:, n - 16:n - 15])
+            graph.replay()
+            assert cache.lengths.tolist() == [n] + [16] * (B - 1)
+            assert cache.positions.tolist() == [n - 1] + [15] * (B - 1)
+            for t, k in zip((cache.k_pages, cache.v_pages), kept):
+                assert torch.equal(t[:, table], k)
+        with pytest.raises(ValueError, match="pages"):
+            m(new, past_key_values=cache)
+        # An eager cache of the first sequence's tokens gives its logits.
+        alone = cdx.PagedKVCache(m.config, 1, 64, page_size=16)
+        want = m(torch.cat([ids[:1], *[ids[:1, :1]] * 4, ids[:1, 2:6]], 1), past_key_values=alone).logits[:, -1]
+        e = errors(logits[:1, -1], want)
+        assert e["max_rel"] <= MAX_REL and e["rel_rms"] <= REL_RMS, e
+        assert bool(logits.isfinite().all())
+        cache.release(range(1, B))
+        m(new, past_key_values=cache)
+        assert cache.lengths.tolist() == [22] + [1] * (B - 1)
 
 
 def test_modules_by_themselves(cdx):

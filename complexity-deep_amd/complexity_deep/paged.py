@@ -659,6 +659,10 @@ class PagedKVCache:
                                       None if packed else tokens)
             self.most, self.prompt = most, False
             return
+        capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()
+        if self.newest == 0 and self._replays and not capturing:  # (replays may have brought tokens since)
+            self._read_longest(self.lengths)
+            self.newest = int(self.positions.max()) + 1
         if self.newest == 0:
             if not 0 < tokens <= self.capacity:
                 raise ValueError(f"PagedKVCache: prompts of {tokens} tokens in a cache of {self.capacity}")
@@ -695,7 +699,6 @@ class PagedKVCache:
             self._step = rows.counts * rows.lengths if self._replays else None
             self.prompt = False
             return
-        capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()
         if self.longest >= self.capacity and not self._exact and not capturing:
             self._read_longest(self.lengths)
         if self.longest >= self.capacity:
@@ -794,9 +797,9 @@ class PagedKVCache:
         """Empty these sequences (their numbers); the pages go back to the pool."""
         to = [2 ** 31 - 1] * self.batch_size
         for i in sequences:
-            if not 0 <= int(i) < self.batch_size:
+            if not 0 <= operator.index(i) < self.batch_size:
                 raise IndexError(f"PagedKVCache: sequence {i} of {self.batch_size}")
-            to[int(i)] = 0
+            to[operator.index(i)] = 0
         self.truncate(to)
 
     def _read_longest(self, lengths: torch.Tensor) -> None:

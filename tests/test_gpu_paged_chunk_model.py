@@ -268,7 +268,20 @@ def test_a_call_after_replayed_ones(cdx, pages):
                 m(ids.expand(2, 33 - want), past_key_values=cache, token_counts=[1, 33 - want])
             assert cache.lengths.tolist() == [want, want]
         m(ids.expand(2, 8), past_key_values=cache, token_counts=[8, 0])
-    assert cache.lengths.tolist() == [32, 24]
+        assert cache.lengths.tolist() == [32, 24]
+        # An emptied cache takes prompts, but not where replays have brought tokens meanwhile.
+        cache.release([0, 1])
+        graph.replay()
+        with pytest.raises(ValueError):
+            m(ids.expand(2, 8), past_key_values=cache)
+        assert cache.lengths.tolist() == [1, 1]
+        cache.release([0, 1])
+        m(ids.expand(2, 8), past_key_values=cache)
+        graph.replay()
+        m(ids, past_key_values=cache)
+    assert cache.lengths.tolist() == [10, 10] and cache.positions.tolist() == [9, 9]
+    with pytest.raises(TypeError):
+        cache.release([0.5])
 
 
 @pytest.mark.parametrize("B", [2, 12])

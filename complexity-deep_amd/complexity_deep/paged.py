@@ -485,6 +485,11 @@ def paged_chunk_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     return out
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    """Whether work on t is being captured into a graph."""
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class PagedLayer(NamedTuple):
     """One layer of a PagedKVCache, as ComplexityAttention takes it for past_key_value."""
     cache: "PagedKVCache"
@@ -624,6 +629,12 @@ class PagedKVCache:
         self._before = None             # what ``cancel`` goes back to after a call that took pages
         self._saved = False             # whether _weights_before holds the weights before it
 
+    def _captured(self) -> bool:
+        """Whether the call at hand is being captured, which is noted: its replays count on the device alone."""
+        capturing = _capturing(self._counts)
+        self._replays |= capturing
+        return capturing
+
     def evict(self) -> None:
         """Cut every sequence of more than ``keep`` slots to ``keep``."""
         if self.keep is None:
@@ -648,6 +659,7 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: a block table {tuple(self.block_table.shape)} of pages of {self.page_size} "
                              f"has no room for {self.capacity} tokens")
         self.rows = self._before = None
+        capturing = self._captured()
         if token_counts is not None:
             if self.keep is not None or prompt_lengths is not None or tokens <= 0:
                 raise ValueError("PagedKVCache: token_counts in a bounded cache, beside prompt_lengths, or without rows")
@@ -659,7 +671,6 @@ class PagedKVCache:
                                       None if packed else tokens)
             self.most, self.prompt = most, False
             return
-        capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()
         if self.newest == 0 and self._replays and not capturing:  # (replays may have brought tokens since)
             self._read_longest(self.lengths)
             self.newest = int(self.positions.max()) + 1
@@ -708,7 +719,6 @@ class PagedKVCache:
         # Every layer adds to the weights in place: a call that raises is taken back from a copy (1B preset, 32
         # sequences of 2048 slots: 14 us of a step of 2.4 ms).  A step that is captured runs as a whole or not
         # at all, and makes none.
-        self._replays |= capturing
         self._saved = self.weights is not None and not capturing
         if self._saved:
             self._weights_before.copy_(self.weights)
@@ -737,8 +747,7 @@ class PagedKVCache:
         """Pages and rows of ``counts`` tokens (on the host ``known``, or at most ``most`` each), which are counted.
         Raises, with nothing changed, if the capacity or the pool does not suffice; a call that is being captured
         is not looked at, and tokens that do not fit are then neither counted nor stored."""
-        capturing = self._counts.is_cuda and torch.cuda.is_current_stream_capturing()
-        self._replays |= capturing
+        capturing = _capturing(self._counts)
         before = (self.longest, self.newest, self._exact, self._lengths)
         lengths = self._lengths if not self._replays else None
         used = self.batch_size * -(-(self.longest + most) // self.page_size)

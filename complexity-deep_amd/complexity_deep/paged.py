@@ -611,6 +611,7 @@ class PagedKVCache:
 
     def reset(self) -> None:
         """Empty every sequence."""
+        self._captured()
         self._counts[0].zero_()
         self._counts[1].fill_(-1)
         if self.pages is not None:
@@ -641,6 +642,7 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: made without keep")
         if self.longest <= self.keep:
             return
+        self._captured()
         new = paged_evict(self.k_pages, self.v_pages, self.block_table, self.lengths, self.positions, self.weights,
                           self.slot_positions, self.keep, self.recent)
         for t, n in zip((self.lengths, self.weights, self.slot_positions), new):
@@ -785,6 +787,7 @@ class PagedKVCache:
         if self.keep is not None:
             raise ValueError("PagedKVCache: a bounded cache does not hold its tokens in order")
         to, known = self._integers(to, "to")
+        self._captured()
         if self.pages is not None:
             new = paged_truncate(to, self.lengths, self.positions, self.block_table, self.page_size, self.free_pages,
                                  self.free_count)

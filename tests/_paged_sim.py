@@ -45,7 +45,21 @@ class Sim:
         monkeypatch.setattr(paged, "paged_reserve", reserve)
         monkeypatch.setattr(paged, "paged_truncate", truncate)
         monkeypatch.setattr(paged, "_capturing", lambda t: self.capturing)
+        integers = cdx.PagedKVCache._integers
+
+        def unread(cache, values, name):
+            t, known = integers(cache, values, name)
+            return t, None if getattr(values, "on_device", False) else known
+
+        monkeypatch.setattr(cdx.PagedKVCache, "_integers", unread)
         self.cache = cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), batch_size, max_length, device="cpu", **kw)
+
+    @staticmethod
+    def device(values):
+        """Integers that the host does not know."""
+        t = torch.tensor(values)
+        t.on_device = True
+        return t
 
     def _tensors(self):
         c = self.cache

@@ -48,3 +48,23 @@ def test_calls_after_replayed_prompts(cdx):
             got, want = (m(more[:, :1], past_key_values=c).logits for c in (cache, eager))
             assert torch.equal(got, want)
         assert cache.lengths.tolist() == eager.lengths.tolist() == ([32, 21] if i % 2 == 0 else [21, 21])
+
+
+@pytest.mark.parametrize("pages", [None, 4])
+@torch.inference_mode()
+def test_calls_after_replayed_cuts(cdx, pages):
+    print(f"counts: replayed truncate, pages={pages}", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    cache, eager, other = (cdx.PagedKVCache(m.config, 2, 32, page_size=16, pages=pages) for _ in range(3))
+    ids = torch.randint(0, 600, (2, 90), generator=torch.Generator().manual_seed(4)).cuda()
+    to = torch.tensor([5, 3]).cuda()
+    for c in (cache, eager):
+        m(ids[:, :20], past_key_values=c, token_counts=[20, 18])
+    graph, _ = _graph(lambda: cache.truncate(to), lambda: other.truncate(to))
+    for i in range(4):
+        graph.replay()
+        eager.truncate(to)
+        assert cache.lengths.tolist() == eager.lengths.tolist() == [5, 3]
+        got, want = (m(ids[:, 20 + i:47 + i], past_key_values=c, token_counts=[27, 26]).logits for c in (cache, eager))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1, :26], want[1, :26])
+        assert torch.equal(cache._state, eager._state) and cache.lengths.tolist() == [32, 29]

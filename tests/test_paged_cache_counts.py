@@ -34,3 +34,27 @@ def test_a_call_after_replayed_prompts(monkeypatch, lengths):
         cache.begin(2, 1)
         assert not cache.prompt
         sim.holds([n + 1 for n in held])
+
+
+@pytest.mark.parametrize("pages", [None, 4])
+@pytest.mark.parametrize("cut", ["truncate", "reset"])
+def test_a_call_after_replayed_cuts(monkeypatch, pages, cut):
+    """The host's lengths are too large after them: they are read, not gone by."""
+    sim = Sim(monkeypatch, 2, 32, page_size=16, pages=pages)
+    cache = sim.cache
+    cache.begin(2, 20, token_counts=[20, 18])
+    sim.holds([20, 18], pages)
+    graph = sim.capture(lambda c: c.truncate(Sim.device([5, 3])) if cut == "truncate" else c.reset())
+    sim.holds([20, 18], pages)
+    held = [5, 3] if cut == "truncate" else [0, 0]
+    for i in range(3):
+        cache.begin(2, 11, token_counts=[11, 11])
+        sim.holds([31, 29] if i == 0 else [n + 11 for n in held], pages)
+        sim.replay(graph)
+        sim.holds(held, pages)
+        with pytest.raises(ValueError, match="full"):
+            cache.begin(2, 33, token_counts=[33 - held[0], 1])
+        cache.begin(2, 32, token_counts=[27, 26])
+        sim.holds([held[0] + 27, held[1] + 26], pages)
+        sim.replay(graph)
+        sim.holds(held, pages)

@@ -518,8 +518,9 @@ class PagedKVCache:
     ``lengths`` and ``positions`` (of the newest tokens) live on the device; ``longest`` and ``newest``
     are the host's bounds, and nothing waits for the device but the first call of a batch whose
     bound, of right-padded prompts with prompt_lengths on the device, has reached the capacity: it reads
-    how long the longest is; with token_counts on the device, or a pool, such a call reads all lengths.  One
-    call at a time may use a cache.  A call that is captured into a graph counts on the device when it is
+    how long the longest is; with token_counts on the device, or a pool, such a call reads all lengths, and
+    the counts, which must fit their rows.  Where it need not read them the device alone leaves out a sequence whose
+    tokens do not fit: it brings none, and its rows attend to nothing.  One call at a time may use a cache.  A call that is captured into a graph counts on the device when it is
     replayed, not here: keep to max_length then (a token past the capacity is not stored).  Calls with
     token_counts, or of a pool, read the lengths first once a call of the cache was captured.  A
     TransformerBlock or ComplexityAttention called by itself takes ``cache[i]``, after ``begin`` has
@@ -667,8 +668,10 @@ class PagedKVCache:
                 raise ValueError("PagedKVCache: token_counts in a bounded cache, beside prompt_lengths, or without rows")
             counts, known = self._integers(token_counts, "token_counts")
             most = tokens if known is None else max(0, *known)
-            if known is not None and (min(known) < 0 or (sum(known) if packed else most) > tokens):
-                raise ValueError(f"PagedKVCache: token_counts {known} in {tokens} rows" + (" each" if not packed else ""))
+            if known is not None:
+                if min(known) < 0:
+                    raise ValueError(f"PagedKVCache: token_counts {known} must not be negative")
+                self._check_rows(known, tokens, packed)
             self.rows = self._reserve(counts, known, most, tokens if packed else batch_size * tokens,
                                       None if packed else tokens)
             self.most, self.prompt = most, False
@@ -745,6 +748,11 @@ class PagedKVCache:
         known = None if values.is_cuda else values.tolist()
         return values.long().clamp(-2 ** 31, 2 ** 31 - 1).to(self.lengths.device, torch.int32), known
 
+    @staticmethod
+    def _check_rows(known, rows: int, packed: bool) -> None:
+        if (sum(known) if packed else max(known)) > rows:
+            raise ValueError(f"PagedKVCache: token_counts {known} in {rows} rows" + (" each" if not packed else ""))
+
     def _reserve(self, counts: torch.Tensor, known, most: int, rows: int, stride: Optional[int]) -> PagedRows:
         """Pages and rows of ``counts`` tokens (on the host ``known``, or at most ``most`` each), which are counted.
         Raises, with nothing changed, if the capacity or the pool does not suffice; a call that is being captured
@@ -756,7 +764,9 @@ class PagedKVCache:
         if not capturing and (self._replays or self.longest + most > self.capacity
                               or (self.pages is not None and used > self.pages)):
             lengths = self.lengths.tolist() if lengths is None else lengths
-            known = [max(0, n) for n in counts.tolist()] if known is None else known
+            if known is None:
+                known = [max(0, n) for n in counts.tolist()]
+                self._check_rows(known, rows if stride is None else stride, stride is None)
             if any(c > 0 and n + c > self.capacity for n, c in zip(lengths, known)):
                 raise ValueError(f"PagedKVCache: full ({self.capacity} tokens)")
             used, needed = (sum(-(-n // self.page_size) for n in ns)

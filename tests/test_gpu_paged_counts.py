@@ -68,3 +68,29 @@ def test_calls_after_replayed_cuts(cdx, pages):
         got, want = (m(ids[:, 20 + i:47 + i], past_key_values=c, token_counts=[27, 26]).logits for c in (cache, eager))
         assert torch.equal(got[0], want[0]) and torch.equal(got[1, :26], want[1, :26])
         assert torch.equal(cache._state, eager._state) and cache.lengths.tolist() == [32, 29]
+
+
+@torch.inference_mode()
+def test_counts_on_the_device_past_their_rows(cdx):
+    print("counts: on the device, past their rows", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    ids = torch.randint(0, 600, (2, 40), generator=torch.Generator().manual_seed(4)).cuda()
+    cache = cdx.PagedKVCache(m.config, 2, 48, page_size=16, pages=4)
+    for _ in range(2):
+        for rows, counts in ((ids, [41, 1]), (ids, [1, 41]), (ids[0], [30, 11])):
+            with pytest.raises(ValueError, match="token_counts"):
+                m(rows, past_key_values=cache, token_counts=torch.tensor(counts).cuda())
+            assert cache.lengths.tolist() == [0, 0] and int(cache.free_count) == 4
+        m(ids, past_key_values=cache, token_counts=torch.tensor([30, 20]).cuda())
+        assert cache.lengths.tolist() == [30, 20]
+        m(ids[:, :3], past_key_values=cache, token_counts=torch.tensor([2, 3]).cuda())
+        assert cache.lengths.tolist() == [32, 23]
+        cache.release([0, 1])
+    # Nothing has to be read: the first sequence's rows attend to nothing, the second's are as ever.
+    cache, other = (cdx.PagedKVCache(m.config, 2, 48, page_size=16) for _ in range(2))
+    got = m(ids[:, :9], past_key_values=cache, token_counts=torch.tensor([10, 5]).cuda()).logits
+    # (On the device too: 9 rows for a bound take another kernel, which rounds its weights to 8 bits, than 5 do.)
+    want = m(ids[:, :9], past_key_values=other, token_counts=torch.tensor([0, 5]).cuda()).logits
+    assert torch.equal(got[1, :5], want[1, :5]) and cache.lengths.tolist() == [0, 5] and cache.longest >= 5
+    m(ids, past_key_values=cache, token_counts=[40, 40])
+    assert cache.lengths.tolist() == [40, 45]

@@ -58,3 +58,38 @@ def test_a_call_after_replayed_cuts(monkeypatch, pages, cut):
         sim.holds([held[0] + 27, held[1] + 26], pages)
         sim.replay(graph)
         sim.holds(held, pages)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("pages", [None, 3])
+def test_counts_on_the_device_that_do_not_fit_their_rows(monkeypatch, pages, packed):
+    """Where a call reads them, they are held against its rows as the host's are; where it does not, the device leaves
+    such a sequence out and the host's bounds stay bounds."""
+    capacity = 48 if packed else 32
+    sim = Sim(monkeypatch, 2, capacity, page_size=16, pages=pages)
+    cache = sim.cache
+    rows = 33 if packed else 20
+    bad = [30, 4]  # past 20 rows each, and past 33 in all
+    for _ in range(2):
+        with pytest.raises(ValueError, match="token_counts"):
+            cache.begin(2, rows, token_counts=bad, packed=packed)
+        if pages is not None:  # (a pool of fewer pages than could be asked for: read)
+            with pytest.raises(ValueError, match="token_counts"):
+                cache.begin(2, rows, token_counts=Sim.device(bad), packed=packed)
+            sim.holds([0, 0], pages)
+        cache.begin(2, rows, token_counts=Sim.device([16, 17]), packed=packed)
+        sim.holds([16, 17], pages)
+        # A bound of the lengths past the capacity: read.
+        with pytest.raises(ValueError, match="token_counts"):
+            cache.begin(2, rows, token_counts=Sim.device([31, 3]), packed=packed)
+        sim.holds([16, 17], pages)
+        cache.begin(2, rows, token_counts=Sim.device([0, 15]), packed=packed)
+        sim.holds([16, 32], pages)
+        cache.reset()
+    if pages is None:
+        cache.begin(2, rows, token_counts=Sim.device(bad), packed=packed)
+        assert cache.rows.counts.tolist() == ([30, 0] if packed else [0, 4])
+        sim.holds(cache.rows.counts.tolist())
+        assert cache.longest >= max(cache.rows.counts.tolist())
+        cache.begin(2, 60, token_counts=[18, 40] if packed else [32, 28], packed=packed)
+        sim.holds([48, 40] if packed else [32, 32])

@@ -785,7 +785,7 @@ class PagedKVCache:
             self.longest, self._exact = max(self._lengths), True
         else:
             self._lengths, self._exact = None, False
-            self.longest += most
+            self.longest = min(self.longest + most, self.capacity)  # (tokens past it are refused)
         self.newest = self.longest  # (without a bound by weight a token's position is its slot)
         self._before = before
         return new

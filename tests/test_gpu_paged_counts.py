@@ -94,3 +94,21 @@ def test_counts_on_the_device_past_their_rows(cdx):
     assert torch.equal(got[1, :5], want[1, :5]) and cache.lengths.tolist() == [0, 5] and cache.longest >= 5
     m(ids, past_key_values=cache, token_counts=[40, 40])
     assert cache.lengths.tolist() == [40, 45]
+
+
+@torch.inference_mode()
+def test_graphs_of_more_rows_than_the_capacity(cdx):
+    """Each graph's rows count for the host's bound, which stays within the capacity: the rotary table need not grow,
+    which no capture can do."""
+    print("counts: graphs of many rows", flush=True)
+    m = _model(cdx, 64, 4, 2, layers=1, max_position_embeddings=128)
+    cache, eager, other = (cdx.PagedKVCache(m.config, 2, 128, page_size=16) for _ in range(3))
+    ids = torch.randint(0, 600, (2, 60), generator=torch.Generator().manual_seed(4)).cuda()
+    counts = torch.tensor([20, 11]).cuda()
+    graphs = [_graph(lambda: m(ids, past_key_values=cache, token_counts=counts).logits,
+                     lambda: m(ids, past_key_values=other, token_counts=counts)) for _ in range(4)]
+    for graph, logits in graphs:
+        graph.replay()
+        want = m(ids, past_key_values=eager, token_counts=counts).logits
+        assert torch.equal(logits[0, :20], want[0, :20]) and torch.equal(logits[1, :11], want[1, :11])
+        assert cache.lengths.tolist() == eager.lengths.tolist()

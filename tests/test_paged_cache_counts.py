@@ -93,3 +93,17 @@ def test_counts_on_the_device_that_do_not_fit_their_rows(monkeypatch, pages, pac
         assert cache.longest >= max(cache.rows.counts.tolist())
         cache.begin(2, 60, token_counts=[18, 40] if packed else [32, 28], packed=packed)
         sim.holds([48, 40] if packed else [32, 32])
+
+
+@pytest.mark.parametrize("pages,step", [(None, False), (5, False), (5, True)])
+def test_captured_calls_do_not_move_the_bounds_past_the_capacity(monkeypatch, pages, step):
+    """No sequence has more tokens than its capacity, however many graphs are made of a cache's calls."""
+    sim = Sim(monkeypatch, 2, 32, page_size=16, pages=pages)
+    cache = sim.cache
+    cache.begin(2, 20, token_counts=[20, 3])
+    for _ in range(20):
+        sim.capture(lambda c: c.begin(2, 1) if step else c.begin(2, 7, token_counts=Sim.device([7, 2])))
+        assert cache.longest <= 32 and cache.newest <= 32
+    assert cache.lengths.tolist() == [20, 3]
+    cache.begin(2, 12, token_counts=[12, 9])
+    sim.holds([32, 12], pages)

@@ -715,7 +715,7 @@ class PagedKVCache:
             self._step = rows.counts * rows.lengths if self._replays else None
             self.prompt = False
             return
-        if self.longest >= self.capacity and not self._exact and not capturing:
+        if self.longest >= self.capacity and (not self._exact or self._replays) and not capturing:
             self._read_longest(self.lengths)
         if self.longest >= self.capacity:
             if self.keep is None:

@@ -107,3 +107,20 @@ def test_captured_calls_do_not_move_the_bounds_past_the_capacity(monkeypatch, pa
     assert cache.lengths.tolist() == [20, 3]
     cache.begin(2, 12, token_counts=[12, 9])
     sim.holds([32, 12], pages)
+
+
+@pytest.mark.parametrize("keep", [None, 16])
+def test_a_step_after_replays_that_emptied_a_full_cache(monkeypatch, keep):
+    """A step is refused as full, or cuts the cache, by the lengths that the device has."""
+    sim = Sim(monkeypatch, 2, 32, page_size=16, keep=keep)
+    cache = sim.cache
+    prompts = sim.capture(lambda c: c.begin(2, 20))
+    for _ in range(2):
+        sim.replay(prompts)
+        for n in range(21, 33):
+            cache.begin(2, 1)
+            sim.holds([n, n])
+        if keep is None:
+            with pytest.raises(ValueError, match="full"):
+                cache.begin(2, 1)
+            sim.holds([32, 32])

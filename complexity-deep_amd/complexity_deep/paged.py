@@ -689,6 +689,8 @@ class PagedKVCache:
             n = None if prompt_lengths is None else prompt_lengths.clamp(0, tokens)
             known = [tokens] * batch_size if n is None else (None if n.is_cuda else n.tolist())
             if self.pages is not None:
+                if capturing:  # (replayed prompts begin the batch anew, as they do on pages of the cache's own)
+                    self._give_back(torch.zeros_like(self.lengths))
                 n = torch.full_like(self.lengths, tokens) if n is None else n.to(self.lengths)
                 self._reserve(n, known, tokens, batch_size * tokens, tokens)
             elif n is None:
@@ -790,6 +792,12 @@ class PagedKVCache:
         self._before = before
         return new
 
+    def _give_back(self, to: torch.Tensor) -> None:
+        """Cut the sequences of a pool to ``to`` tokens (on the device)."""
+        new = paged_truncate(to, self.lengths, self.positions, self.block_table, self.page_size, self.free_pages,
+                             self.free_count)
+        self._state.copy_(torch.as_strided(new[0], (self._state.numel(),), (1,)))
+
     def truncate(self, to) -> None:
         """Cut every sequence of more than ``to`` [B] tokens (integers, on the device or the host) to its first so
         many: speculated tokens that were not accepted, 0 for a sequence that has ended.  The pages
@@ -799,9 +807,7 @@ class PagedKVCache:
         to, known = self._integers(to, "to")
         self._captured()
         if self.pages is not None:
-            new = paged_truncate(to, self.lengths, self.positions, self.block_table, self.page_size, self.free_pages,
-                                 self.free_count)
-            self._state.copy_(torch.as_strided(new[0], (self._state.numel(),), (1,)))
+            self._give_back(to)
         else:
             gone = (self.lengths - to.clamp(min=0)).clamp(min=0)
             self._counts.sub_(gone)

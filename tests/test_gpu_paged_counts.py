@@ -112,3 +112,28 @@ def test_graphs_of_more_rows_than_the_capacity(cdx):
         want = m(ids, past_key_values=eager, token_counts=counts).logits
         assert torch.equal(logits[0, :20], want[0, :20]) and torch.equal(logits[1, :11], want[1, :11])
         assert cache.lengths.tolist() == eager.lengths.tolist()
+
+
+@pytest.mark.parametrize("pages", [None, 4])
+@torch.inference_mode()
+def test_replayed_prompts_begin_the_batch_anew(cdx, pages):
+    print(f"counts: prompts replayed over others, pages={pages}", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    cache, eager, other = (cdx.PagedKVCache(m.config, 2, 32, page_size=16, pages=pages) for _ in range(3))
+    gen = torch.Generator().manual_seed(4)
+    ids, n = torch.empty(2, 20, dtype=torch.int64, device="cuda"), torch.empty(2, dtype=torch.int64, device="cuda")
+    ids.zero_(), n.fill_(20)
+    prompts, logits = _graph(lambda: m(ids, past_key_values=cache, prompt_lengths=n).logits,
+                             lambda: m(ids, past_key_values=other, prompt_lengths=n))
+    for held in ([20, 7], [16, 20], [3, 17], [20, 20]):
+        ids.copy_(torch.randint(0, 600, (2, 20), generator=gen)), n.copy_(torch.tensor(held))
+        prompts.replay()
+        eager.reset()
+        want = m(ids, past_key_values=eager, prompt_lengths=n).logits
+        for b, c in enumerate(held):
+            assert torch.equal(logits[b, :c], want[b, :c])
+        for _ in range(2):
+            got, want = (m(ids[:, :1], past_key_values=c).logits for c in (cache, eager))
+            assert torch.equal(got, want)
+        assert cache.lengths.tolist() == eager.lengths.tolist() == [c + 2 for c in held]
+        assert pages is None or int(cache.free_count) == int(eager.free_count)

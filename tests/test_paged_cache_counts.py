@@ -124,3 +124,18 @@ def test_a_step_after_replays_that_emptied_a_full_cache(monkeypatch, keep):
             with pytest.raises(ValueError, match="full"):
                 cache.begin(2, 1)
             sim.holds([32, 32])
+
+
+@pytest.mark.parametrize("pages", [None, 4])
+@pytest.mark.parametrize("lengths", [None, [20, 7]])
+def test_replayed_prompts_begin_the_batch_anew(monkeypatch, pages, lengths):
+    """Captured prompts are prompts at every replay, also where sequences still hold the tokens of the last."""
+    given = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    sim = Sim(monkeypatch, 2, 32, page_size=16, pages=pages)
+    prompts = sim.capture(lambda c: c.begin(2, 20, given))
+    held = lengths or [20, 20]
+    for _ in range(3):
+        sim.replay(prompts)
+        sim.holds(held, pages)
+        sim.cache.begin(2, 1)
+        sim.holds([n + 1 for n in held], pages)

@@ -39,7 +39,7 @@ from ._grad import forward_only
 from .layer import TransformerBlock
 from .linear import embedding, linear
 from .normalization import RMSNorm, rms_norm
-from .paged import PagedKVCache
+from .paged import PagedKVCache, _to_device
 from .sampling import sample_tokens
 from .token_routed_mlp import RoutePlan, TokenRoutedMLP, route_plans
 
@@ -394,12 +394,13 @@ class ComplexityModel(nn.Module):
         """The logits [B, V] behind each prompt's last token, its tokens taken ``chunk`` at a time."""
         B, S = input_ids.shape
         n = prompt_lengths.clamp(0, S) if prompt_lengths is not None else torch.full((B,), S, dtype=torch.int64)
+        last_row = _to_device(n - 1, input_ids.device)
         last = None
         for at in range(0, S, chunk):
             piece = input_ids[:, at:at + chunk]
             counts = (n - at).clamp(0, piece.shape[1])
             logits = self.forward(piece, past_key_values=cache, token_counts=counts).logits
-            end = (n - 1 - at).to(input_ids.device)
+            end = last_row - at
             mine = logits[torch.arange(B, device=input_ids.device), end.clamp(0, piece.shape[1] - 1)]
             here = ((end >= 0) & (end < piece.shape[1])).unsqueeze(1)
             last = torch.where(here, mine, last if last is not None else torch.zeros_like(mine))

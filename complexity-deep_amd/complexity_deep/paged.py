@@ -490,6 +490,12 @@ def _capturing(t: torch.Tensor) -> bool:
     return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
+def _to_device(t: torch.Tensor, device) -> torch.Tensor:
+    """t on the device, without a wait: the host's is copied from pinned memory, which the allocator keeps
+    until the copy is done."""
+    return t if t.is_cuda or torch.device(device).type != "cuda" else t.pin_memory().to(device, non_blocking=True)
+
+
 class PagedLayer(NamedTuple):
     """One layer of a PagedKVCache, as ComplexityAttention takes it for past_key_value."""
     cache: "PagedKVCache"
@@ -687,7 +693,10 @@ class PagedKVCache:
                 raise ValueError(f"PagedKVCache: prompt_lengths must be {batch_size} integers, got "
                                  f"{prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
             n = None if prompt_lengths is None else prompt_lengths.clamp(0, tokens)
-            known = [tokens] * batch_size if n is None else (None if n.is_cuda else n.tolist())
+            known = [tokens] * batch_size
+            if n is not None:
+                known = self._known(n, "prompt_lengths")
+                n = _to_device(n.to(torch.int32), self.lengths.device)
             if self.pages is not None:
                 if capturing:  # (replayed prompts begin the batch anew, as they do on pages of the cache's own)
                     self._give_back(torch.zeros_like(self.lengths))
@@ -739,6 +748,15 @@ class PagedKVCache:
             self._lengths = [n + 1 for n in self._lengths]
         self.prompt = False
 
+    def _known(self, values: torch.Tensor, name: str):
+        """The values as a list if they are the host's.  A graph would copy those from where they were at its
+        capture."""
+        if values.is_cuda:
+            return None
+        if _capturing(self._counts):
+            raise ValueError(f"PagedKVCache: {name} of a captured call must be on {self.lengths.device}")
+        return values.tolist()
+
     def _integers(self, values, name: str):
         """(int32 [B] on the device, the same as a list if the host has them) of a tensor or a sequence."""
         if not isinstance(values, torch.Tensor):
@@ -747,8 +765,9 @@ class PagedKVCache:
                 or values.dtype == torch.bool:
             raise ValueError(f"PagedKVCache: {name} must be {self.batch_size} integers, got {values.dtype} "
                              f"{tuple(values.shape)}")
-        known = None if values.is_cuda else values.tolist()
-        return values.long().clamp(-2 ** 31, 2 ** 31 - 1).to(self.lengths.device, torch.int32), known
+        known = self._known(values, name)
+        values = _to_device(values.long().clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32), self.lengths.device)
+        return values.to(self.lengths.device), known
 
     @staticmethod
     def _check_rows(known, rows: int, packed: bool) -> None:

@@ -35,6 +35,11 @@ def truncate(to, lengths, positions, block_table, page_size, free_pages, free_co
     return _side_by_side(n, pos, [len(free)])
 
 
+class _Device(torch.Tensor):
+    """Taken for a tensor on the GPU, with what is computed from it."""
+    is_cuda = property(lambda self: True)
+
+
 class Sim:
     """``cache`` (a PagedKVCache on the CPU) with ``capture`` and ``replay`` of its calls."""
 
@@ -45,21 +50,12 @@ class Sim:
         monkeypatch.setattr(paged, "paged_reserve", reserve)
         monkeypatch.setattr(paged, "paged_truncate", truncate)
         monkeypatch.setattr(paged, "_capturing", lambda t: self.capturing)
-        integers = cdx.PagedKVCache._integers
-
-        def unread(cache, values, name):
-            t, known = integers(cache, values, name)
-            return t, None if getattr(values, "on_device", False) else known
-
-        monkeypatch.setattr(cdx.PagedKVCache, "_integers", unread)
         self.cache = cdx.PagedKVCache(cdx.ComplexityConfig.complexity_tiny(), batch_size, max_length, device="cpu", **kw)
 
     @staticmethod
     def device(values):
         """Integers that the host does not know."""
-        t = torch.tensor(values)
-        t.on_device = True
-        return t
+        return torch.tensor(values).as_subclass(_Device)
 
     def _tensors(self):
         c = self.cache

@@ -137,3 +137,68 @@ def test_replayed_prompts_begin_the_batch_anew(cdx, pages):
             assert torch.equal(got, want)
         assert cache.lengths.tolist() == eager.lengths.tolist() == [c + 2 for c in held]
         assert pages is None or int(cache.free_count) == int(eager.free_count)
+
+
+def _no_waits(call):
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        return call()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+
+
+@pytest.mark.parametrize("pages", [None, 20])
+@torch.inference_mode()
+def test_counts_of_the_host_do_not_wait(cdx, pages):
+    print(f"counts: no wait for the host's, pages={pages}", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    ids = torch.randint(0, 600, (3, 40), generator=torch.Generator().manual_seed(4)).cuda()
+    cache, other = (cdx.PagedKVCache(m.config, 3, 96, page_size=16, pages=pages) for _ in range(2))
+    lens = torch.tensor([9, 4, 30])
+    got, held = [], [torch.zeros(2 ** 26, device="cuda") for _ in range(2)]
+    for c in (other, cache):
+        def calls():
+            for t in held:  # (work that is still queued when the counts are given)
+                t.add_(1.0)
+            c.reset()
+            out = [m(ids[:, :30], past_key_values=c, prompt_lengths=lens).logits[2]]
+            out.append(m(ids[:, :9], past_key_values=c, token_counts=[9, 1, 5]).logits[0])
+            out.append(m(ids[0, :9], past_key_values=c, token_counts=torch.tensor([2, 0, 7])).logits)
+            c.truncate([15, 5, 40])
+            c.release([1])
+            out.append(m(ids[:, :1], past_key_values=c).logits)
+            c.reset()
+            out.append(m._prompts_in_pieces(ids, None, c, 16))
+            c.reset()
+            out.append(m._prompts_in_pieces(ids, lens, c, 16))
+            return out
+        got.append(calls() if c is other else _no_waits(calls))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert cache.lengths.tolist() == [9, 4, 30]
+
+
+@torch.inference_mode()
+def test_counts_of_the_host_in_a_captured_call(cdx):
+    """A graph would copy them at every replay from where they were: they are refused, and the capture goes on."""
+    print("counts: the host's in a captured call", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    cache, eager, other = (cdx.PagedKVCache(m.config, 2, 64, page_size=16, pages=8) for _ in range(3))
+    ids = torch.randint(0, 600, (2, 3), generator=torch.Generator().manual_seed(4)).cuda()
+    counts = torch.tensor([3, 2]).cuda()
+
+    def captured():
+        for call in (lambda: m(ids, past_key_values=cache, token_counts=[3, 2]), lambda: cache.truncate([1, 1]),
+                     lambda: cache.release([0]),
+                     lambda: m(ids, past_key_values=cache, prompt_lengths=counts.new_zeros(2, device="cpu"))):
+            with pytest.raises(ValueError, match="captured"):
+                call()
+        return m(ids, past_key_values=cache, token_counts=counts).logits
+
+    graph, logits = _graph(captured, lambda: m(ids, past_key_values=other, token_counts=counts))
+    for i in range(3):
+        graph.replay()
+        want = m(ids, past_key_values=eager, token_counts=counts).logits
+        assert torch.equal(logits[0], want[0]) and torch.equal(logits[1, :2], want[1, :2])
+        assert torch.equal(cache._state, eager._state) and cache.lengths.tolist() == [3 * i + 3, 2 * i + 2]

@@ -12,7 +12,7 @@ from _paged_sim import Sim
 @pytest.mark.parametrize("lengths", [None, [20, 7]])
 def test_a_call_after_replayed_prompts(monkeypatch, lengths):
     """Prompts on pages of the cache's own, captured and replayed on an emptied cache."""
-    given = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    given = None if lengths is None else Sim.device(lengths)
     sim = Sim(monkeypatch, 2, 32, page_size=16)
     cache = sim.cache
     prompts = sim.capture(lambda c: c.begin(2, 20, given))
@@ -130,7 +130,7 @@ def test_a_step_after_replays_that_emptied_a_full_cache(monkeypatch, keep):
 @pytest.mark.parametrize("lengths", [None, [20, 7]])
 def test_replayed_prompts_begin_the_batch_anew(monkeypatch, pages, lengths):
     """Captured prompts are prompts at every replay, also where sequences still hold the tokens of the last."""
-    given = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    given = None if lengths is None else Sim.device(lengths)
     sim = Sim(monkeypatch, 2, 32, page_size=16, pages=pages)
     prompts = sim.capture(lambda c: c.begin(2, 20, given))
     held = lengths or [20, 20]
@@ -139,3 +139,14 @@ def test_replayed_prompts_begin_the_batch_anew(monkeypatch, pages, lengths):
         sim.holds(held, pages)
         sim.cache.begin(2, 1)
         sim.holds([n + 1 for n in held], pages)
+
+
+def test_captured_calls_take_no_counts_of_the_host(monkeypatch):
+    sim = Sim(monkeypatch, 2, 32, page_size=16, pages=4)
+    cache = sim.cache
+    for call in (lambda c: c.begin(2, 3, torch.tensor([3, 2])), lambda c: c.begin(2, 3, token_counts=[3, 2]),
+                 lambda c: c.truncate([1, 1]), lambda c: c.release([0])):
+        with pytest.raises(ValueError, match="captured"):
+            sim.capture(call)
+        assert cache.longest == cache.newest == 0
+    sim.holds([0, 0], 4)

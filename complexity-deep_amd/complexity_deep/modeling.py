@@ -393,7 +393,7 @@ class ComplexityModel(nn.Module):
                            chunk: int) -> torch.Tensor:
         """The logits [B, V] behind each prompt's last token, its tokens taken ``chunk`` at a time."""
         B, S = input_ids.shape
-        n = prompt_lengths.clamp(0, S) if prompt_lengths is not None else torch.full((B,), S, dtype=torch.int64)
+        n = torch.full((B,), S) if prompt_lengths is None else cache.prompt_counts(prompt_lengths, S)
         last_row = _to_device(n - 1, input_ids.device)
         last = None
         for at in range(0, S, chunk):

@@ -688,13 +688,9 @@ class PagedKVCache:
         if self.newest == 0:
             if not 0 < tokens <= self.capacity:
                 raise ValueError(f"PagedKVCache: prompts of {tokens} tokens in a cache of {self.capacity}")
-            if prompt_lengths is not None and (prompt_lengths.shape != (batch_size,)
-                                               or prompt_lengths.is_floating_point()):
-                raise ValueError(f"PagedKVCache: prompt_lengths must be {batch_size} integers, got "
-                                 f"{prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
-            n = None if prompt_lengths is None else prompt_lengths.clamp(0, tokens)
-            known = [tokens] * batch_size
-            if n is not None:
+            n, known = None, [tokens] * batch_size
+            if prompt_lengths is not None:
+                n = self.prompt_counts(prompt_lengths, tokens)
                 known = self._known(n, "prompt_lengths")
                 n = _to_device(n.to(torch.int32), self.lengths.device)
             if self.pages is not None:
@@ -713,8 +709,8 @@ class PagedKVCache:
                 self.slot_positions.copy_(torch.where(at < self.lengths.view(-1, 1, 1), at, -1))
             self.longest = self.newest = tokens
             self._exact = prompt_lengths is None
-            if prompt_lengths is not None and not prompt_lengths.is_cuda:
-                self._read_longest(prompt_lengths.clamp(0, tokens))
+            if prompt_lengths is not None and known is not None:
+                self.longest, self._exact = max(known), True
             self.prompt = True
             return
         if tokens != 1 or prompt_lengths is not None:
@@ -747,6 +743,14 @@ class PagedKVCache:
         if self._lengths is not None:
             self._lengths = [n + 1 for n in self._lengths]
         self.prompt = False
+
+    def prompt_counts(self, prompt_lengths: torch.Tensor, tokens: int) -> torch.Tensor:
+        """``prompt_lengths`` [B] of prompts in ``tokens`` rows each, as int64 of 0 .. tokens."""
+        if prompt_lengths.shape != (self.batch_size,) or prompt_lengths.is_floating_point() \
+                or prompt_lengths.is_complex() or prompt_lengths.dtype == torch.bool:
+            raise ValueError(f"PagedKVCache: prompt_lengths must be {self.batch_size} integers, got "
+                             f"{prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
+        return prompt_lengths.long().clamp(0, tokens)
 
     def _known(self, values: torch.Tensor, name: str):
         """The values as a list if they are the host's.  A graph would copy those from where they were at its

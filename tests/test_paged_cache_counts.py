@@ -150,3 +150,34 @@ def test_captured_calls_take_no_counts_of_the_host(monkeypatch):
             sim.capture(call)
         assert cache.longest == cache.newest == 0
     sim.holds([0, 0], 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_prompt_lengths_of_any_integers(monkeypatch, dtype):
+    """Lengths in types that hold them, but not the prompts' rows nor what is left of them."""
+    import complexity_deep as cdx
+    S, lens = 300, torch.tensor([3, 120, 64, 1], dtype=dtype)
+    sim = Sim(monkeypatch, 4, 320, page_size=16)
+    sim.cache.begin(4, S, lens)
+    sim.holds([3, 120, 64, 1])
+    assert sim.cache.longest == 120
+    sim.cache.reset()
+    taken = []
+
+    class Model:
+        def forward(self, ids, past_key_values, token_counts):
+            past_key_values.begin(*ids.shape, token_counts=token_counts)
+            taken.append(token_counts.tolist())
+            return cdx.CausalLMOutput(loss=None, logits=ids.unsqueeze(-1).float())
+
+    ids = torch.arange(4 * S).view(4, S)
+    last = cdx.ComplexityModel._prompts_in_pieces(Model(), ids, lens, sim.cache, 50)
+    assert [sum(c) for c in zip(*taken)] == [3, 120, 64, 1] and taken[1] == [0, 50, 14, 0]
+    assert last[:, 0].tolist() == [2, S + 119, 2 * S + 63, 3 * S]
+    sim.holds([3, 120, 64, 1])
+    for bad in (lens.float(), lens[:3], lens > 3):
+        with pytest.raises(ValueError, match="prompt_lengths"):
+            cdx.ComplexityModel._prompts_in_pieces(Model(), ids, bad, sim.cache, 50)
+        sim.cache.reset()
+        with pytest.raises(ValueError, match="prompt_lengths"):
+            sim.cache.begin(4, S, bad)

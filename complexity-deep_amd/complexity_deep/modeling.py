@@ -350,12 +350,15 @@ class ComplexityModel(nn.Module):
         produced ``eos_token_id`` (the configuration's by default) repeats it; the generation ends when
         all have.  ``cache`` (emptied first) may bound the memory (PagedKVCache's keep, or its pages); by
         default it has room for every token.  ``chunk`` takes the prompts in pieces of so many tokens each, which
-        bounds the activations and logits of long ones."""
+        bounds the activations and logits of long ones (with a cache that has no keep: that takes its prompts at
+        once)."""
         B, S = input_ids.shape
         if chunk is not None and chunk <= 0:
             raise ValueError(f"generate_paged: chunk={chunk} must be positive")
         if chunk is not None and S == 0:
             raise ValueError("generate_paged: empty prompts")
+        if chunk is not None and cache is not None and cache.keep is not None:
+            raise ValueError("generate_paged: a cache with keep takes its prompts at once, not in pieces (chunk)")
         eos = self.config.eos_token_id if eos_token_id is None else eos_token_id
         dev = input_ids.device
         if uniforms is None:

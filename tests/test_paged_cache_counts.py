@@ -181,3 +181,14 @@ def test_prompt_lengths_of_any_integers(monkeypatch, dtype):
         sim.cache.reset()
         with pytest.raises(ValueError, match="prompt_lengths"):
             sim.cache.begin(4, S, bad)
+
+
+def test_prompts_in_pieces_need_an_unbounded_cache():
+    """Refused before the cache is emptied."""
+    import complexity_deep as cdx
+    cfg = cdx.ComplexityConfig.complexity_tiny()
+    cache = cdx.PagedKVCache(cfg, 2, 40, keep=10, device="cpu")
+    cache.begin(2, 12)
+    with pytest.raises(ValueError, match="keep"):
+        cdx.ComplexityModel.generate_paged(None, torch.zeros(2, 12, dtype=torch.int64), 3, cache=cache, chunk=4)
+    assert cache.lengths.tolist() == [12, 12]

@@ -58,6 +58,22 @@ __device__ __forceinline__ int last_at_most(const T* values, int n, T x) {
   return lo;
 }
 
+// Arrays of a call on the host's side.
+struct Extent {
+  const void* at;
+  int64_t bytes;
+};
+// Whether any result lies over an array that blocks still read while another one writes results.
+template <size_t NIn, size_t NOut>
+bool overlap(const Extent (&in)[NIn], const Extent (&out)[NOut]) {
+  for (const Extent& o : out)
+    for (const Extent& i : in) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(o.at), b = reinterpret_cast<uintptr_t>(i.at);
+      if (o.at && i.at && a < b + (uintptr_t)i.bytes && b < a + (uintptr_t)o.bytes) return true;
+    }
+  return false;
+}
+
 struct ReserveParams {
   const int32_t* counts;     // [B]
   const int32_t* lengths;    // [B]
@@ -327,9 +343,10 @@ extern "C" int cdx_paged_reserve(const int32_t* counts, const int32_t* lengths, 
       (width > 0 && !table) || (rows > 0 && (!row_slots || !row_positions)) || pool != (new_free_count != nullptr) ||
       (free_pages && !pool) || (pool && free_capacity > 0 && !free_pages))
     return fail(CDX_EINVAL, "%s: null pointer", name);
-  if (new_counts == counts || new_lengths == lengths || new_positions == positions ||
-      (pool && new_free_count == free_count))
-    return fail(CDX_EINVAL, "%s: the new counts, lengths and positions need memory of their own", name);
+  const Extent in[] = {{counts, 4 * B}, {lengths, 4 * B}, {positions, 4 * B}, {free_count, 4}};
+  const Extent out[] = {{starts, 4 * B}, {new_counts, 4 * B}, {new_lengths, 4 * B}, {new_positions, 4 * B},
+                        {new_free_count, 4}, {row_slots, 8 * rows}, {row_positions, 4 * rows}};
+  if (overlap(in, out)) return fail(CDX_EINVAL, "%s: the results need memory of their own", name);
   ReserveParams p{};
   p.counts = counts;
   p.lengths = lengths;
@@ -373,8 +390,9 @@ extern "C" int cdx_paged_truncate(const int32_t* to, const int32_t* lengths, con
   if (!to || !lengths || !positions || !free_count || !new_lengths || !new_positions || !new_free_count ||
       (width > 0 && !table) || (free_capacity > 0 && !free_pages))
     return fail(CDX_EINVAL, "%s: null pointer", name);
-  if (new_lengths == lengths || new_lengths == to || new_positions == positions || new_free_count == free_count)
-    return fail(CDX_EINVAL, "%s: the new lengths and positions need memory of their own", name);
+  const Extent in[] = {{to, 4 * B}, {lengths, 4 * B}, {positions, 4 * B}, {free_count, 4}};
+  const Extent out[] = {{new_lengths, 4 * B}, {new_positions, 4 * B}, {new_free_count, 4}};
+  if (overlap(in, out)) return fail(CDX_EINVAL, "%s: the results need memory of their own", name);
   TruncateParams p{};
   p.to = to;
   p.lengths = lengths;

@@ -642,6 +642,7 @@ int cdx_paged_evict(int64_t layers, int64_t B, int32_t nkv, int32_t hd, const in
  * first sequence's first page last: what reserve took it finds again.  Table entries past the new length
  * stay as they are and name pages that may be another's.  Pages that come back must be the
  * sequence's own; past free_capacity, the list's room, they are dropped.
+ * The results of both need memory of their own, apart from all that a call reads (CDX_EINVAL).
  *
  * No counterpart in the reference, which has one cache tensor per batch.
  */

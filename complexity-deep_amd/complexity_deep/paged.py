@@ -668,7 +668,7 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: a block table {tuple(self.block_table.shape)} of pages of {self.page_size} "
                              f"has no room for {self.capacity} tokens")
         self.rows = self._before = None
-        capturing = self._captured()
+        replays, capturing = self._replays, self._captured()
         if token_counts is not None:
             if self.keep is not None or prompt_lengths is not None or tokens <= 0:
                 raise ValueError("PagedKVCache: token_counts in a bounded cache, beside prompt_lengths, or without rows")
@@ -686,6 +686,9 @@ class PagedKVCache:
             self._read_longest(self.lengths)
             self.newest = int(self.positions.max()) + 1
         if self.newest == 0:
+            if capturing and replays and tokens == 1:
+                raise ValueError("PagedKVCache: whether a captured call of one token each is a prompt or a step cannot be "
+                                 "known, as replays may have brought tokens: give token_counts, or make a call first")
             if not 0 < tokens <= self.capacity:
                 raise ValueError(f"PagedKVCache: prompts of {tokens} tokens in a cache of {self.capacity}")
             n, known = None, [tokens] * batch_size

@@ -7,7 +7,8 @@ import torch
 
 import _paged_chunk as chunk
 
-HOST = ("longest", "newest", "_exact", "_lengths", "prompt", "_step", "rows", "most", "_before", "_saved")
+HOST = ("longest", "newest", "_exact", "_lengths", "prompt", "_step", "rows", "most", "_before", "_saved",
+        "_replays")
 
 
 def _side_by_side(*lists):
@@ -79,7 +80,7 @@ class Sim:
     def replay(self, graph):
         """The graph's work on tensors, with the host's side as it was (the branches are the captured ones)."""
         call, host = graph
-        now = self._host(), self.cache._replays
+        now = self._host()
         for name, value in host.items():
             setattr(self.cache, name, value)
         self.capturing = True
@@ -87,9 +88,8 @@ class Sim:
             call(self.cache)
         finally:
             self.capturing = False
-            for name, value in now[0].items():
+            for name, value in now.items():
                 setattr(self.cache, name, value)
-            self.cache._replays = now[1]
 
     def holds(self, lengths, pages=None):
         """The device's lengths, and what a pool of so many pages must have left and in use then."""

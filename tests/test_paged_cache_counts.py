@@ -192,3 +192,28 @@ def test_prompts_in_pieces_need_an_unbounded_cache():
     with pytest.raises(ValueError, match="keep"):
         cdx.ComplexityModel.generate_paged(None, torch.zeros(2, 12, dtype=torch.int64), 3, cache=cache, chunk=4)
     assert cache.lengths.tolist() == [12, 12]
+
+
+@pytest.mark.parametrize("pages", [None, 6])
+def test_a_captured_call_of_one_token_each_on_a_cache_that_replays_may_have_filled(monkeypatch, pages):
+    """A step or a prompt of one token: the host cannot know which, and must not guess."""
+    sim = Sim(monkeypatch, 2, 32, page_size=16, pages=pages)
+    cache = sim.cache
+    first = sim.capture(lambda c: c.begin(2, 1))  # nothing was captured before: a prompt
+    assert cache.prompt
+    cache.reset()
+    prompts = sim.capture(lambda c: c.begin(2, 20))
+    cache.reset()
+    sim.replay(prompts)
+    with pytest.raises(ValueError, match="token_counts"):
+        sim.capture(lambda c: c.begin(2, 1))
+    sim.holds([20, 20], pages)
+    counted = sim.capture(lambda c: c.begin(2, 1, token_counts=Sim.device([1, 1])))
+    sim.replay(counted)
+    sim.holds([21, 21], pages)
+    cache.begin(2, 1)  # (an eager call reads the lengths: after it a captured one is a step)
+    step = sim.capture(lambda c: c.begin(2, 1))
+    sim.replay(step)
+    sim.holds([23, 23], pages)
+    sim.replay(first)
+    sim.holds([1, 1], pages)

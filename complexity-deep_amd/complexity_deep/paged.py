@@ -682,7 +682,9 @@ class PagedKVCache:
                                       None if packed else tokens)
             self.most, self.prompt = most, False
             return
-        if self.newest == 0 and self._replays and not capturing:  # (replays may have brought tokens since)
+        more = tokens != 1 or prompt_lengths is not None
+        # (Replays may have brought tokens to an empty cache; prompts are taken if the device has emptied it.)
+        if not capturing and (self._replays if self.newest == 0 else more and (self._replays or not self._exact)):
             self._read_longest(self.lengths)
             self.newest = int(self.positions.max()) + 1
         if self.newest == 0:
@@ -716,7 +718,7 @@ class PagedKVCache:
                 self.longest, self._exact = max(known), True
             self.prompt = True
             return
-        if tokens != 1 or prompt_lengths is not None:
+        if more:
             raise ValueError("PagedKVCache: after the prompts a call without token_counts takes one token per sequence "
                              "(reset() empties the cache)")
         if self.pages is not None:

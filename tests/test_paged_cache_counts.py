@@ -217,3 +217,24 @@ def test_a_captured_call_of_one_token_each_on_a_cache_that_replays_may_have_fill
     sim.holds([23, 23], pages)
     sim.replay(first)
     sim.holds([1, 1], pages)
+
+
+@pytest.mark.parametrize("pages", [None, 4])
+@pytest.mark.parametrize("replayed", [False, True])
+def test_prompts_of_a_cache_that_the_device_has_emptied(monkeypatch, pages, replayed):
+    """By a cut whose lengths the host does not know."""
+    sim = Sim(monkeypatch, 2, 32, page_size=16, pages=pages)
+    cache = sim.cache
+    cache.begin(2, 20)
+    cut = sim.capture(lambda c: c.truncate(Sim.device([0, 0]))) if replayed else None
+    for prompts in ((20, None), (1, torch.tensor([1, 1])), (9, torch.tensor([2, 9])), (32, None)):
+        with pytest.raises(ValueError, match="after the prompts"):
+            cache.begin(2, *prompts)
+        if replayed:
+            sim.replay(cut)
+        else:
+            cache.truncate(Sim.device([0, 0]))
+        sim.holds([0, 0], pages)
+        cache.begin(2, *prompts)
+        assert cache.prompt
+        sim.holds([prompts[0]] * 2 if prompts[1] is None else prompts[1].tolist(), pages)

@@ -525,11 +525,17 @@ class PagedKVCache:
     are the host's bounds, and nothing waits for the device but the first call of a batch whose
     bound, of right-padded prompts with prompt_lengths on the device, has reached the capacity: it reads
     how long the longest is; with token_counts on the device, or a pool, such a call reads all lengths, and
-    the counts, which must fit their rows.  Where it need not read them the device alone leaves out a sequence whose
-    tokens do not fit: it brings none, and its rows attend to nothing.  One call at a time may use a cache.  A call that is captured into a graph counts on the device when it is
-    replayed, not here: keep to max_length then (a token past the capacity is not stored).  Calls with
-    token_counts, or of a pool, read the lengths first once a call of the cache was captured.  A
-    TransformerBlock or ComplexityAttention called by itself takes ``cache[i]``, after ``begin`` has
+    the counts, which must fit their rows.  (For the bound, counts on the device are all rows of a sequence,
+    or of the whole call if packed.)  Where it need not read them the device alone leaves out a sequence whose
+    tokens do not fit: it brings none, and its rows attend to nothing.  One call at a time may use a cache.
+
+    A call that is captured into a graph, with its counts on the device, counts on the device when it is
+    replayed, not here: keep to max_length then (a token past the capacity is not stored).  Captured prompts
+    begin the batch anew at every replay.  Once a call of the cache was captured, calls with token_counts, or of a
+    pool, prompts, and steps that would be refused as full read the lengths first.  A captured call of one token
+    each that could be a prompt or a step, replays having filled the cache or not, is refused.
+
+    A TransformerBlock or ComplexityAttention called by itself takes ``cache[i]``, after ``begin`` has
     counted the call's tokens."""
 
     def __init__(self, config, batch_size: int, max_length: int, *, page_size: int = 64, keep: Optional[int] = None,
@@ -689,8 +695,9 @@ class PagedKVCache:
             self.newest = int(self.positions.max()) + 1
         if self.newest == 0:
             if capturing and replays and tokens == 1:
-                raise ValueError("PagedKVCache: whether a captured call of one token each is a prompt or a step cannot be "
-                                 "known, as replays may have brought tokens: give token_counts, or make a call first")
+                raise ValueError("PagedKVCache: whether a captured call of one token each is a prompt or a step cannot "
+                                 "be known, as replays may have brought tokens: give token_counts, or make a call "
+                                 "first")
             if not 0 < tokens <= self.capacity:
                 raise ValueError(f"PagedKVCache: prompts of {tokens} tokens in a cache of {self.capacity}")
             n, known = None, [tokens] * batch_size

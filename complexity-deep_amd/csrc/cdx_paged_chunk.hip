@@ -18,10 +18,11 @@
 //     latency: paged_attn_kernel's walk of the pages, the slots over eight waves and over splits, with the
 //     columns of the matrix instruction taken by queries of several rows.
 //
-// Measured (us a call, issued back to back, and what of it bounds the call), 16/8 heads of 128 unless said: 2048 new tokens
-// over 65536 slots 990 (1090 TFLOP/s), 8 x 1024 over 2048 113 (915), 8 prompts of 2048 156 (885); 4 chunks of 512
-// among 60 single tokens, up to 2048 slots, 50 (227 MB: 4.5 TB/s); 16 of 1 .. 777 over up to 4099, 16/4 of 80, 82
-// (590); 64 single tokens over 2049 94 (537 MB: 5.7 TB/s); 8 over 32768 31; 5 over 505, 8/4 of 40, 5.8.
+// Measured (us a call, issued back to back, and what of it bounds the call), 16/8 heads of 128 unless said:
+// 2048 new tokens over 65536 slots 990 (1090 TFLOP/s), 8 x 1024 over 2048 113 to 117 (915), 8 prompts of 2048 158
+// (871); 4 chunks of 512 among 60 single tokens, up to 2048 slots, 50 to 57 (227 MB: 4.0 to 4.5 TB/s); 16 of
+// 1 .. 777 over up to 4099, 16/4 of 80, 82 to 85 (590); 4 x 512 over 4096, 12/4 of 64, 50 (481); 64 single tokens
+// over 2049 94 (537 MB: 5.7 TB/s); 8 over 32768 31; 5 over 505, 8/4 of 40, 5.8.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -660,7 +661,9 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_tile_kernel(const ChunkPar
       }
     };
     // P of two neighbouring keys of slab sl, rounded to bf16 (the sum l is of the rounded ones, so that the
-    // weights that V is multiplied by add up to 1), and its place among the slab's operand.
+    // weights that V is multiplied by add up to 1), and its place among the slab's operand.  One bf16 part leaves
+    // 2^-9 of a weight, and 0.0023 of the output against 64 bits where rounding the result alone leaves 0.0017; a
+    // second part, as in the few kernel, would be half as many products again where products bound the call.
     auto p_pair = [&](int set, int u) __attribute__((always_inline)) {
       const int sl = u / 4, j = u % 4, kb = sl >> 1, v = 8 * (sl & 1) + 2 * j;
       const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[set][kb][v], p.scale_log2, -m_ref));
@@ -952,6 +955,8 @@ struct ChunkPlan {
 // as three, and every block's sums, written and read at 5 TB/s, 0.02 (a tile of 128 queries and 64 keys:
 // 1.3 us).  4 x 512 tokens over 4096 of 12/4 heads of 64: one split 55 us, two 51, three 56; 64 over 8192
 // of 16/8 heads of 128: one split 137, two 77, four 45, eight 31; 2048 over 65536: one 1133, two 994, four 999.
+// The host knows the table's width alone, and not the lengths: 256 tokens over 4096 slots take 31 us in a table
+// of that width, 33 in one of 16384 and 76 in one of 65536 slots; 2048 over 8192 136, 149 and 148.
 int tile_splits(int64_t blocks, int64_t key_tiles) {
   const int64_t slots = 2 * device_cu_count();
   int best = 1;
@@ -969,7 +974,8 @@ ChunkPlan chunk_plan(int64_t rows, int64_t B, int64_t nq, int64_t nkv, int64_t h
   ChunkPlan c{};
   const int64_t group = nq / nkv;
   // Calls of so few queries: 1 x 8 tokens over 4096 slots 13.4 us, by the tile kernel 21.5; 32 x 4 over 1024 29, 41;
-  // 64 x 1 over 2048 94, 113; 64 x 4 over 1000 of 8/4 heads of 40 13, 27; but 64 x 8 over 2048 120, 100.
+  // 64 x 1 over 2048 94, 113; 64 x 4 over 1000 of 8/4 heads of 40 13, 27; but 64 x 8 over 2048 120, 100, which a
+  // rule by the queries alone does not tell from the others.
   c.few = std::min(most, rows) * group <= kFew;
   const int64_t size = c.few ? kFew : kTileM;
   c.tiles = rows * group / size + B;

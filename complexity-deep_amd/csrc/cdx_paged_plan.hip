@@ -14,10 +14,11 @@
 //   chunk_append_kernel  per row of the packed projection: per-head RMSNorm, RoPE, q out, k and v into the
 //                    row's slot; 16 lanes a head, as paged_append_kernel.
 //
-// Measured (us of a kernel): reserve 3.0 for one sequence, 4.5 for 256 with 8432 rows or 64 with 131072 (launch and two
-// rounds of loads); truncate 2.9 for 256 sequences, 5.0 for 1024 that give 32000 pages back; append of 8192 rows of
-// 16/8 heads of 128 25 (134 MB read and written, 5.4 TB/s, a plain copy's rate), of 5 rows 2.7.  Two heads a group of
-// lanes, loaded together, took as long.
+// Measured (us of a kernel): reserve 3.1 for one sequence, 4.6 for 256 with 8432 rows or 64 with 131072 (launch and
+// two rounds of loads); truncate 2.9 for 256 sequences, 5.2 for 1024 that give 32000 pages back; append of 8192
+// rows of 16/8 heads of 128 25 (134 MB read and written, 5.4 TB/s, a plain copy's rate), of 5 rows 2.9.  Two heads a
+// group of lanes, loaded together, took as long.  Narrower heads leave lanes of their 16 without dims: 8192 rows of
+// 16/4 heads of 80 17 (63 MB: 3.7 TB/s), 12/4 of 64 14 (42 MB: 3.0), 8/4 of 40 12 (21 MB: 1.8).
 #include "cdx_paged.h"
 #include "cdx_wave.h"
 

@@ -397,7 +397,7 @@ class ComplexityModel(nn.Module):
         """The logits [B, V] behind each prompt's last token, its tokens taken ``chunk`` at a time."""
         B, S = input_ids.shape
         n = torch.full((B,), S) if prompt_lengths is None else cache.prompt_counts(prompt_lengths, S)
-        last_row = _to_device(n - 1, input_ids.device)
+        last_row = _to_device(n - 1, input_ids.device).to(input_ids.device)
         last = None
         for at in range(0, S, chunk):
             piece = input_ids[:, at:at + chunk]

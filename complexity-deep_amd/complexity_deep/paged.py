@@ -716,6 +716,8 @@ class PagedKVCache:
                 self._counts[0].copy_(n)
             self._lengths = known
             torch.sub(self._counts[0], 1, out=self._counts[1])
+            if self.weights is not None and capturing:  # (replays begin the batch anew)
+                self.weights.zero_()
             if self.slot_positions is not None:
                 at = torch.arange(self.capacity, dtype=torch.int32, device=self.slot_positions.device)
                 self.slot_positions.copy_(torch.where(at < self.lengths.view(-1, 1, 1), at, -1))

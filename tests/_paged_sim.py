@@ -60,7 +60,8 @@ class Sim:
 
     def _tensors(self):
         c = self.cache
-        return [t for t in (c._state, c._undo, c.block_table, c.free_pages) if t is not None]
+        return [t for t in (c._state, c._undo, c.block_table, c.free_pages, c.weights, c.slot_positions)
+                if t is not None]
 
     def _host(self):
         return {name: getattr(self.cache, name) for name in HOST}

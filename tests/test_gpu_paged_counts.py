@@ -202,3 +202,25 @@ def test_counts_of_the_host_in_a_captured_call(cdx):
         want = m(ids, past_key_values=eager, token_counts=counts).logits
         assert torch.equal(logits[0], want[0]) and torch.equal(logits[1, :2], want[1, :2])
         assert torch.equal(cache._state, eager._state) and cache.lengths.tolist() == [3 * i + 3, 2 * i + 2]
+
+
+@torch.inference_mode()
+def test_replayed_prompts_of_a_bounded_cache(cdx):
+    """Cuts go by the weights of the batch at hand, not by those of the last one."""
+    print("counts: prompts replayed on a bounded cache", flush=True)
+    m = _model(cdx, 64, 4, 2)
+    cache, eager, other = (cdx.PagedKVCache(m.config, 2, 32, page_size=16, keep=14, recent=4) for _ in range(3))
+    gen = torch.Generator().manual_seed(4)
+    ids = torch.zeros(2, 12, dtype=torch.int64, device="cuda")
+    prompts, logits = _graph(lambda: m(ids, past_key_values=cache).logits, lambda: m(ids, past_key_values=other))
+    for _ in range(3):
+        ids.copy_(torch.randint(0, 600, (2, 12), generator=gen))
+        prompts.replay()
+        eager.reset()
+        assert torch.equal(logits, m(ids, past_key_values=eager).logits)
+        for i in range(45):
+            x = torch.randint(0, 600, (2, 1), generator=gen).cuda()
+            got, want = (m(x, past_key_values=c).logits for c in (cache, eager))
+            assert torch.equal(got, want) and torch.equal(cache.lengths, eager.lengths), i
+        assert torch.equal(cache.slot_positions[..., :14], eager.slot_positions[..., :14])
+        assert int(cache.lengths.max()) < 32 and cache.positions.tolist() == [56, 56]

@@ -238,3 +238,18 @@ def test_prompts_of_a_cache_that_the_device_has_emptied(monkeypatch, pages, repl
         cache.begin(2, *prompts)
         assert cache.prompt
         sim.holds([prompts[0]] * 2 if prompts[1] is None else prompts[1].tolist(), pages)
+
+
+def test_replayed_prompts_of_a_bounded_cache_have_no_weights_of_the_last_batch(monkeypatch):
+    """The weights say what a later cut keeps."""
+    sim = Sim(monkeypatch, 2, 32, page_size=16, keep=20)
+    cache = sim.cache
+    cache.weights.fill_(3.0)  # (as steps leave them)
+    prompts = sim.capture(lambda c: c.begin(2, 9))
+    assert bool((cache.weights == 3.0).all())
+    for _ in range(2):
+        sim.replay(prompts)
+        sim.holds([9, 9])
+        assert not cache.weights.any()
+        assert cache.slot_positions[..., :9].eq(torch.arange(9)).all() and cache.slot_positions[..., 9:].eq(-1).all()
+        cache.weights.fill_(2.0)

@@ -70,7 +70,7 @@ bool overlap(const Extent (&in)[NIn], const Extent (&out)[NOut]) {
   for (const Extent& o : out)
     for (const Extent& i : in) {
       const uintptr_t a = reinterpret_cast<uintptr_t>(o.at), b = reinterpret_cast<uintptr_t>(i.at);
-      if (o.at && i.at && a < b + (uintptr_t)i.bytes && b < a + (uintptr_t)o.bytes) return true;
+      if (o.at && i.at && o.bytes > 0 && a < b + (uintptr_t)i.bytes && b < a + (uintptr_t)o.bytes) return true;
     }
   return false;
 }

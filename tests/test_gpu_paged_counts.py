@@ -224,3 +224,16 @@ def test_replayed_prompts_of_a_bounded_cache(cdx):
             assert torch.equal(got, want) and torch.equal(cache.lengths, eager.lengths), i
         assert torch.equal(cache.slot_positions[..., :14], eager.slot_positions[..., :14])
         assert int(cache.lengths.max()) < 32 and cache.positions.tolist() == [56, 56]
+
+
+def test_reserve_without_rows_by_the_entry_point(cdx):
+    """Results of no bytes lie over nothing, wherever their pointers are."""
+    print("counts: reserve without rows", flush=True)
+    from complexity_deep import _native as nat
+    x = torch.tensor([[0, 0], [5, 9], [4, 8]], dtype=torch.int32, device="cuda")  # counts, lengths, positions
+    table = torch.tensor([[3, 4], [1, 2]], dtype=torch.int32, device="cuda")
+    out = torch.empty(4, 2, dtype=torch.int32, device="cuda")
+    nat.check(nat.lib().cdx_paged_reserve(
+        *(t.data_ptr() for t in x), 2, 0, 0, table.data_ptr(), 2, 2, 16, None, 0, None, *(t.data_ptr() for t in out), None,
+        x.data_ptr() + 4, x.data_ptr() + 4, nat.stream_of(x)), "cdx_paged_reserve")
+    assert out.tolist() == [[0, 0], [0, 0], [5, 9], [4, 8]]
